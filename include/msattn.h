@@ -356,6 +356,54 @@ int msattn_paged_attention_append(const void* query, const void* k_new, const vo
                                   float scale, int q_dtype, int kv_dtype, void* stream);
 
 /*
+ * msattn_write_kv with the keys rotated on the way, and the step's queries rotated beside them,
+ * in one launch. Token t of row b goes to cache position starts[b] + t as in msattn_write_kv
+ * (holes and positions outside the table are skipped); it is rotated at row
+ *   starts[b] + t                 position == NULL
+ *   position[b] + t               position_per_token == 0, position int32 [batch]
+ *   position[b * tokens + t]      position_per_token != 0, position int32 [batch, tokens]
+ * of rope_cos / rope_sin, fp32 [max_position, rotary_dim] contiguous, clamped to
+ * [0, max_position): rotate-half (miniserve/attention.py:41-62) of the first rotary_dim dims
+ * (even, at most head_dim), the others unchanged, in fp32, every product and the sum rounded on
+ * its own. Queries are rounded once to src_dtype, keys once to kv_dtype (straight from fp32),
+ * values as msattn_write_kv rounds them. query [batch, tokens, num_heads, head_dim] goes to
+ * query_out, holes or not; query_out may be query itself with the same strides, no other overlap
+ * of a source with query_out or the caches is allowed. query == NULL: keys and values alone
+ * (query_out, both query strides and num_heads are not read). *_strides: batch, token and head
+ * strides in elements, at least 0, read on the host; head dim contiguous. src_dtype is fp32, fp16
+ * or bf16, head_dim up to 256. Two tokens of one launch in one cache slot: either's row remains.
+ * The reference makes these calls one by one (miniserve/model_runner.py:62-76).
+ */
+int msattn_write_kv_rope(const void* query, const int64_t* q_strides, void* query_out,
+                         const int64_t* q_out_strides, const void* k, const int64_t* k_strides,
+                         const void* v, const int64_t* v_strides, void* k_cache, void* v_cache,
+                         int64_t cache_block_stride, int64_t cache_slot_stride,
+                         int64_t cache_head_stride, const int32_t* block_table,
+                         const int32_t* starts, const float* rope_cos, const float* rope_sin,
+                         const int32_t* position, int position_per_token, int max_position,
+                         int rotary_dim, int batch, int tokens, int num_heads, int num_kv_heads,
+                         int head_dim, int block_size, int num_blocks, int table_width,
+                         int src_dtype, int kv_dtype, void* stream);
+
+/*
+ * msattn_paged_attention_append with rotate-half RoPE on the query and on the new key: k_new is
+ * rotated as msattn_write_kv_rope rotates it (rotary_dim == head_dim) on its way to position
+ * context_lens[b] - 1, the query as msattn_paged_attention_rope rotates it, both at row
+ * position[b] of the tables (position == NULL: context_lens[b] - 1), clamped to
+ * [0, max_position). rope_cos / rope_sin are 16-byte aligned. One launch where
+ * msattn_paged_attention_append is one, else the write, then the decode: the same caches and
+ * output as msattn_write_kv_rope of the new token followed by msattn_paged_attention_rope.
+ */
+int msattn_paged_attention_append_rope(
+    const void* query, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+    int64_t cache_block_stride, int64_t cache_slot_stride, int64_t cache_head_stride,
+    const int32_t* block_table, const int32_t* context_lens, void* out, void* workspace,
+    size_t workspace_bytes, int batch, int num_heads, int num_kv_heads, int head_dim,
+    int block_size, int num_blocks, int table_width, int max_context, int window, float scale,
+    int q_dtype, int kv_dtype, const float* rope_cos, const float* rope_sin,
+    const int32_t* position, int max_position, void* stream);
+
+/*
  * Block-table gather: out[b, p] = cache[table[b, p / block_size], p % block_size]
  * for p < context_lens[b]; positions p >= context_lens[b] read page 0 (as the
  * reference does), holes give zero rows. out is [batch, max_context,

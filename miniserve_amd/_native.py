@@ -85,6 +85,14 @@ SIGNATURES = {
         c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_size,
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
         c_float, c_int, c_int, c_vp]),
+    "msattn_write_kv_rope": (c_int, [
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64,
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "msattn_paged_attention_append_rope": (c_int, [
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_size,
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_float, c_int, c_int, c_vp, c_vp, c_vp, c_int, c_vp]),
     "msattn_gather_kv": (c_int, [
         c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp,
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),

@@ -28,6 +28,7 @@ from typing import Sequence
 import torch
 
 from . import _native as nat
+from .rotary import on_device, rope_table, write_kv_rope
 
 _BACKENDS = ("sdpa", "triton_flash")
 
@@ -163,6 +164,20 @@ def context_lens_i32(context_lens, device: torch.device, batch: int) -> tuple[to
     return lens, host_max
 
 
+def starts_i32(start, batch: int, device: torch.device) -> torch.Tensor:
+    """int32 device tensor of each row's first position: an int, one entry per row (at least),
+    or an int tensor."""
+    if isinstance(start, torch.Tensor):
+        starts = start.reshape(-1).to(device=device, dtype=torch.int32)
+    elif isinstance(start, Sequence):
+        starts = _host_ints_to_device([int(s) for s in start], device)
+    else:
+        starts = torch.full((batch,), int(start), dtype=torch.int32, device=device)
+    if starts.numel() < batch:
+        raise ValueError("start needs one entry per batch row")
+    return starts.contiguous()
+
+
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """A zeroed workspace of at least `nbytes` for calls on the current stream of `device`.
 
@@ -262,15 +277,7 @@ class PagedAttention:
         table = block_table_i32(block_table, dev)
         if table.shape[0] < B:
             raise ValueError("block_table has fewer rows than k")
-        if isinstance(start, torch.Tensor):
-            starts = start.reshape(-1).to(device=dev, dtype=torch.int32)
-        elif isinstance(start, Sequence):
-            starts = _host_ints_to_device([int(s) for s in start], dev)
-        else:
-            starts = torch.full((B,), int(start), dtype=torch.int32, device=dev)
-        if starts.numel() < B:
-            raise ValueError("start needs one entry per batch row")
-        starts = starts.contiguous()
+        starts = starts_i32(start, B, dev)
         if not (k.is_contiguous() and v.is_contiguous()) and \
                 _readable_in_place(k, k_cache, v_cache) and \
                 _readable_in_place(v, k_cache, v_cache) and _worth_in_place(k) and _worth_in_place(v):
@@ -291,6 +298,24 @@ class PagedAttention:
             B, T, KVH, D, k_cache.shape[1], k_cache.shape[0], table.shape[1],
             nat.dtype_code(k.dtype), nat.dtype_code(k_cache.dtype), nat.stream_handle(dev))
         nat.check("msattn_write_kv", status)
+
+    def write_kv_rope(
+        self,
+        k_cache: torch.Tensor,
+        v_cache: torch.Tensor,
+        query: torch.Tensor | None,
+        k: torch.Tensor,
+        v: torch.Tensor,
+        block_table: torch.Tensor,
+        start: int | Sequence[int] | torch.Tensor = 0,
+        *,
+        cos: torch.Tensor,
+        sin: torch.Tensor,
+        position: torch.Tensor | None = None,
+    ) -> torch.Tensor | None:
+        """``write_kv`` with the keys rotated on the way; returns the rotated ``query``
+        (miniserve_amd.rotary.write_kv_rope: one launch for apply_rope and write_kv)."""
+        return write_kv_rope(query, k, v, k_cache, v_cache, block_table, start, cos, sin, position)
 
     def build_mask(
         self,
@@ -497,7 +522,8 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
                            context_lens, *, window: int | None = None,
                            scale: float | None = None, max_context: int | None = None,
                            workspace: torch.Tensor | None = None,
-                           out: torch.Tensor | None = None) -> torch.Tensor:
+                           out: torch.Tensor | None = None,
+                           rope: tuple | None = None) -> torch.Tensor:
     """One decode step with the new token appended: ``write_kv`` of k_new / v_new
     ([batch, 1, kv_heads, head_dim], the query's dtype) at position context_lens[b] - 1
     of each row, then the causal decode over ``context_lens`` (which count the new
@@ -505,6 +531,11 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
     nothing. On the partition kernel (small decodes, bf16/fp16 query, at most 8 query rows
     per KV head) both happen in one launch; the caches and the output equal those of
     ``write_kv`` followed by ``paged_attention`` bit for bit.
+    ``rope`` = (cos, sin) or (cos, sin, position): the query and the new key are rotated on the
+    way (rotate-half, fp32 tables [max_pos, rotary_dim]), at context_lens[b] - 1 or at
+    position[b], clamped to [0, max_pos): ``write_kv_rope`` of the new token, then the decode,
+    in the launches of the call without it (msattn_paged_attention_append_rope). A rotary_dim
+    below head_dim makes the two calls.
     """
     _require_gpu(query, "query")
     _require_gpu(k_cache, "k_cache")
@@ -554,6 +585,35 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
         workspace = _workspace(dev, ws_bytes)
     if out is None:
         out = torch.empty((B, 1, H, D), dtype=query.dtype, device=dev)
+    if rope is not None:
+        if len(rope) not in (2, 3):
+            raise ValueError("rope must be (cos, sin) or (cos, sin, position)")
+        cos, sin = rope_table(rope[0], dev, "cos"), rope_table(rope[1], dev, "sin")
+        if cos.shape != sin.shape or cos.shape[1] % 2 or not 0 < cos.shape[1] <= D:
+            raise ValueError(f"cos/sin must share one [max_pos, rotary_dim] shape, rotary_dim even "
+                             f"and at most {D}")
+        pos = None
+        if len(rope) == 3 and rope[2] is not None:
+            pos = torch.as_tensor(rope[2], device=dev).reshape(-1).to(torch.int32)
+            if pos.numel() == 1:
+                pos = pos.expand(B)
+            if pos.numel() != B:
+                raise ValueError(f"position has {pos.numel()} entries for a batch of {B}")
+            pos = pos.contiguous()
+        if cos.shape[1] < D:
+            q = write_kv_rope(q, kn, vn, k_cache, v_cache, table, lens - 1, cos, sin, pos)
+            return paged_attention(q, k_cache, v_cache, table, lens, window=window, scale=scale,
+                                   max_context=max_context, workspace=workspace, out=out)
+        status = on_device(
+            dev, L.msattn_paged_attention_append_rope,
+            q.data_ptr(), kn.data_ptr(), vn.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), table.data_ptr(),
+            lens.data_ptr(), out.data_ptr(), workspace.data_ptr(), ws_bytes, B, H, KVH, D, bs, nb,
+            W, max_context, int(window or 0), float(scale), nat.dtype_code(query.dtype),
+            nat.dtype_code(k_cache.dtype), cos.data_ptr(), sin.data_ptr(),
+            pos.data_ptr() if pos is not None else None, cos.shape[0])
+        nat.check("msattn_paged_attention_append_rope", status)
+        return out
     status = L.msattn_paged_attention_append(
         q.data_ptr(), kn.data_ptr(), vn.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
         k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), table.data_ptr(),

@@ -69,6 +69,16 @@ int write_kv_impl(void* k_cache, void* v_cache, int64_t cache_block_stride,
                   int start_offset, int batch, int tokens, int num_kv_heads, int head_dim,
                   int block_size, int num_blocks, int table_width, int src_dtype, int kv_dtype,
                   void* stream, const int64_t* src_strides = nullptr);
+int write_kv_rope_impl(const void* query, const int64_t* q_strides, void* query_out,
+                       const int64_t* q_out_strides, const void* k, const int64_t* k_strides,
+                       const void* v, const int64_t* v_strides, void* k_cache, void* v_cache,
+                       int64_t cache_block_stride, int64_t cache_slot_stride,
+                       int64_t cache_head_stride, const int32_t* block_table,
+                       const int32_t* starts, int start_offset, const float* rope_cos,
+                       const float* rope_sin, const int32_t* position, int position_per_token,
+                       int max_position, int rotary_dim, int batch, int tokens, int num_heads,
+                       int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                       int table_width, int src_dtype, int kv_dtype, void* stream);
 #ifndef MSATTN_WIDE_ROUTE
 #define MSATTN_WIDE_ROUTE 1
 #endif
@@ -527,6 +537,7 @@ struct RopeArgs {
   const float* sin;
   const int32_t* pos;
   int max_pos;
+  int pos_add;  // added to pos[b] (-1: pos are context lengths that count the new token)
 };
 
 // Which partials kernel a call takes (kind as the workspace header records it: 1 stream-K,
@@ -693,6 +704,7 @@ int partials_impl(const void* query, const void* k_cache, const void* v_cache,
   p.rope_sin = rope.sin;
   p.rope_pos = rope.pos;
   p.rope_max_pos = rope.max_pos;
+  p.rope_pos_add = rope.pos_add;
   p.out = nullptr;
   p.tickets = nullptr;
   p.k_new = nullptr;
@@ -1612,9 +1624,157 @@ int msattn_paged_attention_append(const void* query, const void* k_new, const vo
                                 scale, q_dtype, kv_dtype, stream);
 }
 
+int msattn_write_kv_rope(const void* query, const int64_t* q_strides, void* query_out,
+                         const int64_t* q_out_strides, const void* k, const int64_t* k_strides,
+                         const void* v, const int64_t* v_strides, void* k_cache, void* v_cache,
+                         int64_t cache_block_stride, int64_t cache_slot_stride,
+                         int64_t cache_head_stride, const int32_t* block_table,
+                         const int32_t* starts, const float* rope_cos, const float* rope_sin,
+                         const int32_t* position, int position_per_token, int max_position,
+                         int rotary_dim, int batch, int tokens, int num_heads, int num_kv_heads,
+                         int head_dim, int block_size, int num_blocks, int table_width,
+                         int src_dtype, int kv_dtype, void* stream) {
+  return write_kv_rope_impl(query, q_strides, query_out, q_out_strides, k, k_strides, v, v_strides,
+                            k_cache, v_cache, cache_block_stride, cache_slot_stride,
+                            cache_head_stride, block_table, starts, 0, rope_cos, rope_sin, position,
+                            position_per_token, max_position, rotary_dim, batch, tokens, num_heads,
+                            num_kv_heads, head_dim, block_size, num_blocks, table_width, src_dtype,
+                            kv_dtype, stream);
+}
+
+int msattn_paged_attention_append_rope(
+    const void* query, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+    int64_t cache_block_stride, int64_t cache_slot_stride, int64_t cache_head_stride,
+    const int32_t* block_table, const int32_t* context_lens, void* out, void* workspace,
+    size_t workspace_bytes, int batch, int num_heads, int num_kv_heads, int head_dim,
+    int block_size, int num_blocks, int table_width, int max_context, int window, float scale,
+    int q_dtype, int kv_dtype, const float* rope_cos, const float* rope_sin,
+    const int32_t* position, int max_position, void* stream) {
+  if (!query || !k_new || !v_new || !k_cache || !v_cache || !block_table || !context_lens || !out ||
+      !workspace)
+    return MSATTN_ERR_INVALID_ARG;
+  if (!dtype_ok(q_dtype) || q_dtype == MSATTN_FP8_E4M3 || !dtype_ok(kv_dtype))
+    return MSATTN_ERR_INVALID_ARG;
+  if (!geometry_ok(batch, 1, num_heads, num_kv_heads, head_dim, max_context) ||
+      !std::isfinite(scale))
+    return MSATTN_ERR_INVALID_ARG;
+  if (!rope_cos || !rope_sin || max_position <= 0 || !aligned(rope_cos, 16) ||
+      !aligned(rope_sin, 16) || !aligned(position, 4) || !aligned(out, dtype_bytes(q_dtype)) ||
+      !aligned(query, dtype_bytes(q_dtype)) || !aligned(workspace, 16))
+    return MSATTN_ERR_INVALID_ARG;
+  const int rc = check_cache_args(k_cache, v_cache, cache_block_stride, cache_slot_stride,
+                                  cache_head_stride, kv_dtype, block_size, num_blocks, table_width);
+  if (rc != MSATTN_OK) return rc;
+  // Everything the decode refuses is refused before the append writes.
+  const Layout L = workspace_layout(batch, 1, num_heads, num_kv_heads, head_dim, max_context);
+  if (workspace_bytes < L.total()) return MSATTN_ERR_WORKSPACE;
+  const PartialsPlan plan = plan_partials(
+      query, q_dtype, kv_dtype, head_dim, block_size, cache_slot_stride,
+      cache_rows16(k_cache, v_cache, cache_block_stride, cache_slot_stride, cache_head_stride,
+                   head_dim, kv_dtype),
+      batch, 1, num_heads, num_kv_heads, max_context, true, 0, window);
+  const int64_t gx = static_cast<int64_t>(L.max_parts) * num_kv_heads *
+                     ceil_div(num_heads / num_kv_heads, plan.RT);
+  if (gx >= (int64_t(1) << 31) || batch > 65535) return MSATTN_ERR_UNSUPPORTED;
+  // Without positions of its own the new token sits where the cache has it, at length - 1.
+  const RopeArgs rope{rope_cos, rope_sin, position ? position : context_lens, max_position,
+                      position ? 0 : -1};
+  const bool fused = kFusedAppend && append_built(plan, q_dtype, kv_dtype) && aligned(k_new, 16) &&
+                     aligned(v_new, 16);
+  if (!fused) {  // the write, then the decode (the same result)
+    const int64_t row = head_dim, tok = row * num_kv_heads;
+    const int64_t dense[3] = {tok, tok, row};
+    const int rw = write_kv_rope_impl(
+        nullptr, nullptr, nullptr, nullptr, k_new, dense, v_new, dense, k_cache, v_cache,
+        cache_block_stride, cache_slot_stride, cache_head_stride, block_table, context_lens, -1,
+        rope_cos, rope_sin, position, 0, max_position, head_dim, batch, 1, 0, num_kv_heads,
+        head_dim, block_size, num_blocks, table_width, q_dtype, kv_dtype, stream);
+    if (rw != MSATTN_OK) return rw;
+  }
+  int kind = -1;
+  const int rd = partials_impl(
+      query, k_cache, v_cache, cache_block_stride, cache_slot_stride, cache_head_stride,
+      block_table, context_lens, workspace, workspace_bytes, batch, 1, num_heads, num_kv_heads,
+      head_dim, block_size, num_blocks, table_width, max_context, 1, window, scale, q_dtype,
+      kv_dtype, rope, 0, &kind, stream, out, fused ? k_new : nullptr, fused ? v_new : nullptr);
+  if (rd != MSATTN_OK) return rd;
+  if (kind == 2) return MSATTN_OK;  // merged in-kernel
+  return merge_impl(workspace, workspace_bytes, context_lens, out, batch, 1, num_heads,
+                    num_kv_heads, head_dim, max_context, q_dtype, nullptr, nullptr, 0, kind, stream);
+}
+
 }  // extern "C"
 
 namespace {
+
+int write_kv_rope_impl(const void* query, const int64_t* q_strides, void* query_out,
+                       const int64_t* q_out_strides, const void* k, const int64_t* k_strides,
+                       const void* v, const int64_t* v_strides, void* k_cache, void* v_cache,
+                       int64_t cache_block_stride, int64_t cache_slot_stride,
+                       int64_t cache_head_stride, const int32_t* block_table,
+                       const int32_t* starts, int start_offset, const float* rope_cos,
+                       const float* rope_sin, const int32_t* position, int position_per_token,
+                       int max_position, int rotary_dim, int batch, int tokens, int num_heads,
+                       int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                       int table_width, int src_dtype, int kv_dtype, void* stream) {
+  if (!k || !v || !k_strides || !v_strides || !k_cache || !v_cache || !block_table || !starts ||
+      !rope_cos || !rope_sin)
+    return MSATTN_ERR_INVALID_ARG;
+  if (query != nullptr && (!query_out || !q_strides || !q_out_strides || num_heads <= 0))
+    return MSATTN_ERR_INVALID_ARG;
+  if (batch <= 0 || tokens < 0 || num_kv_heads <= 0 || head_dim <= 0 || head_dim > kMaxHeadDim)
+    return MSATTN_ERR_INVALID_ARG;
+  if (rotary_dim <= 0 || rotary_dim % 2 || rotary_dim > head_dim || max_position <= 0)
+    return MSATTN_ERR_INVALID_ARG;
+  if (!dtype_ok(src_dtype) || src_dtype == MSATTN_FP8_E4M3 || !dtype_ok(kv_dtype))
+    return MSATTN_ERR_INVALID_ARG;
+  const int rc = check_cache_args(k_cache, v_cache, cache_block_stride, cache_slot_stride,
+                                  cache_head_stride, kv_dtype, block_size, num_blocks, table_width);
+  if (rc != MSATTN_OK) return rc;
+  const int eb = dtype_bytes(src_dtype);
+  if (!aligned(k, eb) || !aligned(v, eb) || !aligned(query, eb) || !aligned(query_out, eb) ||
+      !aligned(rope_cos, 4) || !aligned(rope_sin, 4) || !aligned(position, 4))
+    return MSATTN_ERR_INVALID_ARG;
+  RopeWriteParams p{};
+  for (int i = 0; i < 3; ++i) {
+    p.k_src[i] = k_strides[i];
+    p.v_src[i] = v_strides[i];
+    if (query != nullptr) {
+      p.q_src[i] = q_strides[i];
+      p.q_dst[i] = q_out_strides[i];
+    }
+    if (p.k_src[i] < 0 || p.v_src[i] < 0 || p.q_src[i] < 0 || p.q_dst[i] < 0)
+      return MSATTN_ERR_INVALID_ARG;
+  }
+  if (tokens == 0) return MSATTN_OK;
+  p.q = query;
+  p.q_out = query_out;
+  p.k = k;
+  p.v = v;
+  p.k_cache = k_cache;
+  p.v_cache = v_cache;
+  p.table = block_table;
+  p.starts = starts;
+  p.cos = rope_cos;
+  p.sin = rope_sin;
+  p.position = position;
+  p.position_per_token = position_per_token ? 1 : 0;
+  p.blk_stride = cache_block_stride;
+  p.slot_stride = cache_slot_stride;
+  p.head_stride = cache_head_stride;
+  p.batch = batch;
+  p.tokens = tokens;
+  p.QH = query != nullptr ? num_heads : 0;
+  p.KVH = num_kv_heads;
+  p.D = head_dim;
+  p.R = rotary_dim;
+  p.max_pos = max_position;
+  p.bs = block_size;
+  p.num_blocks = num_blocks;
+  p.W = table_width;
+  p.start_offset = start_offset;
+  return hip_status(launch_rope_write(p, src_dtype, kv_dtype, static_cast<hipStream_t>(stream)));
+}
 
 int write_kv_impl(void* k_cache, void* v_cache, int64_t cache_block_stride,
                   int64_t cache_slot_stride, int64_t cache_head_stride, const void* k,

@@ -652,8 +652,54 @@ __device__ __forceinline__ void rope_chunks(typename QChunk<T>::type (&qb)[D / 3
   }
 }
 
+// The new token's key row, held as append chunks of the query type (chunk j of lane group g as
+// rope_chunks' query chunks), rotated at row cs / sn of the tables and cast once, from fp32, to
+// the cache's chunks: what msattn_write_kv_rope writes. Lanes l and l ^ 32 (the same token) are
+// both active or both not.
+template <typename T, typename KT, int D>
+__device__ __forceinline__ void rope_new_key(const SrcChunk<T> (&kn)[D / 32], const float* cs,
+                                             const float* sn, int g,
+                                             typename Kv8<T, KT>::raw_t (&out)[D / 32]) {
+  typedef typename Kv8<T, KT>::raw_t raw_t;
+  static_assert(sizeof(raw_t) == 8 * sizeof(KT) && sizeof(T) == 2, "eight cache elements a chunk");
+  constexpr int JD = D / 32;
+  constexpr bool kCross = sizeof(KT) == 1 && D == 64;  // the partner is in the other half-wave
+  float k[JD][8], kp[JD][8];
+#pragma unroll
+  for (int j = 0; j < JD; ++j) {
+    const uint4 x = __builtin_bit_cast(uint4, kn[j]);
+    Chunk<T>::unpack(x, k[j]);
+    if constexpr (kCross) {
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const auto t = __builtin_amdgcn_permlane32_swap(w[i], w[i], false, false);
+        o[i] = g < 2 ? t[1] : t[0];
+      }
+      Chunk<T>::unpack(make_uint4(o[0], o[1], o[2], o[3]), kp[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < JD; ++j) {
+    const int d0 = Kv8<T, KT>::qk_dim0(j, g, JD);
+    CacheChunk<KT> c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float r;
+      if constexpr (kCross)
+        r = g < 2 ? -kp[j][e] : kp[j][e];
+      else
+        r = j < JD / 2 ? -k[j + JD / 2][e] : k[j - JD / 2][e];
+      Elt<KT>::store(&c.v[e], rope_mix(k[j][e], r, cs[d0 + e], sn[d0 + e]));
+    }
+    out[j] = __builtin_bit_cast(raw_t, c);
+  }
+}
+
+// APPEND: 1 the fused append, 2 the fused append of a key that is rotated on the way.
 template <typename T, typename KT, int D, int RT, int W = kMfmaWaves, int WPC = kMfmaWgPerCu,
-          bool APPEND = false>
+          int APPEND = 0>
 __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParams p) {
   constexpr int kWaves = W;               // waves per workgroup
   constexpr int kThreads = W * kWave;
@@ -967,6 +1013,23 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
     return;
   }
 
+  // The fused append of a rotated key (APPEND 2): the wave whose run holds the new position
+  // requests the key beside the query and rotates it after it, at the same row of the tables.
+  constexpr bool kAppendTurns = APPEND == 2 && !kPvMfma && sizeof(T) == 2 && RT <= 8;
+  const int k_turn = kAppendTurns && ctx > 0 ? (ctx - 1) / 16 - tw0 : -1;
+  const bool turn_lane = kAppendTurns && p.k_new != nullptr && k_turn >= 0 && k_turn < nt &&
+                         tile_token<D>(n) == ((ctx - 1) & 15);
+  SrcChunk<T> k_in[kAppendTurns ? JD : 1];
+  raw_t k_turned[kAppendTurns ? JD : 1];
+  if constexpr (kAppendTurns) {
+    if (turn_lane) {
+      const T* const src = static_cast<const T*>(p.k_new) + (static_cast<int64_t>(b) * p.KVH + kvh) * D;
+#pragma unroll
+      for (int j = 0; j < JD; ++j)
+        k_in[j] = *reinterpret_cast<const SrcChunk<T>*>(src + KV::qk_dim0(j, g, JD));
+    }
+  }
+
   // Query rows as the MFMA B operand: lane (g, n) holds Q[row n][dims 8*(4j+g) .. +8].
   typename QChunk<T>::type qb[JD];
 
@@ -981,6 +1044,12 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
     if (p.rope_cos != nullptr && n < nrows) {
       const int64_t po = static_cast<int64_t>(rope_position(p, b)) * D;
       rope_chunks<T, KT, D>(qb, p.rope_cos + po, p.rope_sin + po, g);
+    }
+  }
+  if constexpr (kAppendTurns) {
+    if (turn_lane) {
+      const int64_t po = static_cast<int64_t>(rope_position(p, b)) * D;
+      rope_new_key<T, KT, D>(k_in, p.rope_cos + po, p.rope_sin + po, g, k_turned);
     }
   }
   // Tiles a wave may own: partitions of the fp32 16-row route reach kPartLongF32 tokens.
@@ -1094,7 +1163,7 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
   // the store.
   // (Built as its own instantiation, APPEND, for 2-byte queries at up to 8 rows per tile:
   // the chunks held for it take 16-36 registers, which cost the decode without it 0.5-2.6 %.)
-  constexpr bool kAppendOk = APPEND && !kPvMfma && sizeof(T) == 2 && RT <= 8;
+  constexpr bool kAppendOk = APPEND != 0 && !kPvMfma && sizeof(T) == 2 && RT <= 8;
   const bool app = kAppendOk && p.k_new != nullptr && ctx > 0;
   const int k_app = app ? (ctx - 1) / 16 - tw0 : -1;  // run index of the new token's tile
   const bool app_here = k_app >= 0 && k_app < nt;      // wave-uniform
@@ -1104,7 +1173,7 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
   SrcChunk<T> kn[JD], vn;
   if (app_here) {
     const int64_t row = (static_cast<int64_t>(b) * p.KVH + kvh) * D;
-    if (k_lane) {
+    if (!kAppendTurns && k_lane) {
 #pragma unroll
       for (int j = 0; j < JD; ++j)
         kn[j] = *reinterpret_cast<const SrcChunk<T>*>(static_cast<const T*>(p.k_new) + row +
@@ -1119,7 +1188,9 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
     if (k_lane) {
 #pragma unroll
       for (int j = 0; j < JD; ++j) {
-        const raw_t x = append_raw<KT, T, raw_t>(kn[j]);
+        raw_t x;
+        if constexpr (kAppendTurns) x = k_turned[j];
+        else x = append_raw<KT, T, raw_t>(kn[j]);
         kb[j] = x;
         *reinterpret_cast<raw_t*>(const_cast<KT*>(kbase) + rowoff + KV::qk_dim0(j, g, JD)) = x;
       }
@@ -1277,8 +1348,12 @@ hipError_t launch_decode_mfma_one(const SplitParams& p_in, hipStream_t stream) {
   // the fused append's instantiation (the host sets k_new only where it is built)
   if constexpr (sizeof(T) == 2 && RT <= 8) {
     if (p.k_new != nullptr) {
-      hipLaunchKernelGGL((decode_mfma_kernel<T, KT, D, RT, W, WPC, true>), grid, dim3(W * kWave),
-                         0, stream, p);
+      if (p.rope_cos != nullptr)
+        hipLaunchKernelGGL((decode_mfma_kernel<T, KT, D, RT, W, WPC, 2>), grid, dim3(W * kWave), 0,
+                           stream, p);
+      else
+        hipLaunchKernelGGL((decode_mfma_kernel<T, KT, D, RT, W, WPC, 1>), grid, dim3(W * kWave), 0,
+                           stream, p);
       return hipGetLastError();
     }
   }

@@ -86,7 +86,8 @@ __host__ __device__ constexpr int64_t streamk_pieces(int64_t n_chunks, int64_t n
   return n_chunks + n_segments;
 }
 
-template <typename T, typename KT, int D, int RT, bool APPEND = false>
+// APPEND: 1 the fused append, 2 the fused append of a key that is rotated on the way.
+template <typename T, typename KT, int D, int RT, int APPEND = 0>
 __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decode_streamk_kernel(
     const SplitParams p) {
   constexpr int kSkWaves = sk_waves(sizeof(KT), sizeof(T));
@@ -358,7 +359,7 @@ __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decod
   // reads that position, so nothing waits for the store.
   // (Not over an fp8 cache: its 8-wave workgroups keep two waves a SIMD, where the held
   // chunks would spill.)
-  constexpr bool kAppendOk = APPEND && sizeof(T) == 2 && sizeof(KT) != 1 && RT <= 8;
+  constexpr bool kAppendOk = APPEND != 0 && sizeof(T) == 2 && sizeof(KT) != 1 && RT <= 8;
   int app_t = -1;  // absolute tile index of the current piece to patch, or -1
   int app_r = 0;   // the new token's row in that tile
   SrcChunk<T> kn[JD], vn;
@@ -382,9 +383,18 @@ __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decod
     if (base < 0) return;  // a hole: write_kv writes nothing there either
     const int64_t rowoff = base + static_cast<int64_t>(app_r) * p.slot_stride;
     if (tile_token<D>(n) == app_r) {
+      // A rotated key is turned here, once a sequence: holding its table rows from the piece's
+      // start on would take 64 registers.
+      raw_t turned[APPEND == 2 ? JD : 1];
+      if constexpr (APPEND == 2) {
+        const int64_t po = static_cast<int64_t>(rope_position(p, cur.b)) * D;
+        rope_new_key<T, KT, D>(kn, p.rope_cos + po, p.rope_sin + po, g, turned);
+      }
 #pragma unroll
       for (int j = 0; j < JD; ++j) {
-        const raw_t x = append_raw<KT, T, raw_t>(kn[j]);
+        raw_t x;
+        if constexpr (APPEND == 2) x = turned[j];
+        else x = append_raw<KT, T, raw_t>(kn[j]);
         kb[j] = x;
         *reinterpret_cast<raw_t*>(const_cast<KT*>(kbase) + rowoff + KV::qk_dim0(j, g, JD)) = x;
       }
@@ -609,9 +619,13 @@ hipError_t launch_decode_streamk_one(const SplitParams& p, int grid, hipStream_t
   // the fused append's instantiation (the host sets k_new only where it is built)
   if constexpr (sizeof(T) == 2 && sizeof(KT) != 1 && RT <= 8) {
     if (p.k_new != nullptr) {
-      hipLaunchKernelGGL((decode_streamk_kernel<T, KT, D, RT, true>),
-                         dim3(static_cast<unsigned>(grid)),
-                         dim3(sk_waves(sizeof(KT), sizeof(T)) * kWave), 0, stream, p);
+      const dim3 threads(sk_waves(sizeof(KT), sizeof(T)) * kWave);
+      if (p.rope_cos != nullptr)
+        hipLaunchKernelGGL((decode_streamk_kernel<T, KT, D, RT, 2>), dim3(static_cast<unsigned>(grid)),
+                           threads, 0, stream, p);
+      else
+        hipLaunchKernelGGL((decode_streamk_kernel<T, KT, D, RT, 1>), dim3(static_cast<unsigned>(grid)),
+                           threads, 0, stream, p);
       return hipGetLastError();
     }
   }

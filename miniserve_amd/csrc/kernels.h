@@ -45,6 +45,32 @@ struct WriteKVParams {
 hipError_t launch_write_kv(const WriteKVParams& p, int src_dtype, int dst_dtype,
                            hipStream_t stream, bool* supported);
 
+// msattn_write_kv_rope (rope_write.hip): write_kv with the keys rotated on the way, and the
+// queries rotated beside them.
+struct RopeWriteParams {
+  const void* q;  // QH == 0: no queries
+  void* q_out;
+  const void* k;
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  const int32_t* table;
+  const int32_t* starts;
+  const float* cos;  // [max_pos, R]
+  const float* sin;
+  const int32_t* position;  // null: the cache position; else [batch] first positions or, with
+  int position_per_token;   // position_per_token, [batch, tokens]
+  int64_t q_src[3], k_src[3], v_src[3], q_dst[3];  // batch, token and head strides (elements)
+  int64_t blk_stride, slot_stride, head_stride;
+  int batch, tokens, QH, KVH, D, R, max_pos;
+  int bs, num_blocks, W;
+  int start_offset;  // added to starts[b] (-1: starts are context lengths after the append)
+  int items, slices;  // set by the launcher: lanes a row, waves a token
+};
+
+hipError_t launch_rope_write(const RopeWriteParams& p, int src_dtype, int kv_dtype,
+                             hipStream_t stream);
+
 struct GatherParams {
   const void* cache;
   const int32_t* table;

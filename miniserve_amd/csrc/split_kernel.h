@@ -103,6 +103,7 @@ struct SplitParams {
   const float* rope_sin;
   const int32_t* rope_pos;
   int rope_max_pos;
+  int rope_pos_add;  // added to rope_pos[b] (-1: rope_pos are context lengths after an append)
   // In-kernel merge (partition MFMA kernel only): non-null `out` [rows][D] of the query
   // type makes the last partition of each (sequence, KV head, row tile) to arrive merge
   // its partials and write the output; `tickets` are the header's arrival counters.
@@ -118,7 +119,8 @@ struct SplitParams {
   int rows16;      // cache rows start on 16-byte boundaries and hold whole 16-byte chunks
   // Fused append (partition MFMA kernel, q_len 1): non-null k_new / v_new, contiguous
   // [batch, KVH, D] rows of the query type, 16-byte aligned: row (b, kvh) goes to cache
-  // position lens[b] - 1 (cast to the cache type) before the decode reads it.
+  // position lens[b] - 1 (cast to the cache type) before the decode reads it; with rope_cos set
+  // the key is rotated at the query's position first (and cast once, from fp32).
   const void* k_new;
   const void* v_new;
 };
@@ -148,7 +150,7 @@ __device__ __forceinline__ uint4 load_kv_chunk(const KT* src, int valid, bool ve
 
 // Position of row b's query for RoPE, clamped into the tables.
 __device__ __forceinline__ int rope_position(const SplitParams& p, int b) {
-  int pos = p.rope_pos[b];
+  int pos = p.rope_pos[b] + p.rope_pos_add;
   pos = pos < 0 ? 0 : (pos >= p.rope_max_pos ? p.rope_max_pos - 1 : pos);
   return pos;
 }

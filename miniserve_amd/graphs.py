@@ -35,6 +35,7 @@ import torch
 
 from . import _native as nat
 from .attention import PagedAttention, paged_attention, paged_attention_append
+from .rotary import rope_table, write_kv_rope
 
 
 def fill_table(tab: np.ndarray, tables, batch: int) -> None:
@@ -79,10 +80,13 @@ class GraphedDecodeRunner:
 
     def __init__(self, layers: Sequence[DecodeLayer], table_width: int,
                  buckets: Sequence[int] = (1, 2, 4, 8, 16, 32, 64),
-                 dtype: torch.dtype | None = None, fused_append: bool = True) -> None:
+                 dtype: torch.dtype | None = None, fused_append: bool = True,
+                 rope: tuple[torch.Tensor, torch.Tensor] | None = None) -> None:
         """fused_append: each layer's write_kv and decode through one
         msattn_paged_attention_append call (one launch where the partition kernel takes
-        it, the same caches and output bit for bit); False keeps the two calls."""
+        it, the same caches and output bit for bit); False keeps the two calls.
+        rope: (cos, sin) tables [max_pos, rotary_dim]; decode() then takes unrotated q and k,
+        which are rotated at each row's new position on the way, in the same launches."""
         buckets = list(buckets)
         if not buckets or sorted(buckets) != buckets or buckets[0] < 1:
             raise ValueError("buckets must be sorted, start at 1")
@@ -110,6 +114,9 @@ class GraphedDecodeRunner:
         L, Bm, H, KVH, D = (len(self.layers), self.max_batch, self.num_heads,
                             self.num_kv_heads, self.head_dim)
         dev = self._device
+        # (the captured graphs hold the tables' addresses: the runner keeps them)
+        self.rope = None if rope is None else (rope_table(rope[0], dev, "cos"),
+                                               rope_table(rope[1], dev, "sin"))
 
         Wt = self.table_width
 
@@ -156,11 +163,17 @@ class GraphedDecodeRunner:
                                        buf["v"][li, :bucket], layer.k_cache, layer.v_cache,
                                        table, lens, window=layer.pa.window,
                                        max_context=self.max_context, workspace=self._ws,
-                                       out=self._out[li, :bucket])
+                                       out=self._out[li, :bucket], rope=self.rope)
                 continue
-            layer.pa.write_kv(layer.k_cache, layer.v_cache, buf["k"][li, :bucket],
-                              buf["v"][li, :bucket], table, start=start)
-            paged_attention(buf["q"][li, :bucket], layer.k_cache, layer.v_cache, table, lens,
+            q = buf["q"][li, :bucket]
+            if self.rope is not None:
+                # (a pad row's start, 0, is on a hole: nothing of it is written)
+                q = write_kv_rope(q, buf["k"][li, :bucket], buf["v"][li, :bucket], layer.k_cache,
+                                  layer.v_cache, table, start, *self.rope)
+            else:
+                layer.pa.write_kv(layer.k_cache, layer.v_cache, buf["k"][li, :bucket],
+                                  buf["v"][li, :bucket], table, start=start)
+            paged_attention(q, layer.k_cache, layer.v_cache, table, lens,
                             window=layer.pa.window, max_context=self.max_context,
                             workspace=self._ws, out=self._out[li, :bucket])
 

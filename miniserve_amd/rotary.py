@@ -1,0 +1,187 @@
+"""miniserve_amd.rotary -- rotated queries and keys on their way into the paged cache.
+
+``write_kv_rope`` is ``write_kv`` (miniserve/attention.py:111-133) with rotate-half RoPE
+(miniserve/attention.py:41-62) of the keys on the way and of the step's queries beside them, in
+one launch of libmsattn.so (msattn_write_kv_rope). The single-token form that goes on to attend is
+``paged_attention_append(..., rope=)``.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Sequence
+
+import torch
+
+from . import _native as nat
+
+_I64x3 = ctypes.c_int64 * 3
+
+
+def on_device(dev: torch.device, fn, *args) -> int:
+    """fn(*args, stream) with `dev` current and torch's current stream on it."""
+    if torch.cuda.current_device() == dev.index or dev.index is None:
+        return fn(*args, nat.stream_handle(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, nat.stream_handle(dev))
+
+
+def rope_table(t, dev: torch.device, what: str) -> torch.Tensor:
+    """A rotation table as the kernels read it: fp32 [max_pos, dims], contiguous, on `dev`."""
+    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.float32:
+        t = torch.as_tensor(t, device=dev).to(torch.float32)
+    if t.ndim != 2 or t.shape[0] < 1:
+        raise ValueError(f"{what} must be [max_pos, dims] with at least one position")
+    return t.contiguous()
+
+
+def extent(t: torch.Tensor) -> tuple[int, int]:
+    """First byte that `t` addresses and the one past its last."""
+    lo = t.data_ptr()
+    if t.numel() == 0:
+        return lo, lo
+    return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [batch, tokens, heads, dims] views of one buffer interleave token by token
+    without sharing an element, as the slices of a fused projection do."""
+    if a.dtype != b.dtype or a.stride()[:2] != b.stride()[:2] or a.shape[:2] != b.shape[:2]:
+        return False
+    token, batch, es = a.stride(1), a.stride(0), a.element_size()
+    gap = b.data_ptr() - a.data_ptr()
+    if gap < 0:
+        return _rows_apart(b, a)
+    row = [(t.shape[2] - 1) * t.stride(2) + t.shape[3] for t in (a, b)]
+    return gap % es == 0 and row[0] <= gap // es and gap // es + row[1] <= token and \
+        (a.shape[0] == 1 or batch >= a.shape[1] * token)
+
+
+def _apart(t: torch.Tensor, written: Sequence[torch.Tensor]) -> bool:
+    lo, hi = extent(t)
+    for w in written:
+        wlo, whi = extent(w)
+        if lo < whi and wlo < hi and not (t.ndim == w.ndim == 4 and _rows_apart(t, w)):
+            return False
+    return True
+
+
+def _source(t: torch.Tensor, written: Sequence[torch.Tensor]) -> torch.Tensor:
+    """`t` as the kernel may read it through its strides: rows of contiguous dims that share no
+    memory with what the call writes (a copy otherwise)."""
+    if t.is_neg():
+        t = t.resolve_neg()
+    if t.stride(3) != 1 and t.shape[3] != 1 or not _apart(t, written):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def write_kv_rope(query: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                  k_cache: torch.Tensor, v_cache: torch.Tensor, block_table, start,
+                  cos: torch.Tensor, sin: torch.Tensor, position=None, *,
+                  out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Rotate a step's queries and keys, and scatter the keys and values into the cache.
+
+    ``query`` [batch, tokens, heads, head_dim] (or None), ``k``/``v`` [batch, tokens, kv_heads,
+    head_dim] of one fp32, fp16 or bf16 type, in any strides: the views of a fused projection are
+    read where they lie. Row b's token t goes to cache position start[b] + t (``start``: an int,
+    one entry per row, or an int tensor); tokens on holes of the block table or outside it are
+    not written. It is rotated at that position, or at ``position``: an int, [batch] positions of
+    the rows' first tokens, or [batch, tokens]. ``cos``/``sin`` [max_pos, rotary_dim] are read as
+    fp32, positions clamped to [0, max_pos); the first rotary_dim dims (even) are rotated
+    (x * cos + rotate_half(x) * sin), the others kept.
+
+    Everything is computed in fp32 and rounded once: queries to their type, keys and values to
+    the cache's. Returns the rotated queries, contiguous, or ``out``, which may be ``query``
+    itself (rotated in place). Two tokens of one call that land in one cache slot leave either's
+    row there.
+    """
+    from .attention import _require_gpu, block_table_i32, starts_i32
+
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k", k), ("v", v)):
+        _require_gpu(t, name)
+    if k.ndim != 4 or k.shape != v.shape:
+        raise ValueError("k and v must both be [batch, tokens, kv_heads, head_dim]")
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or \
+            k_cache.stride() != v_cache.stride():
+        raise ValueError("k_cache and v_cache must share a [num_blocks, block_size, kv_heads, "
+                         "head_dim] shape, dtype and strides")
+    B, T, KVH, D = k.shape
+    nb, bs = k_cache.shape[:2]
+    if k_cache.shape[2] != KVH or k_cache.shape[3] != D:
+        raise ValueError("k/v heads or head_dim do not match the cache")
+    if k_cache.stride(3) != 1:
+        raise ValueError("cache head_dim must be contiguous")
+    if D > nat.MAX_HEAD_DIM:
+        raise ValueError(f"head_dim {D}: the kernels take head sizes up to {nat.MAX_HEAD_DIM}")
+    dev = k_cache.device
+    if query is None:
+        if out is not None:
+            raise ValueError("out holds rotated queries: it needs a query")
+    else:
+        _require_gpu(query, "query")
+        if query.ndim != 4 or query.shape[:2] != k.shape[:2] or query.shape[3] != D or \
+                query.shape[2] == 0:
+            raise ValueError("query must be [batch, tokens, heads, head_dim] beside k and v")
+    for name, t in (("v", v), ("query", query)):
+        if t is not None and t.dtype != k.dtype:
+            raise ValueError(f"{name} must have k's dtype")
+    if k.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"unsupported dtype for a rotation: {k.dtype}")
+    if any(t is not None and t.device != dev for t in (v_cache, k, v, query, out)):
+        raise ValueError("query, k, v, out and the caches must be on one device")
+    cos, sin = rope_table(cos, dev, "cos"), rope_table(sin, dev, "sin")
+    R = cos.shape[1]
+    if cos.shape != sin.shape or R % 2 or not 0 < R <= D:
+        raise ValueError(f"cos/sin must share one [max_pos, rotary_dim] shape, rotary_dim even and "
+                         f"at most {D}")
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or
+                            out.stride(3) != 1 or
+                            any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride()))):
+        raise ValueError("out must have the query's shape and dtype, rows of contiguous dims and "
+                         "no element twice")
+    if B == 0 or T == 0 or KVH == 0 or nb == 0:
+        return None if query is None else _rest(query, out)
+    table = block_table_i32(block_table, dev)
+    if table.shape[0] < B:
+        raise ValueError("block_table has fewer rows than k")
+    if table.shape[1] == 0:
+        raise ValueError("block_table has no columns")
+    starts = starts_i32(start, B, dev)
+    pos, per_token = None, 0
+    if position is not None:
+        pos = torch.as_tensor(position, device=dev).to(torch.int32)
+        if pos.ndim == 0:
+            pos = pos.expand(B)
+        if tuple(pos.shape) not in ((B,), (B, T)):
+            raise ValueError(f"position must be an int, [{B}] or [{B}, {T}]")
+        per_token = 1 if pos.ndim == 2 else 0
+        pos = pos.contiguous()
+    q_args = (None, None, None, None, 0)
+    written = [k_cache, v_cache]
+    if query is not None:
+        if out is None:
+            out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+        in_place = out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
+        q = query if in_place and not query.is_neg() else _source(query, [k_cache, v_cache, out])
+        if not _apart(out, [k_cache, v_cache]):
+            raise ValueError("out shares memory with a cache")
+        written.append(out)
+        q_args = (q.data_ptr(), _I64x3(*q.stride()[:3]), out.data_ptr(),
+                  _I64x3(*out.stride()[:3]), query.shape[2])
+    ks, vs = _source(k, written), _source(v, written)
+    status = on_device(
+        dev, nat.lib().msattn_write_kv_rope, *q_args[:4], ks.data_ptr(), _I64x3(*ks.stride()[:3]),
+        vs.data_ptr(), _I64x3(*vs.stride()[:3]), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), table.data_ptr(),
+        starts.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        pos.data_ptr() if pos is not None else None, per_token, cos.shape[0], R, B, T, q_args[4],
+        KVH, D, bs, nb, table.shape[1], nat.dtype_code(k.dtype), nat.dtype_code(k_cache.dtype))
+    nat.check("msattn_write_kv_rope", status)
+    return out
+
+
+def _rest(query: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    """The answer of a call without a token (or without a KV head to write): nothing to rotate."""
+    if query.numel():
+        raise ValueError("a query needs keys and values beside it")
+    return torch.empty(query.shape, dtype=query.dtype, device=query.device) if out is None else out
