@@ -404,6 +404,41 @@ int msattn_paged_attention_append_rope(
     const int32_t* position, int max_position, void* stream);
 
 /*
+ * Workspace bytes of msattn_paged_attention_shared (at least msattn_workspace_bytes of the same
+ * geometry); 0 for an invalid geometry. No reference counterpart.
+ */
+size_t msattn_shared_workspace_bytes(int batch, int q_len, int num_heads, int num_kv_heads,
+                                     int head_dim, int max_context, int groups);
+
+/*
+ * Causal attention (no window) for a batch whose rows come in groups, each group behind a prefix
+ * of its own: rows group_rows[g] .. group_rows[g + 1] - 1 hold the same physical pages in their
+ * first prefix_pages[g] table entries, as RadixPrefixCache.match hands them out
+ * (miniserve/prefix_cache.py:66-96). group_rows int32 [groups + 1] ascends within [0, batch],
+ * prefix_pages int32 [groups]; both on the device, read there (capture-safe; values outside
+ * [0, batch] and [0, table_width] are taken as the nearest bound). Rows outside every group share
+ * nothing. Same result as msattn_paged_attention(causal = 1, window = 0) within float rounding,
+ * any q_len: each prefix is read once per KV head and 128 query rows for the whole group, through
+ * the table of the group's first row; the caller is trusted that the other rows' entries are the
+ * same. A row whose context ends inside the prefix sees its own length of it.
+ * Other types and layouts than a bf16 or fp16 query (16-byte aligned) over a cache of its type or
+ * of fp8 e4m3, head_dim 64 or 128, block_size a multiple of 16, 16-byte aligned cache rows, up to
+ * 1024 rows and groups and 128 query rows a KV head and batch row, and calls without a group, run
+ * msattn_paged_attention. msattn_paged_attention_prefix is the form for one prefix under the
+ * whole batch and one query token. The reference reads the shared pages once a row
+ * (miniserve/attention.py:155-171).
+ */
+int msattn_paged_attention_shared(const void* query, const void* k_cache, const void* v_cache,
+                                  int64_t cache_block_stride, int64_t cache_slot_stride,
+                                  int64_t cache_head_stride, const int32_t* block_table,
+                                  const int32_t* context_lens, const int32_t* group_rows,
+                                  const int32_t* prefix_pages, int groups, void* out,
+                                  void* workspace, size_t workspace_bytes, int batch, int q_len,
+                                  int num_heads, int num_kv_heads, int head_dim, int block_size,
+                                  int num_blocks, int table_width, int max_context, float scale,
+                                  int q_dtype, int kv_dtype, void* stream);
+
+/*
  * Block-table gather: out[b, p] = cache[table[b, p / block_size], p % block_size]
  * for p < context_lens[b]; positions p >= context_lens[b] read page 0 (as the
  * reference does), holes give zero rows. out is [batch, max_context,

@@ -7,6 +7,7 @@ include/msattn.h).
 from .attention import (PagedAttention, apply_rope, gather_kv, kernel_route, paged_attention,
                         paged_attention_append)
 from .rotary import write_kv_rope
+from .shared import paged_attention_shared
 
 __all__ = ["PagedAttention", "apply_rope", "gather_kv", "kernel_route", "paged_attention",
-           "paged_attention_append", "write_kv_rope"]
+           "paged_attention_append", "paged_attention_shared", "write_kv_rope"]

@@ -357,6 +357,7 @@ class PagedAttention:
         position: torch.Tensor | None = None,
         scale: float | None = None,
         shared_prefix_pages: int | None = None,
+        prefix_groups: tuple | None = None,
     ) -> torch.Tensor:
         """Paged attention; ``window`` overrides the constructor value.
 
@@ -366,6 +367,9 @@ class PagedAttention:
         (cos/sin/position, kernels/paged_attn_triton.py:135-139).
         ``shared_prefix_pages``: the leading block-table entries every row shares (a
         radix-cache hit, prefix_cache.py:66-96); a decode reads them once per KV head.
+        ``prefix_groups`` = (group_rows, prefix_pages): groups of rows, each behind shared pages
+        of its own (paged_attention_shared), read once a group where the call is causal and
+        without a window or RoPE.
         """
         if backend not in _BACKENDS:
             raise ValueError(f"unknown attention backend: {backend!r}")
@@ -386,6 +390,10 @@ class PagedAttention:
                                    causal=True, window=None, scale=scale, rope=rope,
                                    prefix_pages=shared_prefix_pages if rope is None else None)
         window = self.window if window is None else window
+        if prefix_groups is not None and causal and window is None:
+            from .shared import paged_attention_shared
+            return paged_attention_shared(query, k_cache, v_cache, block_table, context_lens,
+                                          *prefix_groups, scale=scale)
         cascade = shared_prefix_pages if (query.shape[1] == 1 and causal and window is None) \
             else None
         return paged_attention(query, k_cache, v_cache, block_table, context_lens,

@@ -48,6 +48,8 @@ FILE_FLAGS = {
     "prefill_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "prefill_mfma_fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "prefill_mfma_f32kv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "shared_prefix.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "shared_prefix_fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 # The any-layout prefill kernels do the same.
 FILE_FLAGS.update({f"prefill_any_{q}_{kv}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]

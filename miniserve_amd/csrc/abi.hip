@@ -11,6 +11,7 @@
 #include "decode_streamk.h"
 #include "prefill_any.h"
 #include "prefill_mfma.h"
+#include "shared_prefix.h"
 #include "kernels.h"
 #include "msattn.h"
 
@@ -1701,6 +1702,147 @@ int msattn_paged_attention_append_rope(
   if (kind == 2) return MSATTN_OK;  // merged in-kernel
   return merge_impl(workspace, workspace_bytes, context_lens, out, batch, 1, num_heads,
                     num_kv_heads, head_dim, max_context, q_dtype, nullptr, nullptr, 0, kind, stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+// ---- attention behind several shared prefixes (shared_prefix.h) ----
+
+// Workgroups of a launch: one a CU, or as many as there can be tiles, in whole rounds of the XCDs.
+constexpr int kShMaxShares = 256;
+int64_t shared_most_tiles(int batch, int q_len, int num_heads, int num_kv_heads, int max_context,
+                          int groups) {
+  const int64_t rps = static_cast<int64_t>(q_len) * (num_heads / num_kv_heads);
+  const int64_t own = static_cast<int64_t>(batch) * ((rps + kShRows - 1) / kShRows);
+  const int64_t prefix = groups + (batch * rps) / kShRows;
+  return (own + prefix) * num_kv_heads * std::max(1, ceil_div(max_context, kShTile));
+}
+int shared_shares(int64_t most_tiles, int64_t cus) {
+  int64_t n = std::min<int64_t>(std::min<int64_t>(cus, kShMaxShares), most_tiles);
+  n = n >= kXcds ? (n + kXcds - 1) / kXcds * kXcds : n;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(n, kShMaxShares)));
+}
+
+struct SharedLayout {
+  size_t plan_off, ml_off, acc_off, total;
+};
+// After the header that other calls on the workspace keep their counters in.
+SharedLayout shared_layout(int batch, int q_len, int num_heads, int head_dim, int groups) {
+  SharedLayout X;
+  const int64_t slots = sh_slots(static_cast<int64_t>(batch) * q_len * num_heads, kShMaxShares);
+  X.plan_off = round256(sizeof(int) * kHdrPrefix);
+  X.ml_off = X.plan_off + round256(sizeof(int) * sh_plan_words(batch, groups));
+  X.acc_off = X.ml_off + round256(static_cast<size_t>(slots) * 2 * sizeof(float));
+  X.total = X.acc_off + static_cast<size_t>(slots) * head_dim * sizeof(float);
+  return X;
+}
+
+// Whether the kernel takes a geometry (types and alignment aside): its plan holds kShMaxBatch rows,
+// and rows of more than kShMaxQueryRows query rows a KV head read their keys once for so many
+// queries that the prefill kernels' products, not the reads, set the time.
+#ifndef MSATTN_SHARED_MAX_QUERY_ROWS
+#define MSATTN_SHARED_MAX_QUERY_ROWS 128
+#endif
+constexpr int64_t kShMaxQueryRows = MSATTN_SHARED_MAX_QUERY_ROWS;
+bool shared_geometry_ok(int batch, int q_len, int num_heads, int num_kv_heads, int head_dim,
+                        int max_context, int groups) {
+  return groups > 0 && groups <= kShMaxBatch && batch <= kShMaxBatch &&
+         (head_dim == 64 || head_dim == 128) &&
+         static_cast<int64_t>(q_len) * (num_heads / num_kv_heads) <= kShMaxQueryRows &&
+         shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups) <
+             (int64_t(1) << 30);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t msattn_shared_workspace_bytes(int batch, int q_len, int num_heads, int num_kv_heads,
+                                     int head_dim, int max_context, int groups) {
+  if (groups < 0 || !geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context))
+    return 0;
+  size_t most = workspace_layout(batch, q_len, num_heads, num_kv_heads, head_dim, max_context).total();
+  if (shared_geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, groups))
+    most = std::max(most, shared_layout(batch, q_len, num_heads, head_dim, groups).total);
+  return most;
+}
+
+int msattn_paged_attention_shared(const void* query, const void* k_cache, const void* v_cache,
+                                  int64_t cache_block_stride, int64_t cache_slot_stride,
+                                  int64_t cache_head_stride, const int32_t* block_table,
+                                  const int32_t* context_lens, const int32_t* group_rows,
+                                  const int32_t* prefix_pages, int groups, void* out,
+                                  void* workspace, size_t workspace_bytes, int batch, int q_len,
+                                  int num_heads, int num_kv_heads, int head_dim, int block_size,
+                                  int num_blocks, int table_width, int max_context, float scale,
+                                  int q_dtype, int kv_dtype, void* stream) {
+  if (!query || !block_table || !context_lens || !out || !workspace || groups < 0 ||
+      (groups > 0 && (!group_rows || !prefix_pages)))
+    return MSATTN_ERR_INVALID_ARG;
+  if (!geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context))
+    return MSATTN_ERR_INVALID_ARG;
+  if (!dtype_ok(q_dtype) || q_dtype == MSATTN_FP8_E4M3 || !dtype_ok(kv_dtype) ||
+      !std::isfinite(scale))
+    return MSATTN_ERR_INVALID_ARG;
+  const int rc = check_cache_args(k_cache, v_cache, cache_block_stride, cache_slot_stride,
+                                  cache_head_stride, kv_dtype, block_size, num_blocks, table_width);
+  if (rc != MSATTN_OK) return rc;
+  if (!aligned(query, dtype_bytes(q_dtype)) || !aligned(out, dtype_bytes(q_dtype)) ||
+      !aligned(workspace, 16) || !aligned(group_rows, 4) || !aligned(prefix_pages, 4))
+    return MSATTN_ERR_INVALID_ARG;
+  if (workspace_bytes < msattn_shared_workspace_bytes(batch, q_len, num_heads, num_kv_heads,
+                                                      head_dim, max_context, groups))
+    return MSATTN_ERR_WORKSPACE;
+  const bool rows16 = cache_rows16(k_cache, v_cache, cache_block_stride, cache_slot_stride,
+                                   cache_head_stride, head_dim, kv_dtype);
+  if (!shared_geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, groups) ||
+      kv_dtype == MSATTN_F32 ||
+      !mfma_route_ok(query, q_dtype, kv_dtype, head_dim, block_size, cache_slot_stride, rows16))
+    return msattn_paged_attention(query, k_cache, v_cache, cache_block_stride, cache_slot_stride,
+                                  cache_head_stride, block_table, context_lens, out, workspace,
+                                  workspace_bytes, batch, q_len, num_heads, num_kv_heads, head_dim,
+                                  block_size, num_blocks, table_width, max_context, 1, 0, scale,
+                                  q_dtype, kv_dtype, stream);
+  const SharedLayout X = shared_layout(batch, q_len, num_heads, head_dim, groups);
+  char* ws = static_cast<char*>(workspace);
+  SharedParams p{};
+  p.q = query;
+  p.k = k_cache;
+  p.v = v_cache;
+  p.table = block_table;
+  p.lens = context_lens;
+  p.group_rows = group_rows;
+  p.prefix_pages = prefix_pages;
+  p.out = out;
+  p.blk_stride = cache_block_stride;
+  p.slot_stride = cache_slot_stride;
+  p.head_stride = cache_head_stride;
+  p.batch = batch;
+  p.groups = groups;
+  p.q_len = q_len;
+  p.H = num_heads;
+  p.KVH = num_kv_heads;
+  p.G = num_heads / num_kv_heads;
+  p.bs = block_size;
+  p.bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
+  p.num_blocks = num_blocks;
+  p.W = table_width;
+  p.max_ctx = max_context;
+  p.scale_log2 = scale * kLog2e;
+  p.plan = reinterpret_cast<int*>(ws + X.plan_off);
+  p.ml = reinterpret_cast<float*>(ws + X.ml_off);
+  p.acc = reinterpret_cast<float*>(ws + X.acc_off);
+  p.rows = static_cast<int64_t>(batch) * q_len * num_heads;
+  p.shares = shared_shares(
+      shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups), device_cus());
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (q_dtype == MSATTN_BF16)
+    return hip_status(kv_dtype == MSATTN_FP8_E4M3 ? launch_shared<bf16_t, fp8_t>(p, head_dim, st)
+                                                  : launch_shared<bf16_t, bf16_t>(p, head_dim, st));
+  return hip_status(kv_dtype == MSATTN_FP8_E4M3 ? launch_shared<_Float16, fp8_t>(p, head_dim, st)
+                                                : launch_shared<_Float16, _Float16>(p, head_dim, st));
 }
 
 }  // extern "C"
