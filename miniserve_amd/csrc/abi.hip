@@ -1713,11 +1713,11 @@ namespace {
 // Workgroups of a launch: one a CU, or as many as there can be tiles, in whole rounds of the XCDs.
 constexpr int kShMaxShares = 256;
 int64_t shared_most_tiles(int batch, int q_len, int num_heads, int num_kv_heads, int max_context,
-                          int groups) {
+                          int groups, int tile) {
   const int64_t rps = static_cast<int64_t>(q_len) * (num_heads / num_kv_heads);
   const int64_t own = static_cast<int64_t>(batch) * ((rps + kShRows - 1) / kShRows);
   const int64_t prefix = groups + (batch * rps) / kShRows;
-  return (own + prefix) * num_kv_heads * std::max(1, ceil_div(max_context, kShTile));
+  return (own + prefix) * num_kv_heads * std::max(1, ceil_div(max_context, tile));
 }
 int shared_shares(int64_t most_tiles, int64_t cus) {
   int64_t n = std::min<int64_t>(std::min<int64_t>(cus, kShMaxShares), most_tiles);
@@ -1751,8 +1751,11 @@ bool shared_geometry_ok(int batch, int q_len, int num_heads, int num_kv_heads, i
   return groups > 0 && groups <= kShMaxBatch && batch <= kShMaxBatch &&
          (head_dim == 64 || head_dim == 128) &&
          static_cast<int64_t>(q_len) * (num_heads / num_kv_heads) <= kShMaxQueryRows &&
-         shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups) <
-             (int64_t(1) << 30);
+         num_kv_heads < 65536 &&
+         // (the kernel's query offsets are 32-bit)
+         static_cast<int64_t>(batch) * q_len * num_heads * head_dim * 2 < (int64_t(1) << 31) &&
+         shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups,
+                           sh_tile(head_dim, 2)) < (int64_t(1) << 30);
 }
 
 }  // namespace
@@ -1826,7 +1829,6 @@ int msattn_paged_attention_shared(const void* query, const void* k_cache, const 
   p.KVH = num_kv_heads;
   p.G = num_heads / num_kv_heads;
   p.bs = block_size;
-  p.bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(block_size)) : -1;
   p.num_blocks = num_blocks;
   p.W = table_width;
   p.max_ctx = max_context;
@@ -1835,8 +1837,12 @@ int msattn_paged_attention_shared(const void* query, const void* k_cache, const 
   p.ml = reinterpret_cast<float*>(ws + X.ml_off);
   p.acc = reinterpret_cast<float*>(ws + X.acc_off);
   p.rows = static_cast<int64_t>(batch) * q_len * num_heads;
+  p.by_bs = fast_div(static_cast<uint32_t>(block_size));
+  p.by_rps = fast_div(static_cast<uint32_t>(q_len * p.G));
+  p.by_g = fast_div(static_cast<uint32_t>(p.G));
   p.shares = shared_shares(
-      shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups), device_cus());
+      shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups,
+                        sh_tile(head_dim, dtype_bytes(kv_dtype))), device_cus());
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (q_dtype == MSATTN_BF16)
     return hip_status(kv_dtype == MSATTN_FP8_E4M3 ? launch_shared<bf16_t, fp8_t>(p, head_dim, st)

@@ -5,22 +5,27 @@
 // The work is a list of segments: one a group (the prefix's keys, read once for the query rows of
 // every member) and one a batch row (the keys past its prefix, or all of them). A segment falls
 // into units, one a KV head and block of up to 128 query rows; a unit's keys are cut into tiles
-// of 128. All tiles of all units, in order, are dealt in equal contiguous shares, one a
-// workgroup, whatever the lengths (they are read on the device, so a call is capture-safe). A
-// share's part of one unit is a piece; it leaves, for each of its query rows,
+// of 32 KB of K and 32 KB of V. All tiles of all units, in order, are dealt in equal contiguous
+// shares, one a workgroup, whatever the lengths (they are read on the device, so a call is
+// capture-safe). A share's part of one unit is a piece; it leaves, for each of its query rows,
 //   m = max_j s_j,  l = sum_j 2^(s_j - m),  acc = sum_j 2^(s_j - m) V_j,   s_j = scale log2(e) q.K_j
 // over the piece's visible keys, and the merge kernel below joins a row's pieces:
 //   out = sum 2^(m - M) acc / sum 2^(m - M) l,   M = max m.
 //
-// A tile's 16 KB to 32 KB each of K and V are copied into LDS by the load unit, two tiles in
-// flight while one is computed, across piece and unit boundaries, so the memory pipe does not run
-// dry between units. Scores are S^T = K Q^T on v_mfma_f32_16x16x32, 16 query rows a wave: lane
-// (g, n) = (l / 16, l % 16) then holds row n's scores of keys 4 g .. 4 g + 3 of a 16-key block,
-// and two such blocks, rounded to the query type and packed, are its B operand of
-// O^T += V^T P^T (V^T by transposed LDS reads), so softmax and rescaling stay in the lane.
-// A unit of more than 64 query rows gives each of the 8 waves 16 rows and all keys; fewer rows
-// leave waves over, which take every second or fourth 32-key block of the same rows and are
-// joined through LDS at the piece's end.
+// A workgroup has four copying and four computing waves, one of each a SIMD. The copying waves
+// bring the share's tiles into two LDS slots with the load unit, one tile ahead of the computation
+// and on across pieces and units, so that the memory pipe does not run dry between them, and keep
+// the page walk out of the computing waves. Those take 32 query rows each, as two sets of 16:
+// scores are S^T = K Q^T on v_mfma_f32_16x16x32, so that lane (g, n) = (l / 16, l % 16) holds row
+// n's scores of keys 4 g .. 4 g + 3 of a 16-key block, and two such blocks, rounded to the query
+// type and packed, are its B operand of O^T += V^T P^T (V^T by transposed LDS reads): softmax and
+// rescaling stay in the lane, and K and V are read from LDS once for 32 rows. A unit of 64 rows or
+// fewer leaves computing waves over, which take every second or fourth 32-key block of the same
+// rows and are joined through LDS at the piece's end.
+//
+// The kernel runs each part of its code a few times a workgroup, so its size counts: every part
+// stands once, divisions by the call's constants are multiplications, and the plan's searches are
+// made for 64 tiles at a time, a lane each.
 //
 // Semantics: miniserve/attention.py:205-250 (causal), whose gather reads a shared page once a row.
 #pragma once
@@ -29,12 +34,38 @@
 
 namespace msattn {
 
-constexpr int kShWaves = 8;
-constexpr int kShThreads = kShWaves * kWave;
-constexpr int kShTile = 16 * kShWaves;  // keys of a tile: 16 a copying wave
-constexpr int kShRows = 16 * kShWaves;  // query rows of a unit, at most
+constexpr int kShThreads = 512;
+constexpr int kShSide = 4;              // computing waves, and copying waves: one each a SIMD
+constexpr int kShRows = 32 * kShSide;   // query rows of a unit, at most: 32 a computing wave
 constexpr int kShMaxBatch = 1024;       // rows (and groups) of a launch: its plan sits in LDS
-constexpr int kShIds = kWave;           // page ids a wave holds: its sub-tile's in 64 tiles
+constexpr int kShHalf = 32 * 1024;      // bytes of K, and of V, of a tile
+constexpr int kShSlots = 2;             // tiles in LDS
+// Keys of a tile.
+__host__ __device__ constexpr int sh_tile(int head_dim, int kv_bytes) {
+  return kShHalf / (head_dim * kv_bytes);
+}
+// Cache policy of the K/V reads (2: nontemporal).
+#ifndef MSATTN_SHARED_AUX
+#define MSATTN_SHARED_AUX 0
+#endif
+constexpr int kShAux = MSATTN_SHARED_AUX;
+
+// Division of x < 2^31 by a constant of the call: with s = ceil(log2 d) and m = ceil(2^(31+s) / d),
+// x m 2^-(31+s) exceeds x / d by less than 1 / d, so its integer part is the quotient.
+struct FastDiv {
+  uint32_t m;
+  int s;
+};
+inline FastDiv fast_div(uint32_t d) {
+  FastDiv f;
+  f.s = 0;
+  while ((uint32_t(1) << f.s) < d) ++f.s;
+  f.m = static_cast<uint32_t>(((uint64_t(1) << (31 + f.s)) + d - 1) / d);
+  return f;
+}
+__device__ __forceinline__ int fast_quot(int x, FastDiv f) {
+  return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(x), f.m) >> f.s);
+}
 
 struct SharedParams {
   const void* q;
@@ -47,7 +78,8 @@ struct SharedParams {
   void* out;
   int64_t blk_stride, slot_stride, head_stride;
   int batch, groups, q_len, H, KVH, G;
-  int bs, bs_shift, num_blocks, W, max_ctx;
+  int bs, num_blocks, W, max_ctx;
+  FastDiv by_bs, by_rps, by_g;  // page size, query rows a KV head and batch row, query heads a KV head
   float scale_log2;
   // Workspace: the plan (written by workgroup 0 for the merge) and the pieces' partials. A
   // unit's first piece goes to slot kind * rows + output row (kind 0: the group's segment, 1: the
@@ -67,34 +99,58 @@ __host__ __device__ constexpr int64_t sh_slots(int64_t rows, int shares) {
   return 2 * rows + static_cast<int64_t>(shares) * kShRows;
 }
 
-// s_waitcnt immediates (gfx9 encoding): at most N vector memory operations outstanding.
-constexpr int sh_wait_vm(int n) { return 0x0F70 | (n & 15); }
+// As lds_copy16, with the cache policy above.
+__device__ __forceinline__ void sh_copy16(__amdgpu_buffer_rsrc_t r, char* dst, uint32_t voff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 16, voff, 0, 0, kShAux);
+#endif
+}
+// A barrier of the workgroup that waits for LDS accesses only: the copies into LDS that are in
+// flight stay so (__syncthreads would wait for them). What a wave copied is awaited by its own
+// vmcnt before the barrier that publishes it.
+__device__ __forceinline__ void sh_barrier() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#endif
+}
+// s_waitcnt immediate (gfx9 encoding): at most N vector memory operations outstanding.
+constexpr int sh_wait_vm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
+
+// 16-byte chunk c of a row of ROW bytes sits at chunk c ^ sh_swz(row): the 16 rows of a K operand
+// read, and the rows of a transposed V read, then fall on distinct banks (pf_swz's patterns for
+// rows of 256 and 128 bytes; rows of 64 bytes, four to a turn of the banks).
+template <int ROW>
+__device__ __forceinline__ int sh_swz(int r) {
+  if constexpr (ROW >= 128) return pf_swz<ROW / 2>(r);
+  return (r >> 2) & 3;
+}
 
 template <typename T, typename KT, int D>
-__global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(
-    const SharedParams p) {
+__global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const SharedParams p) {
   typedef Kv8<T, KT> KV;
   static_assert(D == 64 || D == 128, "head_dim 64 and 128");
   constexpr int EB = static_cast<int>(sizeof(KT));
-  constexpr bool WIDEN = !std::is_same<T, KT>::value;  // fp8 rows pass through registers
-  constexpr int JD = D / 32;  // MFMA k-steps of a score block
-  constexpr int ND = D / 16;  // 16-dim tiles of O^T
-  constexpr int CPR = D * EB / 16;   // 16-byte chunks a cache row
-  constexpr int RPI = kWave / CPR;   // rows a copy instruction
-  constexpr int NI = 16 / RPI;       // copy instructions a 16-row sub-tile
+  constexpr bool FP8 = EB == 1;  // its rows are widened as the matrix operands are read
+  constexpr int ROW = D * EB;             // bytes of a cache row
+  constexpr int TK = sh_tile(D, EB);      // keys of a tile
+  constexpr int SUB = TK / 16 / kShSide;  // 16-key sub-tiles a copying wave brings
+  constexpr int CPR = ROW / 16;           // 16-byte chunks a row
+  constexpr int RPI = kWave / CPR;        // rows a copy instruction (1 KiB)
+  constexpr int NI = 16 / RPI;            // copy instructions a sub-tile, of K and of V each
+  constexpr int JD = D / 32;              // MFMA k-steps of a score block
+  constexpr int ND = D / 16;              // 16-dim tiles of O^T
+  static_assert(2 * SUB * NI == 16, "copy instructions a wave and tile");
 
-  __shared__ __attribute__((aligned(256))) uint16_t s_k0[kShTile * D];
-  __shared__ __attribute__((aligned(256))) uint16_t s_v0[kShTile * D];
-  __shared__ __attribute__((aligned(256))) uint16_t s_k1[kShTile * D];
-  __shared__ __attribute__((aligned(256))) uint16_t s_v1[kShTile * D];
+  __shared__ __attribute__((aligned(256))) char s_tile[kShSlots * 2 * kShHalf];
   __shared__ int s_cum[2 * kShMaxBatch + 1];  // tiles before each segment: groups, then rows
   __shared__ int s_g0[kShMaxBatch + 1];       // a group's first row
   __shared__ int s_hi[kShMaxBatch];           // a group's last visible prefix key + 1
   __shared__ int s_len[kShMaxBatch];
   __shared__ int s_own[kShMaxBatch];          // where a row's own keys begin
-  __shared__ float2 s_ml[kShWaves][16];
-  __shared__ int s_live[2][kShWaves];         // sub-tiles of the two tiles that are no holes
-  __shared__ int s_wsum[kShWaves];
+  __shared__ float s_m[kShRows], s_l[kShRows];  // a piece's end: (m, l) of the computing waves' rows
+  __shared__ int s_orow[kShRows];
+  __shared__ __attribute__((aligned(8))) unsigned char s_live[kShSlots][kShSide];  // sub-tiles in the slots that are no holes
+  __shared__ int s_wsum[kShThreads / kWave];
 
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
@@ -103,72 +159,79 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(
   const int n = lane & 15;
   const int B = p.batch, NG = p.groups, NS = NG + B;
   const int RPS = p.q_len * p.G;  // query rows a KV head and batch row
+  const auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
 
   // ---- the plan: tiles before each segment ----
+#pragma unroll 1
   for (int i = tid; i <= NG; i += kShThreads) {
-    const int r = NG > 0 ? p.group_rows[i] : 0;
+    const int r = p.group_rows[i];
+    const int pages = p.prefix_pages[i < NG ? i : 0];
     s_g0[i] = r < 0 ? 0 : (r > B ? B : r);
-    if (i < NG) s_hi[i] = 0;
+    if (i < NG) {
+      const int64_t pt = static_cast<int64_t>(pages < 0 ? 0 : (pages > p.W ? p.W : pages)) * p.bs;
+      s_cum[i] = static_cast<int>(pt < p.max_ctx ? pt : p.max_ctx);  // (for now: prefix tokens)
+      s_hi[i] = 0;
+    }
   }
+#pragma unroll 1
   for (int b = tid; b < B; b += kShThreads) {
     const int len = p.lens[b];
     s_len[b] = len < 0 ? 0 : (len > p.max_ctx ? p.max_ctx : len);
   }
   __syncthreads();
-  const int own_rtiles = ceil_div(RPS, kShRows);
+  const int own_units = ceil_div(RPS, kShRows) * p.KVH;
+#pragma unroll 1
   for (int b = tid; b < B; b += kShThreads) {
     int lo = 0, hi = NG;  // the last group that begins at or before row b
+#pragma unroll 1
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (s_g0[mid] <= b) lo = mid; else hi = mid;
     }
     int own = 0, grp = -1;
     // (a group of one row has nothing to share: its prefix is the row's own)
-    if (NG > 0 && s_g0[lo] <= b && b < s_g0[lo + 1] && s_g0[lo + 1] - s_g0[lo] > 1) {
-      int pages = p.prefix_pages[lo];
-      pages = pages < 0 ? 0 : (pages > p.W ? p.W : pages);
-      const int64_t pt = static_cast<int64_t>(pages) * p.bs;
-      own = static_cast<int>(pt < p.max_ctx ? pt : p.max_ctx);
+    const int g0 = s_g0[lo], g1 = s_g0[lo + 1];
+    if (g0 <= b && b < g1 && g1 - g0 > 1) {
+      own = s_cum[lo];
       grp = lo;
       atomicMax(&s_hi[lo], min(own, s_len[b]));
     }
     s_own[b] = own;
-    s_cum[NG + b] = s_len[b] > own ? ceil_div(s_len[b] - own, kShTile) * p.KVH * own_rtiles : 0;
+    s_cum[NG + b] = s_len[b] > own ? ceil_div(s_len[b] - own, TK) * own_units : 0;
     if (blockIdx.x == 0) p.plan[kShPlanCum + NS + 1 + b] = grp;
   }
   __syncthreads();
+#pragma unroll 1
   for (int i = tid; i < NG; i += kShThreads)
-    s_cum[i] = ceil_div(s_hi[i], kShTile) * p.KVH *
+    s_cum[i] = ceil_div(s_hi[i], TK) * p.KVH *
                ceil_div(max(0, s_g0[i + 1] - s_g0[i]) * RPS, kShRows);
-  __syncthreads();
-  {
-    constexpr int kPer = 2 * kShMaxBatch / kShThreads;
-    int c[kPer], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = tid * kPer + i;
-      c[i] = e < NS ? s_cum[e] : 0;
-      sum += c[i];
-    }
-    const int incl = wave_inclusive_sum(sum);
+  int total = 0;  // the exclusive sum, 512 segments at a time
+#pragma unroll 1
+  for (int e0 = 0; e0 < NS; e0 += kShThreads) {
+    __syncthreads();
+    const int e = e0 + tid;
+    const int c = e < NS ? s_cum[e] : 0;
+    const int incl = wave_inclusive_sum(c);
     if (lane == kWave - 1) s_wsum[w] = incl;
     __syncthreads();
-    int at = incl - sum;
-    for (int i = 0; i < w; ++i) at += s_wsum[i];
+    int at = total + incl - c;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = tid * kPer + i;
-      if (e < NS) s_cum[e] = at;
-      at += c[i];
-      if (e == NS - 1) s_cum[NS] = at;
+    for (int i = 0; i < kShThreads / kWave; ++i) {
+      const int x = s_wsum[i];
+      at += i < w ? x : 0;
+      total += x;
     }
-    __syncthreads();
+    if (e < NS) s_cum[e] = at;
   }
-  const int total = __builtin_amdgcn_readfirstlane(s_cum[NS]);
+  if (tid == 0) s_cum[NS] = total;
+  __syncthreads();
+  total = uni(total);
   const int per = max(1, ceil_div(total, p.shares));
   if (blockIdx.x == 0) {
     if (tid == 0) p.plan[0] = per;
+#pragma unroll 1
     for (int i = tid; i <= NS; i += kShThreads) p.plan[kShPlanCum + i] = s_cum[i];
+#pragma unroll 1
     for (int i = tid; i <= NG; i += kShThreads) p.plan[kShPlanCum + NS + 1 + B + i] = s_g0[i];
   }
   // Contiguous shares to one XCD (workgroup i runs on XCD i % 8): the row blocks of one KV head
@@ -182,356 +245,382 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(
   const int first = static_cast<int>(first64);
   const int last = min(total, first + per);
 
-  // A piece: tiles t0 .. t1 - 1 of one unit.
-  struct Piece {
-    int kind;         // 0: a group's segment, 1: a row's own
-    int b0;           // the batch row whose table names the pages, and the segment's first row
-    int kvh, row0, nrows;  // query rows row0 .. row0 + nrows - 1 of the segment, for one KV head
-    int key0, hi;     // the segment's keys are key0 .. hi - 1
-    int t0, t1;
+  const bool copies = w >= kShSide;  // a copying wave
+  const int cw = w & (kShSide - 1);  // its place among its side's
+
+  // ---- a window of 64 tiles: lane i describes tile base + i ----
+  // Everything the loops need of the plan is found here, each lane one tile, and later taken with
+  // lane reads.
+  //   tok  the key the tile begins at      hi  where the segment's keys end
+  //   unit KV head | row block << 16       id  the pages of a copying wave's sub-tiles
+  //   bits segment's first row | kind << 10 | the unit's first tile << 11 |
+  //        the piece's last tile << 12 | (query rows - 1) << 13 | the piece's first tile << 20
+  struct Tile {
+    int tok, hi, unit, bits;
+    __device__ bool starts() const { return (bits >> 20) & 1; }
+    __device__ bool ends() const { return (bits >> 12) & 1; }
+    __device__ int rows() const { return ((bits >> 13) & 127) + 1; }
+    // Computing waves that take different rows; the others take other keys of the same.
+    __device__ int row_waves() const { return rows() > 64 ? 4 : (rows() > 32 ? 2 : 1); }
+    __device__ int first_row() const { return bits & 1023; }
+    __device__ int kvh() const { return unit & 0xffff; }
+    __device__ Tile at(int lane) const {
+      return Tile{__builtin_amdgcn_readlane(tok, lane), __builtin_amdgcn_readlane(hi, lane),
+                  __builtin_amdgcn_readlane(unit, lane), __builtin_amdgcn_readlane(bits, lane)};
+    }
   };
-  const auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  auto locate = [&](int pos) __attribute__((always_inline)) {
+  auto window = [&](int base) __attribute__((always_inline)) {
+    const int pos = min(base + lane, last - 1);
     int lo = 0, hi = NS;  // the last segment that begins at or before pos
+#pragma unroll 1
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (uni(s_cum[mid]) <= pos) lo = mid; else hi = mid;
+      if (s_cum[mid] <= pos) lo = mid; else hi = mid;
     }
-    Piece c;
-    int members = 1;
-    if (lo < NG) {
-      c.kind = 0;
-      c.b0 = uni(s_g0[lo]);
-      members = uni(s_g0[lo + 1]) - c.b0;
-      c.key0 = 0;
-      c.hi = uni(s_hi[lo]);
-    } else {
-      c.kind = 1;
-      c.b0 = lo - NG;
-      c.key0 = uni(s_own[c.b0]);
-      c.hi = uni(s_len[c.b0]);
-    }
-    const int tiles = ceil_div(c.hi - c.key0, kShTile);
-    const int off = pos - uni(s_cum[lo]);
-    const int unit = off / tiles;
-    const int rtiles = ceil_div(members * RPS, kShRows);
-    c.kvh = unit / rtiles;
-    c.row0 = (unit - c.kvh * rtiles) * kShRows;
-    c.nrows = min(kShRows, members * RPS - c.row0);
-    c.t0 = off - unit * tiles;
-    c.t1 = min(tiles, c.t0 + (last - pos));
+    const bool own = lo >= NG;
+    const int b0 = own ? lo - NG : s_g0[lo];
+    const int members = own ? 1 : s_g0[lo + 1] - b0;
+    const int key0 = own ? s_own[b0] : 0;
+    Tile c;
+    c.hi = own ? s_len[b0] : s_hi[lo];
+    const uint32_t tiles = static_cast<uint32_t>(ceil_div(c.hi - key0, TK));
+    const uint32_t off = static_cast<uint32_t>(pos - s_cum[lo]);
+    const uint32_t unit = off / tiles;
+    const uint32_t t = off - unit * tiles;
+    const uint32_t rtiles = static_cast<uint32_t>(ceil_div(members * RPS, kShRows));
+    const uint32_t kvh = rtiles == 1 ? unit : unit / rtiles;
+    const uint32_t rt = unit - kvh * rtiles;
+    c.tok = key0 + static_cast<int>(t) * TK;
+    c.unit = static_cast<int>(kvh | (rt << 16));
+    c.bits = b0 | (own ? 1 << 10 : 0) | (t == 0 ? 1 << 11 : 0) |
+             (t + 1 == tiles || pos + 1 == last ? 1 << 12 : 0) |
+             ((min(kShRows, members * RPS - static_cast<int>(rt) * kShRows) - 1) << 13) |
+             (t == 0 || pos == first ? 1 << 20 : 0);
     return c;
   };
 
-  // ---- copying: wave w takes keys 16 w .. 16 w + 15 of each tile ----
-  const KT* const kbase = static_cast<const KT*>(p.k);
-  const KT* const vbase = static_cast<const KT*>(p.v);
-  const int64_t row_bytes = p.slot_stride * EB;
-  uint32_t dvo[NI];
+  // Both sides meet, for each tile, at a barrier where it has landed and at one where its slot
+  // has been read; at a piece's end, whose rows leave through the slot, at two more.
+  int slot = 0;  // the tile's slot
+  if (copies) {
+    // ================= the copying waves: SUB sub-tiles of K and of V each =================
+#pragma unroll 1
+    for (int wbase = first; wbase < last; wbase += kWave) {
+      const int count = min(kWave, last - wbase);
+      const Tile wt = window(wbase);
+      int w_id[SUB];
 #pragma unroll
-  for (int j = 0; j < NI; ++j) {
-    const int lr = RPI * j + lane / CPR;
-    dvo[j] = static_cast<uint32_t>(lr * row_bytes +
-                                   16 * (WIDEN ? lane % CPR : (lane % CPR) ^ pf_swz<D>(lr)));
-  }
-  auto page_of = [&](int tok) { return p.bs_shift >= 0 ? tok >> p.bs_shift : tok / p.bs; };
-  // Lane i: the page id of this wave's sub-tile in tile t + i of the piece (-1: none).
-  auto load_ids = [&](const Piece& c, int t) __attribute__((always_inline)) {
-    const int64_t tok = c.key0 + static_cast<int64_t>(t + lane) * kShTile + 16 * w;
-    int id = -1;
-    if (t + lane < c.t1 && tok < c.hi) {
-      const int pg = page_of(static_cast<int>(tok));
-      if (pg < p.W) id = p.table[static_cast<int64_t>(c.b0) * p.W + pg];
-    }
-    return id;
-  };
-
-  // The copying cursor runs two tiles ahead of the computing one.
-  Piece lp = locate(first);
-  int lpos = first, lt = lp.t0, lw = lp.t0;  // tile lt, its piece, the first tile of the ids held
-  int ids = load_ids(lp, lw);
-  constexpr int HOLD = WIDEN ? 2 : 1;  // fp8: two tiles are held in registers
-  uint4 k_held[HOLD][NI], v_held[HOLD][NI];
-  int live_held[HOLD];
-  // Requests tile lpos into slot `buf` (fp8: into register set `buf`, which land() widens into
-  // the slot), and moves the cursor on. The page ids of a new piece or window are requested
-  // first, so that the next tile waits for them alone.
-  auto request = [&](uint16_t* sk, uint16_t* sv, int buf, auto set_c) __attribute__((always_inline)) {
-    constexpr int set = decltype(set_c)::value;
-    const bool live = lpos < last;
-    int phys = -1, tok = 0, kvh = 0, hi = 0;
-    if (live) {
-      phys = __builtin_amdgcn_readlane(ids, lt - lw);
-      tok = lp.key0 + lt * kShTile + 16 * w;
-      kvh = lp.kvh;
-      hi = lp.hi;
-      ++lpos;
-      ++lt;
-      if (lpos < last) {
-        if (lt == lp.t1) {
-          lp = locate(lpos);
-          lt = lw = lp.t0;
-          ids = load_ids(lp, lw);
-        } else if (lt - lw == kShIds) {
-          lw = lt;
-          ids = load_ids(lp, lw);
-        }
+      for (int i = 0; i < SUB; ++i) {
+        const int tok = wt.tok + 16 * (SUB * cw + i);
+        const int pg = fast_quot(tok, p.by_bs);
+        w_id[i] = -1;
+        if (tok < wt.hi && pg < p.W)
+          w_id[i] = p.table[static_cast<int64_t>(wt.first_row()) * p.W + pg];
       }
-    }
-    const bool in = phys >= 0 && phys < p.num_blocks;
-    const int slot = tok - page_of(tok) * p.bs;
-    const int64_t off = in ? static_cast<int64_t>(phys) * p.blk_stride +
-                                 static_cast<int64_t>(slot) * p.slot_stride +
-                                 static_cast<int64_t>(kvh) * p.head_stride
-                           : 0;
-    const int nbytes = in ? static_cast<int>((min(16, hi - tok) - 1) * row_bytes + D * EB) : 0;
-    const __amdgpu_buffer_rsrc_t rk = tile_rsrc(kbase + off, nbytes);
-    const __amdgpu_buffer_rsrc_t rv = tile_rsrc(vbase + off, nbytes);
-    if constexpr (WIDEN) {
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        k_held[set][j] = buffer_load16<2>(rk, dvo[j]);
-        v_held[set][j] = buffer_load16<2>(rv, dvo[j]);
-      }
-      live_held[set] = in ? 1 : 0;
-    } else {
-#pragma unroll
-      for (int j = 0; j < NI; ++j) lds_copy16(rk, sk + (16 * w + RPI * j) * D, dvo[j]);
-#pragma unroll
-      for (int j = 0; j < NI; ++j) lds_copy16(rv, sv + (16 * w + RPI * j) * D, dvo[j]);
-      if (lane == 0) s_live[buf][w] = in ? 1 : 0;
-    }
-  };
-  // fp8: the held set's rows, widened, into the slot.
-  auto land = [&](uint16_t* sk, uint16_t* sv, int buf, auto set_c) __attribute__((always_inline)) {
-    constexpr int set = decltype(set_c)::value;
-    if constexpr (WIDEN) {
+      const int64_t row_bytes = p.slot_stride * EB;
+      uint32_t dvo[NI];
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
         const int lr = RPI * j + lane / CPR;
-        const int c = 2 * (lane % CPR);
-        typedef typename KV::raw_t raw_t;
-        const uint4 a = k_held[set][j], b = v_held[set][j];
-        uint16_t* const rk = sk + (16 * w + lr) * D;
-        uint16_t* const rv = sv + (16 * w + lr) * D;
-        *reinterpret_cast<uint4*>(rk + 8 * (c ^ pf_swz<D>(lr))) = KV::operand(raw_t{a.x, a.y});
-        *reinterpret_cast<uint4*>(rk + 8 * ((c + 1) ^ pf_swz<D>(lr))) = KV::operand(raw_t{a.z, a.w});
-        *reinterpret_cast<uint4*>(rv + 8 * (c ^ pf_swz<D>(lr))) = KV::operand(raw_t{b.x, b.y});
-        *reinterpret_cast<uint4*>(rv + 8 * ((c + 1) ^ pf_swz<D>(lr))) = KV::operand(raw_t{b.z, b.w});
+        dvo[j] = static_cast<uint32_t>(lr * row_bytes + 16 * ((lane % CPR) ^ sh_swz<ROW>(lr)));
       }
-      if (lane == 0) s_live[buf][w] = live_held[set];
-    }
-  };
-
-  // ---- a piece's query rows ----
-  uint4 qb[JD];       // the B operand Q^T: row n, dims 8 (4 j + g) ..
-  int hi_n = 0;       // the lane's row sees keys below hi_n
-  int wave_all = 0;   // every row of the wave sees keys below wave_all,
-  int wave_any = 0;   // none sees one at or past wave_any
-  int64_t orow = -1;  // the row's place in the output, -1: none
-  int RW = 1, rw = 0, ks = 0, KS = 1;  // the wave takes rows 16 rw .., every KS-th 32-key block
-  float m_run, l_run;
-  mf_f32x4 acc[ND];
-  auto begin = [&](const Piece& c) __attribute__((always_inline)) {
-    RW = c.nrows > 64 ? 8 : (c.nrows > 32 ? 4 : (c.nrows > 16 ? 2 : 1));
-    rw = w & (RW - 1);
-    KS = kShWaves / RW;
-    ks = w / RW;
-    const int r = 16 * rw + n;
-    hi_n = 0;
-    orow = -1;
-    if (r < c.nrows) {
-      const int row = c.row0 + r;
-      const int member = row / RPS;
-      const int rest = row - member * RPS;
-      const int i = rest / p.G;
-      const int b = c.b0 + member;
-      orow = (static_cast<int64_t>(b) * p.q_len + i) * p.H + c.kvh * p.G + (rest - i * p.G);
-      hi_n = min(c.hi, s_len[b] - p.q_len + i + 1);
-    }
-    const T* const q = static_cast<const T*>(p.q) + (orow < 0 ? 0 : orow) * D;
-#pragma unroll
-    for (int j = 0; j < JD; ++j) qb[j] = *reinterpret_cast<const uint4*>(q + 8 * (4 * j + g));
-    int lo = orow < 0 ? INT_MAX : hi_n, hi = hi_n;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-      lo = min(lo, __shfl_xor(lo, o, kWave));
-      hi = max(hi, __shfl_xor(hi, o, kWave));
-    }
-    wave_all = uni(lo);
-    wave_any = uni(hi);
-    m_run = -INFINITY;
-    l_run = 0.0f;
-#pragma unroll
-    for (int t = 0; t < ND; ++t) acc[t] = mf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  };
-
-  // ---- one tile: the wave's 32-key blocks ks, ks + KS, .. ----
-  const uint32_t kx = static_cast<uint32_t>(n * 2 * D);
-  const int vtok = 4 * g + (n >> 2);  // the token a lane names in a transposed read, and its dims
-  auto tile = [&](const uint16_t* sk, const uint16_t* sv, int buf, const Piece& c, int t)
-                  __attribute__((always_inline)) {
-    const int key_t = c.key0 + t * kShTile;
-    for (int kb = ks; kb < kShTile / 32; kb += KS) {
-      const int key = key_t + 32 * kb;
-      if (key >= wave_any) break;
-      const int live = uni(s_live[buf][2 * kb]) & 1, live2 = uni(s_live[buf][2 * kb + 1]) & 1;
-      mf_f32x4 s[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        s[h] = mf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const char* const base = reinterpret_cast<const char*>(sk) + (32 * kb + 16 * h) * 2 * D + kx;
-#pragma unroll
-        for (int j = 0; j < JD; ++j)
-          s[h] = Mfma16<T>::mac(
-              *reinterpret_cast<const uint4*>(base + 16 * ((4 * j + g) ^ pf_swz<D>(n))), qb[j], s[h]);
-      }
-      float sc[8];
-      const bool full = key + 32 <= wave_all && live && live2;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          sc[4 * h + r] = s[h][r] * p.scale_log2;
-          if (!full) {
-            const bool ok = (h ? live2 : live) && key + 16 * h + 4 * g + r < hi_n;
-            sc[4 * h + r] = ok ? sc[4 * h + r] : -INFINITY;
+      int to = slot;  // the slot the next tile is brought to
+      __builtin_amdgcn_s_waitcnt(sh_wait_vm(0));  // (the page ids: no later use waits for them)
+#pragma unroll 1
+      for (int i = -kShSlots; i < count; ++i) {
+        if (i >= 0) {
+          // tile i has landed: all but the copies of the tile after it
+          __builtin_amdgcn_s_waitcnt(sh_wait_vm(16 * (kShSlots - 1)));
+          sh_barrier();
+          sh_barrier();  // it has been read
+          if ((__builtin_amdgcn_readlane(wt.bits, i) >> 12) & 1) {
+            sh_barrier();
+            sh_barrier();
           }
+          slot ^= 1;
         }
-      float mt = sc[0];
+        const int r = i + kShSlots;  // the tile requested (past the window: nothing is read)
+        const int rl = min(r, count - 1);
+        const Tile c = wt.at(rl);
+        int live = 0;
+        char* const d = s_tile + to * 2 * kShHalf + SUB * cw * 16 * ROW;
 #pragma unroll
-      for (int e = 1; e < 8; ++e) mt = fmaxf(mt, sc[e]);
-      const float m_new = fmaxf(m_run, rows4_max(mt));
-      const bool some = m_new != -INFINITY;
-      const float alpha = some ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-      const float m_use = some ? m_new : 0.0f;  // (masked scores weigh 2^-inf = 0, NaN stays NaN)
-      float pr[8];
+        for (int h = 0; h < SUB; ++h) {
+          const int id = __builtin_amdgcn_readlane(w_id[h], rl);
+          const bool in = r < count && id >= 0 && id < p.num_blocks;
+          const int tok = c.tok + 16 * (SUB * cw + h);
+          const int64_t o = static_cast<int64_t>(in ? id : 0) * p.blk_stride +
+                            static_cast<int64_t>(tok - fast_quot(tok, p.by_bs) * p.bs) * p.slot_stride +
+                            static_cast<int64_t>(c.kvh()) * p.head_stride;
+          const int64_t off = static_cast<int64_t>(
+              (static_cast<uint64_t>(static_cast<uint32_t>(uni(static_cast<int>(o >> 32)))) << 32) |
+              static_cast<uint32_t>(uni(static_cast<int>(o))));
+          const int nbytes = uni(in ? static_cast<int>((min(16, c.hi - tok) - 1) * row_bytes + ROW) : 0);
+          const __amdgpu_buffer_rsrc_t rk = tile_rsrc(static_cast<const KT*>(p.k) + off, nbytes);
+          const __amdgpu_buffer_rsrc_t rv = tile_rsrc(static_cast<const KT*>(p.v) + off, nbytes);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pr[e] = __builtin_amdgcn_exp2f(sc[e] - m_use);
-      // The weights are rounded to the query type for the matrix cores (half a step of it, at
-      // most 1); l sums the rounded ones, so that the weights used still sum to one.
-      const uint4 pb = make_uint4(Pack2<T>::pack(pr[0], pr[1]), Pack2<T>::pack(pr[2], pr[3]),
-                                  Pack2<T>::pack(pr[4], pr[5]), Pack2<T>::pack(pr[6], pr[7]));
-      const uint32_t one2 = Pack2<T>::pack(1.0f, 1.0f);
-      l_run = fmaf(l_run, alpha,
-                   Dot2<T>::dot(pb.w, one2, Dot2<T>::dot(pb.z, one2, Dot2<T>::dot(pb.y, one2,
-                   Dot2<T>::dot(pb.x, one2, 0.0f)))));
-      m_run = m_new;
-      if (__any(alpha != 1.0f)) {
-#pragma unroll
-        for (int u = 0; u < ND; ++u) acc[u] *= alpha;
+          for (int j = 0; j < NI; ++j) {
+            sh_copy16(rk, d + (16 * h + RPI * j) * ROW, dvo[j]);
+            sh_copy16(rv, d + kShHalf + (16 * h + RPI * j) * ROW, dvo[j]);
+          }
+          if (in) live |= 1 << h;
+        }
+        if (lane == 0) s_live[to][cw] = static_cast<unsigned char>(live);
+        to ^= 1;
       }
-      const char* const vb = reinterpret_cast<const char*>(sv) + (32 * kb + vtok) * 2 * D + 8 * (n & 1);
-#pragma unroll
-      for (int u = 0; u < ND; ++u) {
-        const int ch = 2 * u + ((n & 3) >> 1);  // the 16-byte chunk of dims 16 u + 4 (n & 3)
-        const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s4*)(vb + 16 * (ch ^ pf_swz<D>(vtok)))));
-        const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s4*)(vb + 16 * 2 * D + 16 * (ch ^ pf_swz<D>(vtok)))));
-        acc[u] = Mfma16<T>::mac(make_uint4(a.x, a.y, b.x, b.y), pb, acc[u]);
-      }
+      // (the copies past the window read nothing, and have landed before its slots are used again)
+      __builtin_amdgcn_s_waitcnt(sh_wait_vm(0));
     }
-  };
+    return;
+  }
 
-  // ---- a piece's end: its key-splitting waves are joined through the tile's slot (read for the
-  // last time before the barrier that precedes this), and the partials stored ----
-  constexpr int kSlotF4 = ND * kWave;  // float4 a wave's accumulators take
-  static_assert(4 * kSlotF4 * 16 == sizeof(s_k0), "four waves' accumulators fill a K slot");
-  auto finish = [&](uint16_t* sk, uint16_t* sv, const Piece& c) __attribute__((always_inline)) {
-    l_run = rows4_sum(l_run);
-    auto slot_of = [&](int i) {
-      return (i < 4 ? reinterpret_cast<float4*>(sk) + i * kSlotF4
-                    : reinterpret_cast<float4*>(sv) + (i - 4) * kSlotF4) + lane;
-    };
-    const int KA = min(KS, kShTile / 32);  // waves of a row block that took keys
-    if (KA > 1) {
-      if (ks > 0 && ks < KA) {
-        float4* const d = slot_of((ks - 1) * RW + rw);
+  // ================= the computing waves =================
+  uint4 qb[2][JD];  // B operands Q^T of the two 16-row sets: row n, dims KV::qk_dim0(j, g) ..
+  int orow[2] = {-1, -1}, hi_n[2] = {0, 0};  // their places in the output; they see keys below hi_n
+  int wave_all = 0, wave_any = 0;  // all rows of the wave see keys below wave_all, none past wave_any
+  int RW = 1, rw = 0, ks = 0, KS = 1;  // the wave takes rows 32 rw .., every KS-th 32-key block
+  bool unit_first = false;  // the piece holds its unit's first tile
+  float m_run[2], l_run[2];
+  mf_f32x4 acc[2][ND];
+#pragma unroll 1
+  for (int wbase = first; wbase < last; wbase += kWave) {
+    const int count = min(kWave, last - wbase);
+    const Tile wt = window(wbase);
+    // A negative scale goes into the query's sign, so that the largest score weighs most. (A scale
+    // of zero weighs every visible key alike; a tiny one does the same and keeps the masked scores
+    // infinite.)
+    const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    const uint32_t flip = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+    const int vtok = FP8 ? 16 * (n >> 3) + 4 * g + ((n >> 1) & 3)  // the token a lane names in a
+                         : 4 * g + (n >> 2);                       // transposed V read
+#pragma unroll 1
+    for (int i = -1; i < count; ++i) {  // (i == -1: before the window's first tile)
+      const Tile c = wt.at(i < 0 ? 0 : i);
+      char* const base = s_tile + slot * 2 * kShHalf;
+      const bool ends = i >= 0 && c.ends();
+      if (i >= 0) {
+        sh_barrier();  // the tile has landed
+        const uint32_t live4 = static_cast<uint32_t>(uni(*reinterpret_cast<const int*>(s_live[slot])));
+        // (blocks past every row's last key, and a wave without rows, have nothing to do)
+        const int blocks = min(TK / 32, (wave_any - c.tok + 31) >> 5);
+#pragma unroll 1
+        for (int kb = ks; kb < blocks; kb += KS) {
+          const int key = c.tok + 32 * kb;
+          const int live = (live4 >> (8 * (2 * kb / SUB) + 2 * kb % SUB)) & 3;
+          char* const kv = base + kb * 32 * ROW;
+          mf_f32x4 s[2][2];
 #pragma unroll
-        for (int u = 0; u < ND; ++u)
-          d[u * kWave] = make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
-        if (g == 0) s_ml[w][n] = make_float2(m_run, l_run);
-      }
-      __syncthreads();
-      if (ks == 0) {
-        for (int k = 1; k < KA; ++k) {
-          const float2 ml = s_ml[k * RW + rw][n];
-          const float M = fmaxf(m_run, ml.x);
-          const bool some = M != -INFINITY;
-          const float a0 = some ? __builtin_amdgcn_exp2f(m_run - M) : 1.0f;
-          const float a1 = some ? __builtin_amdgcn_exp2f(ml.x - M) : 0.0f;
-          const float4* const d = slot_of((k - 1) * RW + rw);
+          for (int k = 0; k < 2; ++k) {
+            uint4 kk[JD];
+            const char* const row = kv + (16 * k + n) * ROW;
+            if constexpr (FP8) {
+#pragma unroll
+              for (int j = 0; j < JD / 2; ++j) {
+                const uint4 x = *reinterpret_cast<const uint4*>(row + 16 * ((4 * j + g) ^ sh_swz<ROW>(n)));
+                kk[2 * j] = KV::operand(typename KV::raw_t{x.x, x.y});
+                kk[2 * j + 1] = KV::operand(typename KV::raw_t{x.z, x.w});
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < JD; ++j)
+                kk[j] = *reinterpret_cast<const uint4*>(row + 16 * ((4 * j + g) ^ sh_swz<ROW>(n)));
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[h][k] = mf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+              for (int j = 0; j < JD; ++j) s[h][k] = Mfma16<T>::mac(kk[j], qb[h][j], s[h][k]);
+            }
+          }
+          if (key + 32 > wave_all || live != 3) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const bool ok = ((live >> k) & 1) && key + 16 * k + 4 * g + r < hi_n[h];
+                  s[h][k][r] = ok ? s[h][k][r] : -INFINITY;
+                }
+          }
+          uint4 pb[2];
+          float alpha[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mt = fmaxf(s[h][0][0], s[h][1][0]);
+#pragma unroll
+            for (int r = 1; r < 4; ++r) mt = fmaxf(mt, fmaxf(s[h][0][r], s[h][1][r]));
+            mt = rows4_max(mt);
+            const float m_new = fmaxf(m_run[h], mt * scale);
+            const bool some = m_new != -INFINITY;
+            alpha[h] = some ? __builtin_amdgcn_exp2f(m_run[h] - m_new) : 1.0f;
+            const float m_use = some ? m_new : 0.0f;
+            float pr[8];  // (masked scores weigh 2^-inf = 0, NaN stays NaN)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                pr[4 * k + r] = __builtin_amdgcn_exp2f(fmaf(s[h][k][r], scale, -m_use));
+            // The weights are rounded to the query type for the matrix cores (half a step of it,
+            // at most 1); l sums the rounded ones, so that the weights used still sum to one.
+            pb[h] = make_uint4(Pack2<T>::pack(pr[0], pr[1]), Pack2<T>::pack(pr[2], pr[3]),
+                               Pack2<T>::pack(pr[4], pr[5]), Pack2<T>::pack(pr[6], pr[7]));
+            const uint32_t one2 = Pack2<T>::pack(1.0f, 1.0f);
+            l_run[h] = fmaf(l_run[h], alpha[h],
+                            Dot2<T>::dot(pb[h].w, one2, Dot2<T>::dot(pb[h].z, one2, 0.0f)) +
+                                Dot2<T>::dot(pb[h].y, one2, Dot2<T>::dot(pb[h].x, one2, 0.0f)));
+            m_run[h] = m_new;
+          }
+          if (__any(alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int u = 0; u < ND; ++u) acc[h][u] *= alpha[h];
+          }
+          // V^T: tokens 4 g .. + 3 of the block's first 16 keys and of its second, as pb holds them.
 #pragma unroll
           for (int u = 0; u < ND; ++u) {
-            const float4 o = d[u * kWave];
-            acc[u][0] = fmaf(o.x, a1, acc[u][0] * a0);
-            acc[u][1] = fmaf(o.y, a1, acc[u][1] * a0);
-            acc[u][2] = fmaf(o.z, a1, acc[u][2] * a0);
-            acc[u][3] = fmaf(o.w, a1, acc[u][3] * a0);
+            uint4 vv;
+            if constexpr (FP8) {
+              char* const v = kv + kShHalf + vtok * ROW + 16 * (u ^ sh_swz<ROW>(vtok)) + 8 * (n & 1);
+              typedef int sh_i2 __attribute__((ext_vector_type(2)));
+              typedef __attribute__((address_space(3))) sh_i2 lds_i2;
+              const sh_i2 a = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)v);
+              vv = KV::operand(typename KV::raw_t{static_cast<uint32_t>(a.x), static_cast<uint32_t>(a.y)});
+            } else {
+              char* const v = kv + kShHalf + vtok * ROW +
+                              16 * ((2 * u + ((n & 3) >> 1)) ^ sh_swz<ROW>(vtok)) + 8 * (n & 1);
+              const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)v));
+              const uint2 b = __builtin_bit_cast(
+                  uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(v + 16 * ROW)));
+              vv = make_uint4(a.x, a.y, b.x, b.y);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc[h][u] = Mfma16<T>::mac(vv, pb[h], acc[h][u]);
           }
-          l_run = fmaf(ml.y, a1, l_run * a0);
-          m_run = M;
+        }
+        sh_barrier();  // the slot has been read
+        slot ^= 1;
+      }
+
+      // ---- the next piece's query rows are requested here (its first tile is the next one) ----
+      const bool next = i + 1 < count;
+      const Tile nx = wt.at(next ? i + 1 : 0);
+      const bool starts = next && nx.starts();
+      int n_row[2], n_hi[2];  // the rows requested
+      if (starts) {
+        const int b0 = nx.first_row();
+        const T* const q = static_cast<const T*>(p.q) + static_cast<int64_t>(b0) * p.q_len * p.H * D;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 32 * (cw & (nx.row_waves() - 1)) + 16 * h + n;
+          const int row = (nx.unit >> 16) * kShRows + (r < nx.rows() ? r : 0);
+          const int member = fast_quot(row, p.by_rps);
+          const int rest = row - member * RPS;
+          const int tq = fast_quot(rest, p.by_g);
+          const int o = (member * p.q_len + tq) * p.H + nx.kvh() * p.G + (rest - tq * p.G);
+          n_row[h] = r < nx.rows() ? b0 * p.q_len * p.H + o : -1;
+          n_hi[h] = n_row[h] < 0 ? 0 : min(nx.hi, s_len[b0 + member] - p.q_len + tq + 1);
+#pragma unroll
+          for (int j = 0; j < JD; ++j)
+            qb[h][j] = *reinterpret_cast<const uint4*>(q + static_cast<int64_t>(o) * D +
+                                                       KV::qk_dim0(j, g, JD));
         }
       }
-    }
-    if (ks == 0 && orow >= 0) {
-      const int64_t slot = c.t0 == 0 ? c.kind * p.rows + orow
-                                     : 2 * p.rows + static_cast<int64_t>(share) * kShRows + 16 * rw + n;
-      if (g == 0) *reinterpret_cast<float2*>(p.ml + 2 * slot) = make_float2(m_run, l_run);
-      float* const a = p.acc + slot * D + 4 * g;
+      // ---- a piece's end: the waves' rows go to the slot ----
+      // Row r = 32 rw + 16 h + n of key wave ks at row 32 RW ks + r, its 16-byte chunk j at chunk
+      // j ^ n (the 16 lanes of a set hold 16 rows).
+      const int e_rows = 32 * RW;
+      const int e_ks = KS;
+      const int64_t e_slot0 = unit_first ? ((c.bits >> 10) & 1) * p.rows
+                                         : 2 * p.rows + static_cast<int64_t>(share) * kShRows;
+      const bool e_first = unit_first;
+      float* const f = reinterpret_cast<float*>(base);
+      if (ends) {
 #pragma unroll
-      for (int u = 0; u < ND; ++u)
-        *reinterpret_cast<float4*>(a + 16 * u) = make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
-    }
-    if (KA > 1) __syncthreads();  // the slot is free again
-  };
-
-  using I0 = std::integral_constant<int, 0>;
-  using I1 = std::integral_constant<int, 1>;
-  Piece cp = lp;
-  int cpos = first, ct = cp.t0;
-  request(s_k0, s_v0, 0, I0{});
-  if constexpr (WIDEN) {
-    request(s_k1, s_v1, 1, I1{});
-    land(s_k0, s_v0, 0, I0{});
-    request(s_k0, s_v0, 0, I0{});
-    land(s_k1, s_v1, 1, I1{});
-    request(s_k1, s_v1, 1, I1{});
-  } else {
-    request(s_k1, s_v1, 1, I1{});
-  }
-  begin(cp);
-  // Tile cpos sits in slot `buf`; after it the slot takes tile cpos + 2 (fp8: which set `buf`
-  // holds, while the set takes tile cpos + 4).
-  auto step = [&](uint16_t* sk, uint16_t* sv, int buf, auto set_c) __attribute__((always_inline)) {
-    // tile cpos has landed: everything but the last tile requested
-    if constexpr (!WIDEN) __builtin_amdgcn_s_waitcnt(sh_wait_vm(2 * NI));
-    __syncthreads();
-    tile(sk, sv, buf, cp, ct);
-    __syncthreads();  // the slot has been read
-    ++cpos;
-    ++ct;
-    if (ct == cp.t1) {
-      finish(sk, sv, cp);
-      if (cpos < last) {
-        cp = locate(cpos);
-        ct = cp.t0;
-        begin(cp);
+        for (int h = 0; h < 2; ++h) {
+          const float l = rows4_sum(l_run[h]);
+          const int r = 32 * rw + 16 * h + n;
+          const int at = ks * e_rows + r;
+#pragma unroll
+          for (int u = 0; u < ND; ++u)
+            *reinterpret_cast<float4*>(f + at * D + 4 * ((4 * u + g) ^ n)) =
+                make_float4(acc[h][u][0], acc[h][u][1], acc[h][u][2], acc[h][u][3]);
+          if (g == 0) {
+            s_m[at] = m_run[h];
+            s_l[at] = l;
+            if (ks == 0) s_orow[r] = orow[h];
+          }
+        }
+        sh_barrier();
+      }
+      // (taken over before the partials' stores, which a later wait would wait for too)
+      if (starts) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < JD; ++j) {
+            qb[h][j] = make_uint4(qb[h][j].x ^ flip, qb[h][j].y ^ flip, qb[h][j].z ^ flip, qb[h][j].w ^ flip);
+            keep_here(qb[h][j]);
+          }
+      }
+      // ---- the piece's partials: the waves that split the keys are joined, a thread 4 dims ----
+      if (ends) {
+#pragma unroll 1
+        for (int x = cw * kWave + lane; x < c.rows() * (D / 4); x += kShSide * kWave) {
+          const int r = x / (D / 4), j = x % (D / 4);
+          float M = s_m[r];
+#pragma unroll 1
+          for (int k = 1; k < e_ks; ++k) M = fmaxf(M, s_m[k * e_rows + r]);
+          const float m_use = M != -INFINITY ? M : 0.0f;
+          float L = 0.0f;
+          float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+          for (int k = 0; k < e_ks; ++k) {
+            const int at = k * e_rows + r;
+            const float e = __builtin_amdgcn_exp2f(s_m[at] - m_use);
+            const float4 y = *reinterpret_cast<const float4*>(f + at * D + 4 * (j ^ (r & 15)));
+            L = fmaf(s_l[at], e, L);
+            o.x = fmaf(y.x, e, o.x);
+            o.y = fmaf(y.y, e, o.y);
+            o.z = fmaf(y.z, e, o.z);
+            o.w = fmaf(y.w, e, o.w);
+          }
+          const int64_t at = e_slot0 + (e_first ? s_orow[r] : r);
+          if (j == 0) *reinterpret_cast<float2*>(p.ml + 2 * at) = make_float2(M, L);
+          *reinterpret_cast<float4*>(p.acc + at * D + 4 * j) = o;
+        }
+        sh_barrier();  // the slot is free
+      }
+      // ---- the next piece begins ----
+      if (starts) {
+        unit_first = (nx.bits >> 11) & 1;
+        RW = nx.row_waves();
+        rw = cw & (RW - 1);
+        KS = kShSide / RW;
+        ks = cw / RW;
+        int lo = INT_MAX, hi = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          orow[h] = n_row[h];
+          hi_n[h] = n_hi[h];
+          lo = orow[h] < 0 ? lo : min(lo, hi_n[h]);
+          hi = max(hi, hi_n[h]);
+          m_run[h] = -INFINITY;
+          l_run[h] = 0.0f;
+#pragma unroll
+          for (int u = 0; u < ND; ++u) acc[h][u] = mf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+          lo = min(lo, __shfl_xor(lo, o, kWave));
+          hi = max(hi, __shfl_xor(hi, o, kWave));
+        }
+        wave_all = uni(lo);
+        wave_any = uni(hi);
       }
     }
-    land(sk, sv, buf, set_c);
-    request(sk, sv, buf, set_c);
-  };
-  while (true) {
-    step(s_k0, s_v0, 0, I0{});
-    if (cpos >= last) break;
-    step(s_k1, s_v1, 1, I1{});
-    if (cpos >= last) break;
   }
-  // (copies of tiles past the share read nothing; they land before the workgroup's LDS is given
-  // to another)
-  __builtin_amdgcn_s_waitcnt(sh_wait_vm(0));
 }
 
 // Joins a row's pieces: one wave a query row, D / 64 dims a lane. Its pieces: for the group's
