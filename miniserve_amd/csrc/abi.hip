@@ -1752,10 +1752,10 @@ bool shared_geometry_ok(int batch, int q_len, int num_heads, int num_kv_heads, i
          (head_dim == 64 || head_dim == 128) &&
          static_cast<int64_t>(q_len) * (num_heads / num_kv_heads) <= kShMaxQueryRows &&
          num_kv_heads < 65536 &&
-         // (the kernel's query offsets are 32-bit)
+         // (the kernel's query offsets and costs are 32-bit)
          static_cast<int64_t>(batch) * q_len * num_heads * head_dim * 2 < (int64_t(1) << 31) &&
          shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups,
-                           sh_tile(head_dim, 2)) < (int64_t(1) << 30);
+                           sh_tile(head_dim, 2)) < (int64_t(1) << 23);
 }
 
 }  // namespace

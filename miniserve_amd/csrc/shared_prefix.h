@@ -50,6 +50,21 @@ __host__ __device__ constexpr int sh_tile(int head_dim, int kv_bytes) {
 #endif
 constexpr int kShAux = MSATTN_SHARED_AUX;
 
+// What a share is to cost a workgroup, in units of about 500 clocks: a piece (its query, its plan,
+// its partials), and each 32-key block of a unit of so many rows. Few rows wait for the memory pipe,
+// many for the matrix cores and the softmax.
+#ifndef MSATTN_SHARED_COSTS
+#define MSATTN_SHARED_COSTS 11, 2, 3, 5
+#endif
+__host__ __device__ constexpr int sh_cost(int which) {
+  constexpr int c[] = {MSATTN_SHARED_COSTS};
+  return c[which];
+}
+constexpr int kShPieceCost = sh_cost(0);
+__host__ __device__ constexpr int sh_block_cost(int rows) {
+  return sh_cost(rows > 64 ? 3 : (rows > 32 ? 2 : 1));
+}
+
 // Division of x < 2^31 by a constant of the call: with s = ceil(log2 d) and m = ceil(2^(31+s) / d),
 // x m 2^-(31+s) exceeds x / d by less than 1 / d, so its integer part is the quotient.
 struct FastDiv {
@@ -84,7 +99,7 @@ struct SharedParams {
   // Workspace: the plan (written by workgroup 0 for the merge) and the pieces' partials. A
   // unit's first piece goes to slot kind * rows + output row (kind 0: the group's segment, 1: the
   // row's own), a later one to slot 2 * rows + share * kShRows + row of the unit.
-  int* plan;   // [0] tiles a share, [kShPlanCum ..] tiles before each segment, then group ids
+  int* plan;   // [0] cost of a share, [kShPlanCum ..] cost before each segment, then group ids
   float* ml;   // [slots][2]
   float* acc;  // [slots][D]
   int64_t rows;  // batch * q_len * H
@@ -150,7 +165,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   __shared__ float s_m[kShRows], s_l[kShRows];  // a piece's end: (m, l) of the computing waves' rows
   __shared__ int s_orow[kShRows];
   __shared__ __attribute__((aligned(8))) unsigned char s_live[kShSlots][kShSide];  // sub-tiles in the slots that are no holes
-  __shared__ int s_wsum[kShThreads / kWave];
+  __shared__ int s_wsum[2 * (kShThreads / kWave)];
 
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
@@ -161,7 +176,8 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   const int RPS = p.q_len * p.G;  // query rows a KV head and batch row
   const auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
 
-  // ---- the plan: tiles before each segment ----
+  // ---- the plan: tiles and costs before each segment ----
+  int* const s_cost = reinterpret_cast<int*>(s_tile);  // (until the first tile is brought)
 #pragma unroll 1
   for (int i = tid; i <= NG; i += kShThreads) {
     const int r = p.group_rows[i];
@@ -179,7 +195,11 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
     s_len[b] = len < 0 ? 0 : (len > p.max_ctx ? p.max_ctx : len);
   }
   __syncthreads();
-  const int own_units = ceil_div(RPS, kShRows) * p.KVH;
+  // (groups out of order: every row by itself)
+  bool descend = false;
+#pragma unroll 1
+  for (int i = tid; i < NG; i += kShThreads) descend |= s_g0[i] > s_g0[i + 1];
+  descend = __syncthreads_or(descend);
 #pragma unroll 1
   for (int b = tid; b < B; b += kShThreads) {
     int lo = 0, hi = NG;  // the last group that begins at or before row b
@@ -191,46 +211,71 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
     int own = 0, grp = -1;
     // (a group of one row has nothing to share: its prefix is the row's own)
     const int g0 = s_g0[lo], g1 = s_g0[lo + 1];
-    if (g0 <= b && b < g1 && g1 - g0 > 1) {
+    if (!descend && g0 <= b && b < g1 && g1 - g0 > 1) {
       own = s_cum[lo];
       grp = lo;
       atomicMax(&s_hi[lo], min(own, s_len[b]));
     }
     s_own[b] = own;
-    s_cum[NG + b] = s_len[b] > own ? ceil_div(s_len[b] - own, TK) * own_units : 0;
     if (blockIdx.x == 0) p.plan[kShPlanCum + NS + 1 + b] = grp;
   }
-  __syncthreads();
-#pragma unroll 1
-  for (int i = tid; i < NG; i += kShThreads)
-    s_cum[i] = ceil_div(s_hi[i], TK) * p.KVH *
-               ceil_div(max(0, s_g0[i + 1] - s_g0[i]) * RPS, kShRows);
-  int total = 0;  // the exclusive sum, 512 segments at a time
+  struct Segment {
+    int b0, members, key0, hi;  // its first row and rows, its keys
+  };
+  auto segment = [&](int e) __attribute__((always_inline)) {
+    const bool own = e >= NG;
+    Segment x;
+    x.b0 = own ? e - NG : s_g0[e];
+    x.members = own ? 1 : s_g0[e + 1] - x.b0;
+    x.key0 = own ? s_own[x.b0] : 0;
+    x.hi = own ? s_len[x.b0] : s_hi[e];
+    return x;
+  };
+  int total = 0, total_cost = 0;  // the exclusive sums, 512 segments at a time
 #pragma unroll 1
   for (int e0 = 0; e0 < NS; e0 += kShThreads) {
     __syncthreads();
     const int e = e0 + tid;
-    const int c = e < NS ? s_cum[e] : 0;
-    const int incl = wave_inclusive_sum(c);
-    if (lane == kWave - 1) s_wsum[w] = incl;
+    int c = 0, cost = 0;
+    if (e < NS) {
+      const Segment x = segment(e);
+      const int blocks = (x.hi - x.key0 + 31) >> 5;
+      if (blocks > 0) {
+        const int units = p.KVH * ceil_div(x.members * RPS, kShRows);
+        c = units * ceil_div(blocks, TK / 32);
+        cost = units * (kShPieceCost + blocks * sh_block_cost(x.members * RPS));
+      }
+    }
+    const int incl = wave_inclusive_sum(c), incl_cost = wave_inclusive_sum(cost);
+    if (lane == kWave - 1) {
+      s_wsum[w] = incl;
+      s_wsum[kShThreads / kWave + w] = incl_cost;
+    }
     __syncthreads();
-    int at = total + incl - c;
+    int at = total + incl - c, at_cost = total_cost + incl_cost - cost;
 #pragma unroll
     for (int i = 0; i < kShThreads / kWave; ++i) {
-      const int x = s_wsum[i];
+      const int x = s_wsum[i], y = s_wsum[kShThreads / kWave + i];
       at += i < w ? x : 0;
+      at_cost += i < w ? y : 0;
       total += x;
+      total_cost += y;
     }
-    if (e < NS) s_cum[e] = at;
+    if (e < NS) {
+      s_cum[e] = at;
+      s_cost[e] = at_cost;
+    }
   }
-  if (tid == 0) s_cum[NS] = total;
+  if (tid == 0) {
+    s_cum[NS] = total;
+    s_cost[NS] = total_cost;
+  }
   __syncthreads();
-  total = uni(total);
-  const int per = max(1, ceil_div(total, p.shares));
+  const int per = max(1, ceil_div(uni(total_cost), p.shares));
   if (blockIdx.x == 0) {
     if (tid == 0) p.plan[0] = per;
 #pragma unroll 1
-    for (int i = tid; i <= NS; i += kShThreads) p.plan[kShPlanCum + i] = s_cum[i];
+    for (int i = tid; i <= NS; i += kShThreads) p.plan[kShPlanCum + i] = s_cost[i];
 #pragma unroll 1
     for (int i = tid; i <= NG; i += kShThreads) p.plan[kShPlanCum + NS + 1 + B + i] = s_g0[i];
   }
@@ -240,10 +285,33 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
                         ? static_cast<int>(blockIdx.x % kXcds) * (p.shares / kXcds) +
                               static_cast<int>(blockIdx.x / kXcds)
                         : static_cast<int>(blockIdx.x);
-  const int64_t first64 = static_cast<int64_t>(share) * per;
-  if (first64 >= total) return;
-  const int first = static_cast<int>(first64);
-  const int last = min(total, first + per);
+  // The share's tiles are those that begin at costs [share per, (share + 1) per): lane 0 finds the
+  // first, lane 1 the next share's.
+  int bound = total;
+  const int64_t edge = static_cast<int64_t>(share + (lane & 1)) * per;
+  if (edge < total_cost) {
+    const int x = static_cast<int>(edge);
+    int lo = 0, hi = NS;  // the last segment that begins at or before x
+#pragma unroll 1
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_cost[mid] <= x) lo = mid; else hi = mid;
+    }
+    const Segment e = segment(lo);
+    const uint32_t blocks = static_cast<uint32_t>((e.hi - e.key0 + 31) >> 5);
+    const uint32_t step = static_cast<uint32_t>(sh_block_cost(e.members * RPS));
+    const uint32_t unit_cost = kShPieceCost + blocks * step;
+    const uint32_t off = static_cast<uint32_t>(x - s_cost[lo]);
+    const uint32_t unit = off / unit_cost;
+    const int r = static_cast<int>(off - unit * unit_cost);
+    const int tiles = ceil_div(static_cast<int>(blocks), TK / 32);
+    const int t = r == 0 ? 0 : max(1, ceil_div(r - kShPieceCost, static_cast<int>(step) * (TK / 32)));
+    bound = s_cum[lo] + static_cast<int>(unit) * tiles + min(t, tiles);
+  }
+  const int first = __builtin_amdgcn_readlane(bound, 0);
+  const int last = __builtin_amdgcn_readlane(bound, 1);
+  __syncthreads();
+  if (first >= last) return;
 
   const bool copies = w >= kShSide;  // a copying wave
   const int cw = w & (kShSide - 1);  // its place among its side's
@@ -278,23 +346,21 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
       if (s_cum[mid] <= pos) lo = mid; else hi = mid;
     }
     const bool own = lo >= NG;
-    const int b0 = own ? lo - NG : s_g0[lo];
-    const int members = own ? 1 : s_g0[lo + 1] - b0;
-    const int key0 = own ? s_own[b0] : 0;
+    const Segment e = segment(lo);
     Tile c;
-    c.hi = own ? s_len[b0] : s_hi[lo];
-    const uint32_t tiles = static_cast<uint32_t>(ceil_div(c.hi - key0, TK));
+    c.hi = e.hi;
+    const uint32_t tiles = static_cast<uint32_t>(ceil_div(e.hi - e.key0, TK));
     const uint32_t off = static_cast<uint32_t>(pos - s_cum[lo]);
     const uint32_t unit = off / tiles;
     const uint32_t t = off - unit * tiles;
-    const uint32_t rtiles = static_cast<uint32_t>(ceil_div(members * RPS, kShRows));
+    const uint32_t rtiles = static_cast<uint32_t>(ceil_div(e.members * RPS, kShRows));
     const uint32_t kvh = rtiles == 1 ? unit : unit / rtiles;
     const uint32_t rt = unit - kvh * rtiles;
-    c.tok = key0 + static_cast<int>(t) * TK;
+    c.tok = e.key0 + static_cast<int>(t) * TK;
     c.unit = static_cast<int>(kvh | (rt << 16));
-    c.bits = b0 | (own ? 1 << 10 : 0) | (t == 0 ? 1 << 11 : 0) |
+    c.bits = e.b0 | (own ? 1 << 10 : 0) | (t == 0 ? 1 << 11 : 0) |
              (t + 1 == tiles || pos + 1 == last ? 1 << 12 : 0) |
-             ((min(kShRows, members * RPS - static_cast<int>(rt) * kShRows) - 1) << 13) |
+             ((min(kShRows, e.members * RPS - static_cast<int>(rt) * kShRows) - 1) << 13) |
              (t == 0 || pos == first ? 1 << 20 : 0);
     return c;
   };
@@ -432,6 +498,27 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
               for (int j = 0; j < JD; ++j) s[h][k] = Mfma16<T>::mac(kk[j], qb[h][j], s[h][k]);
             }
           }
+          // V^T, on its way during the softmax: tokens 4 g .. + 3 of the block's first 16 keys and of
+          // its second, as pb holds them.
+          typename KV::raw_t vv[ND];
+#pragma unroll
+          for (int u = 0; u < ND; ++u) {
+            if constexpr (FP8) {
+              char* const v = kv + kShHalf + vtok * ROW + 16 * (u ^ sh_swz<ROW>(vtok)) + 8 * (n & 1);
+              typedef int sh_i2 __attribute__((ext_vector_type(2)));
+              typedef __attribute__((address_space(3))) sh_i2 lds_i2;
+              const sh_i2 a = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)v);
+              vv[u] = typename KV::raw_t{static_cast<uint32_t>(a.x), static_cast<uint32_t>(a.y)};
+            } else {
+              char* const v = kv + kShHalf + vtok * ROW +
+                              16 * ((2 * u + ((n & 3) >> 1)) ^ sh_swz<ROW>(vtok)) + 8 * (n & 1);
+              const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)v));
+              const uint2 b = __builtin_bit_cast(
+                  uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(v + 16 * ROW)));
+              vv[u] = typename KV::raw_t{a.x, a.y, b.x, b.y};
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
           if (key + 32 > wave_all || live != 3) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -477,26 +564,11 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
 #pragma unroll
               for (int u = 0; u < ND; ++u) acc[h][u] *= alpha[h];
           }
-          // V^T: tokens 4 g .. + 3 of the block's first 16 keys and of its second, as pb holds them.
 #pragma unroll
           for (int u = 0; u < ND; ++u) {
-            uint4 vv;
-            if constexpr (FP8) {
-              char* const v = kv + kShHalf + vtok * ROW + 16 * (u ^ sh_swz<ROW>(vtok)) + 8 * (n & 1);
-              typedef int sh_i2 __attribute__((ext_vector_type(2)));
-              typedef __attribute__((address_space(3))) sh_i2 lds_i2;
-              const sh_i2 a = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)v);
-              vv = KV::operand(typename KV::raw_t{static_cast<uint32_t>(a.x), static_cast<uint32_t>(a.y)});
-            } else {
-              char* const v = kv + kShHalf + vtok * ROW +
-                              16 * ((2 * u + ((n & 3) >> 1)) ^ sh_swz<ROW>(vtok)) + 8 * (n & 1);
-              const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)v));
-              const uint2 b = __builtin_bit_cast(
-                  uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(v + 16 * ROW)));
-              vv = make_uint4(a.x, a.y, b.x, b.y);
-            }
+            const uint4 x = KV::operand(vv[u]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) acc[h][u] = Mfma16<T>::mac(vv, pb[h], acc[h][u]);
+            for (int h = 0; h < 2; ++h) acc[h][u] = Mfma16<T>::mac(x, pb[h], acc[h][u]);
           }
         }
         sh_barrier();  // the slot has been read
@@ -544,8 +616,9 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
           const int at = ks * e_rows + r;
 #pragma unroll
           for (int u = 0; u < ND; ++u)
-            *reinterpret_cast<float4*>(f + at * D + 4 * ((4 * u + g) ^ n)) =
-                make_float4(acc[h][u][0], acc[h][u][1], acc[h][u][2], acc[h][u][3]);
+            if (r < c.rows())
+              *reinterpret_cast<float4*>(f + at * D + 4 * ((4 * u + g) ^ n)) =
+                  make_float4(acc[h][u][0], acc[h][u][1], acc[h][u][2], acc[h][u][3]);
           if (g == 0) {
             s_m[at] = m_run[h];
             s_l[at] = l;
@@ -554,7 +627,8 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
         }
         sh_barrier();
       }
-      // (taken over before the partials' stores, which a later wait would wait for too)
+      // (the query has arrived before the partials' stores, which a later wait would wait for too)
+      __builtin_amdgcn_s_waitcnt(sh_wait_vm(0));
       if (starts) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -628,7 +702,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
 // that the unit runs on into.
 constexpr int kShMergeThreads = 256;
 constexpr int kShMergeWaves = kShMergeThreads / kWave;
-template <typename T, int D>
+template <typename T, int D, int TB>  // TB: 32-key blocks of a tile
 __global__ __launch_bounds__(kShMergeThreads) void shared_merge_kernel(const SharedParams p) {
   constexpr int DPL = D / 64;
   const int lane = threadIdx.x & (kWave - 1);
@@ -674,12 +748,20 @@ __global__ __launch_bounds__(kShMergeThreads) void shared_merge_kernel(const Sha
       members = g0[grp + 1] - g0[grp];
     }
     const int rtiles = ceil_div(members * RPS, kShRows);
-    const int tiles = (c1 - c0) / (rtiles * p.KVH);
-    const int t0 = c0 + (kvh * rtiles + r / kShRows) * tiles;
-    const int s0 = t0 / per, s1 = (t0 + tiles - 1) / per;
+    const int unit = (c1 - c0) / (rtiles * p.KVH);  // a unit's cost
+    const int step = sh_block_cost(members * RPS);
+    const int tile = step * TB;  // a tile's cost
+    const int last = ((unit - kShPieceCost) / step - 1) / TB;  // its last tile
+    const int t0 = c0 + (kvh * rtiles + r / kShRows) * unit;
     take(kind * p.rows + row);
-    for (int s = s0 + 1; s <= s1 && s < p.shares; ++s)
+    for (int s = t0 / per;;) {
+      // the first tile past share s, and its share
+      const int past = (s + 1) * per - t0 - kShPieceCost;
+      const int t = past <= tile ? 1 : ceil_div(past, tile);
+      if (t > last) break;
+      s = (t0 + kShPieceCost + t * tile) / per;
       take(2 * p.rows + static_cast<int64_t>(s) * kShRows + r % kShRows);
+    }
   }
   const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
   T* const out = static_cast<T*>(p.out) + row * D + DPL * lane;
@@ -706,7 +788,7 @@ hipError_t launch_shared_one(const SharedParams& p, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t blocks = (p.rows + kShMergeWaves - 1) / kShMergeWaves;
-  hipLaunchKernelGGL((shared_merge_kernel<T, D>), dim3(static_cast<unsigned>(blocks)),
+  hipLaunchKernelGGL((shared_merge_kernel<T, D, sh_tile(D, sizeof(KT)) / 32>), dim3(static_cast<unsigned>(blocks)),
                      dim3(kShMergeThreads), 0, stream, p);
   return hipGetLastError();
 }
