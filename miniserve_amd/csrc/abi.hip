@@ -1729,11 +1729,11 @@ struct SharedLayout {
   size_t plan_off, ml_off, acc_off, total;
 };
 // After the header that other calls on the workspace keep their counters in.
-SharedLayout shared_layout(int batch, int q_len, int num_heads, int head_dim, int groups) {
+SharedLayout shared_layout(int batch, int q_len, int num_heads, int head_dim) {
   SharedLayout X;
   const int64_t slots = sh_slots(static_cast<int64_t>(batch) * q_len * num_heads, kShMaxShares);
   X.plan_off = round256(sizeof(int) * kHdrPrefix);
-  X.ml_off = X.plan_off + round256(sizeof(int) * sh_plan_words(batch, groups));
+  X.ml_off = X.plan_off + round256(sizeof(int) * sh_plan_words(batch));
   X.acc_off = X.ml_off + round256(static_cast<size_t>(slots) * 2 * sizeof(float));
   X.total = X.acc_off + static_cast<size_t>(slots) * head_dim * sizeof(float);
   return X;
@@ -1768,7 +1768,7 @@ size_t msattn_shared_workspace_bytes(int batch, int q_len, int num_heads, int nu
     return 0;
   size_t most = workspace_layout(batch, q_len, num_heads, num_kv_heads, head_dim, max_context).total();
   if (shared_geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, groups))
-    most = std::max(most, shared_layout(batch, q_len, num_heads, head_dim, groups).total);
+    most = std::max(most, shared_layout(batch, q_len, num_heads, head_dim).total);
   return most;
 }
 
@@ -1808,7 +1808,7 @@ int msattn_paged_attention_shared(const void* query, const void* k_cache, const 
                                   workspace_bytes, batch, q_len, num_heads, num_kv_heads, head_dim,
                                   block_size, num_blocks, table_width, max_context, 1, 0, scale,
                                   q_dtype, kv_dtype, stream);
-  const SharedLayout X = shared_layout(batch, q_len, num_heads, head_dim, groups);
+  const SharedLayout X = shared_layout(batch, q_len, num_heads, head_dim);
   char* ws = static_cast<char*>(workspace);
   SharedParams p{};
   p.q = query;
@@ -1840,6 +1840,8 @@ int msattn_paged_attention_shared(const void* query, const void* k_cache, const 
   p.by_bs = fast_div(static_cast<uint32_t>(block_size));
   p.by_rps = fast_div(static_cast<uint32_t>(q_len * p.G));
   p.by_g = fast_div(static_cast<uint32_t>(p.G));
+  p.by_h = fast_div(static_cast<uint32_t>(num_heads));
+  p.by_q = fast_div(static_cast<uint32_t>(q_len));
   p.shares = shared_shares(
       shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups,
                         sh_tile(head_dim, dtype_bytes(kv_dtype))), device_cus());

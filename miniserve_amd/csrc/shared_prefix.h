@@ -34,9 +34,10 @@
 
 namespace msattn {
 
-constexpr int kShThreads = 512;
-constexpr int kShSide = 4;              // computing waves, and copying waves: one each a SIMD
-constexpr int kShRows = 32 * kShSide;   // query rows of a unit, at most: 32 a computing wave
+constexpr int kShCopy = 4;              // copying waves: one a SIMD
+constexpr int kShComp = 8;              // computing waves: two a SIMD
+constexpr int kShThreads = 64 * (kShComp + kShCopy);
+constexpr int kShRows = 16 * kShComp;   // query rows of a unit, at most: 16 a computing wave
 constexpr int kShMaxBatch = 1024;       // rows (and groups) of a launch: its plan sits in LDS
 constexpr int kShHalf = 32 * 1024;      // bytes of K, and of V, of a tile
 constexpr int kShSlots = 2;             // tiles in LDS
@@ -94,22 +95,27 @@ struct SharedParams {
   int64_t blk_stride, slot_stride, head_stride;
   int batch, groups, q_len, H, KVH, G;
   int bs, num_blocks, W, max_ctx;
-  FastDiv by_bs, by_rps, by_g;  // page size, query rows a KV head and batch row, query heads a KV head
+  // page size, query rows a KV head and batch row, query heads a KV head, query heads, query tokens
+  FastDiv by_bs, by_rps, by_g, by_h, by_q;
   float scale_log2;
-  // Workspace: the plan (written by workgroup 0 for the merge) and the pieces' partials. A
+  // Workspace: the plan (for the merge) and the pieces' partials. A
   // unit's first piece goes to slot kind * rows + output row (kind 0: the group's segment, 1: the
   // row's own), a later one to slot 2 * rows + share * kShRows + row of the unit.
-  int* plan;   // [0] cost of a share, [kShPlanCum ..] cost before each segment, then group ids
+  int* plan;   // [sh_plan_words]
   float* ml;   // [slots][2]
   float* acc;  // [slots][D]
   int64_t rows;  // batch * q_len * H
   int shares;
 };
 
-constexpr int kShPlanCum = 16;
-__host__ __device__ constexpr int sh_plan_words(int batch, int groups) {
-  return kShPlanCum + (groups + batch + 1) + batch + (groups + 1);
-}
+// The plan's words: the cost of a share, then for each batch row, for the merge, what its own
+// segment and its group's begin at and their 32-key blocks (none: 0), the group's first row and rows.
+constexpr int kShPlanRows = 16, kShPlanRow = 8;
+struct ShPlanRow {
+  int own_cost, own_blocks, cost, blocks, first, members, pad[2];
+};
+static_assert(sizeof(ShPlanRow) == kShPlanRow * sizeof(int), "the plan's row");
+__host__ __device__ constexpr int sh_plan_words(int batch) { return kShPlanRows + kShPlanRow * batch; }
 __host__ __device__ constexpr int64_t sh_slots(int64_t rows, int shares) {
   return 2 * rows + static_cast<int64_t>(shares) * kShRows;
 }
@@ -131,6 +137,13 @@ __device__ __forceinline__ void sh_barrier() {
 // s_waitcnt immediate (gfx9 encoding): at most N vector memory operations outstanding.
 constexpr int sh_wait_vm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
 
+// The least lo and the largest hi of each 16 lanes, one step: with those N lanes around.
+template <int N>
+__device__ __forceinline__ void sh_fold16(int& lo, int& hi) {
+  lo = min(lo, __builtin_amdgcn_update_dpp(lo, lo, 0x120 + N, 0xF, 0xF, false));  // row_ror
+  hi = max(hi, __builtin_amdgcn_update_dpp(hi, hi, 0x120 + N, 0xF, 0xF, false));
+}
+
 // 16-byte chunk c of a row of ROW bytes sits at chunk c ^ sh_swz(row): the 16 rows of a K operand
 // read, and the rows of a transposed V read, then fall on distinct banks (pf_swz's patterns for
 // rows of 256 and 128 bytes; rows of 64 bytes, four to a turn of the banks).
@@ -141,14 +154,14 @@ __device__ __forceinline__ int sh_swz(int r) {
 }
 
 template <typename T, typename KT, int D>
-__global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const SharedParams p) {
+__global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const SharedParams p) {
   typedef Kv8<T, KT> KV;
   static_assert(D == 64 || D == 128, "head_dim 64 and 128");
   constexpr int EB = static_cast<int>(sizeof(KT));
   constexpr bool FP8 = EB == 1;  // its rows are widened as the matrix operands are read
   constexpr int ROW = D * EB;             // bytes of a cache row
   constexpr int TK = sh_tile(D, EB);      // keys of a tile
-  constexpr int SUB = TK / 16 / kShSide;  // 16-key sub-tiles a copying wave brings
+  constexpr int SUB = TK / 16 / kShCopy;  // 16-key sub-tiles a copying wave brings
   constexpr int CPR = ROW / 16;           // 16-byte chunks a row
   constexpr int RPI = kWave / CPR;        // rows a copy instruction (1 KiB)
   constexpr int NI = 16 / RPI;            // copy instructions a sub-tile, of K and of V each
@@ -162,10 +175,12 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   __shared__ int s_hi[kShMaxBatch];           // a group's last visible prefix key + 1
   __shared__ int s_len[kShMaxBatch];
   __shared__ int s_own[kShMaxBatch];          // where a row's own keys begin
+  __shared__ short s_grp[kShMaxBatch];        // a row's group, or -1
   __shared__ float s_m[kShRows], s_l[kShRows];  // a piece's end: (m, l) of the computing waves' rows
   __shared__ int s_orow[kShRows];
-  __shared__ __attribute__((aligned(8))) unsigned char s_live[kShSlots][kShSide];  // sub-tiles in the slots that are no holes
+  __shared__ __attribute__((aligned(8))) unsigned char s_live[kShSlots][kShCopy];  // sub-tiles in the slots that are no holes
   __shared__ int s_wsum[2 * (kShThreads / kWave)];
+  __shared__ int s_edge[4];
 
   const int tid = threadIdx.x;
   const int lane = tid & (kWave - 1);
@@ -178,28 +193,33 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
 
   // ---- the plan: tiles and costs before each segment ----
   int* const s_cost = reinterpret_cast<int*>(s_tile);  // (until the first tile is brought)
+  // (the first round's loads all at once: each is a miss to memory)
+  int r0 = p.group_rows[min(tid, NG)], r1 = p.group_rows[min(tid + 1, NG)];
+  int pages = p.prefix_pages[min(tid, NG - 1)], len = p.lens[min(tid, B - 1)];
+  const auto row_in = [&](int r) { return r < 0 ? 0 : (r > B ? B : r); };
+  bool descend = false;  // groups out of order: every row by itself
 #pragma unroll 1
-  for (int i = tid; i <= NG; i += kShThreads) {
-    const int r = p.group_rows[i];
-    const int pages = p.prefix_pages[i < NG ? i : 0];
-    s_g0[i] = r < 0 ? 0 : (r > B ? B : r);
+  for (int i = tid;;) {
+    if (i <= NG) s_g0[i] = row_in(r0);
     if (i < NG) {
       const int64_t pt = static_cast<int64_t>(pages < 0 ? 0 : (pages > p.W ? p.W : pages)) * p.bs;
       s_cum[i] = static_cast<int>(pt < p.max_ctx ? pt : p.max_ctx);  // (for now: prefix tokens)
       s_hi[i] = 0;
+      descend |= row_in(r0) > row_in(r1);
     }
+    if (i < B) s_len[i] = len < 0 ? 0 : (len > p.max_ctx ? p.max_ctx : len);
+    i += kShThreads;
+    if (i > NG && i >= B) break;
+    r0 = p.group_rows[min(i, NG)];
+    r1 = p.group_rows[min(i + 1, NG)];
+    pages = p.prefix_pages[min(i, NG - 1)];
+    len = p.lens[min(i, B - 1)];
   }
-#pragma unroll 1
-  for (int b = tid; b < B; b += kShThreads) {
-    const int len = p.lens[b];
-    s_len[b] = len < 0 ? 0 : (len > p.max_ctx ? p.max_ctx : len);
-  }
+  descend = __any(descend);
+  if (lane == 0) s_wsum[w] = descend;
   __syncthreads();
-  // (groups out of order: every row by itself)
-  bool descend = false;
-#pragma unroll 1
-  for (int i = tid; i < NG; i += kShThreads) descend |= s_g0[i] > s_g0[i + 1];
-  descend = __syncthreads_or(descend);
+#pragma unroll
+  for (int i = 0; i < kShThreads / kWave; ++i) descend |= s_wsum[i] != 0;
 #pragma unroll 1
   for (int b = tid; b < B; b += kShThreads) {
     int lo = 0, hi = NG;  // the last group that begins at or before row b
@@ -217,7 +237,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
       atomicMax(&s_hi[lo], min(own, s_len[b]));
     }
     s_own[b] = own;
-    if (blockIdx.x == 0) p.plan[kShPlanCum + NS + 1 + b] = grp;
+    s_grp[b] = static_cast<short>(grp);
   }
   struct Segment {
     int b0, members, key0, hi;  // its first row and rows, its keys
@@ -237,7 +257,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
     __syncthreads();
     const int e = e0 + tid;
     int c = 0, cost = 0;
-    if (e < NS) {
+    if (e < NS) {  // (idle waves skip it)
       const Segment x = segment(e);
       const int blocks = (x.hi - x.key0 + 31) >> 5;
       if (blocks > 0) {
@@ -272,12 +292,16 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   }
   __syncthreads();
   const int per = max(1, ceil_div(uni(total_cost), p.shares));
-  if (blockIdx.x == 0) {
-    if (tid == 0) p.plan[0] = per;
+  if (blockIdx.x == 0 && tid == 0) p.plan[0] = per;
 #pragma unroll 1
-    for (int i = tid; i <= NS; i += kShThreads) p.plan[kShPlanCum + i] = s_cost[i];
-#pragma unroll 1
-    for (int i = tid; i <= NG; i += kShThreads) p.plan[kShPlanCum + NS + 1 + B + i] = s_g0[i];
+  for (int b = static_cast<int>(blockIdx.x) + tid * p.shares; b < B; b += kShThreads * p.shares) {
+    const int grp = s_grp[b];
+    const Segment e = segment(grp < 0 ? 0 : grp);
+    ShPlanRow* const o = reinterpret_cast<ShPlanRow*>(p.plan + kShPlanRows) + b;
+    *reinterpret_cast<int4*>(o) =
+        make_int4(s_cost[NG + b], max(0, (s_len[b] - s_own[b] + 31) >> 5), grp < 0 ? 0 : s_cost[grp],
+                  grp < 0 ? 0 : (e.hi + 31) >> 5);
+    *reinterpret_cast<int2*>(&o->first) = make_int2(e.b0, e.members);
   }
   // Contiguous shares to one XCD (workgroup i runs on XCD i % 8): the row blocks of one KV head
   // then read their keys through one L2.
@@ -285,36 +309,43 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
                         ? static_cast<int>(blockIdx.x % kXcds) * (p.shares / kXcds) +
                               static_cast<int>(blockIdx.x / kXcds)
                         : static_cast<int>(blockIdx.x);
-  // The share's tiles are those that begin at costs [share per, (share + 1) per): lane 0 finds the
-  // first, lane 1 the next share's.
-  int bound = total;
-  const int64_t edge = static_cast<int64_t>(share + (lane & 1)) * per;
-  if (edge < total_cost) {
-    const int x = static_cast<int>(edge);
-    int lo = 0, hi = NS;  // the last segment that begins at or before x
+  // The share's tiles are those that begin at costs [share per, (share + 1) per): lane 0 of a wave
+  // finds the first and its segment, lane 1 the next share's.
+  if (w == 0) {
+    int bound = total, lo = NS - 1;
+    const int64_t edge = static_cast<int64_t>(share + (lane & 1)) * per;
+    if (edge < total_cost) {
+      const int x = static_cast<int>(edge);
+      int hi = NS;  // the last segment that begins at or before x
+      lo = 0;
 #pragma unroll 1
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_cost[mid] <= x) lo = mid; else hi = mid;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_cost[mid] <= x) lo = mid; else hi = mid;
+      }
+      const Segment e = segment(lo);
+      const uint32_t blocks = static_cast<uint32_t>((e.hi - e.key0 + 31) >> 5);
+      const uint32_t step = static_cast<uint32_t>(sh_block_cost(e.members * RPS));
+      const uint32_t unit_cost = kShPieceCost + blocks * step;
+      const uint32_t off = static_cast<uint32_t>(x - s_cost[lo]);
+      const uint32_t unit = off / unit_cost;
+      const int r = static_cast<int>(off - unit * unit_cost);
+      const int tiles = ceil_div(static_cast<int>(blocks), TK / 32);
+      const int t = r == 0 ? 0 : max(1, ceil_div(r - kShPieceCost, static_cast<int>(step) * (TK / 32)));
+      bound = s_cum[lo] + static_cast<int>(unit) * tiles + min(t, tiles);
     }
-    const Segment e = segment(lo);
-    const uint32_t blocks = static_cast<uint32_t>((e.hi - e.key0 + 31) >> 5);
-    const uint32_t step = static_cast<uint32_t>(sh_block_cost(e.members * RPS));
-    const uint32_t unit_cost = kShPieceCost + blocks * step;
-    const uint32_t off = static_cast<uint32_t>(x - s_cost[lo]);
-    const uint32_t unit = off / unit_cost;
-    const int r = static_cast<int>(off - unit * unit_cost);
-    const int tiles = ceil_div(static_cast<int>(blocks), TK / 32);
-    const int t = r == 0 ? 0 : max(1, ceil_div(r - kShPieceCost, static_cast<int>(step) * (TK / 32)));
-    bound = s_cum[lo] + static_cast<int>(unit) * tiles + min(t, tiles);
+    if (lane < 2) {
+      s_edge[lane] = bound;
+      s_edge[2 + lane] = lo;
+    }
   }
-  const int first = __builtin_amdgcn_readlane(bound, 0);
-  const int last = __builtin_amdgcn_readlane(bound, 1);
   __syncthreads();
+  const int first = uni(s_edge[0]), last = uni(s_edge[1]);
+  const int seg0 = uni(s_edge[2]), seg1 = uni(s_edge[3]) + 1;  // its segments
   if (first >= last) return;
 
-  const bool copies = w >= kShSide;  // a copying wave
-  const int cw = w & (kShSide - 1);  // its place among its side's
+  const bool copies = w >= kShComp;         // a copying wave
+  const int cw = copies ? w - kShComp : w;  // its place among its side's
 
   // ---- a window of 64 tiles: lane i describes tile base + i ----
   // Everything the loops need of the plan is found here, each lane one tile, and later taken with
@@ -329,7 +360,11 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
     __device__ bool ends() const { return (bits >> 12) & 1; }
     __device__ int rows() const { return ((bits >> 13) & 127) + 1; }
     // Computing waves that take different rows; the others take other keys of the same.
-    __device__ int row_waves() const { return rows() > 64 ? 4 : (rows() > 32 ? 2 : 1); }
+    __device__ int row_waves() const {
+      return rows() > 64 ? 8 : (rows() > 32 ? 4 : (rows() > 16 ? 2 : 1));
+    }
+    // Pieces whose waves split the keys are joined through the slot.
+    __device__ bool joins() const { return ends() && rows() <= 64; }
     __device__ int first_row() const { return bits & 1023; }
     __device__ int kvh() const { return unit & 0xffff; }
     __device__ Tile at(int lane) const {
@@ -339,7 +374,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   };
   auto window = [&](int base) __attribute__((always_inline)) {
     const int pos = min(base + lane, last - 1);
-    int lo = 0, hi = NS;  // the last segment that begins at or before pos
+    int lo = seg0, hi = seg1;  // the last segment that begins at or before pos
 #pragma unroll 1
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -369,6 +404,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   // has been read; at a piece's end, whose rows leave through the slot, at two more.
   int slot = 0;  // the tile's slot
   if (copies) {
+    __builtin_amdgcn_s_setprio(2);
     // ================= the copying waves: SUB sub-tiles of K and of V each =================
 #pragma unroll 1
     for (int wbase = first; wbase < last; wbase += kWave) {
@@ -399,7 +435,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
           __builtin_amdgcn_s_waitcnt(sh_wait_vm(16 * (kShSlots - 1)));
           sh_barrier();
           sh_barrier();  // it has been read
-          if ((__builtin_amdgcn_readlane(wt.bits, i) >> 12) & 1) {
+          if (wt.at(i).joins()) {
             sh_barrier();
             sh_barrier();
           }
@@ -441,13 +477,13 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
   }
 
   // ================= the computing waves =================
-  uint4 qb[2][JD];  // B operands Q^T of the two 16-row sets: row n, dims KV::qk_dim0(j, g) ..
-  int orow[2] = {-1, -1}, hi_n[2] = {0, 0};  // their places in the output; they see keys below hi_n
+  uint4 qb[JD];  // B operands Q^T: row n, dims KV::qk_dim0(j, g) ..
+  int orow = -1, hi_n = 0;  // its place in the output; it sees keys below hi_n
   int wave_all = 0, wave_any = 0;  // all rows of the wave see keys below wave_all, none past wave_any
-  int RW = 1, rw = 0, ks = 0, KS = 1;  // the wave takes rows 32 rw .., every KS-th 32-key block
+  int RW = 1, rw = 0, ks = 0, KS = 1;  // the wave takes rows 16 rw .., every KS-th 32-key block
   bool unit_first = false;  // the piece holds its unit's first tile
-  float m_run[2], l_run[2];
-  mf_f32x4 acc[2][ND];
+  float m_run = -INFINITY, l_run = 0.0f;
+  mf_f32x4 acc[ND];
 #pragma unroll 1
   for (int wbase = first; wbase < last; wbase += kWave) {
     const int count = min(kWave, last - wbase);
@@ -463,7 +499,6 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
     for (int i = -1; i < count; ++i) {  // (i == -1: before the window's first tile)
       const Tile c = wt.at(i < 0 ? 0 : i);
       char* const base = s_tile + slot * 2 * kShHalf;
-      const bool ends = i >= 0 && c.ends();
       if (i >= 0) {
         sh_barrier();  // the tile has landed
         const uint32_t live4 = static_cast<uint32_t>(uni(*reinterpret_cast<const int*>(s_live[slot])));
@@ -474,7 +509,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
           const int key = c.tok + 32 * kb;
           const int live = (live4 >> (8 * (2 * kb / SUB) + 2 * kb % SUB)) & 3;
           char* const kv = base + kb * 32 * ROW;
-          mf_f32x4 s[2][2];
+          mf_f32x4 s[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             uint4 kk[JD];
@@ -491,12 +526,9 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
               for (int j = 0; j < JD; ++j)
                 kk[j] = *reinterpret_cast<const uint4*>(row + 16 * ((4 * j + g) ^ sh_swz<ROW>(n)));
             }
+            s[k] = mf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              s[h][k] = mf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-              for (int j = 0; j < JD; ++j) s[h][k] = Mfma16<T>::mac(kk[j], qb[h][j], s[h][k]);
-            }
+            for (int j = 0; j < JD; ++j) s[k] = Mfma16<T>::mac(kk[j], qb[j], s[k]);
           }
           // V^T, on its way during the softmax: tokens 4 g .. + 3 of the block's first 16 keys and of
           // its second, as pb holds them.
@@ -521,108 +553,95 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
           __builtin_amdgcn_sched_barrier(0);
           if (key + 32 > wave_all || live != 3) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const bool ok = ((live >> k) & 1) && key + 16 * k + 4 * g + r < hi_n[h];
-                  s[h][k][r] = ok ? s[h][k][r] : -INFINITY;
-                }
-          }
-          uint4 pb[2];
-          float alpha[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float mt = fmaxf(s[h][0][0], s[h][1][0]);
-#pragma unroll
-            for (int r = 1; r < 4; ++r) mt = fmaxf(mt, fmaxf(s[h][0][r], s[h][1][r]));
-            mt = rows4_max(mt);
-            const float m_new = fmaxf(m_run[h], mt * scale);
-            const bool some = m_new != -INFINITY;
-            alpha[h] = some ? __builtin_amdgcn_exp2f(m_run[h] - m_new) : 1.0f;
-            const float m_use = some ? m_new : 0.0f;
-            float pr[8];  // (masked scores weigh 2^-inf = 0, NaN stays NaN)
-#pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                pr[4 * k + r] = __builtin_amdgcn_exp2f(fmaf(s[h][k][r], scale, -m_use));
-            // The weights are rounded to the query type for the matrix cores (half a step of it,
-            // at most 1); l sums the rounded ones, so that the weights used still sum to one.
-            pb[h] = make_uint4(Pack2<T>::pack(pr[0], pr[1]), Pack2<T>::pack(pr[2], pr[3]),
-                               Pack2<T>::pack(pr[4], pr[5]), Pack2<T>::pack(pr[6], pr[7]));
-            const uint32_t one2 = Pack2<T>::pack(1.0f, 1.0f);
-            l_run[h] = fmaf(l_run[h], alpha[h],
-                            Dot2<T>::dot(pb[h].w, one2, Dot2<T>::dot(pb[h].z, one2, 0.0f)) +
-                                Dot2<T>::dot(pb[h].y, one2, Dot2<T>::dot(pb[h].x, one2, 0.0f)));
-            m_run[h] = m_new;
+              for (int r = 0; r < 4; ++r) {
+                const bool ok = ((live >> k) & 1) && key + 16 * k + 4 * g + r < hi_n;
+                s[k][r] = ok ? s[k][r] : -INFINITY;
+              }
           }
-          if (__any(alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+          float mt = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+          for (int r = 1; r < 4; ++r) mt = fmaxf(mt, fmaxf(s[0][r], s[1][r]));
+          mt = rows4_max(mt);
+          const float m_new = fmaxf(m_run, mt * scale);
+          const bool some = m_new != -INFINITY;
+          const float alpha = some ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+          const float m_use = some ? m_new : 0.0f;
+          float pr[8];  // (masked scores weigh 2^-inf = 0, NaN stays NaN)
 #pragma unroll
-              for (int u = 0; u < ND; ++u) acc[h][u] *= alpha[h];
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              pr[4 * k + r] = __builtin_amdgcn_exp2f(fmaf(s[k][r], scale, -m_use));
+          // The weights are rounded to the query type for the matrix cores (half a step of it,
+          // at most 1); l sums the rounded ones, so that the weights used still sum to one.
+          const uint4 pb = make_uint4(Pack2<T>::pack(pr[0], pr[1]), Pack2<T>::pack(pr[2], pr[3]),
+                                      Pack2<T>::pack(pr[4], pr[5]), Pack2<T>::pack(pr[6], pr[7]));
+          const uint32_t one2 = Pack2<T>::pack(1.0f, 1.0f);
+          l_run = fmaf(l_run, alpha,
+                       Dot2<T>::dot(pb.w, one2, Dot2<T>::dot(pb.z, one2, 0.0f)) +
+                           Dot2<T>::dot(pb.y, one2, Dot2<T>::dot(pb.x, one2, 0.0f)));
+          m_run = m_new;
+          if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int u = 0; u < ND; ++u) acc[u] *= alpha;
           }
 #pragma unroll
-          for (int u = 0; u < ND; ++u) {
-            const uint4 x = KV::operand(vv[u]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) acc[h][u] = Mfma16<T>::mac(x, pb[h], acc[h][u]);
-          }
+          for (int u = 0; u < ND; ++u) acc[u] = Mfma16<T>::mac(KV::operand(vv[u]), pb, acc[u]);
         }
-        sh_barrier();  // the slot has been read
-        slot ^= 1;
       }
 
-      // ---- the next piece's query rows are requested here (its first tile is the next one) ----
+      // ---- the next piece's query rows are requested here (its first tile is the next one), ahead
+      // of the copies that follow the barrier ----
+      const bool ends = i >= 0 && c.ends();
       const bool next = i + 1 < count;
       const Tile nx = wt.at(next ? i + 1 : 0);
       const bool starts = next && nx.starts();
-      int n_row[2], n_hi[2];  // the rows requested
+      int n_row = -1, n_hi = 0;  // the row requested
+      uint4 nq[JD];
       if (starts) {
         const int b0 = nx.first_row();
         const T* const q = static_cast<const T*>(p.q) + static_cast<int64_t>(b0) * p.q_len * p.H * D;
+        const int r = 16 * (cw & (nx.row_waves() - 1)) + n;
+        const int row = (nx.unit >> 16) * kShRows + (r < nx.rows() ? r : 0);
+        const int member = fast_quot(row, p.by_rps);
+        const int rest = row - member * RPS;
+        const int tq = fast_quot(rest, p.by_g);
+        const int o = (member * p.q_len + tq) * p.H + nx.kvh() * p.G + (rest - tq * p.G);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = 32 * (cw & (nx.row_waves() - 1)) + 16 * h + n;
-          const int row = (nx.unit >> 16) * kShRows + (r < nx.rows() ? r : 0);
-          const int member = fast_quot(row, p.by_rps);
-          const int rest = row - member * RPS;
-          const int tq = fast_quot(rest, p.by_g);
-          const int o = (member * p.q_len + tq) * p.H + nx.kvh() * p.G + (rest - tq * p.G);
-          n_row[h] = r < nx.rows() ? b0 * p.q_len * p.H + o : -1;
-          n_hi[h] = n_row[h] < 0 ? 0 : min(nx.hi, s_len[b0 + member] - p.q_len + tq + 1);
-#pragma unroll
-          for (int j = 0; j < JD; ++j)
-            qb[h][j] = *reinterpret_cast<const uint4*>(q + static_cast<int64_t>(o) * D +
-                                                       KV::qk_dim0(j, g, JD));
+        for (int j = 0; j < JD; ++j)
+          nq[j] = *reinterpret_cast<const uint4*>(q + static_cast<int64_t>(o) * D +
+                                                  KV::qk_dim0(j, g, JD));
+        if (r < nx.rows()) {
+          n_row = b0 * p.q_len * p.H + o;
+          n_hi = min(nx.hi, s_len[b0 + member] - p.q_len + tq + 1);
         }
       }
-      // ---- a piece's end: the waves' rows go to the slot ----
-      // Row r = 32 rw + 16 h + n of key wave ks at row 32 RW ks + r, its 16-byte chunk j at chunk
-      // j ^ n (the 16 lanes of a set hold 16 rows).
-      const int e_rows = 32 * RW;
-      const int e_ks = KS;
-      const int64_t e_slot0 = unit_first ? ((c.bits >> 10) & 1) * p.rows
-                                         : 2 * p.rows + static_cast<int64_t>(share) * kShRows;
-      const bool e_first = unit_first;
+      if (i >= 0) {
+        sh_barrier();  // the slot has been read
+        slot ^= 1;
+      }
+      // ---- a piece's end: its partials ----
+      const int64_t slot0 = unit_first ? ((c.bits >> 10) & 1) * p.rows
+                                       : 2 * p.rows + static_cast<int64_t>(share) * kShRows;
+      const int rr = 16 * rw + n;  // the lane's row of the unit
+      const float l = rows4_sum(l_run);
+      const bool joins = ends && KS > 1;
       float* const f = reinterpret_cast<float*>(base);
-      if (ends) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float l = rows4_sum(l_run[h]);
-          const int r = 32 * rw + 16 * h + n;
-          const int at = ks * e_rows + r;
+      if (joins) {
+        // Waves that split the keys put theirs into the slot: row rr of key wave ks at row
+        // 16 RW ks + rr, its 16-byte chunk j at chunk j ^ n (the lanes of a set hold 16 rows).
+        const int at = 16 * RW * ks + rr;
+        if (rr < c.rows()) {
 #pragma unroll
           for (int u = 0; u < ND; ++u)
-            if (r < c.rows())
-              *reinterpret_cast<float4*>(f + at * D + 4 * ((4 * u + g) ^ n)) =
-                  make_float4(acc[h][u][0], acc[h][u][1], acc[h][u][2], acc[h][u][3]);
+            *reinterpret_cast<float4*>(f + at * D + 4 * ((4 * u + g) ^ n)) =
+                make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
           if (g == 0) {
-            s_m[at] = m_run[h];
+            s_m[at] = m_run;
             s_l[at] = l;
-            if (ks == 0) s_orow[r] = orow[h];
+            if (ks == 0) s_orow[rr] = orow;
           }
         }
         sh_barrier();
@@ -631,36 +650,44 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
       __builtin_amdgcn_s_waitcnt(sh_wait_vm(0));
       if (starts) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < JD; ++j) {
-            qb[h][j] = make_uint4(qb[h][j].x ^ flip, qb[h][j].y ^ flip, qb[h][j].z ^ flip, qb[h][j].w ^ flip);
-            keep_here(qb[h][j]);
-          }
+        for (int j = 0; j < JD; ++j) {
+          qb[j] = make_uint4(nq[j].x ^ flip, nq[j].y ^ flip, nq[j].z ^ flip, nq[j].w ^ flip);
+          keep_here(qb[j]);
+        }
       }
-      // ---- the piece's partials: the waves that split the keys are joined, a thread 4 dims ----
-      if (ends) {
+      if (ends && !joins && orow >= 0) {
+        const int64_t at = slot0 + (unit_first ? orow : rr);
+        if (g == 0) *reinterpret_cast<float2*>(p.ml + 2 * at) = make_float2(m_run, l);
+#pragma unroll
+        for (int u = 0; u < ND; ++u)
+          *reinterpret_cast<float4*>(p.acc + at * D + 16 * u + 4 * g) =
+              make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
+      }
+      if (joins) {  // a thread joins 4 dims of a row
 #pragma unroll 1
-        for (int x = cw * kWave + lane; x < c.rows() * (D / 4); x += kShSide * kWave) {
+        for (int x = tid; x < c.rows() * (D / 4); x += kShComp * kWave) {
           const int r = x / (D / 4), j = x % (D / 4);
-          float M = s_m[r];
-#pragma unroll 1
-          for (int k = 1; k < e_ks; ++k) M = fmaxf(M, s_m[k * e_rows + r]);
+          float M = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < kShComp; ++k) M = fmaxf(M, s_m[(k < KS ? k : 0) * 16 * RW + r]);
           const float m_use = M != -INFINITY ? M : 0.0f;
           float L = 0.0f;
           float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-          for (int k = 0; k < e_ks; ++k) {
-            const int at = k * e_rows + r;
-            const float e = __builtin_amdgcn_exp2f(s_m[at] - m_use);
-            const float4 y = *reinterpret_cast<const float4*>(f + at * D + 4 * (j ^ (r & 15)));
-            L = fmaf(s_l[at], e, L);
-            o.x = fmaf(y.x, e, o.x);
-            o.y = fmaf(y.y, e, o.y);
-            o.z = fmaf(y.z, e, o.z);
-            o.w = fmaf(y.w, e, o.w);
+          for (int k0 = 0; k0 < KS; k0 += 2) {  // (KS is 2, 4 or 8)
+#pragma unroll
+            for (int k = k0; k < k0 + 2; ++k) {
+              const int at = k * 16 * RW + r;
+              const float e = __builtin_amdgcn_exp2f(s_m[at] - m_use);
+              const float4 y = *reinterpret_cast<const float4*>(f + at * D + 4 * (j ^ (r & 15)));
+              L = fmaf(s_l[at], e, L);
+              o.x = fmaf(y.x, e, o.x);
+              o.y = fmaf(y.y, e, o.y);
+              o.z = fmaf(y.z, e, o.z);
+              o.w = fmaf(y.w, e, o.w);
+            }
           }
-          const int64_t at = e_slot0 + (e_first ? s_orow[r] : r);
+          const int64_t at = slot0 + (unit_first ? s_orow[r] : r);
           if (j == 0) *reinterpret_cast<float2*>(p.ml + 2 * at) = make_float2(M, L);
           *reinterpret_cast<float4*>(p.acc + at * D + 4 * j) = o;
         }
@@ -671,25 +698,19 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
         unit_first = (nx.bits >> 11) & 1;
         RW = nx.row_waves();
         rw = cw & (RW - 1);
-        KS = kShSide / RW;
+        KS = kShComp / RW;
         ks = cw / RW;
-        int lo = INT_MAX, hi = 0;
+        orow = n_row;
+        hi_n = n_hi;
+        m_run = -INFINITY;
+        l_run = 0.0f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          orow[h] = n_row[h];
-          hi_n[h] = n_hi[h];
-          lo = orow[h] < 0 ? lo : min(lo, hi_n[h]);
-          hi = max(hi, hi_n[h]);
-          m_run[h] = -INFINITY;
-          l_run[h] = 0.0f;
-#pragma unroll
-          for (int u = 0; u < ND; ++u) acc[h][u] = mf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-          lo = min(lo, __shfl_xor(lo, o, kWave));
-          hi = max(hi, __shfl_xor(hi, o, kWave));
-        }
+        for (int u = 0; u < ND; ++u) acc[u] = mf_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        int lo = orow < 0 ? INT_MAX : hi_n, hi = hi_n;
+        sh_fold16<8>(lo, hi);
+        sh_fold16<4>(lo, hi);
+        sh_fold16<2>(lo, hi);
+        sh_fold16<1>(lo, hi);
         wave_all = uni(lo);
         wave_any = uni(hi);
       }
@@ -699,7 +720,7 @@ __global__ __launch_bounds__(kShThreads, 2) void shared_attn_kernel(const Shared
 
 // Joins a row's pieces: one wave a query row, D / 64 dims a lane. Its pieces: for the group's
 // segment (if the row has one) and for its own, the unit's first piece, then those of the shares
-// that the unit runs on into.
+// that the unit runs on into. What few calls take (two pieces of each) is read at once.
 constexpr int kShMergeThreads = 256;
 constexpr int kShMergeWaves = kShMergeThreads / kWave;
 template <typename T, int D, int TB>  // TB: 32-key blocks of a tile
@@ -709,59 +730,88 @@ __global__ __launch_bounds__(kShMergeThreads) void shared_merge_kernel(const Sha
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kShMergeWaves +
                       __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
   if (row >= p.rows) return;
-  const int B = p.batch, NG = p.groups, NS = NG + B;
-  const int* const cum = p.plan + kShPlanCum;
-  const int bi = static_cast<int>(row / p.H);
-  const int h = static_cast<int>(row - static_cast<int64_t>(bi) * p.H);
-  const int b = bi / p.q_len, i = bi - b * p.q_len;
-  const int kvh = h / p.G, gq = h - kvh * p.G;
-  const int RPS = p.q_len * p.G;
   const int per = p.plan[0];
-  const int grp = cum[NS + 1 + b];
+  const int bi = fast_quot(static_cast<int>(row), p.by_h);
+  const int b = fast_quot(bi, p.by_q), i = bi - b * p.q_len;
+  const int h = static_cast<int>(row) - bi * p.H;
+  const int kvh = fast_quot(h, p.by_g);
+  const int r0 = i * p.G + h - kvh * p.G;
+  const int RPS = p.q_len * p.G;
+  const ShPlanRow e = reinterpret_cast<const ShPlanRow*>(p.plan + kShPlanRows)[b];
+  // A unit's pieces: the first at the row's own place, the others at shares' places.
+  struct Unit {
+    int begin, tile, last, r, share;  // its cost, a tile's, the last tile, the row in it, the share
+  };
+  const auto unit = [&](int cost, int blocks, int r, int members) __attribute__((always_inline)) {
+    const int step = sh_block_cost(members * RPS);
+    const int rtiles = (members * RPS + kShRows - 1) / kShRows;
+    Unit u;
+    u.begin = cost + (kvh * rtiles + r / kShRows) * (kShPieceCost + blocks * step);
+    u.tile = TB * step;
+    u.last = (blocks - 1) / TB;
+    u.r = r % kShRows;
+    u.share = blocks > 0 ? static_cast<int>(static_cast<uint32_t>(u.begin) / static_cast<uint32_t>(per))
+                         : -1;
+    return u;
+  };
+  // The place of the unit's next piece, in the share of its first tile past the last one's; -1: none.
+  const auto next = [&](Unit& u) __attribute__((always_inline)) -> int64_t {
+    if (u.share < 0) return -1;
+    const int past = (u.share + 1) * per - u.begin - kShPieceCost;
+    const int t = past <= u.tile ? 1 : ceil_div(past, u.tile);
+    u.share = t > u.last ? -1
+                         : static_cast<int>(static_cast<uint32_t>(u.begin + kShPieceCost + t * u.tile) /
+                                            static_cast<uint32_t>(per));
+    return u.share < 0 ? -1 : 2 * p.rows + static_cast<int64_t>(u.share) * kShRows + u.r;
+  };
+  Unit group = unit(e.cost, e.blocks, (b - e.first) * RPS + r0, e.members);
+  Unit own = unit(e.own_cost, e.own_blocks, r0, 1);
   float M = -INFINITY, L = 0.0f;
   float o[DPL];
 #pragma unroll
   for (int d = 0; d < DPL; ++d) o[d] = 0.0f;
-  auto take = [&](int64_t slot) __attribute__((always_inline)) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.ml + 2 * slot);
-    float a[DPL];
+  int64_t at[4] = {group.share < 0 ? -1 : row, own.share < 0 ? -1 : p.rows + row, next(group), next(own)};
+#pragma unroll 1
+  for (;;) {
+    float2 ml[4];
+    float a[4][DPL];
 #pragma unroll
-    for (int d = 0; d < DPL; ++d) a[d] = p.acc[slot * D + DPL * lane + d];
-    const float Mn = fmaxf(M, ml.x);
+    for (int k = 0; k < 4; ++k) {  // (place 0 in an absent one's stead)
+      const int64_t s = at[k] < 0 ? 0 : at[k];
+      ml[k] = *reinterpret_cast<const float2*>(p.ml + 2 * s);
+#pragma unroll
+      for (int d = 0; d < DPL; ++d) a[k][d] = p.acc[s * D + DPL * lane + d];
+    }
+#if defined(__HIP_DEVICE_COMPILE__)
+    // (all on their way before the first is used)
+    if constexpr (DPL == 2)
+      asm volatile("" : "+v"(a[0][0]), "+v"(a[1][0]), "+v"(a[2][0]), "+v"(a[3][0]),
+                        "+v"(a[0][1]), "+v"(a[1][1]), "+v"(a[2][1]), "+v"(a[3][1]));
+    else
+      asm volatile("" : "+v"(a[0][0]), "+v"(a[1][0]), "+v"(a[2][0]), "+v"(a[3][0]));
+#endif
+    float Mn = M;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) Mn = at[k] < 0 ? Mn : fmaxf(Mn, ml[k].x);
     const bool some = Mn != -INFINITY;
     const float w0 = some ? __builtin_amdgcn_exp2f(M - Mn) : 1.0f;
-    const float w1 = some ? __builtin_amdgcn_exp2f(ml.x - Mn) : 0.0f;
-    L = fmaf(ml.y, w1, L * w0);
+    L *= w0;
 #pragma unroll
-    for (int d = 0; d < DPL; ++d) o[d] = fmaf(a[d], w1, o[d] * w0);
+    for (int d = 0; d < DPL; ++d) o[d] *= w0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (at[k] >= 0) {
+        const float w = some ? __builtin_amdgcn_exp2f(ml[k].x - Mn) : 0.0f;
+        L = fmaf(ml[k].y, w, L);
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) o[d] = fmaf(a[k][d], w, o[d]);
+      }
     M = Mn;
-  };
-  for (int kind = 0; kind < 2; ++kind) {
-    if (kind == 0 && grp < 0) continue;
-    const int seg = kind == 0 ? grp : NG + b;
-    const int c0 = cum[seg], c1 = cum[seg + 1];
-    if (c1 <= c0) continue;
-    int r = i * p.G + gq, members = 1;
-    if (kind == 0) {
-      const int* const g0 = cum + NS + 1 + B;
-      r += (b - g0[grp]) * RPS;
-      members = g0[grp + 1] - g0[grp];
-    }
-    const int rtiles = ceil_div(members * RPS, kShRows);
-    const int unit = (c1 - c0) / (rtiles * p.KVH);  // a unit's cost
-    const int step = sh_block_cost(members * RPS);
-    const int tile = step * TB;  // a tile's cost
-    const int last = ((unit - kShPieceCost) / step - 1) / TB;  // its last tile
-    const int t0 = c0 + (kvh * rtiles + r / kShRows) * unit;
-    take(kind * p.rows + row);
-    for (int s = t0 / per;;) {
-      // the first tile past share s, and its share
-      const int past = (s + 1) * per - t0 - kShPieceCost;
-      const int t = past <= tile ? 1 : ceil_div(past, tile);
-      if (t > last) break;
-      s = (t0 + kShPieceCost + t * tile) / per;
-      take(2 * p.rows + static_cast<int64_t>(s) * kShRows + r % kShRows);
-    }
+    if (group.share < 0 && own.share < 0) break;
+    at[0] = next(group);
+    at[1] = next(own);
+    at[2] = next(group);
+    at[3] = next(own);
   }
   const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
   T* const out = static_cast<T*>(p.out) + row * D + DPL * lane;
