@@ -1755,7 +1755,7 @@ bool shared_geometry_ok(int batch, int q_len, int num_heads, int num_kv_heads, i
          // (the kernel's query offsets and costs are 32-bit)
          static_cast<int64_t>(batch) * q_len * num_heads * head_dim * 2 < (int64_t(1) << 31) &&
          shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups,
-                           sh_tile(head_dim, 2)) < (int64_t(1) << 23);
+                           sh_tile(head_dim, 2)) < (int64_t(1) << 22);
 }
 
 }  // namespace

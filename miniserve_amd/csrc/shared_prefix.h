@@ -51,20 +51,26 @@ __host__ __device__ constexpr int sh_tile(int head_dim, int kv_bytes) {
 #endif
 constexpr int kShAux = MSATTN_SHARED_AUX;
 
-// What a share is to cost a workgroup, in units of about 500 clocks: a piece (its query, its plan,
+// What a share is to cost a workgroup, in units of about 250 clocks: a piece (its query, its plan,
 // its partials), and each 32-key block of a unit of so many rows. Few rows wait for the memory pipe,
-// many for the matrix cores and the softmax.
+// many for the matrix cores and the softmax. (From a fit of the workgroups' clocks to their pieces
+// and blocks, then tried around: 64 rows in 8 groups of bf16 head_dim 128 took 74 us with the same
+// piece cost and half the spread, 58 so; equal tile counts 81.)
 #ifndef MSATTN_SHARED_COSTS
-#define MSATTN_SHARED_COSTS 11, 2, 3, 5
+#define MSATTN_SHARED_COSTS {20, 6, 7, 9, 12}, {20, 3, 4, 5, 7}, {20, 2, 3, 5, 8}, {20, 2, 3, 4, 6}
 #endif
-__host__ __device__ constexpr int sh_cost(int which) {
-  constexpr int c[] = {MSATTN_SHARED_COSTS};
-  return c[which];
-}
-constexpr int kShPieceCost = sh_cost(0);
-__host__ __device__ constexpr int sh_block_cost(int rows) {
-  return sh_cost(rows > 64 ? 3 : (rows > 32 ? 2 : 1));
-}
+template <int D, int EB>
+struct ShCost {
+  static constexpr int row(int i) {  // 16-bit caches of head_dim 128 and 64, fp8 ones
+    constexpr int c[4][5] = {MSATTN_SHARED_COSTS};
+    return c[(EB == 1 ? 2 : 0) + (D == 64 ? 1 : 0)][i];
+  }
+  static constexpr int kPiece = row(0);
+  __device__ static int block(int rows) {
+    constexpr int c[4] = {row(1), row(2), row(3), row(4)};
+    return rows > 64 ? c[3] : (rows > 32 ? c[2] : (rows > 16 ? c[1] : c[0]));
+  }
+};
 
 // Division of x < 2^31 by a constant of the call: with s = ceil(log2 d) and m = ceil(2^(31+s) / d),
 // x m 2^-(31+s) exceeds x / d by less than 1 / d, so its integer part is the quotient.
@@ -156,6 +162,7 @@ __device__ __forceinline__ int sh_swz(int r) {
 template <typename T, typename KT, int D>
 __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const SharedParams p) {
   typedef Kv8<T, KT> KV;
+  typedef ShCost<D, static_cast<int>(sizeof(KT))> Cost;
   static_assert(D == 64 || D == 128, "head_dim 64 and 128");
   constexpr int EB = static_cast<int>(sizeof(KT));
   constexpr bool FP8 = EB == 1;  // its rows are widened as the matrix operands are read
@@ -263,7 +270,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
       if (blocks > 0) {
         const int units = p.KVH * ceil_div(x.members * RPS, kShRows);
         c = units * ceil_div(blocks, TK / 32);
-        cost = units * (kShPieceCost + blocks * sh_block_cost(x.members * RPS));
+        cost = units * (Cost::kPiece + blocks * Cost::block(x.members * RPS));
       }
     }
     const int incl = wave_inclusive_sum(c), incl_cost = wave_inclusive_sum(cost);
@@ -325,13 +332,13 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
       }
       const Segment e = segment(lo);
       const uint32_t blocks = static_cast<uint32_t>((e.hi - e.key0 + 31) >> 5);
-      const uint32_t step = static_cast<uint32_t>(sh_block_cost(e.members * RPS));
-      const uint32_t unit_cost = kShPieceCost + blocks * step;
+      const uint32_t step = static_cast<uint32_t>(Cost::block(e.members * RPS));
+      const uint32_t unit_cost = Cost::kPiece + blocks * step;
       const uint32_t off = static_cast<uint32_t>(x - s_cost[lo]);
       const uint32_t unit = off / unit_cost;
       const int r = static_cast<int>(off - unit * unit_cost);
       const int tiles = ceil_div(static_cast<int>(blocks), TK / 32);
-      const int t = r == 0 ? 0 : max(1, ceil_div(r - kShPieceCost, static_cast<int>(step) * (TK / 32)));
+      const int t = r == 0 ? 0 : max(1, ceil_div(r - Cost::kPiece, static_cast<int>(step) * (TK / 32)));
       bound = s_cum[lo] + static_cast<int>(unit) * tiles + min(t, tiles);
     }
     if (lane < 2) {
@@ -723,8 +730,10 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
 // that the unit runs on into. What few calls take (two pieces of each) is read at once.
 constexpr int kShMergeThreads = 256;
 constexpr int kShMergeWaves = kShMergeThreads / kWave;
-template <typename T, int D, int TB>  // TB: 32-key blocks of a tile
+template <typename T, int D, int EB>
 __global__ __launch_bounds__(kShMergeThreads) void shared_merge_kernel(const SharedParams p) {
+  typedef ShCost<D, EB> Cost;
+  constexpr int TB = sh_tile(D, EB) / 32;  // 32-key blocks of a tile
   constexpr int DPL = D / 64;
   const int lane = threadIdx.x & (kWave - 1);
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kShMergeWaves +
@@ -743,10 +752,10 @@ __global__ __launch_bounds__(kShMergeThreads) void shared_merge_kernel(const Sha
     int begin, tile, last, r, share;  // its cost, a tile's, the last tile, the row in it, the share
   };
   const auto unit = [&](int cost, int blocks, int r, int members) __attribute__((always_inline)) {
-    const int step = sh_block_cost(members * RPS);
+    const int step = Cost::block(members * RPS);
     const int rtiles = (members * RPS + kShRows - 1) / kShRows;
     Unit u;
-    u.begin = cost + (kvh * rtiles + r / kShRows) * (kShPieceCost + blocks * step);
+    u.begin = cost + (kvh * rtiles + r / kShRows) * (Cost::kPiece + blocks * step);
     u.tile = TB * step;
     u.last = (blocks - 1) / TB;
     u.r = r % kShRows;
@@ -757,10 +766,10 @@ __global__ __launch_bounds__(kShMergeThreads) void shared_merge_kernel(const Sha
   // The place of the unit's next piece, in the share of its first tile past the last one's; -1: none.
   const auto next = [&](Unit& u) __attribute__((always_inline)) -> int64_t {
     if (u.share < 0) return -1;
-    const int past = (u.share + 1) * per - u.begin - kShPieceCost;
+    const int past = (u.share + 1) * per - u.begin - Cost::kPiece;
     const int t = past <= u.tile ? 1 : ceil_div(past, u.tile);
     u.share = t > u.last ? -1
-                         : static_cast<int>(static_cast<uint32_t>(u.begin + kShPieceCost + t * u.tile) /
+                         : static_cast<int>(static_cast<uint32_t>(u.begin + Cost::kPiece + t * u.tile) /
                                             static_cast<uint32_t>(per));
     return u.share < 0 ? -1 : 2 * p.rows + static_cast<int64_t>(u.share) * kShRows + u.r;
   };
@@ -838,7 +847,7 @@ hipError_t launch_shared_one(const SharedParams& p, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t blocks = (p.rows + kShMergeWaves - 1) / kShMergeWaves;
-  hipLaunchKernelGGL((shared_merge_kernel<T, D, sh_tile(D, sizeof(KT)) / 32>), dim3(static_cast<unsigned>(blocks)),
+  hipLaunchKernelGGL((shared_merge_kernel<T, D, sizeof(KT)>), dim3(static_cast<unsigned>(blocks)),
                      dim3(kShMergeThreads), 0, stream, p);
   return hipGetLastError();
 }
