@@ -151,4 +151,5 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 def stream_handle(device: torch.device) -> int:
     """hipStream_t of torch's current stream on `device`."""
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)

@@ -117,9 +117,11 @@ def block_table_i32(block_table, device: torch.device) -> torch.Tensor:
     attention.py:237) is converted once and reused while it is unchanged: same object,
     same torch version counter (every in-place write through torch bumps it), same shape
     and strides. Not during graph capture, whose conversions must be captured."""
+    if isinstance(block_table, torch.Tensor) and block_table.dtype == torch.int32 and \
+            block_table.ndim == 2 and block_table.device == device and block_table.is_contiguous():
+        return block_table
     if not isinstance(block_table, torch.Tensor) or block_table.device != device or \
-            (block_table.dtype == torch.int32 and block_table.is_contiguous() and
-             block_table.ndim == 2) or torch.cuda.is_current_stream_capturing():
+            torch.cuda.is_current_stream_capturing():
         return _convert_table(torch.as_tensor(block_table, device=device))
     try:
         version = block_table._version

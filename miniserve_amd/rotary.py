@@ -19,7 +19,7 @@ _I64x3 = ctypes.c_int64 * 3
 
 def on_device(dev: torch.device, fn, *args) -> int:
     """fn(*args, stream) with `dev` current and torch's current stream on it."""
-    if torch.cuda.current_device() == dev.index or dev.index is None:
+    if dev.index is None or torch._C._cuda_getDevice() == dev.index:
         return fn(*args, nat.stream_handle(dev))
     with torch.cuda.device(dev):
         return fn(*args, nat.stream_handle(dev))
@@ -27,7 +27,7 @@ def on_device(dev: torch.device, fn, *args) -> int:
 
 def rope_table(t, dev: torch.device, what: str) -> torch.Tensor:
     """A rotation table as the kernels read it: fp32 [max_pos, dims], contiguous, on `dev`."""
-    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.float32:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != dev:
         t = torch.as_tensor(t, device=dev).to(torch.float32)
     if t.ndim != 2 or t.shape[0] < 1:
         raise ValueError(f"{what} must be [max_pos, dims] with at least one position")
@@ -37,6 +37,8 @@ def rope_table(t, dev: torch.device, what: str) -> torch.Tensor:
 def extent(t: torch.Tensor) -> tuple[int, int]:
     """First byte that `t` addresses and the one past its last."""
     lo = t.data_ptr()
+    if t.is_contiguous():
+        return lo, lo + t.nbytes
     if t.numel() == 0:
         return lo, lo
     return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
@@ -56,21 +58,28 @@ def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
         (a.shape[0] == 1 or batch >= a.shape[1] * token)
 
 
-def _apart(t: torch.Tensor, written: Sequence[torch.Tensor]) -> bool:
+def _spans(tensors: Sequence[torch.Tensor]) -> list[tuple[int, int, torch.Tensor]]:
+    return [(*extent(t), t) for t in tensors]
+
+
+def _clear(t: torch.Tensor, written: Sequence[tuple[int, int, torch.Tensor]]) -> bool:
     lo, hi = extent(t)
-    for w in written:
-        wlo, whi = extent(w)
+    for wlo, whi, w in written:
         if lo < whi and wlo < hi and not (t.ndim == w.ndim == 4 and _rows_apart(t, w)):
             return False
     return True
 
 
-def _source(t: torch.Tensor, written: Sequence[torch.Tensor]) -> torch.Tensor:
+def _apart(t: torch.Tensor, written: Sequence[torch.Tensor]) -> bool:
+    return _clear(t, _spans(written))
+
+
+def _source(t: torch.Tensor, written: Sequence[tuple[int, int, torch.Tensor]]) -> torch.Tensor:
     """`t` as the kernel may read it through its strides: rows of contiguous dims that share no
-    memory with what the call writes (a copy otherwise)."""
+    memory with the `_spans` that the call writes (a copy otherwise)."""
     if t.is_neg():
         t = t.resolve_neg()
-    if t.stride(3) != 1 and t.shape[3] != 1 or not _apart(t, written):
+    if t.stride(3) != 1 and t.shape[3] != 1 or not _clear(t, written):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -157,15 +166,17 @@ def write_kv_rope(query: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
         per_token = 1 if pos.ndim == 2 else 0
         pos = pos.contiguous()
     q_args = (None, None, None, None, 0)
-    written = [k_cache, v_cache]
+    written = _spans((k_cache, v_cache))
     if query is not None:
         if out is None:
             out = torch.empty(query.shape, dtype=query.dtype, device=dev)
-        in_place = out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
-        q = query if in_place and not query.is_neg() else _source(query, [k_cache, v_cache, out])
-        if not _apart(out, [k_cache, v_cache]):
-            raise ValueError("out shares memory with a cache")
-        written.append(out)
+            q = _source(query, written)
+        else:
+            if not _clear(out, written):
+                raise ValueError("out shares memory with a cache")
+            written += _spans((out,))
+            in_place = out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
+            q = query if in_place and not query.is_neg() else _source(query, written)
         q_args = (q.data_ptr(), _I64x3(*q.stride()[:3]), out.data_ptr(),
                   _I64x3(*out.stride()[:3]), query.shape[2])
     ks, vs = _source(k, written), _source(v, written)

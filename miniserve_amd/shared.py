@@ -100,7 +100,8 @@ def paged_attention_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     max_context = max(0, min(int(max_context), cap))
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty((B, q_len, H, D), dtype=query.dtype, device=dev)
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or \
             not out.is_contiguous():
@@ -112,7 +113,7 @@ def paged_attention_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if workspace is None or workspace.numel() * workspace.element_size() < ws_bytes:
         workspace = _workspace(dev, ws_bytes)
     q = query.contiguous()
-    if q is query:  # a kernel reads all of it while the output is written
+    if q is query and not fresh:  # a kernel reads all of it while the output is written
         (lo, hi), (olo, ohi) = extent(q), extent(out)
         if lo < ohi and olo < hi:
             q = q.clone()

@@ -35,10 +35,10 @@ def test_workspace_bytes():
     assert f(4, 1, 4, 4, 64, 100, 0) == base(4, 1, 4, 4, 64, 100)
     assert f(2000, 1, 4, 4, 64, 100, 3) == base(2000, 1, 4, 4, 64, 100)
     assert f(4, 1, 4, 4, 80, 100, 3) == base(4, 1, 4, 4, 80, 100)
-    # the header other calls keep their counters in, the plan, then two partial rows an output row
-    # and 128 a share of 256: (m, l) and an accumulator each
+    # the header other calls keep their counters in, the plan (8 words a row), then two partial
+    # rows an output row and 128 a share of 256: (m, l) and an accumulator each
     r256 = lambda x: -(-x // 256) * 256  # noqa: E731
     slots = 2 * 64 * 32 + 256 * 128
-    want = r256(4 * (64 + 4096)) + r256(4 * (16 + 8 + 64 + 1 + 64 + 9)) + r256(8 * slots) + \
+    want = r256(4 * (64 + 4096)) + r256(4 * (16 + 8 * 64)) + r256(8 * slots) + \
         slots * 128 * 4
     assert f(64, 1, 32, 8, 128, 1024, 8) == max(want, base(64, 1, 32, 8, 128, 1024))
