@@ -544,8 +544,9 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
     ``rope`` = (cos, sin) or (cos, sin, position): the query and the new key are rotated on the
     way (rotate-half, fp32 tables [max_pos, rotary_dim]), at context_lens[b] - 1 or at
     position[b], clamped to [0, max_pos): ``write_kv_rope`` of the new token, then the decode,
-    in the launches of the call without it (msattn_paged_attention_append_rope). A rotary_dim
-    below head_dim makes the two calls.
+    in the launches of the call without it (msattn_paged_attention_append_rope). With at most 8
+    query heads a KV head the rotated query is used to twice its type's digits instead of rounded
+    to it. A rotary_dim below head_dim makes the two calls.
     """
     _require_gpu(query, "query")
     _require_gpu(k_cache, "k_cache")

@@ -539,6 +539,7 @@ struct RopeArgs {
   const int32_t* pos;
   int max_pos;
   int pos_add;  // added to pos[b] (-1: pos are context lengths that count the new token)
+  int split;    // keep what rounding the rotated query leaves (SplitParams::rope_split)
 };
 
 // Which partials kernel a call takes (kind as the workspace header records it: 1 stream-K,
@@ -706,6 +707,7 @@ int partials_impl(const void* query, const void* k_cache, const void* v_cache,
   p.rope_pos = rope.pos;
   p.rope_max_pos = rope.max_pos;
   p.rope_pos_add = rope.pos_add;
+  p.rope_split = rope.split;
   p.out = nullptr;
   p.tickets = nullptr;
   p.k_new = nullptr;
@@ -1679,7 +1681,7 @@ int msattn_paged_attention_append_rope(
   if (gx >= (int64_t(1) << 31) || batch > 65535) return MSATTN_ERR_UNSUPPORTED;
   // Without positions of its own the new token sits where the cache has it, at length - 1.
   const RopeArgs rope{rope_cos, rope_sin, position ? position : context_lens, max_position,
-                      position ? 0 : -1};
+                      position ? 0 : -1, 1};
   const bool fused = kFusedAppend && append_built(plan, q_dtype, kv_dtype) && aligned(k_new, 16) &&
                      aligned(v_new, 16);
   if (!fused) {  // the write, then the decode (the same result)

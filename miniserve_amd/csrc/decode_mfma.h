@@ -605,9 +605,13 @@ __host__ __device__ constexpr int tile_token(int i) {
 // flash_decode_reference (:134-138) keep the rotated query in fp32. That one rounding of
 // the query (relative 2^-9 for bf16) is the only difference. Lanes l and l ^ 32 (the same
 // query row) are both active or both not.
-template <typename T, typename KT, int D>
+// SPLIT (at most 8 query rows a tile): columns 8 .. 15 of the score product, which no row uses,
+// take what the rounding left of rows 0 .. 7 (`rest`), rounded to T in turn, so that column
+// n + 8's score added to column n's (split_score) is that of a query of twice T's digits. Nothing
+// remains of an infinite element.
+template <typename T, typename KT, int D, bool SPLIT = false>
 __device__ __forceinline__ void rope_chunks(typename QChunk<T>::type (&qb)[D / 32], const float* cs,
-                                            const float* sn, int g) {
+                                            const float* sn, int g, bool rest = false) {
   constexpr int JD = D / 32;
   constexpr bool kCross = sizeof(KT) == 1 && D == 64;  // the partner is in the other half-wave
   float q[JD][8];
@@ -649,7 +653,21 @@ __device__ __forceinline__ void rope_chunks(typename QChunk<T>::type (&qb)[D / 3
       o[e] = rope_mix(q[j][e], r, c[e], sv[e]);
     }
     qb[j] = QChunk<T>::pack(o);
+    if constexpr (SPLIT) {
+      if (rest) {
+        float hi[8];
+        QChunk<T>::unpack(qb[j], hi);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fabsf(hi[e]) < INFINITY ? o[e] - hi[e] : 0.0f;
+        qb[j] = QChunk<T>::pack(o);
+      }
+    }
   }
+}
+// Column n's score plus column (n + 8) % 16's (DPP row_ror:8).
+__device__ __forceinline__ void split_score(mf_f32x4& s) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) s[r] += dpp_mov<0x128>(s[r]);
 }
 
 // The new token's key row, held as append chunks of the query type (chunk j of lane group g as
@@ -697,7 +715,8 @@ __device__ __forceinline__ void rope_new_key(const SrcChunk<T> (&kn)[D / 32], co
   }
 }
 
-// APPEND: 1 the fused append, 2 the fused append of a key that is rotated on the way.
+// APPEND: 1 the fused append, 2 the fused append of a key that is rotated on the way (with k_new
+// set) and a rotated query in two parts.
 template <typename T, typename KT, int D, int RT, int W = kMfmaWaves, int WPC = kMfmaWgPerCu,
           int APPEND = 0>
 __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParams p) {
@@ -889,6 +908,7 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
   // This lane's query row n: key range [lo_n, hi_n) and output row.
   int lo_n = 0, hi_n = 0;
   int64_t orow_n = 0;
+  constexpr bool kSplitQ = APPEND == 2 && !kPvMfma && sizeof(T) == 2 && RT <= 8;
   if (n < nrows) {
     const int gr = row0 + n;
     const int i = gr / p.G;
@@ -1036,14 +1056,16 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
   // The query rows (after the first tiles' loads).
   {
     const T* qp = static_cast<const T*>(p.q);
+    const int nq = kSplitQ ? n & 7 : n;  // the query row of the lane's column
+    const int64_t q_row = kSplitQ ? static_cast<int64_t>(b) * p.H + kvh * p.G + row0 + nq : orow_n;
 #pragma unroll
     for (int j = 0; j < JD; ++j) {
       qb[j] = QChunk<T>::zero();
-      if (n < nrows) qb[j] = QChunk<T>::load(qp + orow_n * D + KV::qk_dim0(j, g, JD));
+      if (nq < nrows) qb[j] = QChunk<T>::load(qp + q_row * D + KV::qk_dim0(j, g, JD));
     }
-    if (p.rope_cos != nullptr && n < nrows) {
+    if (p.rope_cos != nullptr && nq < nrows) {
       const int64_t po = static_cast<int64_t>(rope_position(p, b)) * D;
-      rope_chunks<T, KT, D>(qb, p.rope_cos + po, p.rope_sin + po, g);
+      rope_chunks<T, KT, D, kSplitQ>(qb, p.rope_cos + po, p.rope_sin + po, g, n >= 8);
     }
   }
   if constexpr (kAppendTurns) {
@@ -1073,6 +1095,7 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
     mf_f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < JD; ++j) s = Mfma16<T>::mac(KV::operand(kb[j]), qb[j], s);
+    if constexpr (kSplitQ) split_score(s);
     const int t0 = (tw0 + k) * 16;
     const bool hole = base < 0;
     float sc[4];
@@ -1345,10 +1368,11 @@ hipError_t launch_decode_mfma_one(const SplitParams& p_in, hipStream_t stream) {
                                    : static_cast<unsigned>(p.max_parts) * static_cast<unsigned>(p.KVH) *
                                          static_cast<unsigned>(p.rtiles);
   const dim3 grid(gx, 1, p.part_major ? 1u : static_cast<unsigned>(p.batch));
-  // the fused append's instantiation (the host sets k_new only where it is built)
+  // the instantiations of the fused append (the host sets k_new only where it is built) and of the
+  // query in two parts
   if constexpr (sizeof(T) == 2 && RT <= 8) {
-    if (p.k_new != nullptr) {
-      if (p.rope_cos != nullptr)
+    if (p.k_new != nullptr || p.rope_split) {
+      if (p.rope_split)
         hipLaunchKernelGGL((decode_mfma_kernel<T, KT, D, RT, W, WPC, 2>), grid, dim3(W * kWave), 0,
                            stream, p);
       else

@@ -86,7 +86,8 @@ __host__ __device__ constexpr int64_t streamk_pieces(int64_t n_chunks, int64_t n
   return n_chunks + n_segments;
 }
 
-// APPEND: 1 the fused append, 2 the fused append of a key that is rotated on the way.
+// APPEND: 1 the fused append, 2 the fused append of a key that is rotated on the way (with k_new
+// set) and a rotated query in two parts.
 template <typename T, typename KT, int D, int RT, int APPEND = 0>
 __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decode_streamk_kernel(
     const SplitParams p) {
@@ -283,17 +284,19 @@ __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decod
   // The piece's query rows as the MFMA B operand (lane (g, n): row n, chunk j at dim
   // KV::qk_dim0(j, g), the split the K loads use).
   typedef typename QChunk<T>::type qchunk_t;
+  constexpr bool kSplitQ = APPEND == 2 && sizeof(T) == 2 && RT <= 8;
+  const int nq = kSplitQ ? n & 7 : n;  // the query row of the lane's column
   auto load_q = [&](const Piece& pc, qchunk_t (&q)[JD]) __attribute__((always_inline)) {
     const T* qp = static_cast<const T*>(p.q);
-    const int64_t orow_n = static_cast<int64_t>(pc.b) * p.H + pc.kvh * p.G + pc.row0 + n;
+    const int64_t orow_n = static_cast<int64_t>(pc.b) * p.H + pc.kvh * p.G + pc.row0 + nq;
 #pragma unroll
     for (int j = 0; j < JD; ++j) {
       q[j] = QChunk<T>::zero();
-      if (n < pc.nrows) q[j] = QChunk<T>::load(qp + orow_n * D + KV::qk_dim0(j, g, JD));
+      if (nq < pc.nrows) q[j] = QChunk<T>::load(qp + orow_n * D + KV::qk_dim0(j, g, JD));
     }
-    if (p.rope_cos != nullptr && n < pc.nrows) {
+    if (p.rope_cos != nullptr && nq < pc.nrows) {
       const int64_t po = static_cast<int64_t>(rope_position(p, pc.b)) * D;
-      rope_chunks<T, KT, D>(q, p.rope_cos + po, p.rope_sin + po, g);
+      rope_chunks<T, KT, D, kSplitQ>(q, p.rope_cos + po, p.rope_sin + po, g, n >= 8);
     }
   };
 
@@ -306,14 +309,14 @@ __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decod
     // Lanes past the piece's rows load row 0 again: their MFMA columns' scores are
     // replaced by -inf before use (the masking in the tile loop tests n < nrows), and no
     // output or partial row is stored for them.
-    const bool live = n < pc.nrows;
+    const bool live = nq < pc.nrows;
     const int64_t orow_n =
-        static_cast<int64_t>(pc.b) * p.H + pc.kvh * p.G + pc.row0 + (live ? n : 0);
+        static_cast<int64_t>(pc.b) * p.H + pc.kvh * p.G + pc.row0 + (live ? nq : 0);
 #pragma unroll
     for (int j = 0; j < JD; ++j) q[j] = QChunk<T>::load(qp + orow_n * D + KV::qk_dim0(j, g, JD));
     if (p.rope_cos != nullptr && live) {
       const int64_t po = static_cast<int64_t>(rope_position(p, pc.b)) * D;
-      rope_chunks<T, KT, D>(q, p.rope_cos + po, p.rope_sin + po, g);
+      rope_chunks<T, KT, D, kSplitQ>(q, p.rope_cos + po, p.rope_sin + po, g, n >= 8);
     }
   };
   auto table_first = [&](const Piece& pc) -> int64_t __attribute__((always_inline)) {
@@ -367,6 +370,7 @@ __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decod
     const int ctx = s_ctx[pc.b];
     const int t_new = (ctx - 1) / 16;
     app_t = ctx > 0 && t_new >= pc.t_first && t_new < pc.t_first + pc.ntiles ? t_new : -1;
+    if (APPEND == 2 && p.k_new == nullptr) app_t = -1;  // (written before the launch)
     if (app_t < 0) return;
     app_r = (ctx - 1) & 15;
     const int64_t row = (static_cast<int64_t>(pc.b) * p.KVH + pc.kvh) * D;
@@ -471,6 +475,7 @@ __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decod
       mf_f32x4 sv = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < JD; ++j) sv = Mfma16<T>::mac(KV::operand(kb[j]), qb[j], sv);
+      if constexpr (kSplitQ) split_score(sv);
       const int t0 = (cur.t_first + run0 + k) * 16;
       const bool hole = base < 0;
       float sc[4];
@@ -616,17 +621,21 @@ __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decod
 
 template <typename T, typename KT, int D, int RT>
 hipError_t launch_decode_streamk_one(const SplitParams& p, int grid, hipStream_t stream) {
-  // the fused append's instantiation (the host sets k_new only where it is built)
-  if constexpr (sizeof(T) == 2 && sizeof(KT) != 1 && RT <= 8) {
-    if (p.k_new != nullptr) {
-      const dim3 threads(sk_waves(sizeof(KT), sizeof(T)) * kWave);
-      if (p.rope_cos != nullptr)
-        hipLaunchKernelGGL((decode_streamk_kernel<T, KT, D, RT, 2>), dim3(static_cast<unsigned>(grid)),
-                           threads, 0, stream, p);
-      else
+  // the instantiations of the fused append (the host sets k_new only where it is built) and of the
+  // query in two parts
+  if constexpr (sizeof(T) == 2 && RT <= 8) {
+    const dim3 threads(sk_waves(sizeof(KT), sizeof(T)) * kWave);
+    if (p.rope_split) {
+      hipLaunchKernelGGL((decode_streamk_kernel<T, KT, D, RT, 2>), dim3(static_cast<unsigned>(grid)),
+                         threads, 0, stream, p);
+      return hipGetLastError();
+    }
+    if constexpr (sizeof(KT) != 1) {
+      if (p.k_new != nullptr) {
         hipLaunchKernelGGL((decode_streamk_kernel<T, KT, D, RT, 1>), dim3(static_cast<unsigned>(grid)),
                            threads, 0, stream, p);
-      return hipGetLastError();
+        return hipGetLastError();
+      }
     }
   }
   hipLaunchKernelGGL((decode_streamk_kernel<T, KT, D, RT>), dim3(static_cast<unsigned>(grid)),

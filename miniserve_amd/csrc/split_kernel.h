@@ -104,6 +104,9 @@ struct SplitParams {
   const int32_t* rope_pos;
   int rope_max_pos;
   int rope_pos_add;  // added to rope_pos[b] (-1: rope_pos are context lengths after an append)
+  // Keep what rounding the rotated query to its type leaves (an append with rotation): the
+  // matrix-core kernels of a 2-byte query at up to 8 query rows a tile, and the generic kernel.
+  int rope_split;
   // In-kernel merge (partition MFMA kernel only): non-null `out` [rows][D] of the query
   // type makes the last partition of each (sequence, KV head, row tile) to arrive merge
   // its partials and write the output; `tickets` are the header's arrival counters.
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(kSplitThreads) void split_kernel(const SplitParams 
         float qv[EPL];
 #pragma unroll
         for (int e = 0; e < EPL; ++e) qv[e] = (!ELEM || e < c_valid) ? Elt<QT>::load(src + e) : 0.0f;
-        if (p.rope_cos != nullptr) {  // rotate-half RoPE, rounded back to QT
+        if (p.rope_cos != nullptr) {  // rotate-half RoPE, rounded back to QT (rope_split: kept)
           const int64_t po = static_cast<int64_t>(rope_position(p, b)) * HD;
 #pragma unroll
           for (int e = 0; e < EPL; ++e) {
@@ -308,8 +311,9 @@ __global__ __launch_bounds__(kSplitThreads) void split_kernel(const SplitParams 
             const bool lo_half = d < HD / 2;
             const float partner =
                 Elt<QT>::load(qp + orow[r] * HD + (lo_half ? d + HD / 2 : d - HD / 2));
-            qv[e] = round_to<QT>(rope_mix(qv[e], lo_half ? -partner : partner, p.rope_cos[po + d],
-                                          p.rope_sin[po + d]));
+            const float x = rope_mix(qv[e], lo_half ? -partner : partner, p.rope_cos[po + d],
+                                     p.rope_sin[po + d]);
+            qv[e] = p.rope_split ? x : round_to<QT>(x);
           }
         }
 #pragma unroll
