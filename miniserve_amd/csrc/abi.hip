@@ -1743,9 +1743,12 @@ SharedLayout shared_layout(int batch, int q_len, int num_heads, int head_dim) {
 
 // Whether the kernel takes a geometry (types and alignment aside): its plan holds kShMaxBatch rows,
 // and rows of more than kShMaxQueryRows query rows a KV head read their keys once for so many
-// queries that the prefill kernels' products, not the reads, set the time.
+// queries that the prefill kernels' products, not the reads, set the time. (16 rows in 2 groups,
+// prefixes of 2048 to 4096 and up to 512 own keys, this kernel against those: H32/KVH8 of 128 dims
+// at 32 query rows 53 and 105 us, at 64 70 and 73, at 96 76 and 67, at 128 92 and 66; over fp8 at
+// 64 70 and 78, at 128 114 and 82; H14/KVH2 of 64 at 56 28 and 44, at 112 35 and 29.)
 #ifndef MSATTN_SHARED_MAX_QUERY_ROWS
-#define MSATTN_SHARED_MAX_QUERY_ROWS 128
+#define MSATTN_SHARED_MAX_QUERY_ROWS 64
 #endif
 constexpr int64_t kShMaxQueryRows = MSATTN_SHARED_MAX_QUERY_ROWS;
 bool shared_geometry_ok(int batch, int q_len, int num_heads, int num_kv_heads, int head_dim,

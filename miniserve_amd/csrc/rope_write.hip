@@ -24,8 +24,10 @@ namespace msattn {
 
 constexpr int kRwThreads = 256;
 constexpr int kRwWaves = kRwThreads / kWave;
-// Rows a lane has in flight: 4 x 2 loads of 16 bytes.
-constexpr int kRwUnroll = 4;
+// Rows a lane has in flight: 2 x 2 loads of 16 bytes. (More cost resident waves: whole prompts,
+// 4 x 8191 tokens of 32 + 2 x 8 heads of 128 from bf16 into an fp8 cache, 746 MB, took 144 us
+// with 1 or 2 rows, 150 with 4, 163 with 6; stores past the caches 147, and fp32 ones 20 % more.)
+constexpr int kRwUnroll = 2;
 
 struct RwToken {
   int b, t;
@@ -35,7 +37,9 @@ struct RwToken {
 
 __device__ __forceinline__ RwToken rw_token(const RopeWriteParams& p, int64_t token) {
   RwToken k;
-  k.b = static_cast<int>(token / p.tokens);
+  // (a batch's tokens fit 31 bits in every call but the largest: the short division)
+  k.b = token < (int64_t(1) << 31) ? static_cast<int>(static_cast<uint32_t>(token) / static_cast<uint32_t>(p.tokens))
+                                   : static_cast<int>(token / p.tokens);
   k.t = static_cast<int>(token - static_cast<int64_t>(k.b) * p.tokens);
   const int64_t pos = static_cast<int64_t>(p.starts[k.b]) + p.start_offset + k.t;
   int64_t rp = pos;
@@ -117,10 +121,10 @@ __global__ __launch_bounds__(kRwThreads) void rope_write_vec_kernel(const RopeWr
   const ST* const ks = static_cast<const ST*>(p.k) + k.b * p.k_src[0] + k.t * p.k_src[1];
   const ST* const vs = static_cast<const ST*>(p.v) + k.b * p.v_src[0] + k.t * p.v_src[1];
   ST* const qd = static_cast<ST*>(p.q_out) + k.b * p.q_dst[0] + k.t * p.q_dst[1];
-  // Rows 0 .. QH - 1 are query heads, then KVH key heads, then KVH value heads; nothing of the
-  // keys and values is read where their page is a hole.
+  // Rows 0 .. QH - 1 are query heads, then KVH key heads, then KVH value heads (read before the
+  // page is known, not written where it is a hole).
   const int QH = p.QH;
-  const int rows = k.cache_off >= 0 ? QH + 2 * p.KVH : QH;
+  const int rows = QH + 2 * p.KVH;
   const int step = heads * p.slices;
   for (int r0 = slice * heads + hl; r0 < rows; r0 += step * kRwUnroll) {
     RwBytes<E * sizeof(ST)> x0[kRwUnroll], x1[kRwUnroll];
@@ -138,7 +142,7 @@ __global__ __launch_bounds__(kRwThreads) void rope_write_vec_kernel(const RopeWr
 #pragma unroll
     for (int u = 0; u < kRwUnroll; ++u) {
       const int r = r0 + u * step;
-      if (r >= rows) continue;
+      if (r >= (k.cache_off >= 0 ? rows : QH)) continue;
       const bool value = r >= QH + p.KVH;
       if (value && std::is_same<ST, KT>::value) {  // the bits as they are
         ST* const d = static_cast<ST*>(p.v_cache) + k.cache_off + (r - QH - p.KVH) * p.head_stride;

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
   __shared__ __attribute__((aligned(256))) char s_tile[kShSlots * 2 * kShHalf];
   __shared__ int s_cum[2 * kShMaxBatch + 1];  // tiles before each segment: groups, then rows
   __shared__ int s_g0[kShMaxBatch + 1];       // a group's first row
-  __shared__ int s_hi[kShMaxBatch];           // a group's last visible prefix key + 1
+  __shared__ int s_hi[kShMaxBatch];           // a group's prefix keys, 0 if no row reads them
   __shared__ int s_len[kShMaxBatch];
   __shared__ int s_own[kShMaxBatch];          // where a row's own keys begin
   __shared__ short s_grp[kShMaxBatch];        // a row's group, or -1
@@ -236,12 +236,14 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
       if (s_g0[mid] <= b) lo = mid; else hi = mid;
     }
     int own = 0, grp = -1;
-    // (a group of one row has nothing to share: its prefix is the row's own)
+    // (A group of one row has nothing to share: its prefix is the row's own. So is that of a row
+    // whose queries do not all see it whole: what the others read past it, NaN perhaps, would
+    // enter this row's sums with a weight of zero.)
     const int g0 = s_g0[lo], g1 = s_g0[lo + 1];
-    if (!descend && g0 <= b && b < g1 && g1 - g0 > 1) {
+    if (!descend && g0 <= b && b < g1 && g1 - g0 > 1 && s_len[b] - p.q_len >= s_cum[lo] - 1) {
       own = s_cum[lo];
       grp = lo;
-      atomicMax(&s_hi[lo], min(own, s_len[b]));
+      s_hi[lo] = own;  // (every member's is the same)
     }
     s_own[b] = own;
     s_grp[b] = static_cast<short>(grp);
@@ -727,7 +729,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
 
 // Joins a row's pieces: one wave a query row, D / 64 dims a lane. Its pieces: for the group's
 // segment (if the row has one) and for its own, the unit's first piece, then those of the shares
-// that the unit runs on into. What few calls take (two pieces of each) is read at once.
+// that the unit runs on into. A lane finds one piece each and its weight; the accumulators follow.
 constexpr int kShMergeThreads = 256;
 constexpr int kShMergeWaves = kShMergeThreads / kWave;
 template <typename T, int D, int EB>
@@ -747,9 +749,13 @@ __global__ __launch_bounds__(kShMergeThreads) void shared_merge_kernel(const Sha
   const int r0 = i * p.G + h - kvh * p.G;
   const int RPS = p.q_len * p.G;
   const ShPlanRow e = reinterpret_cast<const ShPlanRow*>(p.plan + kShPlanRows)[b];
-  // A unit's pieces: the first at the row's own place, the others at shares' places.
+  // A unit's pieces: the first at the row's own place, the others at the places of the shares up to
+  // the last tile's one (but for shares so small that they hold no tile of the unit).
   struct Unit {
-    int begin, tile, last, r, share;  // its cost, a tile's, the last tile, the row in it, the share
+    int begin, tile, last, r, share, pieces;  // its cost, a tile's, the last tile, the row in it,
+  };                                          // the first tile's share, shares to the last's
+  const auto share_of = [&](int cost) {
+    return static_cast<int>(static_cast<uint32_t>(cost) / static_cast<uint32_t>(per));
   };
   const auto unit = [&](int cost, int blocks, int r, int members) __attribute__((always_inline)) {
     const int step = Cost::block(members * RPS);
@@ -759,68 +765,69 @@ __global__ __launch_bounds__(kShMergeThreads) void shared_merge_kernel(const Sha
     u.tile = TB * step;
     u.last = (blocks - 1) / TB;
     u.r = r % kShRows;
-    u.share = blocks > 0 ? static_cast<int>(static_cast<uint32_t>(u.begin) / static_cast<uint32_t>(per))
-                         : -1;
+    u.share = share_of(u.begin);
+    u.pieces = blocks <= 0 ? 0
+               : u.last == 0 ? 1
+                             : share_of(u.begin + Cost::kPiece + u.last * u.tile) - u.share + 1;
     return u;
   };
-  // The place of the unit's next piece, in the share of its first tile past the last one's; -1: none.
-  const auto next = [&](Unit& u) __attribute__((always_inline)) -> int64_t {
-    if (u.share < 0) return -1;
-    const int past = (u.share + 1) * per - u.begin - Cost::kPiece;
-    const int t = past <= u.tile ? 1 : ceil_div(past, u.tile);
-    u.share = t > u.last ? -1
-                         : static_cast<int>(static_cast<uint32_t>(u.begin + Cost::kPiece + t * u.tile) /
-                                            static_cast<uint32_t>(per));
-    return u.share < 0 ? -1 : 2 * p.rows + static_cast<int64_t>(u.share) * kShRows + u.r;
-  };
-  Unit group = unit(e.cost, e.blocks, (b - e.first) * RPS + r0, e.members);
-  Unit own = unit(e.own_cost, e.own_blocks, r0, 1);
+  const Unit group = unit(e.cost, e.blocks, (b - e.first) * RPS + r0, e.members);
+  const Unit own = unit(e.own_cost, e.own_blocks, r0, 1);
   float M = -INFINITY, L = 0.0f;
   float o[DPL];
 #pragma unroll
   for (int d = 0; d < DPL; ++d) o[d] = 0.0f;
-  int64_t at[4] = {group.share < 0 ? -1 : row, own.share < 0 ? -1 : p.rows + row, next(group), next(own)};
 #pragma unroll 1
-  for (;;) {
-    float2 ml[4];
-    float a[4][DPL];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {  // (place 0 in an absent one's stead)
-      const int64_t s = at[k] < 0 ? 0 : at[k];
-      ml[k] = *reinterpret_cast<const float2*>(p.ml + 2 * s);
-#pragma unroll
-      for (int d = 0; d < DPL; ++d) a[k][d] = p.acc[s * D + DPL * lane + d];
-    }
-#if defined(__HIP_DEVICE_COMPILE__)
-    // (all on their way before the first is used)
-    if constexpr (DPL == 2)
-      asm volatile("" : "+v"(a[0][0]), "+v"(a[1][0]), "+v"(a[2][0]), "+v"(a[3][0]),
-                        "+v"(a[0][1]), "+v"(a[1][1]), "+v"(a[2][1]), "+v"(a[3][1]));
-    else
-      asm volatile("" : "+v"(a[0][0]), "+v"(a[1][0]), "+v"(a[2][0]), "+v"(a[3][0]));
-#endif
-    float Mn = M;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) Mn = at[k] < 0 ? Mn : fmaxf(Mn, ml[k].x);
-    const bool some = Mn != -INFINITY;
-    const float w0 = some ? __builtin_amdgcn_exp2f(M - Mn) : 1.0f;
-    L *= w0;
+  for (int base = 0; base < group.pieces + own.pieces; base += kWave) {
+    // a lane a piece: its place, its maximum and its weight
+    const bool first = base + lane < group.pieces;
+    const int k = base + lane - (first ? 0 : group.pieces);
+    const int begin = first ? group.begin : own.begin, tile = first ? group.tile : own.tile;
+    const int share = (first ? group.share : own.share) + k;
+    const int past = share * per - begin - Cost::kPiece;  // the share's first tile
+    const int t = past <= tile ? 1
+                               : static_cast<int>(static_cast<uint32_t>(past + tile - 1) /
+                                                  static_cast<uint32_t>(tile));
+    const bool on = first || k < own.pieces;
+    const bool holds = k == 0 || (t <= (first ? group.last : own.last) &&
+                                  begin + Cost::kPiece + t * tile < (share + 1) * per);
+    const int64_t place =
+        !(on && holds) ? 0
+        : k == 0       ? (first ? row : p.rows + row)
+                       : 2 * p.rows + static_cast<int64_t>(share) * kShRows + (first ? group.r : own.r);
+    const float2 ml = *reinterpret_cast<const float2*>(p.ml + 2 * place);
+    uint64_t mask = __ballot(on && holds);
+    float mx = on && holds ? ml.x : -INFINITY;
+    mx = fmaxf(M, group_max<kWave>(mx));
+    const bool some = mx != -INFINITY;
+    const float w = !(on && holds) ? 0.0f : (some ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.0f);
+    const float w0 = some ? __builtin_amdgcn_exp2f(M - mx) : 1.0f;
+    L = fmaf(L, w0, group_sum<kWave>(on && holds ? ml.y * w : 0.0f));
+    M = mx;
 #pragma unroll
     for (int d = 0; d < DPL; ++d) o[d] *= w0;
+#pragma unroll 1
+    while (mask != 0) {  // the pieces' accumulators, eight on their way at once
+      constexpr int N = 8;
+      float a[N][DPL], wk[N];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (at[k] >= 0) {
-        const float w = some ? __builtin_amdgcn_exp2f(ml[k].x - Mn) : 0.0f;
-        L = fmaf(ml[k].y, w, L);
+      for (int i = 0; i < N; ++i) {
+        const bool have = mask != 0;
+        const int l = have ? __builtin_ctzll(mask) : 0;
+        mask &= mask - 1;
+        const int64_t at = have ? static_cast<int64_t>(
+            static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place >> 32), l))) << 32 |
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(place), l))) : 0;
+        wk[i] = have ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), l)) : 0.0f;
+        const float* const src = p.acc + at * D + DPL * lane;
 #pragma unroll
-        for (int d = 0; d < DPL; ++d) o[d] = fmaf(a[k][d], w, o[d]);
+        for (int d = 0; d < DPL; ++d) a[i][d] = have ? src[d] : 0.0f;
       }
-    M = Mn;
-    if (group.share < 0 && own.share < 0) break;
-    at[0] = next(group);
-    at[1] = next(own);
-    at[2] = next(group);
-    at[3] = next(own);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) o[d] = fmaf(a[i][d], wk[i], o[d]);
+    }
   }
   const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
   T* const out = static_cast<T*>(p.out) + row * D + DPL * lane;

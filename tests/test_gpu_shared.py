@@ -242,6 +242,25 @@ def test_infinities_and_nan(device):
     assert bool(nan[3, 0, 1].all()) and not bool(nan[3, 0, [0, 2, 3]].any())
 
 
+@pytest.mark.parametrize("q_len,short", [(1, 40), (1, 63), (3, 65), (3, 40), (4, 2)])
+def test_rows_that_do_not_see_the_whole_prefix(device, q_len, short):
+    """A key and a value of NaN and an infinite one where only the other rows of the group see them
+    leave no trace in the short row, which is as exact as ever."""
+    x = Batch(4, 2, 128, BF16, BF16, [(0, 4, 4)], [100, short, 80, 120], q_len)
+    clean = x.call().float().cpu()
+    x.check(clean)
+    # positions that none of the short row's queries but its last may see
+    for pos, t, bad in ((max(short, 50), x.vc, math.nan), (max(short, 51), x.vc, math.inf),
+                        (max(short, 52), x.kc, math.nan)):
+        if pos < 64:
+            t[x.table[0, pos // 16], pos % 16] = bad
+    note(f"short row {short}, {q_len} queries")
+    out = x.call().float().cpu()
+    assert torch.equal(out[1], clean[1])
+    if short < 64:
+        assert bool(out[[0, 2, 3]].isnan().all())
+
+
 # Calls that the kernel does not take run paged_attention: bit for bit its result.
 @pytest.mark.parametrize("name,H,KVH,D,qt,kt,bs,q_len", [
     ("fp32 query", 8, 2, 64, F32, F32, 16, 1), ("fp32 cache", 8, 2, 64, BF16, F32, 16, 1),
