@@ -514,7 +514,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
         // (blocks past every row's last key, and a wave without rows, have nothing to do)
         const int blocks = min(TK / 32, (wave_any - c.tok + 31) >> 5);
 #pragma unroll 1
-        for (int kb = ks; kb < blocks; kb += KS) {
+        for (int kb = ks < KS ? ks : blocks; kb < blocks; kb += KS) {
           const int key = c.tok + 32 * kb;
           const int live = (live4 >> (8 * (2 * kb / SUB) + 2 * kb % SUB)) & 3;
           char* const kv = base + kb * 32 * ROW;
@@ -642,7 +642,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
         // Waves that split the keys put theirs into the slot: row rr of key wave ks at row
         // 16 RW ks + rr, its 16-byte chunk j at chunk j ^ n (the lanes of a set hold 16 rows).
         const int at = 16 * RW * ks + rr;
-        if (rr < c.rows()) {
+        if (rr < c.rows() && ks < KS) {
 #pragma unroll
           for (int u = 0; u < ND; ++u)
             *reinterpret_cast<float4*>(f + at * D + 4 * ((4 * u + g) ^ n)) =
@@ -707,7 +707,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
         unit_first = (nx.bits >> 11) & 1;
         RW = nx.row_waves();
         rw = cw & (RW - 1);
-        KS = kShComp / RW;
+        KS = min(kShComp / RW, TK / 32);  // (waves ks >= KS have no block)
         ks = cw / RW;
         orow = n_row;
         hi_n = n_hi;
