@@ -573,29 +573,31 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
 #pragma unroll
           for (int r = 1; r < 4; ++r) mt = fmaxf(mt, fmaxf(s[0][r], s[1][r]));
           mt = rows4_max(mt);
-          const float m_new = fmaxf(m_run, mt * scale);
-          const bool some = m_new != -INFINITY;
-          const float alpha = some ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
-          const float m_use = some ? m_new : 0.0f;
+          // The running maximum moves, and what was summed is rescaled, only where a row's grew by
+          // more than 8: weights reach 2^8 at most, and 32 products a block are mostly saved.
+          mt *= scale;
+          if (__any(mt > m_run + 8.0f)) {
+            const float m_new = fmaxf(m_run, mt);
+            const float alpha = m_new != -INFINITY ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int u = 0; u < ND; ++u) acc[u] *= alpha;
+          }
+          const float m_use = m_run != -INFINITY ? m_run : 0.0f;
           float pr[8];  // (masked scores weigh 2^-inf = 0, NaN stays NaN)
 #pragma unroll
           for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               pr[4 * k + r] = __builtin_amdgcn_exp2f(fmaf(s[k][r], scale, -m_use));
-          // The weights are rounded to the query type for the matrix cores (half a step of it,
-          // at most 1); l sums the rounded ones, so that the weights used still sum to one.
+          // The weights are rounded to the query type for the matrix cores (half a step of it); l
+          // sums the rounded ones, so that the weights used still sum to one.
           const uint4 pb = make_uint4(Pack2<T>::pack(pr[0], pr[1]), Pack2<T>::pack(pr[2], pr[3]),
                                       Pack2<T>::pack(pr[4], pr[5]), Pack2<T>::pack(pr[6], pr[7]));
           const uint32_t one2 = Pack2<T>::pack(1.0f, 1.0f);
-          l_run = fmaf(l_run, alpha,
-                       Dot2<T>::dot(pb.w, one2, Dot2<T>::dot(pb.z, one2, 0.0f)) +
-                           Dot2<T>::dot(pb.y, one2, Dot2<T>::dot(pb.x, one2, 0.0f)));
-          m_run = m_new;
-          if (__any(alpha != 1.0f)) {
-#pragma unroll
-            for (int u = 0; u < ND; ++u) acc[u] *= alpha;
-          }
+          l_run += Dot2<T>::dot(pb.w, one2, Dot2<T>::dot(pb.z, one2, 0.0f)) +
+                   Dot2<T>::dot(pb.y, one2, Dot2<T>::dot(pb.x, one2, 0.0f));
 #pragma unroll
           for (int u = 0; u < ND; ++u) acc[u] = Mfma16<T>::mac(KV::operand(vv[u]), pb, acc[u]);
         }
