@@ -95,7 +95,7 @@ def _worth_in_place(t: torch.Tensor) -> bool:
 
 
 def _require_gpu(t: torch.Tensor, what: str) -> None:
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(
             f"msattn needs ROCm GPU tensors: {what} is on {t.device} (there is no CPU path)")
 
@@ -154,9 +154,12 @@ def _host_ints_to_device(values: list[int], device: torch.device) -> torch.Tenso
 def context_lens_i32(context_lens, device: torch.device, batch: int) -> tuple[torch.Tensor, int | None]:
     """(int32 [batch] device tensor, host-known max or None) for context_lens."""
     if isinstance(context_lens, torch.Tensor):
-        lens = context_lens.reshape(-1)
-        host_max = int(lens.max()) if (lens.device.type == "cpu" and lens.numel()) else None
-        lens = lens.to(device=device, dtype=torch.int32).contiguous()
+        lens = context_lens if context_lens.ndim == 1 else context_lens.reshape(-1)
+        host_max = int(lens.max()) if (not lens.is_cuda and lens.device.type == "cpu" and
+                                       lens.numel()) else None
+        if lens.dtype != torch.int32 or lens.device != device:
+            lens = lens.to(device=device, dtype=torch.int32)
+        lens = lens.contiguous()
     else:
         values = [int(x) for x in context_lens]
         host_max = max(values) if values else 0
@@ -170,7 +173,9 @@ def starts_i32(start, batch: int, device: torch.device) -> torch.Tensor:
     """int32 device tensor of each row's first position: an int, one entry per row (at least),
     or an int tensor."""
     if isinstance(start, torch.Tensor):
-        starts = start.reshape(-1).to(device=device, dtype=torch.int32)
+        starts = start if start.ndim == 1 else start.reshape(-1)
+        if starts.dtype != torch.int32 or starts.device != device:
+            starts = starts.to(device=device, dtype=torch.int32)
     elif isinstance(start, Sequence):
         starts = _host_ints_to_device([int(s) for s in start], device)
     else:

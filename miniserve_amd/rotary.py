@@ -15,6 +15,7 @@ import torch
 from . import _native as nat
 
 _I64x3 = ctypes.c_int64 * 3
+_SOURCES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def on_device(dev: torch.device, fn, *args) -> int:
@@ -31,7 +32,7 @@ def rope_table(t, dev: torch.device, what: str) -> torch.Tensor:
         t = torch.as_tensor(t, device=dev).to(torch.float32)
     if t.ndim != 2 or t.shape[0] < 1:
         raise ValueError(f"{what} must be [max_pos, dims] with at least one position")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def extent(t: torch.Tensor) -> tuple[int, int]:
@@ -41,7 +42,12 @@ def extent(t: torch.Tensor) -> tuple[int, int]:
         return lo, lo + t.nbytes
     if t.numel() == 0:
         return lo, lo
-    return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    if t.ndim == 4:
+        (a, b, c, d), (sa, sb, sc, sd) = t.shape, t.stride()
+        last = (a - 1) * sa + (b - 1) * sb + (c - 1) * sc + (d - 1) * sd
+    else:
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return lo, lo + (last + 1) * t.element_size()
 
 
 def _rows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -104,39 +110,44 @@ def write_kv_rope(query: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     itself (rotated in place). Two tokens of one call that land in one cache slot leave either's
     row there.
     """
-    from .attention import _require_gpu, block_table_i32, starts_i32
-
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k", k), ("v", v)):
-        _require_gpu(t, name)
+    if not (k_cache.is_cuda and v_cache.is_cuda and k.is_cuda and v.is_cuda):
+        for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k", k), ("v", v)):
+            _att._require_gpu(t, name)
     if k.ndim != 4 or k.shape != v.shape:
         raise ValueError("k and v must both be [batch, tokens, kv_heads, head_dim]")
+    cache_stride = k_cache.stride()
     if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype or \
-            k_cache.stride() != v_cache.stride():
+            cache_stride != v_cache.stride():
         raise ValueError("k_cache and v_cache must share a [num_blocks, block_size, kv_heads, "
                          "head_dim] shape, dtype and strides")
     B, T, KVH, D = k.shape
-    nb, bs = k_cache.shape[:2]
-    if k_cache.shape[2] != KVH or k_cache.shape[3] != D:
+    nb, bs, cache_heads, cache_dim = k_cache.shape
+    if cache_heads != KVH or cache_dim != D:
         raise ValueError("k/v heads or head_dim do not match the cache")
-    if k_cache.stride(3) != 1:
+    if cache_stride[3] != 1:
         raise ValueError("cache head_dim must be contiguous")
     if D > nat.MAX_HEAD_DIM:
         raise ValueError(f"head_dim {D}: the kernels take head sizes up to {nat.MAX_HEAD_DIM}")
-    dev = k_cache.device
+    dev, dtype = k_cache.device, k.dtype
     if query is None:
         if out is not None:
             raise ValueError("out holds rotated queries: it needs a query")
     else:
-        _require_gpu(query, "query")
-        if query.ndim != 4 or query.shape[:2] != k.shape[:2] or query.shape[3] != D or \
-                query.shape[2] == 0:
+        if not query.is_cuda:
+            _att._require_gpu(query, "query")
+        if query.ndim != 4:
             raise ValueError("query must be [batch, tokens, heads, head_dim] beside k and v")
-    for name, t in (("v", v), ("query", query)):
-        if t is not None and t.dtype != k.dtype:
-            raise ValueError(f"{name} must have k's dtype")
-    if k.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-        raise ValueError(f"unsupported dtype for a rotation: {k.dtype}")
-    if any(t is not None and t.device != dev for t in (v_cache, k, v, query, out)):
+        qB, qT, H, qD = query.shape
+        if qB != B or qT != T or qD != D or H == 0:
+            raise ValueError("query must be [batch, tokens, heads, head_dim] beside k and v")
+        if query.dtype != dtype:
+            raise ValueError("query must have k's dtype")
+    if v.dtype != dtype:
+        raise ValueError("v must have k's dtype")
+    if dtype not in _SOURCES:
+        raise ValueError(f"unsupported dtype for a rotation: {dtype}")
+    if v_cache.device != dev or k.device != dev or v.device != dev or \
+            query is not None and query.device != dev or out is not None and out.device != dev:
         raise ValueError("query, k, v, out and the caches must be on one device")
     cos, sin = rope_table(cos, dev, "cos"), rope_table(sin, dev, "sin")
     R = cos.shape[1]
@@ -150,12 +161,12 @@ def write_kv_rope(query: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
                          "no element twice")
     if B == 0 or T == 0 or KVH == 0 or nb == 0:
         return None if query is None else _rest(query, out)
-    table = block_table_i32(block_table, dev)
+    table = _att.block_table_i32(block_table, dev)
     if table.shape[0] < B:
         raise ValueError("block_table has fewer rows than k")
     if table.shape[1] == 0:
         raise ValueError("block_table has no columns")
-    starts = starts_i32(start, B, dev)
+    starts = _att.starts_i32(start, B, dev)
     pos, per_token = None, 0
     if position is not None:
         pos = torch.as_tensor(position, device=dev).to(torch.int32)
@@ -169,7 +180,7 @@ def write_kv_rope(query: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     written = _spans((k_cache, v_cache))
     if query is not None:
         if out is None:
-            out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+            out = torch.empty((B, T, H, D), dtype=dtype, device=dev)
             q = _source(query, written)
         else:
             if not _clear(out, written):
@@ -178,15 +189,15 @@ def write_kv_rope(query: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
             in_place = out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
             q = query if in_place and not query.is_neg() else _source(query, written)
         q_args = (q.data_ptr(), _I64x3(*q.stride()[:3]), out.data_ptr(),
-                  _I64x3(*out.stride()[:3]), query.shape[2])
+                  _I64x3(*out.stride()[:3]), H)
     ks, vs = _source(k, written), _source(v, written)
     status = on_device(
         dev, nat.lib().msattn_write_kv_rope, *q_args[:4], ks.data_ptr(), _I64x3(*ks.stride()[:3]),
         vs.data_ptr(), _I64x3(*vs.stride()[:3]), k_cache.data_ptr(), v_cache.data_ptr(),
-        k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), table.data_ptr(),
+        cache_stride[0], cache_stride[1], cache_stride[2], table.data_ptr(),
         starts.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-        pos.data_ptr() if pos is not None else None, per_token, cos.shape[0], R, B, T, q_args[4],
-        KVH, D, bs, nb, table.shape[1], nat.dtype_code(k.dtype), nat.dtype_code(k_cache.dtype))
+        None if pos is None else pos.data_ptr(), per_token, cos.shape[0], R, B, T, q_args[4],
+        KVH, D, bs, nb, table.shape[1], nat.dtype_code(dtype), nat.dtype_code(k_cache.dtype))
     nat.check("msattn_write_kv_rope", status)
     return out
 
@@ -196,3 +207,6 @@ def _rest(query: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     if query.numel():
         raise ValueError("a query needs keys and values beside it")
     return torch.empty(query.shape, dtype=query.dtype, device=query.device) if out is None else out
+
+
+from . import attention as _att  # noqa: E402  (which imports this module's names)

@@ -25,7 +25,8 @@ def _groups_i32(group_rows, prefix_pages, batch: int, width: int, dev: torch.dev
         if isinstance(x, torch.Tensor) and x.device == dev:
             if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool:
                 raise ValueError(f"{name} must hold whole numbers")
-            out.append(x.reshape(-1).to(torch.int32).contiguous())
+            x = x if x.ndim == 1 else x.reshape(-1)
+            out.append((x if x.dtype == torch.int32 else x.to(torch.int32)).contiguous())
             continue
         values = [int(v) for v in (x.reshape(-1).tolist() if isinstance(x, torch.Tensor) else x)]
         if name == "group_rows":
