@@ -628,6 +628,19 @@ bool append_built(const PartialsPlan& plan, int q_dtype, int kv_dtype) {
   return (q_dtype == MSATTN_BF16 || q_dtype == MSATTN_F16) && plan.RT <= 8 &&
          (plan.kind == 2 || (plan.kind == 1 && kv_dtype != MSATTN_FP8_E4M3));
 }
+// The same with a rotation on the way: the partition kernel for an fp32 query as well (one launch
+// of the two saved, 4 short sequences of H14/KVH2/D64 18.7 -> 15.5 us a call). Over an fp32 cache
+// at head_dim 128 and up to 4 rows a tile its registers leave one workgroup to a CU: only where no
+// more are launched, below 2^15 tokens of table times KV heads and sequences (H8/KVH8, one
+// launch against two: 1 x 2048 tokens 15.9 and 19.1 us, 2 x 2048 23.8 and 22.4, 4 x 512 11.7 and
+// 14.6, 8 x 512 19.5 and 17.5; H8/KVH2 4 x 2048 15.4 and 18.6, 8 x 2048 23.2 and 21.4).
+bool append_rope_built(const PartialsPlan& plan, int q_dtype, int kv_dtype, int head_dim, int batch,
+                       int num_kv_heads, int max_context) {
+  if (append_built(plan, q_dtype, kv_dtype)) return true;
+  if (q_dtype != MSATTN_F32 || plan.RT > 8 || plan.kind != 2) return false;
+  return kv_dtype != MSATTN_F32 || head_dim <= 64 || plan.RT == 8 ||
+         static_cast<int64_t>(batch) * num_kv_heads * max_context < (1 << 15);
+}
 
 int partials_impl(const void* query, const void* k_cache, const void* v_cache,
                   int64_t cache_block_stride, int64_t cache_slot_stride,
@@ -663,7 +676,11 @@ int partials_impl(const void* query, const void* k_cache, const void* v_cache,
                     batch, q_len, num_heads, num_kv_heads, max_context, fused_out != nullptr,
                     key_lo, window);
   // (a kernel without the append would leave the new token out of the cache and the output)
-  if (k_new != nullptr && !append_built(plan, q_dtype, kv_dtype)) return MSATTN_ERR_UNSUPPORTED;
+  if (k_new != nullptr &&
+      !(rope.cos != nullptr ? append_rope_built(plan, q_dtype, kv_dtype, head_dim, batch,
+                                                num_kv_heads, max_context)
+                            : append_built(plan, q_dtype, kv_dtype)))
+    return MSATTN_ERR_UNSUPPORTED;
   const bool use_mfma = plan.use_mfma;
   const int RT = plan.RT;
   char* ws = static_cast<char*>(workspace);
@@ -1682,8 +1699,9 @@ int msattn_paged_attention_append_rope(
   // Without positions of its own the new token sits where the cache has it, at length - 1.
   const RopeArgs rope{rope_cos, rope_sin, position ? position : context_lens, max_position,
                       position ? 0 : -1, 1};
-  const bool fused = kFusedAppend && append_built(plan, q_dtype, kv_dtype) && aligned(k_new, 16) &&
-                     aligned(v_new, 16);
+  const bool fused = kFusedAppend && append_rope_built(plan, q_dtype, kv_dtype, head_dim, batch,
+                                                     num_kv_heads, max_context) &&
+                     aligned(k_new, 16) && aligned(v_new, 16);
   if (!fused) {  // the write, then the decode (the same result)
     const int64_t row = head_dim, tok = row * num_kv_heads;
     const int64_t dense[3] = {tok, tok, row};

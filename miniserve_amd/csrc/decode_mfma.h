@@ -679,23 +679,24 @@ __device__ __forceinline__ void rope_new_key(const SrcChunk<T> (&kn)[D / 32], co
                                              const float* sn, int g,
                                              typename Kv8<T, KT>::raw_t (&out)[D / 32]) {
   typedef typename Kv8<T, KT>::raw_t raw_t;
-  static_assert(sizeof(raw_t) == 8 * sizeof(KT) && sizeof(T) == 2, "eight cache elements a chunk");
+  static_assert(sizeof(raw_t) == 8 * sizeof(KT), "eight cache elements a chunk");
   constexpr int JD = D / 32;
   constexpr bool kCross = sizeof(KT) == 1 && D == 64;  // the partner is in the other half-wave
   float k[JD][8], kp[JD][8];
 #pragma unroll
   for (int j = 0; j < JD; ++j) {
-    const uint4 x = __builtin_bit_cast(uint4, kn[j]);
-    Chunk<T>::unpack(x, k[j]);
+    const typename QChunk<T>::type x = __builtin_bit_cast(typename QChunk<T>::type, kn[j]);
+    QChunk<T>::unpack(x, k[j]);
     if constexpr (kCross) {
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-      uint32_t o[4];
+      constexpr int NW = QChunk<T>::kWords;
+      uint32_t w[NW], o[NW];
+      QChunk<T>::words(x, w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < NW; ++i) {
         const auto t = __builtin_amdgcn_permlane32_swap(w[i], w[i], false, false);
         o[i] = g < 2 ? t[1] : t[0];
       }
-      Chunk<T>::unpack(make_uint4(o[0], o[1], o[2], o[3]), kp[j]);
+      QChunk<T>::unpack(QChunk<T>::from_words(o), kp[j]);
     }
   }
 #pragma unroll
@@ -1035,7 +1036,7 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
 
   // The fused append of a rotated key (APPEND 2): the wave whose run holds the new position
   // requests the key beside the query and rotates it after it, at the same row of the tables.
-  constexpr bool kAppendTurns = APPEND == 2 && !kPvMfma && sizeof(T) == 2 && RT <= 8;
+  constexpr bool kAppendTurns = APPEND == 2 && !kPvMfma && RT <= 8;
   const int k_turn = kAppendTurns && ctx > 0 ? (ctx - 1) / 16 - tw0 : -1;
   const bool turn_lane = kAppendTurns && p.k_new != nullptr && k_turn >= 0 && k_turn < nt &&
                          tile_token<D>(n) == ((ctx - 1) & 15);
@@ -1184,9 +1185,10 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
   // this launch reads what msattn_write_kv followed by a decode would read. No other
   // workgroup reads that position (it lies in the last partition), so nothing waits for
   // the store.
-  // (Built as its own instantiation, APPEND, for 2-byte queries at up to 8 rows per tile:
+  // (Built as its own instantiation, APPEND, for 2-byte queries, with a rotation for fp32 ones too,
+  // at up to 8 rows per tile:
   // the chunks held for it take 16-36 registers, which cost the decode without it 0.5-2.6 %.)
-  constexpr bool kAppendOk = APPEND != 0 && !kPvMfma && sizeof(T) == 2 && RT <= 8;
+  constexpr bool kAppendOk = APPEND != 0 && !kPvMfma && RT <= 8;
   const bool app = kAppendOk && p.k_new != nullptr && ctx > 0;
   const int k_app = app ? (ctx - 1) / 16 - tw0 : -1;  // run index of the new token's tile
   const bool app_here = k_app >= 0 && k_app < nt;      // wave-uniform
@@ -1378,6 +1380,13 @@ hipError_t launch_decode_mfma_one(const SplitParams& p_in, hipStream_t stream) {
       else
         hipLaunchKernelGGL((decode_mfma_kernel<T, KT, D, RT, W, WPC, 1>), grid, dim3(W * kWave), 0,
                            stream, p);
+      return hipGetLastError();
+    }
+  }
+  if constexpr (sizeof(T) == 4 && RT <= 8) {
+    if (p.k_new != nullptr) {  // (with a rotation only)
+      hipLaunchKernelGGL((decode_mfma_kernel<T, KT, D, RT, W, WPC, 2>), grid, dim3(W * kWave), 0,
+                         stream, p);
       return hipGetLastError();
     }
   }

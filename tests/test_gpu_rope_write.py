@@ -312,8 +312,14 @@ APPENDS = {
     "bf16 over fp8 D128": (28, 4, 128, BF16, FP8, 8, 96, 0, "partition-fused"),
     "fp16 over fp8 D64": (16, 2, 64, F16, FP8, 8, 64, 0, "partition-fused"),
     "bf16 over fp32": (14, 2, 64, BF16, F32, 16, 64, 0, "partition-fused"),
-    "fp32 (two launches)": (14, 2, 64, F32, F32, 8, 64, 0, "partition-fused"),
-    "fp32 over fp8 (two launches)": (14, 2, 64, F32, FP8, 8, 64, 0, "partition-fused"),
+    "fp32": (14, 2, 64, F32, F32, 8, 64, 0, "partition-fused"),
+    "fp32 over fp8": (14, 2, 64, F32, FP8, 8, 64, 0, "partition-fused"),
+    "fp32 over bf16, D128": (8, 2, 128, F32, BF16, 8, 64, 0, "partition-fused"),
+    "fp32, one query head, D128": (4, 4, 128, F32, F32, 8, 40, 0, "partition-fused"),
+    "fp32, one query head, D128 (two launches)": (8, 8, 128, F32, F32, 8, 64, 0, "partition-fused"),
+    "fp32 over fp16 window": (8, 1, 64, F32, F16, 8, 64, 200, "partition-fused"),
+    "fp32, G16 (two launches)": (32, 2, 128, F32, F32, 8, 64, 0, "partition-fused"),
+    "fp32, stream-K (two launches)": (32, 8, 128, F32, F32, 16, 512, 0, "stream-K"),
     "G16 (two launches)": (32, 2, 128, BF16, BF16, 8, 64, 0, "partition-fused"),
     "stream-K": (32, 8, 128, BF16, BF16, 16, 512, 0, "stream-K"),
     "stream-K, fp8 (two launches)": (32, 8, 128, BF16, FP8, 16, 512, 0, "stream-K"),
@@ -382,7 +388,7 @@ def test_append_rope_against_its_two_calls(device, name, own_positions):
         assert out[0].abs().max() == 0  # the pad row
 
 
-@pytest.mark.parametrize("name", ["C2 geometry bf16", "bf16 over fp8 D128", "fp32 (two launches)",
+@pytest.mark.parametrize("name", ["C2 geometry bf16", "bf16 over fp8 D128", "fp32",
                                   "stream-K", "fp16 over fp8 D64", "head_dim 80 (two launches)",
                                   "stream-K, fp8 (two launches)", "one query head a KV head",
                                   "bf16 over fp32", "stream-K, D64"])
