@@ -12,20 +12,32 @@
 // over the piece's visible keys, and the merge kernel below joins a row's pieces:
 //   out = sum 2^(m - M) acc / sum 2^(m - M) l,   M = max m.
 //
-// A workgroup has four copying and four computing waves, one of each a SIMD. The copying waves
-// bring the share's tiles into two LDS slots with the load unit, one tile ahead of the computation
-// and on across pieces and units, so that the memory pipe does not run dry between them, and keep
-// the page walk out of the computing waves. Those take 32 query rows each, as two sets of 16:
-// scores are S^T = K Q^T on v_mfma_f32_16x16x32, so that lane (g, n) = (l / 16, l % 16) holds row
-// n's scores of keys 4 g .. 4 g + 3 of a 16-key block, and two such blocks, rounded to the query
-// type and packed, are its B operand of O^T += V^T P^T (V^T by transposed LDS reads): softmax and
-// rescaling stay in the lane, and K and V are read from LDS once for 32 rows. A unit of 64 rows or
-// fewer leaves computing waves over, which take every second or fourth 32-key block of the same
-// rows and are joined through LDS at the piece's end.
+// Few query rows wait for the memory pipe, many for the matrix cores and the softmax (a tile of 128
+// rows costs 2 to 4 times one of 8), so the shares are equal in cost, not in tiles (ShCost).
+//
+// A workgroup has four copying waves, one a SIMD, and eight computing ones. The copying waves bring
+// the share's tiles into two LDS slots with the load unit, one tile ahead of the computation and on
+// across pieces and units, so that the memory pipe does not run dry between them, and keep the page
+// walk out of the computing waves. Those take 16 query rows each: scores are S^T = K Q^T on
+// v_mfma_f32_16x16x32, so that lane (g, n) = (l / 16, l % 16) holds row n's scores of keys
+// 4 g .. 4 g + 3 of a 16-key block, and two such blocks, rounded to the query type and packed, are
+// its B operand of O^T += V^T P^T (V^T by transposed LDS reads): softmax and rescaling stay in the
+// lane. A unit of 64 rows or fewer leaves computing waves over, which take other 32-key blocks of
+// the same rows and are joined through LDS at the piece's end. (Four waves of 32 rows read K and V
+// from LDS half as often, but one wave a SIMD does not hide the reads' and products' latencies:
+// draft rows below 37.5 us against 32.9.)
 //
 // The kernel runs each part of its code a few times a workgroup, so its size counts: every part
 // stands once, divisions by the call's constants are multiplications, and the plan's searches are
 // made for 64 tiles at a time, a lane each.
+//
+// Measured (this launch, then the merge): 64 rows of H32/KVH8/D128 bf16 in 8 groups of 8, prefixes
+// of 1024 to 8192 keys and 64 to 1024 own ones, 56 + 4.9 us (225 MB: 36 us of pure reading); 128
+// rows over an fp8 cache behind one prefix of 8192, 93 + 6.0 us (259 MB, 19 GFLOP); 32 rows of 4
+// draft tokens, H28/KVH4 fp16, in 4 groups, 29 + 5.9 us; 6 rows of a small model 10 + 3.8 us, of
+// which the launch, the plan and the first tile's latency are nearly all. What bounds it: the plan
+// and the first window, 9000 clocks a workgroup before the first copy; about 6000 a piece; between
+// them the reads' rate for few rows and some 1000 clocks a 32-key block for 128.
 //
 // Semantics: miniserve/attention.py:205-250 (causal), whose gather reads a shared page once a row.
 #pragma once
@@ -260,7 +272,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
     x.hi = own ? s_len[x.b0] : s_hi[e];
     return x;
   };
-  int total = 0, total_cost = 0;  // the exclusive sums, 512 segments at a time
+  int total = 0, total_cost = 0;  // the exclusive sums, a segment a thread
 #pragma unroll 1
   for (int e0 = 0; e0 < NS; e0 += kShThreads) {
     __syncthreads();
