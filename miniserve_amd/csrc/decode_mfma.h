@@ -609,9 +609,32 @@ __host__ __device__ constexpr int tile_token(int i) {
 // take what the rounding left of rows 0 .. 7 (`rest`), rounded to T in turn, so that column
 // n + 8's score added to column n's (split_score) is that of a query of twice T's digits. Nothing
 // remains of an infinite element.
+template <typename T, typename KT, int D>
+struct RopeTable {  // a lane's entries of one row of the tables: those of its chunks' dims
+  float4 c[D / 32][2], s[D / 32][2];
+  __device__ __forceinline__ void load(const float* cs, const float* sn, int g) {
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const int d0 = Kv8<T, KT>::qk_dim0(j, g, D / 32);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        c[j][h] = *reinterpret_cast<const float4*>(cs + d0 + 4 * h);
+        s[j][h] = *reinterpret_cast<const float4*>(sn + d0 + 4 * h);
+      }
+    }
+  }
+  __device__ __forceinline__ void chunk(int j, float (&co)[8], float (&si)[8]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      co[4 * h] = c[j][h].x, co[4 * h + 1] = c[j][h].y, co[4 * h + 2] = c[j][h].z, co[4 * h + 3] = c[j][h].w;
+      si[4 * h] = s[j][h].x, si[4 * h + 1] = s[j][h].y, si[4 * h + 2] = s[j][h].z, si[4 * h + 3] = s[j][h].w;
+    }
+  }
+};
 template <typename T, typename KT, int D, bool SPLIT = false>
-__device__ __forceinline__ void rope_chunks(typename QChunk<T>::type (&qb)[D / 32], const float* cs,
-                                            const float* sn, int g, bool rest = false) {
+__device__ __forceinline__ void rope_chunks(typename QChunk<T>::type (&qb)[D / 32],
+                                            const RopeTable<T, KT, D>& table, int g,
+                                            bool rest = false) {
   constexpr int JD = D / 32;
   constexpr bool kCross = sizeof(KT) == 1 && D == 64;  // the partner is in the other half-wave
   float q[JD][8];
@@ -635,13 +658,8 @@ __device__ __forceinline__ void rope_chunks(typename QChunk<T>::type (&qb)[D / 3
   }
 #pragma unroll
   for (int j = 0; j < JD; ++j) {
-    const int d0 = Kv8<T, KT>::qk_dim0(j, g, JD);
-    const float4 c0 = *reinterpret_cast<const float4*>(cs + d0);
-    const float4 c1 = *reinterpret_cast<const float4*>(cs + d0 + 4);
-    const float4 s0 = *reinterpret_cast<const float4*>(sn + d0);
-    const float4 s1 = *reinterpret_cast<const float4*>(sn + d0 + 4);
-    const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    const float sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+    float c[8], sv[8];
+    table.chunk(j, c, sv);
     float o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -664,6 +682,13 @@ __device__ __forceinline__ void rope_chunks(typename QChunk<T>::type (&qb)[D / 3
     }
   }
 }
+template <typename T, typename KT, int D, bool SPLIT = false>
+__device__ __forceinline__ void rope_chunks(typename QChunk<T>::type (&qb)[D / 32], const float* cs,
+                                            const float* sn, int g, bool rest = false) {
+  RopeTable<T, KT, D> table;
+  table.load(cs, sn, g);
+  rope_chunks<T, KT, D, SPLIT>(qb, table, g, rest);
+}
 // Column n's score plus column (n + 8) % 16's (DPP row_ror:8).
 __device__ __forceinline__ void split_score(mf_f32x4& s) {
 #pragma unroll
@@ -671,12 +696,12 @@ __device__ __forceinline__ void split_score(mf_f32x4& s) {
 }
 
 // The new token's key row, held as append chunks of the query type (chunk j of lane group g as
-// rope_chunks' query chunks), rotated at row cs / sn of the tables and cast once, from fp32, to
+// rope_chunks' query chunks), rotated at a row of the tables and cast once, from fp32, to
 // the cache's chunks: what msattn_write_kv_rope writes. Lanes l and l ^ 32 (the same token) are
 // both active or both not.
 template <typename T, typename KT, int D>
-__device__ __forceinline__ void rope_new_key(const SrcChunk<T> (&kn)[D / 32], const float* cs,
-                                             const float* sn, int g,
+__device__ __forceinline__ void rope_new_key(const SrcChunk<T> (&kn)[D / 32],
+                                             const RopeTable<T, KT, D>& table, int g,
                                              typename Kv8<T, KT>::raw_t (&out)[D / 32]) {
   typedef typename Kv8<T, KT>::raw_t raw_t;
   static_assert(sizeof(raw_t) == 8 * sizeof(KT), "eight cache elements a chunk");
@@ -701,8 +726,9 @@ __device__ __forceinline__ void rope_new_key(const SrcChunk<T> (&kn)[D / 32], co
   }
 #pragma unroll
   for (int j = 0; j < JD; ++j) {
-    const int d0 = Kv8<T, KT>::qk_dim0(j, g, JD);
     CacheChunk<KT> c;
+    float co[8], si[8];
+    table.chunk(j, co, si);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float r;
@@ -710,7 +736,7 @@ __device__ __forceinline__ void rope_new_key(const SrcChunk<T> (&kn)[D / 32], co
         r = g < 2 ? -kp[j][e] : kp[j][e];
       else
         r = j < JD / 2 ? -k[j + JD / 2][e] : k[j - JD / 2][e];
-      Elt<KT>::store(&c.v[e], rope_mix(k[j][e], r, cs[d0 + e], sn[d0 + e]));
+      Elt<KT>::store(&c.v[e], rope_mix(k[j][e], r, co[e], si[e]));
     }
     out[j] = __builtin_bit_cast(raw_t, c);
   }
@@ -795,6 +821,33 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
   if (lane < per_wave) {
     const int pg = ((tw0 + lane) * 16) / p.bs;
     if (pg < p.W) phys_pre = p.table[static_cast<int64_t>(b) * p.W + pg];
+  }
+
+  // An append with rotation (APPEND 2): the query rows, the new key and the position are requested
+  // with the length and the page ids, the table entries with the first tiles, ahead of them: two
+  // round trips before the rotation instead of three (32 rows of H14/KVH2/D64 14.6 -> 13.8 us, 16
+  // of H28/KVH4/D128 over fp8 26.2 -> 24.5). (Lanes past the rows take the last row; their scores
+  // are masked.)
+  constexpr bool kTurns = APPEND == 2 && RT <= 8;
+  constexpr bool kSplitQ = kTurns && sizeof(T) == 2;
+  // Query rows as the MFMA B operand: lane (g, n) holds Q[row n][dims 8*(4j+g) .. +8].
+  typename QChunk<T>::type qb[JD];
+  SrcChunk<T> k_in[kTurns ? JD : 1];
+  int rope_row = 0;
+  if constexpr (kTurns) {
+    const int rows = min(RT, p.rows_per_kvh - rtile * RT);
+    const int nq = min(kSplitQ ? n & 7 : n, rows - 1);
+    const T* const qp = static_cast<const T*>(p.q) +
+                        (static_cast<int64_t>(b) * p.H + kvh * p.G + rtile * RT + nq) * D;
+    const T* const kp = (p.k_new != nullptr ? static_cast<const T*>(p.k_new) +
+                                                  (static_cast<int64_t>(b) * p.KVH + kvh) * D
+                                            : qp);
+    rope_row = rope_position(p, b);
+#pragma unroll
+    for (int j = 0; j < JD; ++j) {
+      qb[j] = QChunk<T>::load(qp + KV::qk_dim0(j, g, JD));
+      k_in[j] = *reinterpret_cast<const SrcChunk<T>*>(kp + KV::qk_dim0(j, g, JD));
+    }
   }
 
   const int nparts = ctx > 0 ? ceil_div(ctx - 16 * tile0, p.part) : 1;
@@ -899,6 +952,11 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
   int64_t br[DEPTH];
   // The first tiles' loads go out as soon as the context length is known, ahead of the
   // lanes' row set-up and the query load, which then run under their round trip.
+  RopeTable<T, KT, kTurns ? D : 32> rope_table;
+  if constexpr (kTurns) {
+    const int64_t po = static_cast<int64_t>(rope_row) * D;
+    rope_table.load(p.rope_cos + po, p.rope_sin + po, g);
+  }
   if (a1 > a0) {
     static_for<DEPTH - 1>([&](auto dc) {
       constexpr int d = decltype(dc)::value;
@@ -909,7 +967,6 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
   // This lane's query row n: key range [lo_n, hi_n) and output row.
   int lo_n = 0, hi_n = 0;
   int64_t orow_n = 0;
-  constexpr bool kSplitQ = APPEND == 2 && !kPvMfma && sizeof(T) == 2 && RT <= 8;
   if (n < nrows) {
     const int gr = row0 + n;
     const int i = gr / p.G;
@@ -1036,43 +1093,26 @@ __global__ __launch_bounds__(W * kWave) void decode_mfma_kernel(const SplitParam
 
   // The fused append of a rotated key (APPEND 2): the wave whose run holds the new position
   // requests the key beside the query and rotates it after it, at the same row of the tables.
-  constexpr bool kAppendTurns = APPEND == 2 && !kPvMfma && RT <= 8;
+  constexpr bool kAppendTurns = kTurns;
+  static_assert(!(kTurns && kPvMfma), "appends take up to 8 rows a tile");
   const int k_turn = kAppendTurns && ctx > 0 ? (ctx - 1) / 16 - tw0 : -1;
   const bool turn_lane = kAppendTurns && p.k_new != nullptr && k_turn >= 0 && k_turn < nt &&
                          tile_token<D>(n) == ((ctx - 1) & 15);
-  SrcChunk<T> k_in[kAppendTurns ? JD : 1];
   raw_t k_turned[kAppendTurns ? JD : 1];
-  if constexpr (kAppendTurns) {
-    if (turn_lane) {
-      const T* const src = static_cast<const T*>(p.k_new) + (static_cast<int64_t>(b) * p.KVH + kvh) * D;
-#pragma unroll
-      for (int j = 0; j < JD; ++j)
-        k_in[j] = *reinterpret_cast<const SrcChunk<T>*>(src + KV::qk_dim0(j, g, JD));
-    }
-  }
-
-  // Query rows as the MFMA B operand: lane (g, n) holds Q[row n][dims 8*(4j+g) .. +8].
-  typename QChunk<T>::type qb[JD];
-
   // The query rows (after the first tiles' loads).
-  {
+  if constexpr (kTurns) {
+    rope_chunks<T, KT, D, kSplitQ>(qb, rope_table, g, n >= 8);
+    if (turn_lane) rope_new_key<T, KT, D>(k_in, rope_table, g, k_turned);
+  } else {
     const T* qp = static_cast<const T*>(p.q);
-    const int nq = kSplitQ ? n & 7 : n;  // the query row of the lane's column
-    const int64_t q_row = kSplitQ ? static_cast<int64_t>(b) * p.H + kvh * p.G + row0 + nq : orow_n;
 #pragma unroll
     for (int j = 0; j < JD; ++j) {
       qb[j] = QChunk<T>::zero();
-      if (nq < nrows) qb[j] = QChunk<T>::load(qp + q_row * D + KV::qk_dim0(j, g, JD));
+      if (n < nrows) qb[j] = QChunk<T>::load(qp + orow_n * D + KV::qk_dim0(j, g, JD));
     }
-    if (p.rope_cos != nullptr && nq < nrows) {
+    if (p.rope_cos != nullptr && n < nrows) {
       const int64_t po = static_cast<int64_t>(rope_position(p, b)) * D;
-      rope_chunks<T, KT, D, kSplitQ>(qb, p.rope_cos + po, p.rope_sin + po, g, n >= 8);
-    }
-  }
-  if constexpr (kAppendTurns) {
-    if (turn_lane) {
-      const int64_t po = static_cast<int64_t>(rope_position(p, b)) * D;
-      rope_new_key<T, KT, D>(k_in, p.rope_cos + po, p.rope_sin + po, g, k_turned);
+      rope_chunks<T, KT, D>(qb, p.rope_cos + po, p.rope_sin + po, g);
     }
   }
   // Tiles a wave may own: partitions of the fp32 16-row route reach kPartLongF32 tokens.

@@ -392,7 +392,9 @@ __global__ __launch_bounds__(sk_waves(sizeof(KT), sizeof(T)) * kWave) void decod
       raw_t turned[APPEND == 2 ? JD : 1];
       if constexpr (APPEND == 2) {
         const int64_t po = static_cast<int64_t>(rope_position(p, cur.b)) * D;
-        rope_new_key<T, KT, D>(kn, p.rope_cos + po, p.rope_sin + po, g, turned);
+        RopeTable<T, KT, D> table;
+        table.load(p.rope_cos + po, p.rope_sin + po, g);
+        rope_new_key<T, KT, D>(kn, table, g, turned);
       }
 #pragma unroll
       for (int j = 0; j < JD; ++j) {
