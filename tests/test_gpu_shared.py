@@ -303,6 +303,32 @@ def test_device_groups_out_of_range(device):
     x.check(x.call())
 
 
+@pytest.mark.parametrize("rows", [[0, 4, 2, 6], [3, 1, 0, 0], [6, 6, 6, 2], [2 ** 31 - 1, 0, -7, 4]])
+def test_device_groups_out_of_order(device, rows):
+    """Group rows on the device that do not ascend: every row by itself."""
+    x = Batch(8, 2, 64, BF16, BF16, [], [120, 100, 0, 200, 150, 145], 2)
+    x.rows, x.pages = torch.tensor(rows, device=device), torch.tensor([3, 4, 5], device=device)
+    note(f"group rows {rows}")
+    x.check(x.call())
+
+
+def test_offsets_past_32_bits(device):
+    """Pages whose elements lie past 2^31 in an fp8 pool."""
+    x = Batch(8, 8, 128, BF16, FP8, [(0, 2, 3), (2, 2, 5)], [100, 64, 300, 90], 1)
+    n = x.kc.shape[0]
+    first = 2 ** 31 // (16 * 8 * 128) - n // 2
+    pools = []
+    for t in (x.kc, x.vc):
+        pool = torch.zeros(first + n, 16, 8, 128, dtype=torch.uint8, device=device)
+        pool[first:] = t.view(torch.uint8).to(device)
+        pools.append(pool.view(FP8))
+    note("offsets past 32 bits")
+    lens = torch.tensor(x.lens, dtype=torch.int32, device=device)
+    out = paged_attention_shared(x.q.to(device), *pools, (x.table + first).to(device), lens, x.rows,
+                                 x.pages)
+    x.check(out)
+
+
 def test_refusals(device):
     x = Batch(8, 2, 64, BF16, BF16, [(0, 3, 4)], [150, 120, 110], 1)
     a = [t.to(device) for t in (x.q, x.kc, x.vc, x.table)]
