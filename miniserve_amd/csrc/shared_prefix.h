@@ -32,7 +32,7 @@
 // made for 64 tiles at a time, a lane each.
 //
 // Measured (this launch, then the merge): 64 rows of H32/KVH8/D128 bf16 in 8 groups of 8, prefixes
-// of 1024 to 8192 keys and 64 to 1024 own ones, 56 + 4.9 us (225 MB: 36 us of pure reading); 128
+// of 1024 to 8192 keys and 64 to 1024 own ones, 48 + 4.6 us (225 MB: 36 us of pure reading); 128
 // rows over an fp8 cache behind one prefix of 8192, 93 + 6.0 us (259 MB, 19 GFLOP); 32 rows of 4
 // draft tokens, H28/KVH4 fp16, in 4 groups, 29 + 5.9 us; 6 rows of a small model 10 + 3.8 us, of
 // which the launch, the plan and the first tile's latency are nearly all. What bounds it: the plan
@@ -57,9 +57,12 @@ constexpr int kShSlots = 2;             // tiles in LDS
 __host__ __device__ constexpr int sh_tile(int head_dim, int kv_bytes) {
   return kShHalf / (head_dim * kv_bytes);
 }
-// Cache policy of the K/V reads (2: nontemporal).
+// Cache policy of the reads of a 16-bit cache in units whose keys no other row block reads (2:
+// nontemporal; 64 rows in 8 groups of H32/KVH8/D128 48 us against 56, H16/KVH2/D64 28 and 29 with
+// the merge). Keys that several row blocks read stay in L2 for them (nontemporal, 16 rows of 32
+// query rows took 2 % more), and an fp8 cache's took 1 to 3 % more.
 #ifndef MSATTN_SHARED_AUX
-#define MSATTN_SHARED_AUX 0
+#define MSATTN_SHARED_AUX 2
 #endif
 constexpr int kShAux = MSATTN_SHARED_AUX;
 
@@ -138,10 +141,11 @@ __host__ __device__ constexpr int64_t sh_slots(int64_t rows, int shares) {
   return 2 * rows + static_cast<int64_t>(shares) * kShRows;
 }
 
-// As lds_copy16, with the cache policy above.
+// As lds_copy16, with a cache policy.
+template <int AUX>
 __device__ __forceinline__ void sh_copy16(__amdgpu_buffer_rsrc_t r, char* dst, uint32_t voff) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 16, voff, 0, 0, kShAux);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 16, voff, 0, 0, AUX);
 #endif
 }
 // A barrier of the workgroup that waits for LDS accesses only: the copies into LDS that are in
@@ -374,7 +378,8 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
   //   tok  the key the tile begins at      hi  where the segment's keys end
   //   unit KV head | row block << 16       id  the pages of a copying wave's sub-tiles
   //   bits segment's first row | kind << 10 | the unit's first tile << 11 |
-  //        the piece's last tile << 12 | (query rows - 1) << 13 | the piece's first tile << 20
+  //        the piece's last tile << 12 | (query rows - 1) << 13 | the piece's first tile << 20 |
+  //        its keys are read for one row block only << 21
   struct Tile {
     int tok, hi, unit, bits;
     __device__ bool starts() const { return (bits >> 20) & 1; }
@@ -417,7 +422,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
     c.bits = e.b0 | (own ? 1 << 10 : 0) | (t == 0 ? 1 << 11 : 0) |
              (t + 1 == tiles || pos + 1 == last ? 1 << 12 : 0) |
              ((min(kShRows, e.members * RPS - static_cast<int>(rt) * kShRows) - 1) << 13) |
-             (t == 0 || pos == first ? 1 << 20 : 0);
+             (t == 0 || pos == first ? 1 << 20 : 0) | (rtiles == 1 ? 1 << 21 : 0);
     return c;
   };
 
@@ -465,6 +470,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
         const int r = i + kShSlots;  // the tile requested (past the window: nothing is read)
         const int rl = min(r, count - 1);
         const Tile c = wt.at(rl);
+        const bool once = EB == 2 && ((c.bits >> 21) & 1);
         int live = 0;
         char* const d = s_tile + to * 2 * kShHalf + SUB * cw * 16 * ROW;
 #pragma unroll
@@ -483,8 +489,13 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
           const __amdgpu_buffer_rsrc_t rv = tile_rsrc(static_cast<const KT*>(p.v) + off, nbytes);
 #pragma unroll
           for (int j = 0; j < NI; ++j) {
-            sh_copy16(rk, d + (16 * h + RPI * j) * ROW, dvo[j]);
-            sh_copy16(rv, d + kShHalf + (16 * h + RPI * j) * ROW, dvo[j]);
+            if (once) {
+              sh_copy16<kShAux>(rk, d + (16 * h + RPI * j) * ROW, dvo[j]);
+              sh_copy16<kShAux>(rv, d + kShHalf + (16 * h + RPI * j) * ROW, dvo[j]);
+            } else {
+              sh_copy16<0>(rk, d + (16 * h + RPI * j) * ROW, dvo[j]);
+              sh_copy16<0>(rv, d + kShHalf + (16 * h + RPI * j) * ROW, dvo[j]);
+            }
           }
           if (in) live |= 1 << h;
         }
