@@ -1868,6 +1868,7 @@ int msattn_paged_attention_shared(const void* query, const void* k_cache, const 
   p.shares = shared_shares(
       shared_most_tiles(batch, q_len, num_heads, num_kv_heads, max_context, groups,
                         sh_tile(head_dim, dtype_bytes(kv_dtype))), device_cus());
+  p.by_shares = fast_div(static_cast<uint32_t>(p.shares));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (q_dtype == MSATTN_BF16)
     return hip_status(kv_dtype == MSATTN_FP8_E4M3 ? launch_shared<bf16_t, fp8_t>(p, head_dim, st)

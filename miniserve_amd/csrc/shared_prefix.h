@@ -116,8 +116,9 @@ struct SharedParams {
   int64_t blk_stride, slot_stride, head_stride;
   int batch, groups, q_len, H, KVH, G;
   int bs, num_blocks, W, max_ctx;
-  // page size, query rows a KV head and batch row, query heads a KV head, query heads, query tokens
-  FastDiv by_bs, by_rps, by_g, by_h, by_q;
+  // page size, query rows a KV head and batch row, query heads a KV head, query heads, query
+  // tokens, shares
+  FastDiv by_bs, by_rps, by_g, by_h, by_q, by_shares;
   float scale_log2;
   // Workspace: the plan (for the merge) and the pieces' partials. A
   // unit's first piece goes to slot kind * rows + output row (kind 0: the group's segment, 1: the
@@ -241,8 +242,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
   descend = __any(descend);
   if (lane == 0) s_wsum[w] = descend;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kShThreads / kWave; ++i) descend |= s_wsum[i] != 0;
+  descend = __any(lane < kShThreads / kWave && s_wsum[lane] != 0);
 #pragma unroll 1
   for (int b = tid; b < B; b += kShThreads) {
     int lo = 0, hi = NG;  // the last group that begins at or before row b
@@ -297,15 +297,17 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
       s_wsum[kShThreads / kWave + w] = incl_cost;
     }
     __syncthreads();
-    int at = total + incl - c, at_cost = total_cost + incl_cost - cost;
-#pragma unroll
-    for (int i = 0; i < kShThreads / kWave; ++i) {
-      const int x = s_wsum[i], y = s_wsum[kShThreads / kWave + i];
-      at += i < w ? x : 0;
-      at_cost += i < w ? y : 0;
-      total += x;
-      total_cost += y;
-    }
+    // the waves' sums, scanned by lanes: tiles in lanes 0 .., costs from lane 32 on
+    constexpr int NW = kShThreads / kWave;
+    const int of = lane & 31;
+    const int part = of < NW ? s_wsum[of + (lane >= 32 ? NW : 0)] : 0;
+    const int scan = wave_inclusive_sum(part);
+    const int tiles_before = w > 0 ? __builtin_amdgcn_readlane(scan, w - 1) : 0;
+    const int all_tiles = __builtin_amdgcn_readlane(scan, 31);  // (lanes from 32 on count on top)
+    const int cost_before = w > 0 ? __builtin_amdgcn_readlane(scan, 31 + w) - all_tiles : 0;
+    const int at = total + tiles_before + incl - c, at_cost = total_cost + cost_before + incl_cost - cost;
+    total += all_tiles;
+    total_cost += __builtin_amdgcn_readlane(scan, 63) - all_tiles;
     if (e < NS) {
       s_cum[e] = at;
       s_cost[e] = at_cost;
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
     s_cost[NS] = total_cost;
   }
   __syncthreads();
-  const int per = max(1, ceil_div(uni(total_cost), p.shares));
+  const int per = max(1, fast_quot(uni(total_cost) + p.shares - 1, p.by_shares));
   if (blockIdx.x == 0 && tid == 0) p.plan[0] = per;
 #pragma unroll 1
   for (int b = static_cast<int>(blockIdx.x) + tid * p.shares; b < B; b += kShThreads * p.shares) {
@@ -385,9 +387,9 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
     __device__ bool starts() const { return (bits >> 20) & 1; }
     __device__ bool ends() const { return (bits >> 12) & 1; }
     __device__ int rows() const { return ((bits >> 13) & 127) + 1; }
-    // Computing waves that take different rows; the others take other keys of the same.
+    // log2 of the computing waves that take different rows; the others take other keys of the same.
     __device__ int row_waves() const {
-      return rows() > 64 ? 8 : (rows() > 32 ? 4 : (rows() > 16 ? 2 : 1));
+      return rows() > 64 ? 3 : (rows() > 32 ? 2 : (rows() > 16 ? 1 : 0));
     }
     // Pieces whose waves split the keys are joined through the slot.
     __device__ bool joins() const { return ends() && rows() <= 64; }
@@ -637,7 +639,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
       if (starts) {
         const int b0 = nx.first_row();
         const T* const q = static_cast<const T*>(p.q) + static_cast<int64_t>(b0) * p.q_len * p.H * D;
-        const int r = 16 * (cw & (nx.row_waves() - 1)) + n;
+        const int r = 16 * (cw & ((1 << nx.row_waves()) - 1)) + n;
         const int row = (nx.unit >> 16) * kShRows + (r < nx.rows() ? r : 0);
         const int member = fast_quot(row, p.by_rps);
         const int rest = row - member * RPS;
@@ -730,10 +732,10 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
       // ---- the next piece begins ----
       if (starts) {
         unit_first = (nx.bits >> 11) & 1;
-        RW = nx.row_waves();
+        RW = 1 << nx.row_waves();
         rw = cw & (RW - 1);
-        KS = min(kShComp / RW, TK / 32);  // (waves ks >= KS have no block)
-        ks = cw / RW;
+        KS = min(kShComp >> nx.row_waves(), TK / 32);  // (waves ks >= KS have no block)
+        ks = cw >> nx.row_waves();
         orow = n_row;
         hi_n = n_hi;
         m_run = -INFINITY;
