@@ -421,8 +421,9 @@ size_t msattn_shared_workspace_bytes(int batch, int q_len, int num_heads, int nu
  * [0, batch] and [0, table_width] are taken as the nearest bound). Rows outside every group share
  * nothing. Same result as msattn_paged_attention(causal = 1, window = 0) within float rounding,
  * any q_len: each prefix is read once per KV head and 128 query rows for the whole group, through
- * the table of the group's first row; the caller is trusted that the other rows' entries are the
- * same. A row whose queries do not all see the whole prefix reads its own length of it by itself.
+ * the table of the group's first row whose queries all see it whole; the caller is trusted that
+ * the other such rows' entries are the same. The rows that do not (a padding row of length 0, say)
+ * read what they see of it by themselves, through their own.
  * Other types and layouts than a bf16 or fp16 query (16-byte aligned) over a cache of its type or
  * of fp8 e4m3, head_dim 64 or 128, block_size a multiple of 16, 16-byte aligned cache rows, up to
  * 1024 rows and groups and 64 query rows a KV head and batch row, and calls without a group, run

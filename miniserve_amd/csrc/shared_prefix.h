@@ -197,6 +197,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
   __shared__ int s_cum[2 * kShMaxBatch + 1];  // tiles before each segment: groups, then rows
   __shared__ int s_g0[kShMaxBatch + 1];       // a group's first row
   __shared__ int s_hi[kShMaxBatch];           // a group's prefix keys, 0 if no row reads them
+  __shared__ int s_by[kShMaxBatch];           // the first row that does, whose table gives the pages
   __shared__ int s_len[kShMaxBatch];
   __shared__ int s_own[kShMaxBatch];          // where a row's own keys begin
   __shared__ short s_grp[kShMaxBatch];        // a row's group, or -1
@@ -229,6 +230,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
       const int64_t pt = static_cast<int64_t>(pages < 0 ? 0 : (pages > p.W ? p.W : pages)) * p.bs;
       s_cum[i] = static_cast<int>(pt < p.max_ctx ? pt : p.max_ctx);  // (for now: prefix tokens)
       s_hi[i] = 0;
+      s_by[i] = B - 1;
       descend |= row_in(r0) > row_in(r1);
     }
     if (i < B) s_len[i] = len < 0 ? 0 : (len > p.max_ctx ? p.max_ctx : len);
@@ -260,12 +262,13 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
       own = s_cum[lo];
       grp = lo;
       s_hi[lo] = own;  // (every member's is the same)
+      atomicMin(&s_by[lo], b);
     }
     s_own[b] = own;
     s_grp[b] = static_cast<short>(grp);
   }
   struct Segment {
-    int b0, members, key0, hi;  // its first row and rows, its keys
+    int b0, members, key0, hi, by;  // its first row and rows, its keys, the row whose table has them
   };
   auto segment = [&](int e) __attribute__((always_inline)) {
     const bool own = e >= NG;
@@ -274,6 +277,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
     x.members = own ? 1 : s_g0[e + 1] - x.b0;
     x.key0 = own ? s_own[x.b0] : 0;
     x.hi = own ? s_len[x.b0] : s_hi[e];
+    x.by = own ? x.b0 : s_by[e];
     return x;
   };
   int total = 0, total_cost = 0;  // the exclusive sums, a segment a thread
@@ -381,7 +385,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
   //   unit KV head | row block << 16       id  the pages of a copying wave's sub-tiles
   //   bits segment's first row | kind << 10 | the unit's first tile << 11 |
   //        the piece's last tile << 12 | (query rows - 1) << 13 | the piece's first tile << 20 |
-  //        its keys are read for one row block only << 21
+  //        its keys are read for one row block only << 21 | the row whose table has them << 22
   struct Tile {
     int tok, hi, unit, bits;
     __device__ bool starts() const { return (bits >> 20) & 1; }
@@ -394,6 +398,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
     // Pieces whose waves split the keys are joined through the slot.
     __device__ bool joins() const { return ends() && rows() <= 64; }
     __device__ int first_row() const { return bits & 1023; }
+    __device__ int table_row() const { return static_cast<int>(static_cast<uint32_t>(bits) >> 22); }
     __device__ int kvh() const { return unit & 0xffff; }
     __device__ Tile at(int lane) const {
       return Tile{__builtin_amdgcn_readlane(tok, lane), __builtin_amdgcn_readlane(hi, lane),
@@ -424,7 +429,8 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
     c.bits = e.b0 | (own ? 1 << 10 : 0) | (t == 0 ? 1 << 11 : 0) |
              (t + 1 == tiles || pos + 1 == last ? 1 << 12 : 0) |
              ((min(kShRows, e.members * RPS - static_cast<int>(rt) * kShRows) - 1) << 13) |
-             (t == 0 || pos == first ? 1 << 20 : 0) | (rtiles == 1 ? 1 << 21 : 0);
+             (t == 0 || pos == first ? 1 << 20 : 0) | (rtiles == 1 ? 1 << 21 : 0) |
+             static_cast<int>(static_cast<uint32_t>(e.by) << 22);
     return c;
   };
 
@@ -445,7 +451,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
         const int pg = fast_quot(tok, p.by_bs);
         w_id[i] = -1;
         if (tok < wt.hi && pg < p.W)
-          w_id[i] = p.table[static_cast<int64_t>(wt.first_row()) * p.W + pg];
+          w_id[i] = p.table[static_cast<int64_t>(wt.table_row()) * p.W + pg];
       }
       const int64_t row_bytes = p.slot_stride * EB;
       uint32_t dvo[NI];

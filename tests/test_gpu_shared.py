@@ -261,6 +261,17 @@ def test_rows_that_do_not_see_the_whole_prefix(device, q_len, short):
         assert bool(out[[0, 2, 3]].isnan().all())
 
 
+@pytest.mark.parametrize("gone", [[0], [0, 1], [2], [0, 1, 2, 3]])
+def test_padding_rows_in_a_group(device, gone):
+    """Rows of a group that hold no sequence (length 0, an empty table), its first among them."""
+    lens = [0 if b in gone else n for b, n in enumerate([100, 90, 80, 120])] + [70, 66]
+    x = Batch(8, 2, 64, BF16, BF16, [(0, 4, 4), (4, 2, 2)], lens, 1)
+    for b in gone:
+        x.table[b] = -1
+    note(f"rows {gone} empty")
+    x.check(x.call())
+
+
 # Calls that the kernel does not take run paged_attention: bit for bit its result.
 @pytest.mark.parametrize("name,H,KVH,D,qt,kt,bs,q_len", [
     ("fp32 query", 8, 2, 64, F32, F32, 16, 1), ("fp32 cache", 8, 2, 64, BF16, F32, 16, 1),
