@@ -3,11 +3,12 @@
 Tolerance. Scores are fp32 sums of exact products: off by at most |ds| = (D + 8) 2^-24 scale |q||k|
 (products, D additions, the scale), so a weight is off by a factor e^(2 |ds|); it is rounded to the
 query type (u = eps / 2 relative; fp16 weights below 2^-14 by 2^-25 absolute, beside a largest
-weight of 1), in the numerator and in the sum alike, and the output is rounded once more. Outputs
+weight of 1 or more), in the numerator and in the sum alike, and the output is rounded once more. Outputs
 are weighted means of V: the whole is at most (4.04 |ds| e^(2 |ds|) + 3 u + n 2^-24 [fp16] + 2^-18)
 max |V| over the n visible keys, the last term for the hardware's 2^x and the joins in fp32.
 """
 import math
+import random
 
 import pytest
 import torch
@@ -270,6 +271,32 @@ def test_padding_rows_in_a_group(device, gone):
         x.table[b] = -1
     note(f"rows {gone} empty")
     x.check(x.call())
+
+
+@pytest.mark.parametrize("seed", range(32))
+def test_fuzz(device, seed):
+    """Seeded shapes: loose rows before, between and after groups, groups of one and of many, empty
+    and short rows, prefixes of no page, contexts ending on and off tiles, up to 64 query rows."""
+    r = random.Random(7000 + seed)
+    KVH, G = r.choice((1, 2, 3, 8)), r.choice((1, 2, 4, 7, 8, 16))
+    D, qt = r.choice((64, 128)), r.choice((BF16, F16))
+    kt, bs = r.choice((qt, qt, FP8)), r.choice((16, 32, 48, 64))
+    q_len = r.choice([n for n in (1, 1, 1, 2, 3, 5, 8) if n * G <= 64])
+    groups, lens, at = [], [], r.choice((0, 0, 1, 2))
+    lens += [r.randrange(0, 300) for _ in range(at)]
+    for _ in range(r.randrange(1, 5)):
+        n, pages = r.choice((1, 2, 3, 5, 12, 40)), r.choice((0, 1, 2, 5, 17, 40)) * 16 // bs
+        groups.append((at, n, pages))
+        at += n
+        for _ in range(n):
+            kind = r.random()
+            lens.append(0 if kind < 0.08 else
+                        r.randrange(1, pages * bs + 2) if kind < 0.16 else
+                        pages * bs + r.choice((0, 1, q_len, 15, 16, 31, 128, 200, 256, 511)))
+    lens += [r.randrange(0, 300) for _ in range(r.choice((0, 0, 1, 3)))]
+    x = Batch(KVH * G, KVH, D, qt, kt, groups, lens, q_len, bs, extra=r.choice((0, 3)), seed=seed)
+    note(f"seed {seed}: H{KVH * G}/KVH{KVH}/D{D} {qt} over {kt}, pages of {bs}, q_len {q_len}, {groups}")
+    x.check(x.call(), rows=sorted(r.sample(range(len(lens)), min(12, len(lens)))))
 
 
 # Calls that the kernel does not take run paged_attention: bit for bit its result.
