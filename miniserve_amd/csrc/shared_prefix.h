@@ -34,10 +34,10 @@
 // Measured (this launch, then the merge): 64 rows of H32/KVH8/D128 bf16 in 8 groups of 8, prefixes
 // of 1024 to 8192 keys and 64 to 1024 own ones, 48 + 4.6 us (225 MB: 36 us of pure reading); 128
 // rows over an fp8 cache behind one prefix of 8192, 93 + 6.0 us (259 MB, 19 GFLOP); 32 rows of 4
-// draft tokens, H28/KVH4 fp16, in 4 groups, 29 + 5.9 us; 6 rows of a small model 10 + 3.8 us, of
+// draft tokens, H28/KVH4 fp16, in 4 groups, 30 + 6.0 us; 6 rows of a small model 11 + 3.9 us, of
 // which the launch, the plan and the first tile's latency are nearly all. What bounds it: the plan
 // and the first window, 9000 clocks a workgroup before the first copy; about 6000 a piece; between
-// them the reads' rate for few rows and some 1000 clocks a 32-key block for 128.
+// them the reads' rate for few rows and some 1300 clocks a 32-key block for 128 (1900 over fp8).
 //
 // Semantics: miniserve/attention.py:205-250 (causal), whose gather reads a shared page once a row.
 #pragma once
@@ -69,8 +69,9 @@ constexpr int kShAux = MSATTN_SHARED_AUX;
 // What a share is to cost a workgroup, in units of about 250 clocks: a piece (its query, its plan,
 // its partials), and each 32-key block of a unit of so many rows. Few rows wait for the memory pipe,
 // many for the matrix cores and the softmax. (From a fit of the workgroups' clocks to their pieces
-// and blocks, then tried around: 64 rows in 8 groups of bf16 head_dim 128 took 74 us with the same
-// piece cost and half the spread, 58 so; equal tile counts 81.)
+// and blocks, then tried around. 64 rows in 8 groups of H32/KVH8/D128 took 81 us in shares of equal
+// tiles, 63 with one row of costs for all types and sizes and 56 with these, all before the
+// nontemporal reads.)
 #ifndef MSATTN_SHARED_COSTS
 #define MSATTN_SHARED_COSTS {20, 6, 7, 9, 12}, {20, 3, 4, 5, 7}, {20, 2, 3, 5, 8}, {20, 2, 3, 4, 6}
 #endif
