@@ -392,10 +392,11 @@ int msattn_write_kv_rope(const void* query, const int64_t* q_strides, void* quer
  * position[b] of the tables (position == NULL: context_lens[b] - 1), clamped to
  * [0, max_position). rope_cos / rope_sin are 16-byte aligned. One launch where
  * msattn_paged_attention_append is one, and for most fp32 queries on the partition kernel (in
- * small launches only over an fp32 cache of head_dim 128), else the write, then the decode: the same caches and
- * output as msattn_write_kv_rope of the new token followed by msattn_paged_attention_rope, but
- * for the rotated query: with at most 8 query heads a KV head it is used to twice its type's
- * digits (those of fp32 in the generic kernel), not rounded to the type.
+ * small launches only over an fp32 cache of head_dim 128), else the write, then the decode: the
+ * same caches and output as msattn_write_kv_rope of the new token followed by
+ * msattn_paged_attention_rope, but for the rotated query: a 2-byte one with at most 8 query heads
+ * a KV head is used to twice its type's digits (those of fp32 in the generic kernel), not rounded
+ * to the type.
  */
 int msattn_paged_attention_append_rope(
     const void* query, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
