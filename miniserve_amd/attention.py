@@ -393,6 +393,10 @@ class PagedAttention:
                 raise RuntimeError("triton_flash requires CUDA tensors (a ROCm GPU device)")
             rope = (cos, sin, position) if cos is not None and sin is not None and \
                 position is not None else None
+            if prefix_groups is not None and rope is None:
+                from .shared import paged_attention_shared
+                return paged_attention_shared(query, k_cache, v_cache, block_table, context_lens,
+                                              *prefix_groups, scale=scale)
             return paged_attention(query, k_cache, v_cache, block_table, context_lens,
                                    causal=True, window=None, scale=scale, rope=rope,
                                    prefix_pages=shared_prefix_pages if rope is None else None)

@@ -403,7 +403,9 @@ def test_forward_takes_groups(device):
                         device=device, kv_dtype=BF16)
     a = [t.to(device) for t in (x.q, x.kc, x.vc, x.table)]
     note("forward")
-    assert torch.equal(pa.forward(*a, x.lens, prefix_groups=(x.rows, x.pages)), x.call(lens=x.lens))
+    for backend in ("sdpa", "triton_flash"):
+        got = pa.forward(*a, x.lens, prefix_groups=(x.rows, x.pages), backend=backend)
+        assert torch.equal(got, x.call(lens=x.lens))
     plain = paged_attention(*a, x.lens, window=50)
     assert torch.equal(pa.forward(*a, x.lens, window=50, prefix_groups=(x.rows, x.pages)), plain)
 
