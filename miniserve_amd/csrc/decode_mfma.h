@@ -689,10 +689,15 @@ __device__ __forceinline__ void rope_chunks(typename QChunk<T>::type (&qb)[D / 3
   table.load(cs, sn, g);
   rope_chunks<T, KT, D, SPLIT>(qb, table, g, rest);
 }
-// Column n's score plus column (n + 8) % 16's (DPP row_ror:8).
+// Column n's score plus column (n + 8) % 16's (DPP row_ror:8). An infinite key's score stays as
+// the rounded query has it: the rest, of either sign or zero, would make inf - inf or 0 inf of it,
+// and NaN of a -inf that weighs nothing.
 __device__ __forceinline__ void split_score(mf_f32x4& s) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) s[r] += dpp_mov<0x128>(s[r]);
+  for (int r = 0; r < 4; ++r) {
+    const float rest = dpp_mov<0x128>(s[r]);
+    s[r] = fabsf(s[r]) < INFINITY ? s[r] + rest : s[r];
+  }
 }
 
 // The new token's key row, held as append chunks of the query type (chunk j of lane group g as

@@ -1,0 +1,49 @@
+"""Rotated writes and appends at the ends of what their arguments allow."""
+import math
+
+import pytest
+import torch
+
+import test_gpu_rope_write as base
+from miniserve_amd import paged_attention_append
+from oracle import dense
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16, FP8 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn
+note, tables, rotate64, bits = base.note, base.tables, base.rotate64, base.bits
+
+
+@pytest.mark.parametrize("name", ["C2 geometry bf16", "stream-K", "bf16 over fp32",
+                                  "two query heads a KV head", "stream-K, D64"])
+def test_append_over_an_infinite_key(device, name):
+    """A cached key whose one element is -inf, and queries that are positive there: its score is
+    -inf and it weighs nothing, as in the two calls; queries that are negative there have no finite
+    answer. The bound is that of the appends against 64 bits: the query in two parts of its type
+    (u^2, fp16's least step), the sums in fp32, the output's rounding."""
+    q, k, v, kc, vc, table, lens, cos, sin, _, _, host = base.append_case(name, device)
+    H, KVH, D = q.shape[2], kc.shape[2], q.shape[3]
+    pos, row, dim = torch.tensor(host)[:, None] - 1, 2, 3  # (row 2 fills its table)
+    sign = rotate64(q, cos, sin, pos)[0][row, 0, :, dim].sign()
+    flip = torch.ones(H).double()
+    flip[H - 1] = -1.0  # the last head's score is +inf
+    q[row, 0] *= (sign * flip).to(q.dtype).to(device)[:, None]
+    turned, _ = rotate64(q, cos, sin, pos)
+    bad = 37
+    page = int(table[row, bad // 16])
+    kc[page, bad % 16, :, dim] = -math.inf
+    note(f"infinite key, {name}")
+    out = paged_attention_append(q, k, v, kc, vc, table, lens, rope=(cos, sin))[row].cpu().double()
+    n = host[row]
+    kk = torch.from_numpy(dense.gather_rows(kc.cpu(), table[row].cpu(), n, q.dtype))
+    vv = torch.from_numpy(dense.gather_rows(vc.cpu(), table[row].cpu(), n, q.dtype))
+    kk[bad] = 0
+    keep = dense.keep_mask(n, 1, True, None)
+    keep[:, bad] = False
+    want = torch.from_numpy(dense.attend_f64(turned[row].numpy(), kk.numpy(), vv.numpy(), keep, D ** -0.5))
+    u = torch.finfo(q.dtype).eps / 2
+    ds = (((u * u + 2.0 ** -22) * turned[row].norm(dim=-1).max() +
+           (2.0 ** -25 * D ** 0.5 if q.dtype == F16 else 0)) * D ** -0.5 * kk.norm(dim=-1).max()).item()
+    bound = (2.02 * ds * math.exp(2 * ds) + 4 * u + 2.0 ** -18 +
+             (n * 2.0 ** -24 if q.dtype == F16 else 0)) * vv.abs().max().item()
+    assert (out - want)[:, :H - 1].abs().max().item() <= bound
+    assert not bool(out[:, H - 1].isfinite().any())
