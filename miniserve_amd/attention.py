@@ -169,6 +169,14 @@ def context_lens_i32(context_lens, device: torch.device, batch: int) -> tuple[to
     return lens, host_max
 
 
+def narrow_i32(t: torch.Tensor, lo: int = -2 ** 31, hi: int = 2 ** 31 - 1) -> torch.Tensor:
+    """`t` as int32, wider values taken as the nearest of [lo, hi] (not modulo 2^32), without a
+    read by the host."""
+    if t.dtype == torch.int32:
+        return t
+    return (t.clamp(lo, hi) if t.element_size() > 4 else t).to(torch.int32)
+
+
 def starts_i32(start, batch: int, device: torch.device) -> torch.Tensor:
     """int32 device tensor of each row's first position: an int, one entry per row (at least),
     or an int tensor."""
@@ -614,7 +622,7 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
                              f"and at most {D}")
         pos = None
         if len(rope) == 3 and rope[2] is not None:
-            pos = torch.as_tensor(rope[2], device=dev).reshape(-1).to(torch.int32)
+            pos = narrow_i32(torch.as_tensor(rope[2], device=dev).reshape(-1))
             if pos.numel() == 1:
                 pos = pos.expand(B)
             if pos.numel() != B:

@@ -169,7 +169,7 @@ def write_kv_rope(query: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
     starts = _att.starts_i32(start, B, dev)
     pos, per_token = None, 0
     if position is not None:
-        pos = torch.as_tensor(position, device=dev).to(torch.int32)
+        pos = _att.narrow_i32(torch.as_tensor(position, device=dev))
         if pos.ndim == 0:
             pos = pos.expand(B)
         if tuple(pos.shape) not in ((B,), (B, T)):

@@ -5,12 +5,49 @@ import pytest
 import torch
 
 import test_gpu_rope_write as base
-from miniserve_amd import paged_attention_append
+from miniserve_amd import paged_attention_append, write_kv_rope
 from oracle import dense
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16, FP8 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn
 note, tables, rotate64, bits = base.note, base.tables, base.rotate64, base.bits
+
+
+@pytest.mark.parametrize("form", ["rows", "tokens", "int"])
+def test_positions_past_32_bits_are_clamped(device, form):
+    """int64 positions past int32 are the tables' last row, or their first, as any position outside
+    is; they are not taken modulo 2^32."""
+    g = torch.Generator().manual_seed(5)
+    B, T, H, KVH, D, bs, W = 3, 18, 4, 2, 64, 16, 2
+    q, k, v = base.sources(H, KVH, D, F16, B, T, "fused", g, device)
+    kc, vc = base.pool(B * W, bs, KVH, D, F16, g, device)
+    kc0, vc0 = kc.clone(), vc.clone()
+    table = torch.randperm(B * W, generator=g).view(B, W).to(torch.int32)
+    cos, sin = tables(50, D, device)
+    wide = torch.tensor([2 ** 31, 2 ** 40 + 7, -2 ** 33 + 5])
+    last = torch.tensor([49, 49, 0])
+    given, full = {
+        "rows": (wide, None),
+        "tokens": (wide[:, None].expand(B, T), last[:, None].expand(B, T)),
+        "int": (2 ** 32 + 3, torch.full((B, T), 49)),
+    }[form]
+    if full is None:  # (the first tokens' positions; the others follow)
+        full = (wide[:, None].clamp(-2 ** 31, 2 ** 31 - 1) + torch.arange(T))
+    note(f"positions past 32 bits, {form}")
+    out = write_kv_rope(q, k, v, kc, vc, table.to(device), [2, 0, 5], cos, sin,
+                        given.to(device) if isinstance(given, torch.Tensor) else given)
+    base.check_write(q, k, v, kc0, vc0, kc, vc, out, table, [2, 0, 5], cos, sin, full)
+
+
+def test_append_positions_past_32_bits(device):
+    q, k, v, kc, vc, table, lens, cos, sin, _, _, host = base.append_case("C2 geometry bf16", device)
+    a = (kc.clone(), vc.clone())
+    wide = torch.tensor([2 ** 32 + 5, 2 ** 31, -2 ** 32 + 9, 7] * 8, device=device)
+    near = wide.clamp(0, cos.shape[0] - 1).to(torch.int32)
+    note("append, positions past 32 bits")
+    out = paged_attention_append(q, k, v, kc, vc, table, lens, rope=(cos, sin, wide))
+    want = paged_attention_append(q, k, v, *a, table, lens, rope=(cos, sin, near))
+    assert torch.equal(out, want) and torch.equal(bits(kc), bits(a[0]))
 
 
 @pytest.mark.parametrize("name", ["C2 geometry bf16", "stream-K", "bf16 over fp32",
