@@ -166,6 +166,8 @@ def write_kv_rope(query: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
         raise ValueError("block_table has fewer rows than k")
     if table.shape[1] == 0:
         raise ValueError("block_table has no columns")
+    if isinstance(start, torch.Tensor):
+        start = _att.narrow_i32(start)
     starts = _att.starts_i32(start, B, dev)
     pos, per_token = None, 0
     if position is not None:

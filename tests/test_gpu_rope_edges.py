@@ -39,6 +39,21 @@ def test_positions_past_32_bits_are_clamped(device, form):
     base.check_write(q, k, v, kc0, vc0, kc, vc, out, table, [2, 0, 5], cos, sin, full)
 
 
+def test_starts_past_32_bits_write_nothing(device):
+    """int64 starts past int32 lie outside every table: their tokens are rotated, not written."""
+    g = torch.Generator().manual_seed(6)
+    B, T, H, KVH, D, bs, W = 4, 5, 2, 2, 64, 16, 2
+    q, k, v = base.sources(H, KVH, D, BF16, B, T, "dense", g, device)
+    kc, vc = base.pool(B * W, bs, KVH, D, BF16, g, device)
+    kc0, vc0 = kc.clone(), vc.clone()
+    table = torch.randperm(B * W, generator=g).view(B, W).to(torch.int32)
+    cos, sin = tables(40, D, device)
+    start = [2 ** 32 + 3, 4, -2 ** 32 + 2, 2 ** 31]
+    note("starts past 32 bits")
+    out = write_kv_rope(q, k, v, kc, vc, table.to(device), torch.tensor(start, device=device), cos, sin)
+    base.check_write(q, k, v, kc0, vc0, kc, vc, out, table, start, cos, sin)
+
+
 def test_append_positions_past_32_bits(device):
     q, k, v, kc, vc, table, lens, cos, sin, _, _, host = base.append_case("C2 geometry bf16", device)
     a = (kc.clone(), vc.clone())
