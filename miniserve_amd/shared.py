@@ -13,7 +13,7 @@ import torch
 
 from . import _native as nat
 from .attention import (_host_ints_to_device, _require_gpu, _workspace, block_table_i32,
-                        context_lens_i32, paged_attention)
+                        context_lens_i32, narrow_i32, paged_attention)
 from .rotary import extent, on_device
 
 
@@ -21,12 +21,12 @@ def _groups_i32(group_rows, prefix_pages, batch: int, width: int, dev: torch.dev
                 ) -> tuple[torch.Tensor, torch.Tensor]:
     """(int32 [groups + 1], int32 [groups]) on `dev`; host values are checked."""
     out = []
-    for name, x in (("group_rows", group_rows), ("prefix_pages", prefix_pages)):
+    for name, x, most in (("group_rows", group_rows, batch), ("prefix_pages", prefix_pages, width)):
         if isinstance(x, torch.Tensor) and x.device == dev:
             if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool:
                 raise ValueError(f"{name} must hold whole numbers")
             x = x if x.ndim == 1 else x.reshape(-1)
-            out.append((x if x.dtype == torch.int32 else x.to(torch.int32)).contiguous())
+            out.append(narrow_i32(x, 0, most).contiguous())
             continue
         values = [int(v) for v in (x.reshape(-1).tolist() if isinstance(x, torch.Tensor) else x)]
         if name == "group_rows":

@@ -1,0 +1,29 @@
+"""Attention behind shared prefixes at the ends of its arguments."""
+import pytest
+import torch
+
+from miniserve_amd import shared
+from test_gpu_shared import BF16, Batch, note
+
+pytestmark = pytest.mark.gpu
+
+
+def test_device_groups_past_32_bits(device):
+    """int64 group rows and pages past int32 count as the nearest bound, not modulo 2^32."""
+    x = Batch(8, 2, 64, BF16, BF16, [(0, 3, 6), (3, 3, 9)], [120, 100, 97, 200, 150, 145], 1)
+    want = x.call()
+    note("group rows past 32 bits")
+    x.rows = torch.tensor([-2 ** 40, 3, 2 ** 31], device=device)
+    x.pages = torch.tensor([6, 9], device=device)
+    assert torch.equal(want, x.call())
+    # all pages shared: 2^32 + 1 pages are the table's, not one; -2^32 + 4 none, not four
+    for b in range(3):
+        x.table[b], x.table[3 + b] = x.table[0], x.table[3]
+    x.rows = [0, 3, 6]
+    note("prefix pages past 32 bits")
+    got = {}
+    for name, pages in (("wide", [2 ** 32 + 1, -2 ** 32 + 4]), ("bounds", [x.table.shape[1], 0])):
+        x.pages = torch.tensor(pages, device=device)
+        got[name] = x.call()
+        x.check(got[name])
+    assert torch.equal(got["wide"], got["bounds"])
