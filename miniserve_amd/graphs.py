@@ -86,7 +86,8 @@ class GraphedDecodeRunner:
         msattn_paged_attention_append call (one launch where the partition kernel takes
         it, the same caches and output bit for bit); False keeps the two calls.
         rope: (cos, sin) tables [max_pos, rotary_dim]; decode() then takes unrotated q and k,
-        which are rotated at each row's new position on the way, in the same launches."""
+        which are rotated at each row's new position on the way, in the same launches. A step
+        that has a position past the tables is refused."""
         buckets = list(buckets)
         if not buckets or sorted(buckets) != buckets or buckets[0] < 1:
             raise ValueError("buckets must be sorted, start at 1")
@@ -255,6 +256,8 @@ class GraphedDecodeRunner:
         top = int(lens[:B].max())
         if top > self.max_context:
             raise ValueError(f"context {top} > table capacity {self.max_context}")
+        if self.rope is not None and top > self.rope[0].shape[0]:
+            raise ValueError(f"context {top} > {self.rope[0].shape[0]} positions of the rotation tables")
         self._in[idx]["ints"].copy_(self._stage[idx], non_blocking=True)
         ev = torch.cuda.Event()
         ev.record()

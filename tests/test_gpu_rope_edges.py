@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import test_gpu_rope_write as base
-from miniserve_amd import paged_attention_append, write_kv_rope
+from miniserve_amd import PagedAttention, paged_attention_append, write_kv_rope
+from miniserve_amd.graphs import DecodeLayer, GraphedDecodeRunner
 from oracle import dense
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +100,34 @@ def test_append_over_an_infinite_key(device, name):
              (n * 2.0 ** -24 if q.dtype == F16 else 0)) * vv.abs().max().item()
     assert (out - want)[:, :H - 1].abs().max().item() <= bound
     assert not bool(out[:, H - 1].isfinite().any())
+
+
+def runner_of(device, W, rope, H=14, KVH=2, D=64, fused=True):
+    pa = PagedAttention(H, KVH, D, num_blocks=16, block_size=16, dtype=BF16, device=device,
+                        kv_dtype=BF16)
+    caches = pa.allocate_kv_cache()
+    return GraphedDecodeRunner([DecodeLayer(pa, *caches)], W, buckets=(1, 2), fused_append=fused,
+                               rope=rope), caches
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_runner_refuses_positions_past_its_tables(device, fused):
+    """A context longer than the rotation tables has no position there: the step is refused before
+    it writes; one that fits runs."""
+    cos, sin = tables(40, 64, device)
+    runner, caches = runner_of(device, 4, (cos, sin), fused=fused)
+    g = torch.Generator().manual_seed(3)
+    rnd = lambda n: torch.randn(1, 2, 1, n, 64, generator=g).to(BF16).to(device)  # noqa: E731
+    q, k, v = rnd(14), rnd(2), rnd(2)
+    rows = [[0, 1, 2, 3], [4, 5, 6, 7]]
+    note("positions past the tables")
+    for ctx in ([3, 40], [63, 0]):
+        with pytest.raises(ValueError, match="rotation tables"):
+            runner.decode(q, k, v, rows, ctx)
+        assert not bits(caches[0]).any() and not bits(caches[1]).any()
+    out = runner.decode(q, k, v, rows, [3, 39])
+    a = [torch.zeros_like(c) for c in caches]
+    lens = torch.tensor([4, 40], dtype=torch.int32, device=device)
+    write_kv_rope(q[0], k[0], v[0], *a, torch.tensor(rows, dtype=torch.int32, device=device),
+                  lens - 1, cos, sin)
+    assert torch.equal(caches[0], a[0]) and torch.equal(caches[1], a[1]) and bool(out.isfinite().all())
