@@ -28,7 +28,7 @@ from typing import Sequence
 import torch
 
 from . import _native as nat
-from .rotary import on_device, rope_table, write_kv_rope
+from .rotary import on_16_bytes, on_device, rope_table, write_kv_rope
 
 _BACKENDS = ("sdpa", "triton_flash")
 
@@ -563,7 +563,7 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
     position[b], clamped to [0, max_pos): ``write_kv_rope`` of the new token, then the decode,
     in the launches of the call without it (msattn_paged_attention_append_rope). With at most 8
     query heads a KV head the rotated query is used to twice its type's digits instead of rounded
-    to it. A rotary_dim below head_dim makes the two calls.
+    to it. A rotary_dim below head_dim makes the two calls. Tables off 16 bytes are copied.
     """
     _require_gpu(query, "query")
     _require_gpu(k_cache, "k_cache")
@@ -632,6 +632,7 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
             q = write_kv_rope(q, kn, vn, k_cache, v_cache, table, lens - 1, cos, sin, pos)
             return paged_attention(q, k_cache, v_cache, table, lens, window=window, scale=scale,
                                    max_context=max_context, workspace=workspace, out=out)
+        cos, sin = on_16_bytes(cos), on_16_bytes(sin)
         status = on_device(
             dev, L.msattn_paged_attention_append_rope,
             q.data_ptr(), kn.data_ptr(), vn.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),

@@ -35,7 +35,7 @@ import torch
 
 from . import _native as nat
 from .attention import PagedAttention, paged_attention, paged_attention_append
-from .rotary import rope_table, write_kv_rope
+from .rotary import on_16_bytes, rope_table, write_kv_rope
 
 
 def fill_table(tab: np.ndarray, tables, batch: int) -> None:
@@ -116,8 +116,8 @@ class GraphedDecodeRunner:
                             self.num_kv_heads, self.head_dim)
         dev = self._device
         # (the captured graphs hold the tables' addresses: the runner keeps them)
-        self.rope = None if rope is None else (rope_table(rope[0], dev, "cos"),
-                                               rope_table(rope[1], dev, "sin"))
+        self.rope = None if rope is None else (on_16_bytes(rope_table(rope[0], dev, "cos")),
+                                               on_16_bytes(rope_table(rope[1], dev, "sin")))
 
         Wt = self.table_width
 

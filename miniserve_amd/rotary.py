@@ -35,6 +35,11 @@ def rope_table(t, dev: torch.device, what: str) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def on_16_bytes(t: torch.Tensor) -> torch.Tensor:
+    """`t`, or a copy where it lies off 16 bytes (the decode kernels read 16 of a table at once)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def extent(t: torch.Tensor) -> tuple[int, int]:
     """First byte that `t` addresses and the one past its last."""
     lo = t.data_ptr()

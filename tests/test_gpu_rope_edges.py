@@ -102,6 +102,18 @@ def test_append_over_an_infinite_key(device, name):
     assert not bool(out[:, H - 1].isfinite().any())
 
 
+@pytest.mark.parametrize("name", ["C2 geometry bf16", "fp32", "stream-K, fp8 (two launches)",
+                                  "head_dim 80 (two launches)"])
+def test_append_takes_tables_off_16_bytes(device, name):
+    q, k, v, kc, vc, table, lens, cos, sin, _, _, _ = base.append_case(name, device)
+    a = (kc.clone(), vc.clone())
+    off = lambda t: torch.empty(t.numel() + 1, device=device)[1:].view(t.shape).copy_(t)  # noqa: E731
+    note(f"tables off 16 bytes, {name}")
+    want = paged_attention_append(q, k, v, *a, table, lens, rope=(cos, sin))
+    out = paged_attention_append(q, k, v, kc, vc, table, lens, rope=(off(cos), off(sin)))
+    assert torch.equal(out, want) and torch.equal(bits(kc), bits(a[0]))
+
+
 def runner_of(device, W, rope, H=14, KVH=2, D=64, fused=True):
     pa = PagedAttention(H, KVH, D, num_blocks=16, block_size=16, dtype=BF16, device=device,
                         kv_dtype=BF16)
@@ -131,3 +143,15 @@ def test_runner_refuses_positions_past_its_tables(device, fused):
     write_kv_rope(q[0], k[0], v[0], *a, torch.tensor(rows, dtype=torch.int32, device=device),
                   lens - 1, cos, sin)
     assert torch.equal(caches[0], a[0]) and torch.equal(caches[1], a[1]) and bool(out.isfinite().all())
+
+
+def test_runner_takes_tables_off_16_bytes(device):
+    cos, sin = tables(64, 64, device)
+    off = lambda t: torch.empty(t.numel() + 1, device=device)[1:].view(t.shape).copy_(t)  # noqa: E731
+    g = torch.Generator().manual_seed(4)
+    rnd = lambda n: torch.randn(1, 2, 1, n, 64, generator=g).to(BF16).to(device)  # noqa: E731
+    q, k, v = rnd(14), rnd(2), rnd(2)
+    rows = [[0, 1, 2, 3], [4, 5, 6, 7]]
+    note("runner, tables off 16 bytes")
+    got = [runner_of(device, 4, r)[0].decode(q, k, v, rows, [3, 39]) for r in ((cos, sin), (off(cos), off(sin)))]
+    assert torch.equal(*got)
