@@ -28,7 +28,7 @@ from typing import Sequence
 import torch
 
 from . import _native as nat
-from .rotary import on_16_bytes, on_device, rope_table, write_kv_rope
+from .rotary import current, on_16_bytes, on_device, rope_table, write_kv_rope
 
 _BACKENDS = ("sdpa", "triton_flash")
 
@@ -629,9 +629,10 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
                 raise ValueError(f"position has {pos.numel()} entries for a batch of {B}")
             pos = pos.contiguous()
         if cos.shape[1] < D:
-            q = write_kv_rope(q, kn, vn, k_cache, v_cache, table, lens - 1, cos, sin, pos)
-            return paged_attention(q, k_cache, v_cache, table, lens, window=window, scale=scale,
-                                   max_context=max_context, workspace=workspace, out=out)
+            with current(dev):
+                q = write_kv_rope(q, kn, vn, k_cache, v_cache, table, lens - 1, cos, sin, pos)
+                return paged_attention(q, k_cache, v_cache, table, lens, window=window, scale=scale,
+                                       max_context=max_context, workspace=workspace, out=out)
         cos, sin = on_16_bytes(cos), on_16_bytes(sin)
         status = on_device(
             dev, L.msattn_paged_attention_append_rope,

@@ -7,6 +7,7 @@ one launch of libmsattn.so (msattn_write_kv_rope). The single-token form that go
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Sequence
 
@@ -16,6 +17,12 @@ from . import _native as nat
 
 _I64x3 = ctypes.c_int64 * 3
 _SOURCES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def current(dev: torch.device):
+    """A context with `dev` current."""
+    return contextlib.nullcontext() if dev.index is None or \
+        torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def on_device(dev: torch.device, fn, *args) -> int:

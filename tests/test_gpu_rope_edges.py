@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import test_gpu_rope_write as base
-from miniserve_amd import PagedAttention, paged_attention_append, write_kv_rope
+from miniserve_amd import PagedAttention, attention, paged_attention_append, write_kv_rope
 from miniserve_amd.graphs import DecodeLayer, GraphedDecodeRunner
 from oracle import dense
 
@@ -155,3 +155,31 @@ def test_runner_takes_tables_off_16_bytes(device):
     note("runner, tables off 16 bytes")
     got = [runner_of(device, 4, r)[0].decode(q, k, v, rows, [3, 39]) for r in ((cos, sin), (off(cos), off(sin)))]
     assert torch.equal(*got)
+
+
+def test_partial_rotation_on_another_device_than_the_current_one(device, monkeypatch):
+    """Every launch of an append with a rotary size below head_dim runs with the tensors' device
+    current: here the current one is reported as another, and entering a device is recorded."""
+    q, k, v, kc, vc, table, lens, _, _, _, _, _ = base.append_case("C2 geometry bf16", device)
+    cos, sin = tables(64 * 16, 32, device)
+    inside = []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            inside.append(self.dev)
+
+        def __exit__(self, *e):
+            inside.pop()
+
+    seen = []
+    real_write, real_attend = attention.write_kv_rope, attention.paged_attention
+    monkeypatch.setattr(attention, "write_kv_rope", lambda *a, **kw: (seen.append(list(inside)), real_write(*a, **kw))[1])
+    monkeypatch.setattr(attention, "paged_attention", lambda *a, **kw: (seen.append(list(inside)), real_attend(*a, **kw))[1])
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 7)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    note("another device")
+    paged_attention_append(q, k, v, kc, vc, table, lens, rope=(cos, sin))
+    assert seen[-1] == [device] and len(seen) == 2 and not inside
