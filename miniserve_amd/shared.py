@@ -14,7 +14,7 @@ import torch
 from . import _native as nat
 from .attention import (_host_ints_to_device, _require_gpu, _workspace, block_table_i32,
                         context_lens_i32, narrow_i32, paged_attention)
-from .rotary import extent, on_device
+from .rotary import current, extent, on_device
 
 
 def _groups_i32(group_rows, prefix_pages, batch: int, width: int, dev: torch.device
@@ -90,8 +90,9 @@ def paged_attention_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     rows, pages = _groups_i32(group_rows, prefix_pages, B, W, dev)
     groups = pages.numel()
     if groups == 0 or B == 0 or q_len == 0:
-        return paged_attention(query, k_cache, v_cache, table, context_lens, scale=scale,
-                               max_context=max_context, workspace=workspace, out=out)
+        with current(dev):
+            return paged_attention(query, k_cache, v_cache, table, context_lens, scale=scale,
+                                   max_context=max_context, workspace=workspace, out=out)
     lens, host_max = context_lens_i32(context_lens, dev, B)
     cap = W * bs
     if max_context is None:

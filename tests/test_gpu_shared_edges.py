@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from miniserve_amd import shared
+from miniserve_amd import paged_attention_shared, shared
 from test_gpu_shared import BF16, Batch, note
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +27,30 @@ def test_device_groups_past_32_bits(device):
         got[name] = x.call()
         x.check(got[name])
     assert torch.equal(got["wide"], got["bounds"])
+
+
+def test_no_group_on_another_device_than_the_current_one(device, monkeypatch):
+    """A call without a group runs paged_attention with the tensors' device current."""
+    x = Batch(8, 2, 64, BF16, BF16, [(0, 3, 6)], [120, 100, 97], 1)
+    x.rows, x.pages = [], []
+    inside, seen = [], []
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            inside.append(self.dev)
+
+        def __exit__(self, *e):
+            inside.pop()
+
+    real = shared.paged_attention
+    monkeypatch.setattr(shared, "paged_attention", lambda *a, **kw: (seen.append(list(inside)), real(*a, **kw))[1])
+    args = [t.to(device) for t in (x.q, x.kc, x.vc, x.table)]
+    lens = torch.tensor(x.lens, dtype=torch.int32, device=device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 7)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    note("another device")
+    paged_attention_shared(*args, lens, [], [])
+    assert seen == [[device]] and not inside
