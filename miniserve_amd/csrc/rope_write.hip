@@ -258,7 +258,7 @@ static hipError_t launch_rope_write_one(const RopeWriteParams& p_in, hipStream_t
     int64_t slices = (kRwWant + tokens - 1) / tokens;
     p.slices = static_cast<int>(slices < most ? slices : most);
     const int64_t blocks = (tokens * p.slices + kRwWaves - 1) / kRwWaves;
-    if (blocks < (int64_t(1) << 31)) {
+    if (blocks * kRwThreads < (int64_t(1) << 32)) {  // (a launch's threads are counted in 32 bits)
       hipLaunchKernelGGL((rope_write_vec_kernel<ST, KT, E>), dim3(static_cast<unsigned>(blocks)),
                          dim3(kRwThreads), 0, stream, p);
       return hipGetLastError();

@@ -183,3 +183,29 @@ def test_partial_rotation_on_another_device_than_the_current_one(device, monkeyp
     note("another device")
     paged_attention_append(q, k, v, kc, vc, table, lens, rope=(cos, sin))
     assert seen[-1] == [device] and len(seen) == 2 and not inside
+
+
+def test_more_tokens_than_a_launch_holds_waves(device):
+    """2^26 + 8 tokens: a wave each would be a launch of more than 2^32 threads."""
+    T, D = 2 ** 26 + 8, 16
+    g = torch.Generator().manual_seed(12)
+    some = torch.randn(2 ** 16, 1, D, generator=g).to(BF16).to(device)
+    q = some.repeat(2 ** 10 + 1, 1, 1)[None, :T]
+    k = some[:1].expand(1, T, 1, D)
+    kc, vc = base.pool(2, 16, 1, D, BF16, g, device)
+    kc0, vc0 = kc.clone(), vc.clone()
+    cos, sin = tables(3, D, device)
+    note("more than 2^26 tokens")
+    out = write_kv_rope(q, k, k, kc, vc, torch.tensor([[-1]], dtype=torch.int32, device=device), 0,
+                        cos, sin)
+    x = some.float()
+    turned = torch.cat((-x[..., D // 2:], x[..., :D // 2]), -1)
+    for t in range(2):  # (positions 0 and 1; all others are past the tables: their last row)
+        y = (x[t] * cos[t] + turned[t] * sin[t]).to(BF16)
+        assert torch.equal(out[0, t], y)
+    y = (x * cos[2] + turned * sin[2]).to(BF16)
+    for t in range(0, T, 2 ** 16):
+        n = min(2 ** 16, T - t)
+        lo = 2 if t == 0 else 0
+        assert torch.equal(out[0, t + lo:t + n], y[lo:n])
+    assert torch.equal(kc, kc0) and torch.equal(vc, vc0)
