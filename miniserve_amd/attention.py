@@ -589,6 +589,13 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
     if window is not None and window <= 0:
         raise ValueError("window must be positive")
     dev = query.device
+    if k_cache.device != dev or v_cache.device != dev or k_new.device != dev or v_new.device != dev:
+        raise ValueError("query, k_new, v_new and the caches must be on one device")
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or
+                            out.device != dev or not out.is_contiguous()):
+        raise ValueError("out must be contiguous, of the query's shape, dtype and device")
+    if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
+        raise ValueError("workspace must be contiguous and on the query's device")
     q = query.contiguous()
     kn = k_new.contiguous()
     vn = v_new.contiguous()

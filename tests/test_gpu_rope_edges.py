@@ -209,3 +209,25 @@ def test_more_tokens_than_a_launch_holds_waves(device):
         lo = 2 if t == 0 else 0
         assert torch.equal(out[0, t + lo:t + n], y[lo:n])
     assert torch.equal(kc, kc0) and torch.equal(vc, vc0)
+
+
+@pytest.mark.parametrize("rope", [False, True])
+def test_append_refuses_what_lies_elsewhere(device, rope):
+    """New rows, caches, output and workspace that the kernels could not address."""
+    q, k, v, kc, vc, table, lens, cos, sin, _, _, _ = base.append_case("C2 geometry bf16", device)
+    a = (kc.clone(), vc.clone())
+    B, _, H, D = q.shape
+    ok = dict(k=k, v=v, kc=kc, vc=vc, out=None, workspace=None)
+    bytes_ = 64 << 20
+    note("operands elsewhere")
+    for bad in (dict(k=k.cpu()), dict(v=v.cpu()), dict(out=torch.empty(B, 1, H, D, dtype=BF16)),
+                dict(out=torch.empty(B - 1, 1, H, D, dtype=BF16, device=device)),
+                dict(out=torch.empty(B, 1, H, D, device=device)),
+                dict(out=torch.empty(B, 1, D, H, dtype=BF16, device=device).transpose(2, 3)),
+                dict(workspace=torch.zeros(bytes_, dtype=torch.uint8)),
+                dict(workspace=torch.zeros(2 * bytes_, dtype=torch.uint8, device=device)[::2])):
+        x = dict(ok, **bad)
+        with pytest.raises(ValueError, match="device|out must"):
+            paged_attention_append(q, x["k"], x["v"], x["kc"], x["vc"], table, lens, out=x["out"],
+                                   workspace=x["workspace"], rope=(cos, sin) if rope else None)
+    assert torch.equal(bits(kc), bits(a[0])) and torch.equal(bits(vc), bits(a[1]))
