@@ -108,6 +108,8 @@ def paged_attention_shared(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or \
             not out.is_contiguous():
         raise ValueError("out must be contiguous, of the query's shape, dtype and device")
+    if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
+        raise ValueError("workspace must be contiguous and on the query's device")
     lib = nat.lib()
     ws_bytes = lib.msattn_shared_workspace_bytes(B, q_len, H, KVH, D, max_context, groups)
     if ws_bytes == 0:

@@ -54,3 +54,12 @@ def test_no_group_on_another_device_than_the_current_one(device, monkeypatch):
     note("another device")
     paged_attention_shared(*args, lens, [], [])
     assert seen == [[device]] and not inside
+
+
+def test_refuses_a_workspace_elsewhere(device):
+    x = Batch(8, 2, 64, BF16, BF16, [(0, 3, 6)], [120, 100, 97], 1)
+    note("workspace elsewhere")
+    for ws in (torch.zeros(64 << 20, dtype=torch.uint8),
+               torch.zeros(128 << 20, dtype=torch.uint8, device=device)[::2]):
+        with pytest.raises(ValueError, match="workspace must"):
+            x.call(workspace=ws)
