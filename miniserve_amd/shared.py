@@ -22,13 +22,17 @@ def _groups_i32(group_rows, prefix_pages, batch: int, width: int, dev: torch.dev
     """(int32 [groups + 1], int32 [groups]) on `dev`; host values are checked."""
     out = []
     for name, x, most in (("group_rows", group_rows, batch), ("prefix_pages", prefix_pages, width)):
+        if isinstance(x, torch.Tensor) and (x.dtype.is_floating_point or x.dtype.is_complex or
+                                            x.dtype == torch.bool):
+            raise ValueError(f"{name} must hold whole numbers")
         if isinstance(x, torch.Tensor) and x.device == dev:
-            if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool:
-                raise ValueError(f"{name} must hold whole numbers")
             x = x if x.ndim == 1 else x.reshape(-1)
             out.append(narrow_i32(x, 0, most).contiguous())
             continue
-        values = [int(v) for v in (x.reshape(-1).tolist() if isinstance(x, torch.Tensor) else x)]
+        given = x.reshape(-1).tolist() if isinstance(x, torch.Tensor) else list(x)
+        values = [int(v) for v in given]
+        if values != given:
+            raise ValueError(f"{name} must hold whole numbers")
         if name == "group_rows":
             if any(a > b for a, b in zip(values, values[1:])) or \
                     any(not 0 <= v <= batch for v in values):
