@@ -565,9 +565,12 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
     query heads a KV head the rotated query is used to twice its type's digits instead of rounded
     to it. A rotary_dim below head_dim makes the two calls. Tables off 16 bytes are copied.
     """
-    _require_gpu(query, "query")
-    _require_gpu(k_cache, "k_cache")
-    _require_gpu(v_cache, "v_cache")
+    at = query.get_device()
+    if at < 0 or k_cache.get_device() != at or v_cache.get_device() != at or \
+            k_new.get_device() != at or v_new.get_device() != at:
+        for name, x in (("query", query), ("k_cache", k_cache), ("v_cache", v_cache)):
+            _require_gpu(x, name)
+        raise ValueError("query, k_new, v_new and the caches must be on one device")
     if query.ndim != 4 or query.shape[1] != 1:
         raise ValueError("query must be [batch, 1, heads, head_dim] (decode)")
     if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype \
@@ -589,8 +592,6 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
     if window is not None and window <= 0:
         raise ValueError("window must be positive")
     dev = query.device
-    if k_cache.device != dev or v_cache.device != dev or k_new.device != dev or v_new.device != dev:
-        raise ValueError("query, k_new, v_new and the caches must be on one device")
     if out is not None and (out.shape != query.shape or out.dtype != query.dtype or
                             out.device != dev or not out.is_contiguous()):
         raise ValueError("out must be contiguous, of the query's shape, dtype and device")
