@@ -371,7 +371,8 @@ int msattn_paged_attention_append(const void* query, const void* k_new, const vo
  * of a source with query_out or the caches is allowed. query == NULL: keys and values alone
  * (query_out, both query strides and num_heads are not read). *_strides: batch, token and head
  * strides in elements, at least 0, read on the host; head dim contiguous. src_dtype is fp32, fp16
- * or bf16, head_dim up to 256. Two tokens of one launch in one cache slot: either's row remains.
+ * or bf16, head_dim up to 256. Two tokens of one launch in one cache slot are the caller's to
+ * avoid: parts of either's rows may remain there.
  * The reference makes these calls one by one (miniserve/model_runner.py:62-76).
  */
 int msattn_write_kv_rope(const void* query, const int64_t* q_strides, void* query_out,
@@ -394,9 +395,12 @@ int msattn_write_kv_rope(const void* query, const int64_t* q_strides, void* quer
  * msattn_paged_attention_append is one, and for most fp32 queries on the partition kernel (in
  * small launches only over an fp32 cache of head_dim 128), else the write, then the decode: the
  * same caches and output as msattn_write_kv_rope of the new token followed by
- * msattn_paged_attention_rope, but for the rotated query: a 2-byte one with at most 8 query heads
- * a KV head is used to twice its type's digits (those of fp32 in the generic kernel), not rounded
- * to the type.
+ * msattn_paged_attention_rope, but for the digits of a 2-byte rotated query, which those calls
+ * round to its type: here it keeps twice the type's with at most 8 query heads a KV head, those
+ * of fp32 in the generic kernel whatever the heads, and is rounded elsewhere. (A key with an
+ * infinite element has the rounded query's score.) With a 2-byte query the matrix-core kernels
+ * round the weights of the values to its type, as msattn_paged_attention does; maxima, sums and
+ * accumulators are fp32.
  */
 int msattn_paged_attention_append_rope(
     const void* query, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
@@ -425,7 +429,9 @@ size_t msattn_shared_workspace_bytes(int batch, int q_len, int num_heads, int nu
  * any q_len: each prefix is read once per KV head and 128 query rows for the whole group, through
  * the table of the group's first row whose queries all see it whole; the caller is trusted that
  * the other such rows' entries are the same. The rows that do not (a padding row of length 0, say)
- * read what they see of it by themselves, through their own.
+ * read what they see of it by themselves, through their own. The weights of the values are rounded
+ * to the query type, and their sum is that of the rounded ones; maxima, sums and accumulators are
+ * fp32.
  * Other types and layouts than a bf16 or fp16 query (16-byte aligned) over a cache of its type or
  * of fp8 e4m3, head_dim 64 or 128, block_size a multiple of 16, 16-byte aligned cache rows, up to
  * 1024 rows and groups and 64 query rows a KV head and batch row, and calls without a group, run

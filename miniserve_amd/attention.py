@@ -562,8 +562,9 @@ def paged_attention_append(query: torch.Tensor, k_new: torch.Tensor, v_new: torc
     way (rotate-half, fp32 tables [max_pos, rotary_dim]), at context_lens[b] - 1 or at
     position[b], clamped to [0, max_pos): ``write_kv_rope`` of the new token, then the decode,
     in the launches of the call without it (msattn_paged_attention_append_rope). With at most 8
-    query heads a KV head the rotated query is used to twice its type's digits instead of rounded
-    to it. A rotary_dim below head_dim makes the two calls. Tables off 16 bytes are copied.
+    query heads a KV head, or on the generic kernel, the rotated query is used to twice its type's
+    digits or more instead of rounded to it. A rotary_dim below head_dim makes the two calls, which
+    round it. Tables off 16 bytes are copied.
     """
     at = query.get_device()
     if at < 0 or k_cache.get_device() != at or v_cache.get_device() != at or \

@@ -86,8 +86,10 @@ class GraphedDecodeRunner:
         msattn_paged_attention_append call (one launch where the partition kernel takes
         it, the same caches and output bit for bit); False keeps the two calls.
         rope: (cos, sin) tables [max_pos, rotary_dim]; decode() then takes unrotated q and k,
-        which are rotated at each row's new position on the way, in the same launches. A step
-        that has a position past the tables is refused."""
+        which are rotated at each row's new position on the way, in the same launches. The two
+        calls round the rotated query to its type, where the one may keep more of its digits
+        (paged_attention_append): the same caches, outputs that may differ in the last place. A
+        step that has a position past the tables is refused."""
         buckets = list(buckets)
         if not buckets or sorted(buckets) != buckets or buckets[0] < 1:
             raise ValueError("buckets must be sorted, start at 1")

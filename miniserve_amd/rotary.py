@@ -119,8 +119,8 @@ def write_kv_rope(query: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
 
     Everything is computed in fp32 and rounded once: queries to their type, keys and values to
     the cache's. Returns the rotated queries, contiguous, or ``out``, which may be ``query``
-    itself (rotated in place). Two tokens of one call that land in one cache slot leave either's
-    row there.
+    itself (rotated in place). Two tokens of one call must not land in one cache slot: parts of
+    either's rows may remain there.
     """
     if not (k_cache.is_cuda and v_cache.is_cuda and k.is_cuda and v.is_cuda):
         for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k", k), ("v", v)):

@@ -5,9 +5,11 @@ import pytest
 import torch
 
 import test_gpu_rope_write as base
-from miniserve_amd import PagedAttention, attention, paged_attention_append, write_kv_rope
+from miniserve_amd import (PagedAttention, attention, kernel_route, paged_attention_append,
+                           write_kv_rope)
 from miniserve_amd.graphs import DecodeLayer, GraphedDecodeRunner
 from oracle import dense
+from test_gpu_serving_places import attend
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16, FP8 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn
@@ -231,3 +233,25 @@ def test_append_refuses_what_lies_elsewhere(device, rope):
             paged_attention_append(q, x["k"], x["v"], x["kc"], x["vc"], table, lens, out=x["out"],
                                    workspace=x["workspace"], rope=(cos, sin) if rope else None)
     assert torch.equal(bits(kc), bits(a[0])) and torch.equal(bits(vc), bits(a[1]))
+
+
+@pytest.mark.parametrize("qt", [BF16, F16])
+def test_generic_append_of_many_query_heads(device, qt):
+    """16 query heads a KV head at head_dim 80, the generic kernel: it keeps the rotated query in fp32
+    whatever the heads, so that the bound of the query in two parts holds."""
+    g = torch.Generator().manual_seed(13)
+    B, H, KVH, D, bs, W = 4, 32, 2, 80, 16, 16
+    kc, vc = base.pool(B * W, bs, KVH, D, qt, g, device)
+    table = torch.randperm(B * W, generator=g).view(B, W).to(torch.int32)
+    host = [37, 256, 100, 18]
+    lens = torch.tensor(host, dtype=torch.int32, device=device)
+    q, k, v = (torch.randn(B, 1, n, D, generator=g).to(qt).to(device) for n in (H, KVH, KVH))
+    cos, sin = tables(W * bs, D, device)
+    assert kernel_route(q, kc, table) == "generic"
+    note(f"generic, 16 heads a KV head, {qt}")
+    out = paged_attention_append(q, k, v, kc, vc, table.to(device), lens, rope=(cos, sin)).cpu().double()
+    turned, _ = rotate64(q, cos, sin, torch.tensor(host)[:, None] - 1)
+    for b, n in enumerate(host):
+        kk, vv = (torch.from_numpy(dense.gather_rows(c.cpu(), table[b], n)) for c in (kc, vc))
+        want, bound = attend(turned[b], kk, vv, qt, True, bs)
+        assert ((out[b] - want).abs() - bound).max().item() <= 0
