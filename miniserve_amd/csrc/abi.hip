@@ -1764,7 +1764,11 @@ SharedLayout shared_layout(int batch, int q_len, int num_heads, int head_dim) {
 // queries that the prefill kernels' products, not the reads, set the time. (16 rows in 2 groups,
 // prefixes of 2048 to 4096 and up to 512 own keys, this kernel against those: H32/KVH8 of 128 dims
 // at 32 query rows 53 and 105 us, at 64 70 and 73, at 96 76 and 67, at 128 92 and 66; over fp8 at
-// 64 70 and 78, at 128 114 and 82; H14/KVH2 of 64 at 56 28 and 44, at 112 35 and 29.)
+// 64 70 and 78, at 128 114 and 82; H14/KVH2 of 64 at 56 28 and 44, at 112 35 and 29. The groups' size
+// hardly moves the line: 16 rows in 8 groups, 32 in one and 64 in two, H32/KVH8/D128 bf16 at 64
+// query rows 53 and 63, 85 and 84, 148 and 165, at 96 65 and 64, 112 and 86, 207 and 169; over fp8 at
+// 64 50 and 67, 77 and 92, 140 and 181, at 96 64 and 68, 103 and 94, 188 and 183; H14/KVH2/D64 is
+// ahead up to 91 rows by 3 to 15 % and behind at 126.)
 #ifndef MSATTN_SHARED_MAX_QUERY_ROWS
 #define MSATTN_SHARED_MAX_QUERY_ROWS 64
 #endif

@@ -184,7 +184,12 @@ __global__ __launch_bounds__(kRwThreads) void rope_write_vec_kernel(const RopeWr
 }
 
 // Any sizes and alignments, element by element: a thread takes a pair (d, d + R/2) of one row,
-// or one dim past R.
+// or one dim past R, and finds its token's page and table row for itself. Bound by that: from some
+// 256 tokens on 3 to 6 times the vector form's time (bf16 rows off 16 bytes, H32/KVH8/D128, 64 tokens
+// 4.0 us and 4.0, 1024 24 and 7.9, 16384 386 and 85; 24 + 2 x 8 heads of 96 dims, 8192 tokens, 24
+// rotated, off the chunks, 166 and, 32 rotated, 27). Copying 16-bit sources off 16 bytes first would
+// pay from 5 M elements on (6 M 24.0 and 21.0 with the three copies, 24 M 88 and 43; 1.5 M 7.7 and
+// 11.7), fp32 ones nowhere by much (24 M 84 and 101, 96 M 435 and 409).
 template <typename ST, typename KT>
 __global__ __launch_bounds__(kRwThreads) void rope_write_elt_kernel(const RopeWriteParams p) {
   const int half = p.R / 2;

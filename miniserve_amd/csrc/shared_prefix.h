@@ -1,6 +1,6 @@
 // Attention for a batch whose rows come in groups, each group behind a prefix of its own: the
 // same physical pages in every row of the group (gfx950; a bf16/fp16 query over a cache of its
-// type or of fp8 e4m3, head_dim 64 or 128, any number of query tokens a row).
+// type or of fp8 e4m3, head_dim 64 or 128, one query token a row or several).
 //
 // The work is a list of segments: one a group (the prefix's keys, read once for the query rows of
 // every member) and one a batch row (the keys past its prefix, or all of them). A segment falls
@@ -71,7 +71,10 @@ constexpr int kShAux = MSATTN_SHARED_AUX;
 // many for the matrix cores and the softmax. (From a fit of the workgroups' clocks to their pieces
 // and blocks, then tried around. 64 rows in 8 groups of H32/KVH8/D128 took 81 us in shares of equal
 // tiles, 63 with one row of costs for all types and sizes and 56 with these, all before the
-// nontemporal reads.)
+// nontemporal reads. 40 calls of H14/KVH2/D64, H16/KVH8/D64, H28/KVH4/D128 and H32/KVH8/D128, 16-bit
+// and fp8, 16 to 64 rows in 1 to 8 groups, 1 to 4 tokens: the first row for all 2 % less to 28 % more
+// but for one call of 16 rows (H28/KVH4 over fp8, 18.4 us here, 15.1), block costs halved 2 % less to
+// 26 % more, half as much again 6 % less to 9 % more but for the same call.)
 #ifndef MSATTN_SHARED_COSTS
 #define MSATTN_SHARED_COSTS {20, 6, 7, 9, 12}, {20, 3, 4, 5, 7}, {20, 2, 3, 5, 8}, {20, 2, 3, 4, 6}
 #endif
