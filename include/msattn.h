@@ -429,9 +429,10 @@ size_t msattn_shared_workspace_bytes(int batch, int q_len, int num_heads, int nu
  * any q_len: each prefix is read once per KV head and 128 query rows for the whole group, through
  * the table of the group's first row whose queries all see it whole; the caller is trusted that
  * the other such rows' entries are the same. The rows that do not (a padding row of length 0, say)
- * read what they see of it by themselves, through their own. The weights of the values are rounded
- * to the query type, and their sum is that of the rounded ones; maxima, sums and accumulators are
- * fp32.
+ * read what they see of it by themselves, through their own. An infinite or NaN value reaches the
+ * queries that see its key alone (msattn_paged_attention may let it reach earlier queries of the
+ * row). The weights of the values are rounded to the query type, and their sum is that of the
+ * rounded ones; maxima, sums and accumulators are fp32.
  * Other types and layouts than a bf16 or fp16 query (16-byte aligned) over a cache of its type or
  * of fp8 e4m3, head_dim 64 or 128, block_size a multiple of 16, 16-byte aligned cache rows, up to
  * 1024 rows and groups and 64 query rows a KV head and batch row, and calls without a group, run

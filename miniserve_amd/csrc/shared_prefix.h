@@ -164,6 +164,25 @@ __device__ __forceinline__ void sh_barrier() {
 // s_waitcnt immediate (gfx9 encoding): at most N vector memory operations outstanding.
 constexpr int sh_wait_vm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
 
+// `x`, from here on: what is found from it is not found ahead of the loops around, where it would hold
+// registers that they need (22 in all; 16-bit caches at 128 dims spilled up to 19 without).
+__device__ __forceinline__ int sh_here(int x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(x));
+#endif
+  return x;
+}
+
+__device__ __forceinline__ void sh_here4(uint4& x) {
+  x = make_uint4(sh_here(x.x), sh_here(x.y), sh_here(x.z), sh_here(x.w));
+}
+__device__ __forceinline__ void sh_here4(uint2& x) { x = make_uint2(sh_here(x.x), sh_here(x.y)); }
+
+// The lane, found where it is asked for.
+__device__ __forceinline__ int sh_lane() {
+  return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, sh_here(0)));
+}
+
 // The least lo and the largest hi of each 16 lanes, one step: with those N lanes around.
 template <int N>
 __device__ __forceinline__ void sh_fold16(int& lo, int& hi) {
@@ -178,6 +197,55 @@ template <int ROW>
 __device__ __forceinline__ int sh_swz(int r) {
   if constexpr (ROW >= 128) return pf_swz<ROW / 2>(r);
   return (r >> 2) & 3;
+}
+
+// Infinite values and NaN among the elements of a word of a cache row: the sign's place of each that
+// is one. An exponent of ones (e4m3: all ones past the sign) carries into it.
+template <typename KT>
+__device__ __forceinline__ uint32_t sh_odd(uint32_t w) {
+  constexpr uint32_t kOnes = sizeof(KT) == 1                   ? 0x7f7f7f7fu
+                             : std::is_same<KT, bf16_t>::value ? 0x7f807f80u
+                                                               : 0x7c007c00u;
+  constexpr uint32_t kStep = sizeof(KT) == 1                   ? 0x01010101u
+                             : std::is_same<KT, bf16_t>::value ? 0x00800080u
+                                                               : 0x04000400u;
+  return ((w & kOnes) + kStep) & (sizeof(KT) == 1 ? 0x80808080u : 0x80008000u);
+}
+template <typename T, typename KT>
+__device__ __forceinline__ uint32_t sh_not_finite(const typename Kv8<T, KT>::raw_t& x) {
+  uint32_t any = sh_odd<KT>(x.x) | sh_odd<KT>(x.y);
+  if constexpr (sizeof(KT) != 1) any |= sh_odd<KT>(x.z) | sh_odd<KT>(x.w);
+  return any;
+}
+// Zeros in their places.
+template <typename T, typename KT>
+__device__ __forceinline__ void sh_finite(typename Kv8<T, KT>::raw_t& x) {
+  const auto clear = [](uint32_t& w) {
+    const uint32_t odd = sh_odd<KT>(w);
+    w &= ~(odd | (odd - (odd >> (8 * sizeof(KT) - 1))));
+  };
+  clear(x.x);
+  clear(x.y);
+  if constexpr (sizeof(KT) != 1) {
+    clear(x.z);
+    clear(x.w);
+  }
+}
+// The mask of two 16-bit elements of which the first `n` are kept.
+__device__ __forceinline__ uint32_t sh_pair_mask(int n) {
+  return n >= 2 ? 0xffffffffu : (n == 1 ? 0xffffu : 0u);
+}
+// Ones of type T in the places of NaN and of the infinite values whose sign is `sign`'s, zeros
+// elsewhere.
+template <typename T>
+__device__ __forceinline__ uint4 sh_ones(const uint4& x, uint32_t sign) {
+  const auto ones = [sign](uint32_t w) {
+    constexpr bool kB = std::is_same<T, bf16_t>::value;
+    constexpr uint32_t kFraction = kB ? 0x007f007fu : 0x03ff03ffu;
+    const uint32_t nan = ((w & kFraction) + kFraction) << (kB ? 8 : 5);  // (to the sign's place)
+    return ((sh_odd<T>(w) & (nan | ~(w ^ sign))) >> 15) * (kB ? 0x3f80u : 0x3c00u);
+  };
+  return make_uint4(ones(x.x), ones(x.y), ones(x.z), ones(x.w));
 }
 
 template <typename T, typename KT, int D>
@@ -410,7 +478,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
     }
   };
   auto window = [&](int base) __attribute__((always_inline)) {
-    const int pos = min(base + lane, last - 1);
+    const int pos = min(base + sh_lane(), last - 1);
     int lo = seg0, hi = seg1;  // the last segment that begins at or before pos
 #pragma unroll 1
     while (hi - lo > 1) {
@@ -603,6 +671,36 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
                 const bool ok = ((live >> k) & 1) && key + 16 * k + 4 * g + r < hi_n;
                 s[k][r] = ok ? s[k][r] : -INFINITY;
               }
+            // A key that other rows of the unit see and some of these do not (drafts): a weight of
+            // zero times an infinite value or NaN would be NaN. Where the block holds one, the rows
+            // that see it get it here, and the products take zero in its place. (0 to 2 % of 40
+            // calls' time, under 1 % in all but four; a branch between softmax and products instead,
+            // a pass for each set of rows that see the same keys, took up to 8 % over fp8.)
+            if (wave_all < c.hi) {
+              uint32_t odd = 0;
+#pragma unroll
+              for (int u = 0; u < ND; ++u) odd |= sh_not_finite<T, KT>(vv[u]);
+              if (__builtin_expect(__any(odd != 0), 0)) {
+                const int sees = hi_n - key - 4 * g;
+                const uint32_t one2 = Pack2<T>::pack(1.0f, 1.0f);
+                const uint4 seen = make_uint4(one2 & sh_pair_mask(sees), one2 & sh_pair_mask(sees - 2),
+                                              one2 & sh_pair_mask(sees - 16), one2 & sh_pair_mask(sees - 18));
+#pragma unroll
+                for (int u = 0; u < ND; ++u) {
+                  sh_here4(vv[u]);  // (what the test above found is not held for this)
+#pragma unroll
+                  for (int down = 0; down < 2; ++down) {
+                    const mf_f32x4 has = Mfma16<T>::mac(sh_ones<T>(KV::operand(vv[u]), down ? 0x80008000u : 0u),
+                                                        seen, mf_f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                      acc[u][r] += has[r] > 0.0f ? (down ? -INFINITY : INFINITY) : 0.0f;
+                    __builtin_amdgcn_sched_barrier(0);
+                  }
+                  sh_finite<T, KT>(vv[u]);
+                }
+              }
+            }
           }
           float mt = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -613,7 +711,7 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
           mt *= scale;
           if (__any(mt > m_run + 8.0f)) {
             const float m_new = fmaxf(m_run, mt);
-            const float alpha = m_new != -INFINITY ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+            const float alpha = m_run != -INFINITY ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
             m_run = m_new;
             l_run *= alpha;
 #pragma unroll
@@ -655,10 +753,11 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
         const int rest = row - member * RPS;
         const int tq = fast_quot(rest, p.by_g);
         const int o = (member * p.q_len + tq) * p.H + nx.kvh() * p.G + (rest - tq * p.G);
+        const int at_g = sh_here(g);
 #pragma unroll
         for (int j = 0; j < JD; ++j)
           nq[j] = *reinterpret_cast<const uint4*>(q + static_cast<int64_t>(o) * D +
-                                                  KV::qk_dim0(j, g, JD));
+                                                  KV::qk_dim0(j, at_g, JD));
         if (r < nx.rows()) {
           n_row = b0 * p.q_len * p.H + o;
           n_hi = min(nx.hi, s_len[b0 + member] - p.q_len + tq + 1);
@@ -679,10 +778,11 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
         // Waves that split the keys put theirs into the slot: row rr of key wave ks at row
         // 16 RW ks + rr, its 16-byte chunk j at chunk j ^ n (the lanes of a set hold 16 rows).
         const int at = 16 * RW * ks + rr;
+        const int chunk = sh_here(n);
         if (rr < c.rows() && ks < KS) {
 #pragma unroll
           for (int u = 0; u < ND; ++u)
-            *reinterpret_cast<float4*>(f + at * D + 4 * ((4 * u + g) ^ n)) =
+            *reinterpret_cast<float4*>(f + at * D + 4 * ((4 * u + g) ^ chunk)) =
                 make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
           if (g == 0) {
             s_m[at] = m_run;
@@ -703,15 +803,16 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
       }
       if (ends && !joins && orow >= 0) {
         const int64_t at = slot0 + (unit_first ? orow : rr);
+        const int at_g = sh_here(g);
         if (g == 0) *reinterpret_cast<float2*>(p.ml + 2 * at) = make_float2(m_run, l);
 #pragma unroll
         for (int u = 0; u < ND; ++u)
-          *reinterpret_cast<float4*>(p.acc + at * D + 16 * u + 4 * g) =
+          *reinterpret_cast<float4*>(p.acc + at * D + 16 * u + 4 * at_g) =
               make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
       }
       if (joins) {  // a thread joins 4 dims of a row
 #pragma unroll 1
-        for (int x = tid; x < c.rows() * (D / 4); x += kShComp * kWave) {
+        for (int x = kWave * cw + sh_lane(); x < c.rows() * (D / 4); x += kShComp * kWave) {
           const int r = x / (D / 4), j = x % (D / 4);
           float M = -INFINITY;
 #pragma unroll

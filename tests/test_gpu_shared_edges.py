@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from miniserve_amd import paged_attention_shared, shared
-from test_gpu_shared import BF16, Batch, note
+from test_gpu_shared import BF16, F16, FP8, Batch, note
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,30 @@ def test_refuses_a_workspace_elsewhere(device):
                torch.zeros(128 << 20, dtype=torch.uint8, device=device)[::2]):
         with pytest.raises(ValueError, match="workspace must"):
             x.call(workspace=ws)
+
+
+@pytest.mark.parametrize("H,KVH,D,qt,kt,T", [
+    (4, 2, 64, BF16, BF16, 3), (28, 4, 128, F16, F16, 8), (16, 1, 64, F16, FP8, 4),
+    (32, 8, 128, BF16, BF16, 5), (8, 2, 128, BF16, FP8, 7), (16, 4, 128, BF16, BF16, 16),
+    (14, 2, 64, F16, F16, 2),
+])
+def test_values_that_only_later_drafts_see(device, H, KVH, D, qt, kt, T):
+    """NaN in the last key's values and an infinite value in the key before it: the drafts that see
+    them have NaN and infinity at those dims of those heads, everything else is bit for bit what it
+    is without them. The rows' drafts straddle blocks of 32 keys and tiles."""
+    x = Batch(H, KVH, D, qt, kt, [(0, 3, 4), (3, 2, 2)], [97, 130, 194, 80, 289], T)
+    clean = x.call().cpu()
+    x.check(clean)
+    bad = [(1, 3, float("nan"))] + ([] if kt == FP8 else [(2, 5, float("inf")), (2, 6, float("-inf"))])
+    head = KVH - 1
+    want = clean.clone().view(x.B, T, KVH, H // KVH, D)
+    for b, n in enumerate(x.lens):
+        for back, dim, value in bad:
+            page, slot = int(x.table[b, (n - back) // 16]), (n - back) % 16
+            x.vc.view(torch.uint8 if kt == FP8 else kt)[page, slot, head, dim] = \
+                0x7f if kt == FP8 else value
+            want[b, T - back:, head, :, dim] = value
+    note(f"values of later drafts, {T} tokens, {kt}")
+    got = x.call().cpu().view_as(want)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
