@@ -33,7 +33,7 @@
 //
 // Measured (this launch, then the merge): 64 rows of H32/KVH8/D128 bf16 in 8 groups of 8, prefixes
 // of 1024 to 8192 keys and 64 to 1024 own ones, 48 + 4.6 us (225 MB: 36 us of pure reading); 128
-// rows over an fp8 cache behind one prefix of 8192, 93 + 6.0 us (259 MB, 19 GFLOP); 32 rows of 4
+// rows over an fp8 cache behind one prefix of 8192, 94 + 5.9 us (259 MB, 19 GFLOP); 32 rows of 4
 // draft tokens, H28/KVH4 fp16, in 4 groups, 30 + 6.0 us; 6 rows of a small model 11 + 3.9 us, of
 // which the launch, the plan and the first tile's latency are nearly all. What bounds it: the plan
 // and the first window, 9000 clocks a workgroup before the first copy; about 6000 a piece; between
@@ -673,9 +673,10 @@ __global__ __launch_bounds__(kShThreads, 3) void shared_attn_kernel(const Shared
               }
             // A key that other rows of the unit see and some of these do not (drafts): a weight of
             // zero times an infinite value or NaN would be NaN. Where the block holds one, the rows
-            // that see it get it here, and the products take zero in its place. (0 to 2 % of 40
-            // calls' time, under 1 % in all but four; a branch between softmax and products instead,
-            // a pass for each set of rows that see the same keys, took up to 8 % over fp8.)
+            // that see it get it here, and the products take zero in its place. (Within 1.1 % of the
+            // time without in 36 of 40 calls, 2.7 % at most, with what the registers cost; a branch
+            // between softmax and products instead, a pass for each set of rows that see the same
+            // keys, took up to 8 % over fp8.)
             if (wave_all < c.hi) {
               uint32_t odd = 0;
 #pragma unroll
