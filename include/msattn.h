@@ -465,6 +465,68 @@ int msattn_gather_kv(const void* cache, int64_t cache_block_stride, int64_t cach
                      int table_width, int kv_dtype, void* stream);
 
 /*
+ * A paged cache held in 4 bits. Elements are e2m1 (a sign and 0, 0.5, 1, 1.5, 2, 3, 4, 6); each 32
+ * of a row share a power of two, held in a byte as its exponent + 127 (255: the block reads as
+ * NaN). k_cache and v_cache are uint8 [num_blocks, num_kv_heads, block_size / 16,
+ * 17 * head_dim / 2], 16-byte aligned, strides in bytes and multiples of 16, the last two
+ * dimensions contiguous: one tile for 16 tokens of one head, its elements (two a byte, the earlier
+ * dim low) and then its scales as [head_dim / 32][16 tokens]. Keys' elements lie as
+ * [16 tokens][head_dim / 2 bytes], values' as [head_dim / 8][16 tokens][4 bytes]. head_dim is a
+ * multiple of 32 up to 256, block_size a multiple of 16. No reference counterpart (its caches are
+ * fp32, fp16, bf16 or fp8, miniserve/attention.py:104-109).
+ *
+ * msattn_write_kv_fp4: msattn_write_kv_strided into such a cache. A block whose largest magnitude
+ * is a takes the power of two 2^e with a / 2^e in (3.5, 7] (e from -126 to 125), its elements
+ * x / 2^e to the nearest, ties to the even code, at most 6; one with a NaN or an infinity reads
+ * back as NaN. k_strides / v_strides are the batch, token and head strides of k and v in elements.
+ * The same row gives the same bytes whatever stands beside it. Two tokens of one call must not
+ * land in one slot.
+ */
+int msattn_write_kv_fp4(const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, void* k_cache, void* v_cache,
+                        int64_t cache_block_stride, int64_t cache_head_stride,
+                        const int32_t* block_table, const int32_t* starts, int batch, int tokens,
+                        int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                        int table_width, int src_dtype, void* stream);
+
+/*
+ * The values that positions starts[b] .. starts[b] + tokens - 1 of each row stand for, to k and v
+ * [batch, tokens, num_kv_heads, head_dim], contiguous, of type dst_dtype (fp32 and bf16 hold them
+ * exactly, fp16 rounds them to nearest); positions on holes, outside the table or below 0 give
+ * zeros.
+ */
+int msattn_read_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_block_stride,
+                       int64_t cache_head_stride, const int32_t* block_table,
+                       const int32_t* starts, void* k, void* v, int batch, int tokens,
+                       int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                       int table_width, int dst_dtype, void* stream);
+
+/*
+ * Workspace bytes of msattn_paged_attention_fp4; 0 for an invalid geometry. A workspace is all
+ * zeros when first used, is left reusable by every call, and may be one of the other entry points'
+ * (its counters lie where theirs do). Calls that share one must not overlap in time.
+ */
+size_t msattn_fp4_workspace_bytes(int batch, int q_len, int num_heads, int num_kv_heads,
+                                  int head_dim, int max_context, int q_dtype);
+
+/*
+ * msattn_paged_attention over a 4-bit cache: fp32, fp16 or bf16 query, any q_len, causal or not,
+ * window as there; one launch. q_strides are the query's batch, token and head strides in elements
+ * (16-byte aligned rows); out is contiguous. Rows without a visible key give zeros; an infinity or
+ * NaN reaches the queries that see its key alone. Scores and products take the cache's values
+ * exactly; the weights of a bf16 query are rounded to bf16, in the numerator and in the sum alike;
+ * maxima, sums and accumulators are fp32.
+ */
+int msattn_paged_attention_fp4(const void* query, const int64_t* q_strides, const void* k_cache,
+                               const void* v_cache, int64_t cache_block_stride,
+                               int64_t cache_head_stride, const int32_t* block_table,
+                               const int32_t* context_lens, void* out, void* workspace,
+                               size_t workspace_bytes, int batch, int q_len, int num_heads,
+                               int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                               int table_width, int max_context, int causal, int window,
+                               float scale, int q_dtype, void* stream);
+
+/*
  * Measurement helper, with no counterpart in the reference: one launch of a plain
  * streaming-read kernel over `bytes` (a multiple of 16) of device memory at `buf`
  * (16-byte aligned), each workgroup reading a contiguous 64 KiB chunk with nontemporal

@@ -100,6 +100,17 @@ SIGNATURES = {
     "msattn_gather_kv": (c_int, [
         c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp,
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "msattn_write_kv_fp4": (c_int, [
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp,
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "msattn_read_kv_fp4": (c_int, [
+        c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp,
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "msattn_fp4_workspace_bytes": (c_size, [c_int] * 7),
+    "msattn_paged_attention_fp4": (c_int, [
+        c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_size,
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+        c_float, c_int, c_vp]),
     "msattn_probe_stream_read": (c_int, [c_vp, c_size, c_vp, c_vp]),
 }
 

@@ -254,7 +254,13 @@ class PagedAttention:
         self.group = num_heads // num_kv_heads
 
     def allocate_kv_cache(self) -> tuple[torch.Tensor, torch.Tensor]:
-        """(k_cache, v_cache), each zeros [num_blocks, block_size, kv_heads, head_dim]."""
+        """(k_cache, v_cache), each zeros [num_blocks, block_size, kv_heads, head_dim]; with
+        kv_dtype torch.float4_e2m1fn_x2, those of ``allocate_fp4_cache``, which ``write_kv`` and
+        ``forward`` then take."""
+        if self.kv_dtype == torch.float4_e2m1fn_x2:
+            from .fp4 import allocate_fp4_cache
+            return allocate_fp4_cache(self.num_blocks, self.block_size, self.num_kv_heads,
+                                      self.head_dim, self.device)
         shape = (self.num_blocks, self.block_size, self.num_kv_heads, self.head_dim)
         k = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
         v = torch.zeros(shape, dtype=self.kv_dtype, device=self.device)
@@ -272,8 +278,13 @@ class PagedAttention:
         """Scatter k/v [batch, tokens, kv_heads, head_dim] into the cache.
 
         Row b's token t lands at position start[b] + t (``start`` is an int,
-        one entry per row, or an int tensor already on the device).
+        one entry per row, or an int tensor already on the device). 4-bit caches:
+        ``write_kv_fp4``.
         """
+        if k_cache.dtype == torch.uint8:
+            from .fp4 import write_kv_fp4
+            write_kv_fp4(k, v, k_cache, v_cache, block_table, start)
+            return
         for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache"), (k, "k"), (v, "v")):
             _require_gpu(t, name)
         if k.shape != v.shape or k.ndim != 4:
@@ -384,10 +395,18 @@ class PagedAttention:
         radix-cache hit, prefix_cache.py:66-96); a decode reads them once per KV head.
         ``prefix_groups`` = (group_rows, prefix_pages): groups of rows, each behind shared pages
         of its own (paged_attention_shared), read once a group where the call is causal and
-        without a window or RoPE.
+        without a window or RoPE. Over 4-bit caches (``paged_attention_fp4``) neither changes how
+        pages are read, and "triton_flash" is refused as over FP8 ones.
         """
         if backend not in _BACKENDS:
             raise ValueError(f"unknown attention backend: {backend!r}")
+        if k_cache.dtype == torch.uint8:
+            if backend == "triton_flash":
+                raise ValueError("triton_flash does not support a 4-bit KV cache")
+            from .fp4 import paged_attention_fp4
+            return paged_attention_fp4(query, k_cache, v_cache, block_table, context_lens,
+                                       causal=causal, scale=scale,
+                                       window=self.window if window is None else window)
         if backend == "triton_flash":
             if not causal:
                 raise ValueError("triton_flash supports causal decode only")

@@ -51,7 +51,9 @@ FILE_FLAGS = {
     "shared_prefix.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "shared_prefix_fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
-# The any-layout prefill kernels do the same.
+# The 4-bit cache's attention and the any-layout prefill kernels do the same.
+FILE_FLAGS.update({f"fp4_attn_{q}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+                   for q in ("f32", "f16", "bf16")})
 FILE_FLAGS.update({f"prefill_any_{q}_{kv}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
                    for q in ("f32", "f16", "bf16") for kv in ("f32", "f16", "bf16", "fp8")})
 

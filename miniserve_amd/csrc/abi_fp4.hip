@@ -1,0 +1,219 @@
+// C ABI of the 4-bit paged cache (declared in include/msattn.h): argument checks and launches.
+// No exception crosses this boundary.
+#include <cmath>
+#include <cstdint>
+
+#include <algorithm>
+
+#include "fp4_attn.h"
+#include "msattn.h"
+
+namespace {
+
+using namespace msattn;
+
+bool on(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+bool float_type(int t) { return t == MSATTN_F32 || t == MSATTN_F16 || t == MSATTN_BF16; }
+int type_bytes(int t) { return t == MSATTN_F32 ? 4 : 2; }
+bool dim_ok(int D) { return D > 0 && D % kFp4Block == 0 && D <= kFp4MaxDim; }
+
+// The caches lie on 16 bytes, and so do their pages and heads.
+bool cache_ok(const void* k, const void* v, int64_t blk, int64_t head, int KVH, int D, int bs,
+              int num_blocks, int W) {
+  return k && v && on(k, 16) && on(v, 16) && blk >= 0 && head >= 0 && blk % 16 == 0 &&
+         head % 16 == 0 && KVH > 0 && dim_ok(D) && bs > 0 && bs % kFp4Tile == 0 && num_blocks > 0 &&
+         W > 0;
+}
+
+int status_of(hipError_t e) { return e == hipSuccess ? MSATTN_OK : MSATTN_ERR_HIP; }
+
+// Write or read: the parameters that both have.
+int cache_params(Fp4CacheParams* p, const void* k, const void* v, const int64_t* ks,
+                 const int64_t* vs, void* k_cache, void* v_cache, int64_t blk, int64_t head,
+                 const int32_t* table, const int32_t* starts, int batch, int tokens, int KVH, int D,
+                 int bs, int num_blocks, int W, int dtype) {
+  if (!k || !v || !table || !starts || batch <= 0 || tokens < 0 || !float_type(dtype) ||
+      !cache_ok(k_cache, v_cache, blk, head, KVH, D, bs, num_blocks, W))
+    return MSATTN_ERR_INVALID_ARG;
+  const int eb = type_bytes(dtype);
+  if (!on(k, eb) || !on(v, eb) || !on(table, 4) || !on(starts, 4)) return MSATTN_ERR_INVALID_ARG;
+  if (static_cast<int64_t>(batch) * tokens >= (int64_t(1) << 31) ||
+      static_cast<int64_t>(KVH) * (D / 8) >= (int64_t(1) << 22))
+    return MSATTN_ERR_UNSUPPORTED;
+  p->k_cache = static_cast<uint8_t*>(k_cache);
+  p->v_cache = static_cast<uint8_t*>(v_cache);
+  p->k = const_cast<void*>(k);
+  p->v = const_cast<void*>(v);
+  p->table = table;
+  p->starts = starts;
+  p->blk_stride = blk;
+  p->head_stride = head;
+  p->vec = on(k, 16) && on(v, 16);
+  for (int i = 0; i < 3; ++i) {
+    p->k_st[i] = ks[i];
+    p->v_st[i] = vs[i];
+    if (ks[i] * eb % 16 != 0 || vs[i] * eb % 16 != 0) p->vec = 0;
+  }
+  p->batch = batch;
+  p->tokens = tokens;
+  p->KVH = KVH;
+  p->D = D;
+  p->bs = bs;
+  p->num_blocks = num_blocks;
+  p->W = W;
+  p->by_tokens = fp4_div(static_cast<uint32_t>(tokens > 0 ? tokens : 1));
+  p->by_octets = fp4_div(static_cast<uint32_t>(D / 8));
+  p->by_bs = fp4_div(static_cast<uint32_t>(bs));
+  return MSATTN_OK;
+}
+
+bool geometry_ok(int batch, int q_len, int H, int KVH, int D, int max_ctx) {
+  return batch > 0 && q_len > 0 && H > 0 && KVH > 0 && H % KVH == 0 && dim_ok(D) && max_ctx >= 0;
+}
+
+// How a call is cut: column tiles of 16 query rows a wave, and its shares.
+struct Plan {
+  int ct, rblocks, slot_rows, split, shares;
+  size_t ml_off, acc_off, total;
+};
+
+size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int q_dtype, Plan* p) {
+  const int64_t rows = static_cast<int64_t>(q_len) * (H / KVH);
+  const int most = q_dtype == MSATTN_BF16 && D <= 128 ? 4 : 2;
+  p->ct = rows <= 16 ? 1 : (rows <= 32 || most == 2 ? 2 : 4);
+  const int per = 16 * p->ct;
+  const int64_t rblocks = (rows + per - 1) / per;
+  const int64_t units = batch * rblocks * KVH;
+  if (rows >= (int64_t(1) << 30) || units >= (int64_t(1) << 30)) return false;
+  p->rblocks = static_cast<int>(rblocks);
+  p->slot_rows = static_cast<int>(std::min<int64_t>(per, rows));
+  const int64_t groups = max_ctx / kFp4Group + 2;  // of a unit, at most
+  p->split = batch * rblocks <= kFp4MaxEntries && units * groups < (int64_t(1) << 31);
+  const int64_t want = rows > 32 ? 1024 : 2048;
+  p->shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, units * groups)));
+  const size_t slots = p->split ? 2 * static_cast<size_t>(p->shares) * p->slot_rows : 0;
+  p->ml_off = up256((kHdrTickets + kMaxTickets) * sizeof(int));
+  p->acc_off = p->ml_off + up256(slots * 2 * sizeof(float));
+  p->total = p->acc_off + up256(slots * D * sizeof(float));
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int msattn_write_kv_fp4(const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, void* k_cache, void* v_cache,
+                        int64_t cache_block_stride, int64_t cache_head_stride,
+                        const int32_t* block_table, const int32_t* starts, int batch, int tokens,
+                        int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                        int table_width, int src_dtype, void* stream) {
+  if (!k_strides || !v_strides) return MSATTN_ERR_INVALID_ARG;
+  Fp4CacheParams p{};
+  const int rc = cache_params(&p, k, v, k_strides, v_strides, k_cache, v_cache, cache_block_stride,
+                              cache_head_stride, block_table, starts, batch, tokens, num_kv_heads,
+                              head_dim, block_size, num_blocks, table_width, src_dtype);
+  if (rc != MSATTN_OK || tokens == 0) return rc;
+  return status_of(launch_write_fp4(p, src_dtype, static_cast<hipStream_t>(stream)));
+}
+
+int msattn_read_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_block_stride,
+                       int64_t cache_head_stride, const int32_t* block_table,
+                       const int32_t* starts, void* k, void* v, int batch, int tokens,
+                       int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                       int table_width, int dst_dtype, void* stream) {
+  Fp4CacheParams p{};
+  const int64_t st[3] = {static_cast<int64_t>(tokens) * num_kv_heads * head_dim,
+                         static_cast<int64_t>(num_kv_heads) * head_dim, head_dim};
+  const int rc = cache_params(&p, k, v, st, st, const_cast<void*>(k_cache),
+                              const_cast<void*>(v_cache), cache_block_stride, cache_head_stride,
+                              block_table, starts, batch, tokens, num_kv_heads, head_dim,
+                              block_size, num_blocks, table_width, dst_dtype);
+  if (rc != MSATTN_OK || tokens == 0) return rc;
+  return status_of(launch_read_fp4(p, dst_dtype, static_cast<hipStream_t>(stream)));
+}
+
+size_t msattn_fp4_workspace_bytes(int batch, int q_len, int num_heads, int num_kv_heads,
+                                  int head_dim, int max_context, int q_dtype) {
+  Plan plan;
+  if (!geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context) ||
+      !float_type(q_dtype) ||
+      !plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, q_dtype, &plan))
+    return 0;
+  return plan.total;
+}
+
+int msattn_paged_attention_fp4(const void* query, const int64_t* q_strides, const void* k_cache,
+                               const void* v_cache, int64_t cache_block_stride,
+                               int64_t cache_head_stride, const int32_t* block_table,
+                               const int32_t* context_lens, void* out, void* workspace,
+                               size_t workspace_bytes, int batch, int q_len, int num_heads,
+                               int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                               int table_width, int max_context, int causal, int window,
+                               float scale, int q_dtype, void* stream) {
+  if (!query || !q_strides || !block_table || !context_lens || !out || !workspace ||
+      !float_type(q_dtype) || window < 0 || std::isnan(scale) ||
+      !geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context) ||
+      !cache_ok(k_cache, v_cache, cache_block_stride, cache_head_stride, num_kv_heads, head_dim,
+                block_size, num_blocks, table_width))
+    return MSATTN_ERR_INVALID_ARG;
+  const int eb = type_bytes(q_dtype);
+  if (!on(query, 16) || !on(out, eb) || !on(workspace, 256) || !on(block_table, 4) ||
+      !on(context_lens, 4))
+    return MSATTN_ERR_INVALID_ARG;
+  for (int i = 0; i < 3; ++i)
+    if (q_strides[i] * eb % 16 != 0) return MSATTN_ERR_INVALID_ARG;
+  Plan plan;
+  if (!plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, q_dtype, &plan))
+    return MSATTN_ERR_UNSUPPORTED;
+  if (workspace_bytes < plan.total) return MSATTN_ERR_WORKSPACE;
+  char* const ws = static_cast<char*>(workspace);
+  Fp4Params p{};
+  p.q = query;
+  p.k = static_cast<const uint8_t*>(k_cache);
+  p.v = static_cast<const uint8_t*>(v_cache);
+  p.table = block_table;
+  p.lens = context_lens;
+  p.out = out;
+  p.blk_stride = cache_block_stride;
+  p.head_stride = cache_head_stride;
+  for (int i = 0; i < 3; ++i) p.q_st[i] = q_strides[i];
+  p.batch = batch;
+  p.q_len = q_len;
+  p.H = num_heads;
+  p.KVH = num_kv_heads;
+  p.G = num_heads / num_kv_heads;
+  p.D = head_dim;
+  p.bs = block_size;
+  p.num_blocks = num_blocks;
+  p.W = table_width;
+  // (no key past the table)
+  p.max_ctx = static_cast<int>(std::min<int64_t>(
+      max_context, static_cast<int64_t>(table_width) * block_size));
+  p.causal = causal != 0;
+  p.window = window < p.max_ctx ? window : 0;  // (one as long as any context hides nothing)
+  p.scale_log2 = scale * kLog2e;
+  p.rows_per_kvh = q_len * p.G;
+  p.rblocks = plan.rblocks;
+  p.slot_rows = plan.slot_rows;
+  p.split = plan.split;
+  p.shares = plan.shares;
+  p.min_groups = 1;
+  p.by_tiles = fp4_div(static_cast<uint32_t>(block_size / kFp4Tile));
+  p.by_g = fp4_div(static_cast<uint32_t>(p.G));
+  p.by_rb = fp4_div(static_cast<uint32_t>(plan.rblocks));
+  p.by_kvh = fp4_div(static_cast<uint32_t>(num_kv_heads));
+  p.tickets = reinterpret_cast<int*>(ws) + kHdrTickets;
+  p.ml = reinterpret_cast<float*>(ws + plan.ml_off);
+  p.acc = reinterpret_cast<float*>(ws + plan.acc_off);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (q_dtype) {
+    case MSATTN_F32: return status_of(launch_fp4_attn<float>(p, plan.ct, st));
+    case MSATTN_F16: return status_of(launch_fp4_attn<_Float16>(p, plan.ct, st));
+    default: return status_of(launch_fp4_attn<bf16_t>(p, plan.ct, st));
+  }
+}
+
+}  // extern "C"

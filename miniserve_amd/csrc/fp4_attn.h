@@ -1,0 +1,691 @@
+// Attention over the 4-bit paged cache (fp4_cache.h; gfx950): any query type, any q_len.
+//
+// A unit is a (batch row, KV head, block of up to 16 CT query rows); rows are the pairs (query
+// token i, head g of the KV head's group) r = i G + g. Its keys are cut into groups of 32 tokens
+// (two tiles), and all groups of all units, in order, are dealt in equal contiguous shares, one a
+// wave, whatever the lengths (read on the device, so a call is capture-safe). A share's part of a
+// unit leaves, for each query row,
+//   m,  l = sum_j 2^(s_j - m),  acc = sum_j 2^(s_j - m) V_j,   s_j = scale log2(e) q.K_j
+// over its visible keys; a unit that lies within one share is normalised and written, the shares of
+// another leave partials, and the last of them to arrive joins them.
+//
+// A wave loads a tile's keys and values straight into the registers of the matrix operands, 16
+// bytes a lane, contiguous (fp4_cache.h), two groups ahead. Lane (g, n) = (l / 16, l % 16):
+//   * S^T = K Q^T on v_mfma_f32_16x16x32_bf16: the lane holds 32 dims of key n of the tile (at
+//     D = 128), widened by v_cvt_scalef32_pk_bf16_fp4, which is exact, and the same dims of query
+//     row n; it receives row n's scores of keys 4 g .. 4 g + 3 of the tile.
+//   * Those of the group's two tiles, 8 weights, are in their lane the B operand of
+//     O^T += V^T P^T; the A operand is the 8 dims the lane holds of the same 8 tokens, so that
+//     product c takes dim 8 n + c and the lane receives dims 32 g .. 32 g + 31 of row n. Softmax and
+//     rescaling stay in the lane.
+// The scaled 4-bit matrix instructions are not used: with an e4m3 operand beside the 4-bit one,
+// sums of 128 products came out up to 9e-5 of the sum of magnitudes off, bf16 ones exactly rounded.
+//
+// fp16 and fp32 queries, and their weights, enter the products as 2 and 3 bf16 parts, which hold
+// all their digits (for a weight, 16 and 24 of them); a bf16 query's weights are rounded to bf16
+// once, in the numerator and in the sum alike. Maxima, sums and accumulators are fp32.
+//
+// A masked key's score is -inf, and where a group has masked keys, values that some row must not see
+// are taken as zeros, and their NaN, if any, is given to the rows that do see them.
+//
+// Semantics: miniserve/attention.py:205-250.
+#pragma once
+
+#include "decode_mfma.h"
+#include "fp4_cache.h"
+
+namespace msattn {
+
+constexpr int kFp4Waves = 4;             // waves of a workgroup
+constexpr int kFp4Group = 32;            // tokens of a group
+constexpr int kFp4MaxEntries = 4096;     // (row, row block) pairs whose shares are planned in LDS
+constexpr int kFp4MaxShares = 4096;      // one arrival counter each, at most kMaxTickets
+static_assert(kFp4MaxShares <= kMaxTickets, "a counter a share");
+constexpr float kFp4Slack = 8.0f;        // base-2 headroom before a running maximum moves
+
+struct Fp4Params {
+  const void* q;
+  const uint8_t* k;
+  const uint8_t* v;
+  const int32_t* table;
+  const int32_t* lens;
+  void* out;
+  int64_t blk_stride, head_stride;  // bytes
+  int64_t q_st[3];                  // batch, token and head strides of the query (elements)
+  int batch, q_len, H, KVH, G, D;
+  int bs, num_blocks, W, max_ctx;
+  int causal, window;
+  float scale_log2;
+  int rows_per_kvh;  // q_len * G
+  int rblocks;       // ceil(rows_per_kvh / (16 CT))
+  int slot_rows;     // rows of a partial: min(16 CT, rows_per_kvh)
+  int split;         // shares planned over all units (else one unit a wave)
+  int shares;
+  int min_groups;    // of a share
+  Fp4Div by_tiles;   // tiles of a page
+  Fp4Div by_g, by_rb, by_kvh;
+  int* tickets;
+  float* ml;         // [2 shares][slot_rows][2]
+  float* acc;        // [2 shares][slot_rows][D]
+};
+
+// bf16 parts that a T's value enters a product as.
+template <typename T> constexpr int fp4_parts() {
+  return std::is_same<T, bf16_t>::value ? 1 : (std::is_same<T, _Float16>::value ? 2 : 3);
+}
+
+// One packed pair of bf16 parts of a and b, cut off (not rounded, so that no part overflows), and
+// what is left of them. A part that is not finite leaves nothing.
+__device__ __forceinline__ uint32_t fp4_cut2(float& a, float& b) {
+  const uint32_t x = __float_as_uint(a) & 0xffff0000u, y = __float_as_uint(b) & 0xffff0000u;
+  a = (x & 0x7f800000u) == 0x7f800000u ? 0.0f : a - __uint_as_float(x);
+  b = (y & 0x7f800000u) == 0x7f800000u ? 0.0f : b - __uint_as_float(y);
+  return (x >> 16) | y;
+}
+
+// Byte S of w, two 4-bit elements, as two bf16 times scale.
+template <int S>
+__device__ __forceinline__ uint32_t fp4_widen2(uint32_t w, float scale) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  const b2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, S);
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+// Keys a query row, and a block of rows, may see, and a unit's place in the work list.
+struct Fp4Unit {
+  int b, kvh, rb;
+  int lo, hi;        // keys that some row of the block sees
+  int first, n;      // its groups of keys
+  int u0;            // position of its first group in the list
+};
+
+template <int ROWS>
+__device__ __forceinline__ void fp4_extent(const Fp4Params& p, int ctx, int rb, int* lo, int* hi) {
+  const int r0 = rb * ROWS;
+  const int r1 = min(r0 + ROWS, p.rows_per_kvh) - 1;
+  const int q0 = ctx - p.q_len + fp4_quot(r0, p.by_g), q1 = ctx - p.q_len + fp4_quot(r1, p.by_g);
+  *hi = p.causal ? max(0, min(ctx, q1 + 1)) : ctx;
+  *lo = p.window > 0 ? max(0, q0 - p.window + 1) : 0;
+  if (*lo > *hi) *lo = *hi;
+}
+__device__ __forceinline__ int fp4_first(int lo) { return lo / kFp4Group; }
+__device__ __forceinline__ int fp4_count(int lo, int hi) {  // at least one, so that zeros are written
+  return hi > lo ? ceil_div(hi, kFp4Group) - lo / kFp4Group : 1;
+}
+
+template <typename T, int DP, int CT>
+__global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Params p) {
+  constexpr int HV = DP > 128 ? 2 : 1;   // halves of 128 dims
+  constexpr int DH = DP > 128 ? 128 : DP;
+  constexpr int NJ = DH / 32;            // score products of a half; dwords of keys a lane holds
+  constexpr int VC = DH / 16;            // value products of a half: dims a lane holds of a token
+  constexpr int LD = DH / 4;             // dims a lane receives of a half
+  constexpr int PQ = fp4_parts<T>();
+  constexpr int ROWS = 16 * CT;
+  constexpr int R = 2;                   // groups in flight
+  typedef typename std::conditional<DH == 128, uint4, uint2>::type kraw_t;
+
+  __shared__ int s_pre[kFp4MaxEntries + 1];
+  __shared__ int s_tot[kFp4Waves];
+
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, n = lane & 15;
+  const int share = static_cast<int>(blockIdx.x) * kFp4Waves + w;
+  const int entries = p.batch * p.rblocks;
+
+  auto ctx_of = [&](int b) {
+    const int c = p.lens[b];
+    return c < 0 ? 0 : (c > p.max_ctx ? p.max_ctx : c);
+  };
+
+  // The list: s_pre[e] = groups of one head's units of entries 0 .. e - 1 (entry = row, row block).
+  int c0, c1, chunk = 1;
+  if (p.split) {
+    int base = 0;
+    for (int e0 = 0; e0 < entries; e0 += 64 * kFp4Waves) {
+      const int e = e0 + tid;
+      int cnt = 0;
+      if (e < entries) {
+        const int b = fp4_quot(e, p.by_rb);
+        int lo, hi;
+        fp4_extent<ROWS>(p, ctx_of(b), e - b * p.rblocks, &lo, &hi);
+        cnt = fp4_count(lo, hi);
+      }
+      const int incl = wave_inclusive_sum(cnt);
+      if (lane == 63) s_tot[w] = incl;
+      __syncthreads();
+      int before = base;
+#pragma unroll
+      for (int i = 0; i < kFp4Waves; ++i) {
+        const int t = s_tot[i];
+        if (i < w) before += t;
+        base += t;
+      }
+      if (e < entries) s_pre[e + 1] = before + incl;
+      __syncthreads();
+    }
+    if (tid == 0) s_pre[0] = 0;
+    __syncthreads();
+    const int total = __builtin_amdgcn_readfirstlane(base) * p.KVH;
+    chunk = max(ceil_div(total, p.shares), p.min_groups);
+    c0 = static_cast<int>(min(static_cast<int64_t>(share) * chunk, static_cast<int64_t>(total)));
+    c1 = min(c0 + chunk, total);
+  } else {
+    c0 = 0;
+    c1 = share < entries * p.KVH ? 1 : 0;  // its unit's groups, set below
+  }
+
+  // The unit holding position q of the list (any lane's own q).
+  auto locate = [&](int q) {
+    Fp4Unit u;
+    if (p.split) {
+      int a = 0, z = p.batch;  // the row: KVH s_pre[a rblocks] <= q < KVH s_pre[z rblocks]
+      while (z - a > 1) {
+        const int m = (a + z) >> 1;
+        if (s_pre[m * p.rblocks] * p.KVH <= q) a = m;
+        else z = m;
+      }
+      u.b = a;
+      const int e0 = a * p.rblocks;
+      const int pre0 = s_pre[e0], per = s_pre[e0 + p.rblocks] - pre0;
+      const int rem = q - pre0 * p.KVH;
+      u.kvh = rem / per;
+      const int in = rem - u.kvh * per;
+      int x = 0, y = p.rblocks;
+      while (y - x > 1) {
+        const int m = (x + y) >> 1;
+        if (s_pre[e0 + m] - pre0 <= in) x = m;
+        else y = m;
+      }
+      u.rb = x;
+      u.u0 = pre0 * p.KVH + u.kvh * per + (s_pre[e0 + x] - pre0);
+    } else {
+      const int bk = fp4_quot(share, p.by_rb);
+      u.rb = share - bk * p.rblocks;
+      u.b = fp4_quot(bk, p.by_kvh);
+      u.kvh = bk - u.b * p.KVH;
+      u.u0 = 0;
+    }
+    fp4_extent<ROWS>(p, ctx_of(u.b), u.rb, &u.lo, &u.hi);
+    u.first = fp4_first(u.lo);
+    u.n = fp4_count(u.lo, u.hi);
+    return u;
+  };
+
+  if (c0 >= c1) return;  // (no barrier follows)
+  if (!p.split) c1 = __builtin_amdgcn_readfirstlane(locate(0).n);
+
+  // ---- what a lane holds of a tile: fixed places, one register each ----
+  uint32_t k_at[HV], ks_at[HV], v_at[HV], vs_at[HV];
+  bool k_in[HV];  // dims past D: keys read at the tile's start, times zeros of the query
+#pragma unroll
+  for (int h = 0; h < HV; ++h) {
+    const int dim = 128 * h + g * LD;
+    k_in[h] = dim < p.D;
+    k_at[h] = k_in[h] ? n * (p.D / 2) + dim / 2 : 0;
+    ks_at[h] = 8 * p.D + (k_in[h] ? 16 * (dim / 32) + n : 0);
+    const int o = DH == 128 ? 16 * h + n : n / 2;
+    const bool in = 8 * o < p.D;
+    v_at[h] = in ? 64 * o + 16 * g : 0;
+    vs_at[h] = 8 * p.D + (in ? 16 * (o / 4) + 4 * g : 0);
+  }
+  struct Keys { kraw_t d[HV]; uint32_t s[HV]; };
+  struct Values { uint4 d[HV]; uint32_t s[HV]; };
+  Keys kr[R][2];
+  Values vr[R][2];
+
+  // Places of the tiles of 32 groups from position base on: lane i holds tile i's byte offset, -1
+  // where the table has none.
+  auto places = [&](int base) -> int64_t {
+    const int q = base + (lane >> 1);
+    if (q >= c1) return -1;
+    const Fp4Unit u = locate(q);
+    const int tile = 2 * (u.first + q - u.u0) + (lane & 1);
+    const int pg = fp4_quot(tile, p.by_tiles);
+    if (tile * kFp4Tile >= u.hi || pg >= p.W) return -1;
+    const int phys = p.table[static_cast<int64_t>(u.b) * p.W + pg];
+    if (phys < 0 || phys >= p.num_blocks) return -1;
+    const int tpp = p.bs / kFp4Tile;
+    return static_cast<int64_t>(phys) * p.blk_stride + static_cast<int64_t>(u.kvh) * p.head_stride +
+           static_cast<int64_t>(tile - pg * tpp) * fp4_tile_bytes(p.D);
+  };
+  int64_t here = places(c0), next = -1;  // of this run of 32 groups, and of the next
+  int run = c0;                          // the run's first position
+  auto place_of = [&](int q, int t) -> int64_t {  // q in this run or the next
+    const int i = 2 * (q - run) + t;
+    auto from = [&](int64_t x) {
+      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), i & 63);
+      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), i & 63);
+      return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+    };
+    if (i < 64) return from(here);  // (a branch: the next run's places may be on their way)
+    return from(next);
+  };
+  auto load_keys = [&](Keys& k, int64_t at) {
+    const uint8_t* t = p.k + (at < 0 ? 0 : at);
+#pragma unroll
+    for (int h = 0; h < HV; ++h) {
+      k.d[h] = *reinterpret_cast<const kraw_t*>(t + k_at[h]);
+      k.s[h] = t[ks_at[h]];
+    }
+  };
+  auto load_values = [&](Values& v, int64_t at) {
+    const uint8_t* t = p.v + (at < 0 ? 0 : at);
+#pragma unroll
+    for (int h = 0; h < HV; ++h) {
+      v.d[h] = *reinterpret_cast<const uint4*>(t + v_at[h]);
+      v.s[h] = *reinterpret_cast<const uint32_t*>(t + vs_at[h]);
+    }
+  };
+  int64_t at[R][2];
+  auto issue = [&](auto slot_c, int q) {
+    constexpr int S = decltype(slot_c)::value;
+    if (q >= c1) return;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      at[S][t] = place_of(q, t);
+      load_keys(kr[S][t], at[S][t]);
+      load_values(vr[S][t], at[S][t]);
+    }
+  };
+
+  // ---- a unit's state ----
+  Fp4Unit u;
+  uint4 qf[CT][HV][NJ][PQ];
+  mf_f32x4 acc[CT][HV][VC];
+  float m_run[CT], l_run[CT];
+  int lo_n[CT], hi_n[CT];  // keys the lane's rows see
+  int all_lo, all_hi;      // keys every row of the block sees
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  auto begin = [&](int q) {
+    u = locate(q);
+    u.b = uniform(u.b); u.kvh = uniform(u.kvh); u.rb = uniform(u.rb); u.lo = uniform(u.lo);
+    u.hi = uniform(u.hi); u.first = uniform(u.first); u.n = uniform(u.n); u.u0 = uniform(u.u0);
+    const int ctx = uniform(ctx_of(u.b));
+    const int r0 = u.rb * ROWS;
+    const int r1 = min(r0 + ROWS, p.rows_per_kvh) - 1;
+    const int q0 = ctx - p.q_len + fp4_quot(r0, p.by_g), q1 = ctx - p.q_len + fp4_quot(r1, p.by_g);
+    all_hi = p.causal ? min(ctx, q0 + 1) : ctx;
+    all_lo = p.window > 0 ? max(0, q1 - p.window + 1) : 0;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int r = r0 + 16 * ct + n;
+      const bool ok = r <= r1;
+      const int i = ok ? fp4_quot(r, p.by_g) : 0;
+      const int qpos = ctx - p.q_len + i;
+      hi_n[ct] = !ok ? 0 : (p.causal ? min(ctx, qpos + 1) : ctx);
+      lo_n[ct] = p.window > 0 ? max(0, qpos - p.window + 1) : 0;
+      m_run[ct] = -INFINITY;
+      l_run[ct] = 0.0f;
+      const T* const qp = static_cast<const T*>(p.q) + u.b * p.q_st[0] + i * p.q_st[1] +
+                          (u.kvh * p.G + (ok ? r - i * p.G : 0)) * p.q_st[2];
+#pragma unroll
+      for (int h = 0; h < HV; ++h) {
+#pragma unroll
+        for (int c = 0; c < VC; ++c) acc[ct][h][c] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int dim = 128 * h + g * LD + 8 * j;
+          uint4 raw[sizeof(T) == 4 ? 2 : 1] = {};
+          if (ok && dim < p.D) {
+#pragma unroll
+            for (int i2 = 0; i2 < static_cast<int>(sizeof(T)) / 2; ++i2)
+              raw[i2] = *reinterpret_cast<const uint4*>(qp + dim + i2 * Chunk<T>::kElems);
+          }
+          if constexpr (PQ == 1) {
+            qf[ct][h][j][0] = raw[0];
+          } else {
+            float x[8];
+#pragma unroll
+            for (int i2 = 0; i2 < static_cast<int>(sizeof(T)) / 2; ++i2)
+              Chunk<T>::unpack(raw[i2], x + i2 * Chunk<T>::kElems);
+#pragma unroll
+            for (int a = 0; a < PQ; ++a) {
+              const uint32_t w0 = fp4_cut2(x[0], x[1]), w1 = fp4_cut2(x[2], x[3]);
+              const uint32_t w2 = fp4_cut2(x[4], x[5]), w3 = fp4_cut2(x[6], x[7]);
+              qf[ct][h][j][a] = make_uint4(w0, w1, w2, w3);
+            }
+          }
+        }
+      }
+    }
+  };
+
+  // Scores of one tile.
+  auto scores = [&](const Keys& k, mf_f32x4 (&s)[CT]) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) s[ct] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < HV; ++h) {
+      const float sc = fp4_scale(k_in[h] ? k.s[h] : 127u);
+      static_for<NJ>([&](auto jc) {
+        constexpr int j = decltype(jc)::value;
+        uint32_t x;
+        if constexpr (DH == 128) x = j == 0 ? k.d[h].x : j == 1 ? k.d[h].y : j == 2 ? k.d[h].z : k.d[h].w;
+        else x = j == 0 ? k.d[h].x : k.d[h].y;
+        const uint4 ka = make_uint4(fp4_widen2<0>(x, sc), fp4_widen2<1>(x, sc),
+                                    fp4_widen2<2>(x, sc), fp4_widen2<3>(x, sc));
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int a = 0; a < PQ; ++a) s[ct] = Mfma16<bf16_t>::mac(ka, qf[ct][h][j][a], s[ct]);
+      });
+    }
+  };
+
+  uint4 pw[CT][PQ];  // the weights, as the B operand of the value products
+  float psum[CT];
+  auto weights = [&](int ct, const mf_f32x4& s0, const mf_f32x4& s1, float mul) {
+    const float m = m_run[ct] != -INFINITY ? m_run[ct] : 0.0f;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = __builtin_amdgcn_exp2f(fmaf(s0[i], mul, -m));
+      x[4 + i] = __builtin_amdgcn_exp2f(fmaf(s1[i], mul, -m));
+    }
+    if constexpr (PQ == 1) {
+      const uint4 y = make_uint4(Pack2<bf16_t>::pack(x[0], x[1]), Pack2<bf16_t>::pack(x[2], x[3]),
+                                 Pack2<bf16_t>::pack(x[4], x[5]), Pack2<bf16_t>::pack(x[6], x[7]));
+      const uint32_t one = 0x3f803f80u;
+      psum[ct] = Dot2<bf16_t>::dot(y.x, one, Dot2<bf16_t>::dot(y.y, one, 0.0f)) +
+                 Dot2<bf16_t>::dot(y.z, one, Dot2<bf16_t>::dot(y.w, one, 0.0f));
+      pw[ct][0] = y;
+    } else {
+      psum[ct] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+#pragma unroll
+      for (int a = 0; a < PQ; ++a) {
+        const uint32_t w0 = fp4_cut2(x[0], x[1]), w1 = fp4_cut2(x[2], x[3]);
+        const uint32_t w2 = fp4_cut2(x[4], x[5]), w3 = fp4_cut2(x[6], x[7]);
+        pw[ct][a] = make_uint4(w0, w1, w2, w3);
+      }
+    }
+  };
+  // The weights with the running maximum as it stands, and only where one of them exceeds 2^8 (or
+  // the row has no maximum yet) with one that has moved: their sum bounds each of them.
+  auto softmax = [&](const mf_f32x4 (&s0)[CT], const mf_f32x4 (&s1)[CT], float mul) {
+    bool over = false;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      weights(ct, s0[ct], s1[ct], mul);
+      over = over || psum[ct] > 256.0f || m_run[ct] == -INFINITY;
+    }
+    if (__builtin_expect(__any(over), 0)) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float t = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t = fmaxf(t, fmaxf(s0[ct][i] * mul, s1[ct][i] * mul));
+        t = rows4_max(t);
+        const float m = fmaxf(m_run[ct], t);
+        const float alpha = m != -INFINITY ? __builtin_amdgcn_exp2f(m_run[ct] - m) : 1.0f;
+        m_run[ct] = m;
+        l_run[ct] *= alpha;
+#pragma unroll
+        for (int h = 0; h < HV; ++h)
+#pragma unroll
+          for (int c = 0; c < VC; ++c) acc[ct][h][c] *= alpha;
+        weights(ct, s0[ct], s1[ct], mul);
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) l_run[ct] += psum[ct];
+  };
+
+  // O^T += V^T P^T for half h: d0, d1 the tiles' elements, sc the 8 tokens' scales.
+  auto product = [&](auto h_c, const uint4& d0, const uint4& d1, const float (&sc)[8],
+                     const uint4 (&b)[CT][PQ]) {
+    constexpr int h = decltype(h_c)::value;
+    uint32_t x[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+    if constexpr (DH == 64) {  // two lanes share 8 dims
+      const int sh = 16 * (n & 1);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) x[t] >>= sh;
+    }
+    static_for<VC / 2>([&](auto cc) {
+      constexpr int c = decltype(cc)::value;
+      uint32_t y[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) y[t] = fp4_widen2<c>(x[t], sc[t]);
+      uint32_t e[4], o[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        e[t] = __builtin_amdgcn_perm(y[2 * t + 1], y[2 * t], 0x05040100u);
+        o[t] = __builtin_amdgcn_perm(y[2 * t + 1], y[2 * t], 0x07060302u);
+      }
+      const uint4 ea = make_uint4(e[0], e[1], e[2], e[3]), oa = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int a = 0; a < PQ; ++a) {
+          acc[ct][h][2 * c] = Mfma16<bf16_t>::mac(ea, b[ct][a], acc[ct][h][2 * c]);
+          acc[ct][h][2 * c + 1] = Mfma16<bf16_t>::mac(oa, b[ct][a], acc[ct][h][2 * c + 1]);
+        }
+    });
+  };
+  auto byte_of = [](uint32_t x, int i) { return (x >> (8 * i)) & 255u; };
+
+  auto consume = [&](auto slot_c, int q) {
+    constexpr int S = decltype(slot_c)::value;
+    const int tok = (u.first + q - u.u0) * kFp4Group;
+    mf_f32x4 s0[CT], s1[CT];
+    scores(kr[S][0], s0);
+    scores(kr[S][1], s1);
+    const bool full = tok >= all_lo && tok + kFp4Group <= all_hi && at[S][0] >= 0 && at[S][1] >= 0;
+    if (full) {
+      softmax(s0, s1, p.scale_log2);
+      static_for<HV>([&](auto hc) {
+        constexpr int h = decltype(hc)::value;
+        float sc[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[i] = fp4_scale(byte_of(vr[S][0].s[h], i));
+          sc[4 + i] = fp4_scale(byte_of(vr[S][1].s[h], i));
+        }
+        product(hc, vr[S][0].d[h], vr[S][1].d[h], sc, pw);
+      });
+      return;
+    }
+    // Keys 4 g + i of tile t for i < 4: bit 4 t + i of `dead` where no row sees it (or the table has
+    // no page), of `seen[ct]` where the lane's row does.
+    uint32_t dead = 0, seen[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) seen[ct] = 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int key = tok + 16 * (x / 4) + 4 * g + x % 4;
+      const bool live = key >= u.lo && key < u.hi && at[S][x / 4] >= 0;
+      dead |= live ? 0u : 1u << x;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const bool see = live && key >= lo_n[ct] && key < hi_n[ct];
+        seen[ct] |= see ? 1u << x : 0u;
+        // (scaled first: a scale of 0 or below must not touch the mask)
+        if (x < 4) s0[ct][x % 4] = see ? s0[ct][x % 4] * p.scale_log2 : -INFINITY;
+        else s1[ct][x % 4] = see ? s1[ct][x % 4] * p.scale_log2 : -INFINITY;
+      }
+    }
+    softmax(s0, s1, 1.0f);
+    static_for<HV>([&](auto hc) {
+      constexpr int h = decltype(hc)::value;
+      float sc[8];
+      uint32_t bad = 0;
+      const uint4 d0 = vr[S][0].d[h], d1 = vr[S][1].d[h];
+      uint32_t el[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const uint32_t byte = byte_of(vr[S][x / 4].s[h], x % 4);
+        const bool gone = (dead >> x) & 1u;
+        const bool nan = !gone && byte == kFp4NaN;
+        bad |= nan ? 1u << x : 0u;
+        sc[x] = gone || nan ? 1.0f : fp4_scale(byte);
+        el[x] = gone || nan ? 0u : el[x];
+      }
+      product(hc, make_uint4(el[0], el[1], el[2], el[3]), make_uint4(el[4], el[5], el[6], el[7]), sc, pw);
+      if (__builtin_expect(__any(bad != 0), 0)) {
+        // Rows that see a NaN block of dims: ones for the blocks times ones for what the rows see.
+        uint32_t aw[4], one[CT][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          aw[t] = ((bad >> (2 * t)) & 1u ? 0x3f80u : 0u) | ((bad >> (2 * t + 1)) & 1u ? 0x3f800000u : 0u);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            one[ct][t] = ((seen[ct] >> (2 * t)) & 1u ? 0x3f80u : 0u) |
+                         ((seen[ct] >> (2 * t + 1)) & 1u ? 0x3f800000u : 0u);
+        }
+        const uint4 av = make_uint4(aw[0], aw[1], aw[2], aw[3]);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const mf_f32x4 hit = Mfma16<bf16_t>::mac(
+              av, make_uint4(one[ct][0], one[ct][1], one[ct][2], one[ct][3]), mf_f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[ct][h][c][i] = hit[i] > 0.0f ? __uint_as_float(0x7fc00000u) : acc[ct][h][c][i];
+        }
+      }
+    });
+  };
+
+  auto out_at = [&](int r) {  // element offset of row r of the unit's KV head in the output
+    const int i = fp4_quot(r, p.by_g);
+    return ((static_cast<int64_t>(u.b) * p.q_len + i) * p.H + (u.kvh * p.G + (r - i * p.G))) * p.D;
+  };
+  // Normalised rows, or a partial and perhaps the join.
+  auto finish = [&]() {
+    const int r0 = u.rb * ROWS;
+    const int rows = min(ROWS, p.rows_per_kvh - r0);
+    float l[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) l[ct] = rows4_sum(l_run[ct]);
+    const bool whole = u.u0 >= c0 && u.u0 + u.n <= c1;
+    if (whole) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        if (16 * ct + n >= rows) continue;
+        const float inv = l[ct] != 0.0f ? 1.0f / l[ct] : 0.0f;  // (a NaN stays one)
+        T* const o = static_cast<T*>(p.out) + out_at(r0 + 16 * ct + n);
+#pragma unroll
+        for (int h = 0; h < HV; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int dim = 128 * h + LD * g + VC * i;
+            if (dim >= p.D) continue;
+#pragma unroll
+            for (int c = 0; c < VC; ++c) Elt<T>::store(o + dim + c, acc[ct][h][c][i] * inv);
+          }
+      }
+      return;
+    }
+    const int64_t slot = 2 * static_cast<int64_t>(share) + (u.u0 >= c0 ? 1 : 0);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int r = 16 * ct + n;
+      if (r >= rows) continue;
+      const int64_t row = slot * p.slot_rows + r;
+      if (g == 0) store2_device(p.ml + row * 2, m_run[ct], l[ct]);
+#pragma unroll
+      for (int h = 0; h < HV; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int dim = 128 * h + LD * g + VC * i;
+          if (dim >= p.D) continue;
+#pragma unroll
+          for (int c = 0; c < VC; c += 2)
+            store2_device(p.acc + row * p.D + dim + c, acc[ct][h][c][i], acc[ct][h][c + 1][i]);
+        }
+    }
+    // The shares that hold the unit's groups; the first names its counter. The partials above are
+    // written through (agent scope) before the counter moves, and read the same way after it.
+    const int s_first = u.u0 / chunk, s_last = (u.u0 + u.n - 1) / chunk;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    int last = 0;
+    if (lane == 0) {
+      int* const t = p.tickets + s_first;
+      const int old = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = old == s_last - s_first;
+      if (last) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    last = uniform(last);
+    asm volatile("" ::: "memory");
+    if (!last) return;
+    const int per = p.D / 4;
+    for (int idx = lane; idx < rows * per; idx += 64) {
+      const int r = idx / per, d = 4 * (idx - r * per);
+      float M = -INFINITY, L = 0.0f;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      constexpr int N = 8;
+      for (int j0 = s_first; j0 <= s_last; j0 += N) {
+        float2 x0[N], x1[N], ml[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {  // shares past the last repeat it, unused
+          const int j = min(j0 + i, s_last);
+          const int64_t row = (2 * static_cast<int64_t>(j) + (j == s_first ? 1 : 0)) * p.slot_rows + r;
+          ml[i] = load2_device(p.ml + row * 2);
+          x0[i] = load2_device(p.acc + row * p.D + d);
+          x1[i] = load2_device(p.acc + row * p.D + d + 2);
+        }
+        float mb = M;
+#pragma unroll
+        for (int i = 0; i < N; ++i) mb = fmaxf(mb, j0 + i <= s_last ? ml[i].x : -INFINITY);
+        const float keep = mb != -INFINITY ? __builtin_amdgcn_exp2f(M - mb) : 1.0f;
+        L *= keep;
+        a.x *= keep; a.y *= keep; a.z *= keep; a.w *= keep;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          // a share without a visible key of the row has nothing (its m is -inf, its sum 0)
+          const bool live = j0 + i <= s_last && !(ml[i].x == -INFINITY && ml[i].y == 0.0f);
+          const float f = __builtin_amdgcn_exp2f(live && mb != -INFINITY ? ml[i].x - mb : 0.0f);
+          L = live ? fmaf(f, ml[i].y, L) : L;
+          a.x = live ? fmaf(f, x0[i].x, a.x) : a.x;
+          a.y = live ? fmaf(f, x0[i].y, a.y) : a.y;
+          a.z = live ? fmaf(f, x1[i].x, a.z) : a.z;
+          a.w = live ? fmaf(f, x1[i].y, a.w) : a.w;
+        }
+        M = mb;
+      }
+      const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+      T* const o = static_cast<T*>(p.out) + out_at(r0 + r) + d;
+      Elt<T>::store(o + 0, a.x * inv);
+      Elt<T>::store(o + 1, a.y * inv);
+      Elt<T>::store(o + 2, a.z * inv);
+      Elt<T>::store(o + 3, a.w * inv);
+    }
+  };
+
+  // ---- the share ----
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  issue(S0{}, c0);
+  issue(S1{}, c0 + 1);
+  next = places(c0 + 32);
+  begin(c0);
+  auto step = [&](auto slot_c, int q) {
+    consume(slot_c, q);
+    issue(slot_c, q + R);
+    if (q + 1 == c1 || q + 1 == u.u0 + u.n) {
+      finish();
+      if (q + 1 < c1) begin(q + 1);
+    }
+  };
+  for (int q = c0; q < c1; q += 2) {
+    if (q - run == 32) {
+      run = q;
+      here = next;
+      next = places(run + 32);
+    }
+    step(S0{}, q);
+    if (q + 1 < c1) step(S1{}, q + 1);
+  }
+}
+
+// Rows a wave takes, in column tiles of 16: as many as the KV head has, up to what the registers
+// hold beside two groups in flight.
+template <typename T> constexpr int fp4_max_ct() { return fp4_parts<T>() == 1 ? 4 : 2; }
+
+template <typename T>
+hipError_t launch_fp4_attn(const Fp4Params& p, int ct, hipStream_t stream);
+
+}  // namespace msattn

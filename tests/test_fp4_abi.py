@@ -1,0 +1,114 @@
+"""CPU checks of the 4-bit cache's entry points: refusals, workspace sizes, CPU tensors."""
+import ctypes
+
+import pytest
+import torch
+
+from miniserve_amd import (PagedAttention, _native as nat, allocate_fp4_cache, paged_attention_fp4,
+                           read_kv_fp4, write_kv_fp4)
+
+I64x3 = ctypes.c_int64 * 3
+ST = I64x3(4 * 128, 128, 128)
+
+
+def write_args(**over):
+    a = dict(k=1024, ks=ST, v=2048, vs=ST, kc=4096, vc=8192, blk=1088 * 2, head=1088, table=256,
+             starts=512, B=2, T=3, KVH=2, D=128, bs=16, nb=10, W=4, t=nat.BF16, stream=None)
+    a.update(over)
+    return list(a.values())
+
+
+BAD_CACHE = [(dict(kc=None), 1), (dict(vc=None), 1), (dict(kc=4100), 1), (dict(vc=8200), 1),
+             (dict(blk=-16), 1), (dict(blk=8), 1), (dict(head=1080), 1), (dict(table=None), 1),
+             (dict(table=258), 1), (dict(KVH=0), 1), (dict(D=0), 1), (dict(D=48), 1),
+             (dict(D=288), 1), (dict(bs=8), 1), (dict(bs=0), 1), (dict(bs=24), 1), (dict(nb=0), 1),
+             (dict(W=0), 1), (dict(B=0), 1), (dict(t=nat.FP8_E4M3), 1), (dict(t=7), 1)]
+
+
+def named(d):
+    return ",".join(f"{k}={v}" for k, v in d.items()) if isinstance(d, dict) else str(d)
+
+
+@pytest.mark.parametrize("bad,status", BAD_CACHE + [
+    (dict(k=None), 1), (dict(v=None), 1), (dict(ks=None), 1), (dict(vs=None), 1),
+    (dict(starts=None), 1), (dict(starts=514), 1), (dict(k=1025), 1), (dict(T=-1), 1),
+    (dict(B=1 << 20, T=1 << 11), 2)], ids=named)
+def test_write_refuses(bad, status):
+    assert nat.lib().msattn_write_kv_fp4(*write_args(**bad)) == status
+
+
+def read_args(**over):
+    a = dict(kc=4096, vc=8192, blk=1088 * 2, head=1088, table=256, starts=512, k=1024, v=2048, B=2,
+             T=3, KVH=2, D=128, bs=16, nb=10, W=4, t=nat.BF16, stream=None)
+    a.update(over)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad,status", BAD_CACHE + [
+    (dict(k=None), 1), (dict(v=None), 1), (dict(starts=None), 1), (dict(v=2049), 1),
+    (dict(T=-1), 1), (dict(B=1 << 20, T=1 << 11), 2)], ids=named)
+def test_read_refuses(bad, status):
+    assert nat.lib().msattn_read_kv_fp4(*read_args(**bad)) == status
+
+
+def attend_args(**over):
+    a = dict(q=1024, qs=I64x3(8 * 128, 8 * 128, 128), kc=4096, vc=8192, blk=1088 * 2, head=1088,
+             table=256, lens=512, out=2048, ws=1 << 20, ws_bytes=1 << 40, B=2, q_len=1, H=8, KVH=2,
+             D=128, bs=16, nb=10, W=4, max_context=64, causal=1, window=0, scale=0.1, t=nat.BF16,
+             stream=None)
+    a.update(over)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad,status", BAD_CACHE + [
+    (dict(q=None), 1), (dict(qs=None), 1), (dict(lens=None), 1), (dict(lens=513), 1),
+    (dict(out=None), 1), (dict(ws=None), 1), (dict(q=1032), 1), (dict(out=2049), 1),
+    (dict(ws=(1 << 20) + 64), 1), (dict(q_len=0), 1), (dict(H=0), 1), (dict(H=3), 1),
+    (dict(max_context=-1), 1), (dict(window=-1), 1), (dict(scale=float("nan")), 1),
+    (dict(qs=I64x3(1028, 1024, 128)), 1), (dict(qs=I64x3(1024, 1024, 132)), 1),
+    (dict(ws_bytes=1024), 3), (dict(q_len=1 << 29), 2)], ids=named)
+def test_attention_refuses(bad, status):
+    assert nat.lib().msattn_paged_attention_fp4(*attend_args(**bad)) == status
+
+
+def test_nothing_to_do():
+    assert nat.lib().msattn_write_kv_fp4(*write_args(T=0)) == 0
+    assert nat.lib().msattn_read_kv_fp4(*read_args(T=0)) == 0
+
+
+def test_workspace_bytes():
+    f = nat.lib().msattn_fp4_workspace_bytes
+    header = (64 + 4096) * 4
+    assert f(4, 1, 6, 4, 64, 100, nat.BF16) == 0 and f(4, 1, 4, 4, 48, 100, nat.BF16) == 0
+    assert f(4, 1, 4, 4, 64, 100, nat.FP8_E4M3) == 0 and f(0, 1, 4, 4, 64, 100, nat.BF16) == 0
+    assert f(4, 1, 4, 4, 64, 100, nat.BF16) > header
+    # as many contexts as one likes need no more
+    assert f(1 << 15, 1, 32, 8, 128, 1 << 16, nat.BF16) <= f(64, 1, 32, 8, 128, 1 << 16, nat.BF16)
+
+
+def test_allocation():
+    k, v = allocate_fp4_cache(5, 32, 3, 96, device="cpu")
+    assert k.shape == v.shape == (5, 3, 2, 816) and k.dtype == torch.uint8 and not k.any()
+    for bad in (dict(num_blocks=0), dict(block_size=24), dict(block_size=0), dict(num_kv_heads=0),
+                dict(head_dim=80), dict(head_dim=288), dict(head_dim=0)):
+        with pytest.raises(ValueError):
+            allocate_fp4_cache(**{**dict(num_blocks=5, block_size=16, num_kv_heads=3, head_dim=64,
+                                         device="cpu"), **bad})
+    pa = PagedAttention(8, 2, 128, num_blocks=4, block_size=32, kv_dtype=torch.float4_e2m1fn_x2)
+    k, v = pa.allocate_kv_cache()
+    assert k.shape == v.shape == (4, 2, 2, 1088) and k.dtype == torch.uint8
+    with pytest.raises(ValueError, match="tiles"):
+        PagedAttention(8, 2, 128, num_blocks=4, block_size=8,
+                       kv_dtype=torch.float4_e2m1fn_x2).allocate_kv_cache()
+
+
+def test_cpu_tensors_raise():
+    k, v = allocate_fp4_cache(5, 16, 2, 64, device="cpu")
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    x = torch.zeros(1, 1, 2, 64)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        write_kv_fp4(x, x, k, v, table)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        read_kv_fp4(k, v, table, 0, 1)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        paged_attention_fp4(x, k, v, table, [1])
