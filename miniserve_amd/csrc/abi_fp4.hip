@@ -81,8 +81,8 @@ size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int q_dtype, Plan* p) {
   const int64_t rows = static_cast<int64_t>(q_len) * (H / KVH);
-  const int most = q_dtype == MSATTN_BF16 && D <= 128 ? 4 : 2;
-  p->ct = rows <= 16 ? 1 : (rows <= 32 || most == 2 ? 2 : 4);
+  const int most = 2;
+  p->ct = rows <= 16 ? 1 : most;
   const int per = 16 * p->ct;
   const int64_t rblocks = (rows + per - 1) / per;
   const int64_t units = batch * rblocks * KVH;
@@ -91,7 +91,7 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int q_dty
   p->slot_rows = static_cast<int>(std::min<int64_t>(per, rows));
   const int64_t groups = max_ctx / kFp4Group + 2;  // of a unit, at most
   p->split = batch * rblocks <= kFp4MaxEntries && units * groups < (int64_t(1) << 31);
-  const int64_t want = rows > 32 ? 1024 : 2048;
+    const int64_t want = 256;  // a workgroup a CU
   p->shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, units * groups)));
   const size_t slots = p->split ? 2 * static_cast<size_t>(p->shares) * p->slot_rows : 0;
   p->ml_off = up256((kHdrTickets + kMaxTickets) * sizeof(int));
@@ -160,7 +160,7 @@ int msattn_paged_attention_fp4(const void* query, const int64_t* q_strides, cons
                 block_size, num_blocks, table_width))
     return MSATTN_ERR_INVALID_ARG;
   const int eb = type_bytes(q_dtype);
-  if (!on(query, 16) || !on(out, eb) || !on(workspace, 256) || !on(block_table, 4) ||
+  if (!on(query, 16) || !on(out, 16) || !on(workspace, 256) || !on(block_table, 4) ||
       !on(context_lens, 4))
     return MSATTN_ERR_INVALID_ARG;
   for (int i = 0; i < 3; ++i)
@@ -200,7 +200,6 @@ int msattn_paged_attention_fp4(const void* query, const int64_t* q_strides, cons
   p.slot_rows = plan.slot_rows;
   p.split = plan.split;
   p.shares = plan.shares;
-  p.min_groups = 1;
   p.by_tiles = fp4_div(static_cast<uint32_t>(block_size / kFp4Tile));
   p.by_g = fp4_div(static_cast<uint32_t>(p.G));
   p.by_rb = fp4_div(static_cast<uint32_t>(plan.rblocks));

@@ -3,7 +3,7 @@
 // A unit is a (batch row, KV head, block of up to 16 CT query rows); rows are the pairs (query
 // token i, head g of the KV head's group) r = i G + g. Its keys are cut into groups of 32 tokens
 // (two tiles), and all groups of all units, in order, are dealt in equal contiguous shares, one a
-// wave, whatever the lengths (read on the device, so a call is capture-safe). A share's part of a
+// workgroup, whatever the lengths (read on the device, so a call is capture-safe). A share's part of a
 // unit leaves, for each query row,
 //   m,  l = sum_j 2^(s_j - m),  acc = sum_j 2^(s_j - m) V_j,   s_j = scale log2(e) q.K_j
 // over its visible keys; a unit that lies within one share is normalised and written, the shares of
@@ -34,11 +34,14 @@
 #include "decode_mfma.h"
 #include "fp4_cache.h"
 
+#define FP4_INLINE __attribute__((always_inline))
+
 namespace msattn {
 
-constexpr int kFp4Waves = 4;             // waves of a workgroup
+constexpr int kFp4Waves = 8;             // waves of a workgroup, two a SIMD
+constexpr int kFp4Threads = 64 * kFp4Waves;
 constexpr int kFp4Group = 32;            // tokens of a group
-constexpr int kFp4MaxEntries = 4096;     // (row, row block) pairs whose shares are planned in LDS
+constexpr int kFp4MaxEntries = 2048;     // (row, row block) pairs whose shares are planned in LDS
 constexpr int kFp4MaxShares = 4096;      // one arrival counter each, at most kMaxTickets
 static_assert(kFp4MaxShares <= kMaxTickets, "a counter a share");
 constexpr float kFp4Slack = 8.0f;        // base-2 headroom before a running maximum moves
@@ -59,9 +62,8 @@ struct Fp4Params {
   int rows_per_kvh;  // q_len * G
   int rblocks;       // ceil(rows_per_kvh / (16 CT))
   int slot_rows;     // rows of a partial: min(16 CT, rows_per_kvh)
-  int split;         // shares planned over all units (else one unit a wave)
+  int split;         // shares planned over all units (else one unit a workgroup)
   int shares;
-  int min_groups;    // of a share
   Fp4Div by_tiles;   // tiles of a page
   Fp4Div by_g, by_rb, by_kvh;
   int* tickets;
@@ -91,6 +93,38 @@ __device__ __forceinline__ uint32_t fp4_widen2(uint32_t w, float scale) {
   return __builtin_bit_cast(uint32_t, r);
 }
 
+// Four neighbouring outputs (on 4 elements' alignment), rounded to nearest.
+template <typename T>
+__device__ __forceinline__ void fp4_store4(T* o, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(o) = make_float4(a, b, c, d);
+  else *reinterpret_cast<uint2*>(o) = make_uint2(Pack2<T>::pack(a, b), Pack2<T>::pack(c, d));
+}
+
+#ifndef MSATTN_FP4_NT
+#define MSATTN_FP4_NT 0
+#endif
+#ifndef MSATTN_FP4_OCC
+#define MSATTN_FP4_OCC 2
+#endif
+template <typename V>
+__device__ __forceinline__ V fp4_load(const uint8_t* p) {
+#if MSATTN_FP4_NT
+  if constexpr (sizeof(V) == 16) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const u4 x = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p));
+    return V{x.x, x.y, x.z, x.w};
+  } else if constexpr (sizeof(V) == 8) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const u2 x = __builtin_nontemporal_load(reinterpret_cast<const u2*>(p));
+    return V{x.x, x.y};
+  } else {
+    return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+  }
+#else
+  return *reinterpret_cast<const V*>(p);
+#endif
+}
+
 // Keys a query row, and a block of rows, may see, and a unit's place in the work list.
 struct Fp4Unit {
   int b, kvh, rb;
@@ -114,7 +148,7 @@ __device__ __forceinline__ int fp4_count(int lo, int hi) {  // at least one, so 
 }
 
 template <typename T, int DP, int CT>
-__global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Params p) {
+__global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Params p) {
   constexpr int HV = DP > 128 ? 2 : 1;   // halves of 128 dims
   constexpr int DH = DP > 128 ? 128 : DP;
   constexpr int NJ = DH / 32;            // score products of a half; dwords of keys a lane holds
@@ -122,35 +156,48 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
   constexpr int LD = DH / 4;             // dims a lane receives of a half
   constexpr int PQ = fp4_parts<T>();
   constexpr int ROWS = 16 * CT;
-  constexpr int R = 2;                   // groups in flight
   typedef typename std::conditional<DH == 128, uint4, uint2>::type kraw_t;
 
   __shared__ int s_pre[kFp4MaxEntries + 1];
-  __shared__ int s_tot[kFp4Waves];
+  __shared__ int s_ctx[kFp4MaxEntries];
+  __shared__ int s_tot[kFp4Waves];  // and whether this workgroup joins a unit's shares
+  // The waves' accumulators of 16 rows, rows 4 floats apart beyond DP (so that the 16 rows of a
+  // store fall on different banks), and their maxima and sums.
+  __shared__ float s_acc[kFp4Waves][16][DP + 4];
+  __shared__ float2 s_ml[kFp4Waves][16];
 
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n = lane & 15;
-  const int share = static_cast<int>(blockIdx.x) * kFp4Waves + w;
+  const int share = static_cast<int>(blockIdx.x);
   const int entries = p.batch * p.rblocks;
 
-  auto ctx_of = [&](int b) {
+  auto ctx_of = [&](int b) FP4_INLINE {
+    if (p.split) return s_ctx[b];
     const int c = p.lens[b];
     return c < 0 ? 0 : (c > p.max_ctx ? p.max_ctx : c);
+  };
+  // Barrier for what lies in LDS: loads into registers stay on their way.
+  auto lds_barrier = [&]() FP4_INLINE {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   };
 
   // The list: s_pre[e] = groups of one head's units of entries 0 .. e - 1 (entry = row, row block).
   int c0, c1, chunk = 1;
   if (p.split) {
     int base = 0;
-    for (int e0 = 0; e0 < entries; e0 += 64 * kFp4Waves) {
+    for (int e0 = 0; e0 < entries; e0 += kFp4Threads) {
       const int e = e0 + tid;
       int cnt = 0;
       if (e < entries) {
-        const int b = fp4_quot(e, p.by_rb);
+        const int b = fp4_quot(e, p.by_rb), rb = e - b * p.rblocks;
+        const int c = p.lens[b], ctx = c < 0 ? 0 : (c > p.max_ctx ? p.max_ctx : c);
+        if (rb == 0) s_ctx[b] = ctx;
         int lo, hi;
-        fp4_extent<ROWS>(p, ctx_of(b), e - b * p.rblocks, &lo, &hi);
+        fp4_extent<ROWS>(p, ctx, rb, &lo, &hi);
         cnt = fp4_count(lo, hi);
       }
       const int incl = wave_inclusive_sum(cnt);
@@ -169,7 +216,8 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
     if (tid == 0) s_pre[0] = 0;
     __syncthreads();
     const int total = __builtin_amdgcn_readfirstlane(base) * p.KVH;
-    chunk = max(ceil_div(total, p.shares), p.min_groups);
+    // whole rounds of the waves: a part of one takes as long, and leaves more to join
+    chunk = ceil_div(ceil_div(total, p.shares), kFp4Waves) * kFp4Waves;
     c0 = static_cast<int>(min(static_cast<int64_t>(share) * chunk, static_cast<int64_t>(total)));
     c1 = min(c0 + chunk, total);
   } else {
@@ -178,7 +226,7 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
   }
 
   // The unit holding position q of the list (any lane's own q).
-  auto locate = [&](int q) {
+  auto locate = [&](int q) FP4_INLINE {
     Fp4Unit u;
     if (p.split) {
       int a = 0, z = p.batch;  // the row: KVH s_pre[a rblocks] <= q < KVH s_pre[z rblocks]
@@ -214,7 +262,7 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
     return u;
   };
 
-  if (c0 >= c1) return;  // (no barrier follows)
+  if (c0 >= c1) return;  // (the workgroup as one)
   if (!p.split) c1 = __builtin_amdgcn_readfirstlane(locate(0).n);
 
   // ---- what a lane holds of a tile: fixed places, one register each ----
@@ -231,31 +279,37 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
     v_at[h] = in ? 64 * o + 16 * g : 0;
     vs_at[h] = 8 * p.D + (in ? 16 * (o / 4) + 4 * g : 0);
   }
-  struct Keys { kraw_t d[HV]; uint32_t s[HV]; };
-  struct Values { uint4 d[HV]; uint32_t s[HV]; };
-  Keys kr[R][2];
-  Values vr[R][2];
+  struct Tile {  // a tile's keys and values, and the scales of the lane's
+    kraw_t k[HV];
+    uint32_t ks[HV];
+    uint4 v[HV];
+    uint32_t vs[HV];
+  };
+  struct Group {  // two tiles, and where they lie (-1: nowhere)
+    Tile t[2];
+    int64_t at[2];
+  };
 
-  // Places of the tiles of 32 groups from position base on: lane i holds tile i's byte offset, -1
-  // where the table has none.
-  auto places = [&](int base) -> int64_t {
-    const int q = base + (lane >> 1);
-    if (q >= c1) return -1;
+  // Wave w takes positions c0 + w + 8 s of the share. Places of the tiles of its 32 groups from s =
+  // base on: lane i holds tile i's byte offset, -1 where the table has none.
+  auto places = [&](int base) FP4_INLINE {
+    const int q = c0 + w + kFp4Waves * (base + (lane >> 1));
+    if (q >= c1) return int64_t(-1);
     const Fp4Unit u = locate(q);
     const int tile = 2 * (u.first + q - u.u0) + (lane & 1);
     const int pg = fp4_quot(tile, p.by_tiles);
-    if (tile * kFp4Tile >= u.hi || pg >= p.W) return -1;
+    if (tile * kFp4Tile >= u.hi || pg >= p.W) return int64_t(-1);
     const int phys = p.table[static_cast<int64_t>(u.b) * p.W + pg];
-    if (phys < 0 || phys >= p.num_blocks) return -1;
+    if (phys < 0 || phys >= p.num_blocks) return int64_t(-1);
     const int tpp = p.bs / kFp4Tile;
     return static_cast<int64_t>(phys) * p.blk_stride + static_cast<int64_t>(u.kvh) * p.head_stride +
            static_cast<int64_t>(tile - pg * tpp) * fp4_tile_bytes(p.D);
   };
-  int64_t here = places(c0), next = -1;  // of this run of 32 groups, and of the next
-  int run = c0;                          // the run's first position
-  auto place_of = [&](int q, int t) -> int64_t {  // q in this run or the next
-    const int i = 2 * (q - run) + t;
-    auto from = [&](int64_t x) {
+  int64_t here = places(0), next = -1;  // of this run of 32 groups, and of the next
+  int run = 0;                          // the run's first
+  auto place_of = [&](int s, int t) FP4_INLINE {  // s in this run or the next
+    const int i = 2 * (s - run) + t;
+    auto from = [&](int64_t x) FP4_INLINE {
       const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), i & 63);
       const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), i & 63);
       return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
@@ -263,31 +317,21 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
     if (i < 64) return from(here);  // (a branch: the next run's places may be on their way)
     return from(next);
   };
-  auto load_keys = [&](Keys& k, int64_t at) {
-    const uint8_t* t = p.k + (at < 0 ? 0 : at);
-#pragma unroll
-    for (int h = 0; h < HV; ++h) {
-      k.d[h] = *reinterpret_cast<const kraw_t*>(t + k_at[h]);
-      k.s[h] = t[ks_at[h]];
-    }
-  };
-  auto load_values = [&](Values& v, int64_t at) {
-    const uint8_t* t = p.v + (at < 0 ? 0 : at);
-#pragma unroll
-    for (int h = 0; h < HV; ++h) {
-      v.d[h] = *reinterpret_cast<const uint4*>(t + v_at[h]);
-      v.s[h] = *reinterpret_cast<const uint32_t*>(t + vs_at[h]);
-    }
-  };
-  int64_t at[R][2];
-  auto issue = [&](auto slot_c, int q) {
-    constexpr int S = decltype(slot_c)::value;
-    if (q >= c1) return;
+  auto load = [&](Group& x, int s) FP4_INLINE {
+    if (c0 + w + kFp4Waves * s >= c1) return;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      at[S][t] = place_of(q, t);
-      load_keys(kr[S][t], at[S][t]);
-      load_values(vr[S][t], at[S][t]);
+      x.at[t] = place_of(s, t);
+      const int64_t at = x.at[t] < 0 ? 0 : x.at[t];
+      const uint8_t* const kt = p.k + at;
+      const uint8_t* const vt = p.v + at;
+#pragma unroll
+      for (int h = 0; h < HV; ++h) {
+        x.t[t].k[h] = fp4_load<kraw_t>(kt + k_at[h]);
+        x.t[t].ks[h] = fp4_load<uint8_t>(kt + ks_at[h]);
+        x.t[t].v[h] = fp4_load<uint4>(vt + v_at[h]);
+        x.t[t].vs[h] = fp4_load<uint32_t>(vt + vs_at[h]);
+      }
     }
   };
 
@@ -298,8 +342,8 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
   float m_run[CT], l_run[CT];
   int lo_n[CT], hi_n[CT];  // keys the lane's rows see
   int all_lo, all_hi;      // keys every row of the block sees
-  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  auto begin = [&](int q) {
+  auto uniform = [](int x) FP4_INLINE { return __builtin_amdgcn_readfirstlane(x); };
+  auto begin = [&](int q) FP4_INLINE {
     u = locate(q);
     u.b = uniform(u.b); u.kvh = uniform(u.kvh); u.rb = uniform(u.rb); u.lo = uniform(u.lo);
     u.hi = uniform(u.hi); u.first = uniform(u.first); u.n = uniform(u.n); u.u0 = uniform(u.u0);
@@ -354,17 +398,17 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
   };
 
   // Scores of one tile.
-  auto scores = [&](const Keys& k, mf_f32x4 (&s)[CT]) {
+  auto scores = [&](const Tile& k, mf_f32x4 (&s)[CT]) FP4_INLINE {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) s[ct] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int h = 0; h < HV; ++h) {
-      const float sc = fp4_scale(k_in[h] ? k.s[h] : 127u);
-      static_for<NJ>([&](auto jc) {
+      const float sc = fp4_scale(k_in[h] ? k.ks[h] : 127u);
+      static_for<NJ>([&](auto jc) FP4_INLINE {
         constexpr int j = decltype(jc)::value;
         uint32_t x;
-        if constexpr (DH == 128) x = j == 0 ? k.d[h].x : j == 1 ? k.d[h].y : j == 2 ? k.d[h].z : k.d[h].w;
-        else x = j == 0 ? k.d[h].x : k.d[h].y;
+        if constexpr (DH == 128) x = j == 0 ? k.k[h].x : j == 1 ? k.k[h].y : j == 2 ? k.k[h].z : k.k[h].w;
+        else x = j == 0 ? k.k[h].x : k.k[h].y;
         const uint4 ka = make_uint4(fp4_widen2<0>(x, sc), fp4_widen2<1>(x, sc),
                                     fp4_widen2<2>(x, sc), fp4_widen2<3>(x, sc));
 #pragma unroll
@@ -377,7 +421,7 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
 
   uint4 pw[CT][PQ];  // the weights, as the B operand of the value products
   float psum[CT];
-  auto weights = [&](int ct, const mf_f32x4& s0, const mf_f32x4& s1, float mul) {
+  auto weights = [&](int ct, const mf_f32x4& s0, const mf_f32x4& s1, float mul) FP4_INLINE {
     const float m = m_run[ct] != -INFINITY ? m_run[ct] : 0.0f;
     float x[8];
 #pragma unroll
@@ -404,7 +448,7 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
   };
   // The weights with the running maximum as it stands, and only where one of them exceeds 2^8 (or
   // the row has no maximum yet) with one that has moved: their sum bounds each of them.
-  auto softmax = [&](const mf_f32x4 (&s0)[CT], const mf_f32x4 (&s1)[CT], float mul) {
+  auto softmax = [&](const mf_f32x4 (&s0)[CT], const mf_f32x4 (&s1)[CT], float mul) FP4_INLINE {
     bool over = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
@@ -435,7 +479,7 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
 
   // O^T += V^T P^T for half h: d0, d1 the tiles' elements, sc the 8 tokens' scales.
   auto product = [&](auto h_c, const uint4& d0, const uint4& d1, const float (&sc)[8],
-                     const uint4 (&b)[CT][PQ]) {
+                     const uint4 (&b)[CT][PQ]) FP4_INLINE {
     constexpr int h = decltype(h_c)::value;
     uint32_t x[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
     if constexpr (DH == 64) {  // two lanes share 8 dims
@@ -443,7 +487,7 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
 #pragma unroll
       for (int t = 0; t < 8; ++t) x[t] >>= sh;
     }
-    static_for<VC / 2>([&](auto cc) {
+    static_for<VC / 2>([&](auto cc) FP4_INLINE {
       constexpr int c = decltype(cc)::value;
       uint32_t y[8];
 #pragma unroll
@@ -466,162 +510,187 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
   };
   auto byte_of = [](uint32_t x, int i) { return (x >> (8 * i)) & 255u; };
 
-  auto consume = [&](auto slot_c, int q) {
-    constexpr int S = decltype(slot_c)::value;
+  auto consume = [&](Group& x, int q) FP4_INLINE {
     const int tok = (u.first + q - u.u0) * kFp4Group;
     mf_f32x4 s0[CT], s1[CT];
-    scores(kr[S][0], s0);
-    scores(kr[S][1], s1);
-    const bool full = tok >= all_lo && tok + kFp4Group <= all_hi && at[S][0] >= 0 && at[S][1] >= 0;
-    if (full) {
-      softmax(s0, s1, p.scale_log2);
-      static_for<HV>([&](auto hc) {
-        constexpr int h = decltype(hc)::value;
-        float sc[8];
+    scores(x.t[0], s0);
+    scores(x.t[1], s1);
+    const bool full = tok >= all_lo && tok + kFp4Group <= all_hi && x.at[0] >= 0 && x.at[1] >= 0;
+    float mul = p.scale_log2;
+    // Of keys 4 g + i of tile t, bit 4 t + i: where the lane's row sees them, and where a value's
+    // block is NaN (in groups that have masked keys).
+    uint32_t seen[CT], bad[HV], any_bad = 0;
+    if (!full) {
+      uint32_t dead = 0;  // no row sees it, or the table has no page
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sc[i] = fp4_scale(byte_of(vr[S][0].s[h], i));
-          sc[4 + i] = fp4_scale(byte_of(vr[S][1].s[h], i));
-        }
-        product(hc, vr[S][0].d[h], vr[S][1].d[h], sc, pw);
-      });
-      return;
-    }
-    // Keys 4 g + i of tile t for i < 4: bit 4 t + i of `dead` where no row sees it (or the table has
-    // no page), of `seen[ct]` where the lane's row does.
-    uint32_t dead = 0, seen[CT];
+      for (int ct = 0; ct < CT; ++ct) seen[ct] = 0;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) seen[ct] = 0;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const int key = tok + 16 * (x / 4) + 4 * g + x % 4;
-      const bool live = key >= u.lo && key < u.hi && at[S][x / 4] >= 0;
-      dead |= live ? 0u : 1u << x;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const bool see = live && key >= lo_n[ct] && key < hi_n[ct];
-        seen[ct] |= see ? 1u << x : 0u;
-        // (scaled first: a scale of 0 or below must not touch the mask)
-        if (x < 4) s0[ct][x % 4] = see ? s0[ct][x % 4] * p.scale_log2 : -INFINITY;
-        else s1[ct][x % 4] = see ? s1[ct][x % 4] * p.scale_log2 : -INFINITY;
-      }
-    }
-    softmax(s0, s1, 1.0f);
-    static_for<HV>([&](auto hc) {
-      constexpr int h = decltype(hc)::value;
-      float sc[8];
-      uint32_t bad = 0;
-      const uint4 d0 = vr[S][0].d[h], d1 = vr[S][1].d[h];
-      uint32_t el[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const uint32_t byte = byte_of(vr[S][x / 4].s[h], x % 4);
-        const bool gone = (dead >> x) & 1u;
-        const bool nan = !gone && byte == kFp4NaN;
-        bad |= nan ? 1u << x : 0u;
-        sc[x] = gone || nan ? 1.0f : fp4_scale(byte);
-        el[x] = gone || nan ? 0u : el[x];
-      }
-      product(hc, make_uint4(el[0], el[1], el[2], el[3]), make_uint4(el[4], el[5], el[6], el[7]), sc, pw);
-      if (__builtin_expect(__any(bad != 0), 0)) {
-        // Rows that see a NaN block of dims: ones for the blocks times ones for what the rows see.
-        uint32_t aw[4], one[CT][4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          aw[t] = ((bad >> (2 * t)) & 1u ? 0x3f80u : 0u) | ((bad >> (2 * t + 1)) & 1u ? 0x3f800000u : 0u);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-            one[ct][t] = ((seen[ct] >> (2 * t)) & 1u ? 0x3f80u : 0u) |
-                         ((seen[ct] >> (2 * t + 1)) & 1u ? 0x3f800000u : 0u);
-        }
-        const uint4 av = make_uint4(aw[0], aw[1], aw[2], aw[3]);
+      for (int i = 0; i < 8; ++i) {
+        const int key = tok + 16 * (i / 4) + 4 * g + i % 4;
+        const bool live = key >= u.lo && key < u.hi && x.at[i / 4] >= 0;
+        dead |= live ? 0u : 1u << i;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          const mf_f32x4 hit = Mfma16<bf16_t>::mac(
-              av, make_uint4(one[ct][0], one[ct][1], one[ct][2], one[ct][3]), mf_f32x4{0.f, 0.f, 0.f, 0.f});
+          const bool see = live && key >= lo_n[ct] && key < hi_n[ct];
+          seen[ct] |= see ? 1u << i : 0u;
+          // (scaled first: a scale of 0 or below must not touch the mask)
+          if (i < 4) s0[ct][i % 4] = see ? s0[ct][i % 4] * p.scale_log2 : -INFINITY;
+          else s1[ct][i % 4] = see ? s1[ct][i % 4] * p.scale_log2 : -INFINITY;
+        }
+      }
+      mul = 1.0f;
+#pragma unroll
+      for (int h = 0; h < HV; ++h) {
+        bad[h] = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          uint32_t e[4] = {x.t[t].v[h].x, x.t[t].v[h].y, x.t[t].v[h].z, x.t[t].v[h].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool gone = (dead >> (4 * t + i)) & 1u;
+            const bool nan = byte_of(x.t[t].vs[h], i) == kFp4NaN;
+            bad[h] |= nan && !gone ? 1u << (4 * t + i) : 0u;
+            e[i] = gone || nan ? 0u : e[i];
+            x.t[t].vs[h] = gone || nan ? (x.t[t].vs[h] & ~(255u << (8 * i))) | 127u << (8 * i)
+                                       : x.t[t].vs[h];
+          }
+          x.t[t].v[h] = make_uint4(e[0], e[1], e[2], e[3]);
+        }
+        any_bad |= bad[h];
+      }
+    }
+    softmax(s0, s1, mul);
+    static_for<HV>([&](auto hc) FP4_INLINE {
+      constexpr int h = decltype(hc)::value;
+      float sc[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[i] = fp4_scale(byte_of(x.t[0].vs[h], i));
+        sc[4 + i] = fp4_scale(byte_of(x.t[1].vs[h], i));
+      }
+      product(hc, x.t[0].v[h], x.t[1].v[h], sc, pw);
+    });
+    if (!full && __any(any_bad != 0)) {
+      // Rows that see a NaN block of dims: ones for the blocks times ones for what the rows see.
+      auto ones = [](uint32_t bits) FP4_INLINE {
+        uint32_t y[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          y[t] = ((bits >> (2 * t)) & 1u ? 0x3f80u : 0u) | ((bits >> (2 * t + 1)) & 1u ? 0x3f800000u : 0u);
+        return make_uint4(y[0], y[1], y[2], y[3]);
+      };
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int h = 0; h < HV; ++h) {
+          const mf_f32x4 hit =
+              Mfma16<bf16_t>::mac(ones(bad[h]), ones(seen[ct]), mf_f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
           for (int c = 0; c < VC; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               acc[ct][h][c][i] = hit[i] > 0.0f ? __uint_as_float(0x7fc00000u) : acc[ct][h][c][i];
         }
-      }
-    });
+    }
   };
 
-  auto out_at = [&](int r) {  // element offset of row r of the unit's KV head in the output
+  auto out_at = [&](int r) FP4_INLINE {  // element offset of row r of the unit's KV head in the output
     const int i = fp4_quot(r, p.by_g);
     return ((static_cast<int64_t>(u.b) * p.q_len + i) * p.H + (u.kvh * p.G + (r - i * p.G))) * p.D;
   };
-  // Normalised rows, or a partial and perhaps the join.
-  auto finish = [&]() {
+  // The waves' parts of the unit joined, 16 rows at a time: normalised rows, or a partial of the
+  // share and perhaps the join of the unit's shares.
+  auto finish = [&]() FP4_INLINE {
     const int r0 = u.rb * ROWS;
     const int rows = min(ROWS, p.rows_per_kvh - r0);
-    float l[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) l[ct] = rows4_sum(l_run[ct]);
+    const int per = p.D / 4;  // items of a row
     const bool whole = u.u0 >= c0 && u.u0 + u.n <= c1;
-    if (whole) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        if (16 * ct + n >= rows) continue;
-        const float inv = l[ct] != 0.0f ? 1.0f / l[ct] : 0.0f;  // (a NaN stays one)
-        T* const o = static_cast<T*>(p.out) + out_at(r0 + 16 * ct + n);
-#pragma unroll
-        for (int h = 0; h < HV; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int dim = 128 * h + LD * g + VC * i;
-            if (dim >= p.D) continue;
-#pragma unroll
-            for (int c = 0; c < VC; ++c) Elt<T>::store(o + dim + c, acc[ct][h][c][i] * inv);
-          }
-      }
-      return;
-    }
     const int64_t slot = 2 * static_cast<int64_t>(share) + (u.u0 >= c0 ? 1 : 0);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const int r = 16 * ct + n;
-      if (r >= rows) continue;
-      const int64_t row = slot * p.slot_rows + r;
-      if (g == 0) store2_device(p.ml + row * 2, m_run[ct], l[ct]);
+      const int here_rows = min(16, rows - 16 * ct);
+      if (here_rows <= 0) break;
+      const float l = rows4_sum(l_run[ct]);
+      if (n < here_rows) {
+        if (g == 0) s_ml[w][n] = make_float2(m_run[ct], l);
 #pragma unroll
-      for (int h = 0; h < HV; ++h)
+        for (int h = 0; h < HV; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int dim = 128 * h + LD * g + VC * i;
-          if (dim >= p.D) continue;
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int c = 0; c < VC; c += 2)
-            store2_device(p.acc + row * p.D + dim + c, acc[ct][h][c][i], acc[ct][h][c + 1][i]);
+            for (int c = 0; c < VC; c += 4)
+              *reinterpret_cast<float4*>(&s_acc[w][n][128 * h + LD * g + VC * i + c]) =
+                  make_float4(acc[ct][h][c][i], acc[ct][h][c + 1][i], acc[ct][h][c + 2][i],
+                              acc[ct][h][c + 3][i]);
+      }
+      lds_barrier();
+      for (int idx = tid; idx < here_rows * per; idx += kFp4Threads) {
+        const int r = idx / per, d = 4 * (idx - r * per);
+        float2 ml[kFp4Waves];
+        float M = -INFINITY, L = 0.0f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kFp4Waves; ++i) {
+          ml[i] = s_ml[i][r];
+          M = fmaxf(M, ml[i].x);
         }
+#pragma unroll
+        for (int i = 0; i < kFp4Waves; ++i) {
+          const float f = __builtin_amdgcn_exp2f(M != -INFINITY ? ml[i].x - M : 0.0f);
+          const float4 x = *reinterpret_cast<const float4*>(&s_acc[i][r][d]);
+          L = fmaf(f, ml[i].y, L);
+          a.x = fmaf(f, x.x, a.x);
+          a.y = fmaf(f, x.y, a.y);
+          a.z = fmaf(f, x.z, a.z);
+          a.w = fmaf(f, x.w, a.w);
+        }
+        if (whole) {
+          const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // (a NaN stays one)
+          fp4_store4<T>(static_cast<T*>(p.out) + out_at(r0 + 16 * ct + r) + d, a.x * inv, a.y * inv,
+                        a.z * inv, a.w * inv);
+        } else {
+          const int64_t row = slot * p.slot_rows + 16 * ct + r;
+          if (d == 0) store2_device(p.ml + row * 2, M, L);
+          store2_device(p.acc + row * p.D + d, a.x, a.y);
+          store2_device(p.acc + row * p.D + d + 2, a.z, a.w);
+        }
+      }
+      lds_barrier();
     }
+    if (whole) return;
     // The shares that hold the unit's groups; the first names its counter. The partials above are
     // written through (agent scope) before the counter moves, and read the same way after it.
     const int s_first = u.u0 / chunk, s_last = (u.u0 + u.n - 1) / chunk;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    int last = 0;
-    if (lane == 0) {
+    lds_barrier();
+    if (tid == 0) {
       int* const t = p.tickets + s_first;
       const int old = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      last = old == s_last - s_first;
+      const int last = old == s_last - s_first;
       if (last) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_tot[0] = last;
     }
-    last = uniform(last);
+    lds_barrier();
+    const int last = uniform(s_tot[0]);
     asm volatile("" ::: "memory");
     if (!last) return;
-    const int per = p.D / 4;
-    for (int idx = lane; idx < rows * per; idx += 64) {
-      const int r = idx / per, d = 4 * (idx - r * per);
+    // Threads left over take other shares of the same items, and are joined through LDS.
+    const int items = rows * per;
+    const int fold = items >= kFp4Threads ? 1 : kFp4Threads / items;
+    float* const s_part = &s_acc[0][0][0];  // [thread][6]
+    for (int i0 = 0; i0 < items; i0 += kFp4Threads) {
+      const int k = fold == 1 ? 0 : tid / items;
+      const int idx = fold == 1 ? i0 + tid : tid - k * items;
+      const bool mine = idx < items && k < fold;
+      const int r = mine ? idx / per : 0, d = mine ? 4 * (idx - r * per) : 0;
       float M = -INFINITY, L = 0.0f;
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-      constexpr int N = 8;
-      for (int j0 = s_first; j0 <= s_last; j0 += N) {
+      constexpr int N = 4;
+      for (int j0 = s_first + k; mine && j0 <= s_last; j0 += N * fold) {
         float2 x0[N], x1[N], ml[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {  // shares past the last repeat it, unused
-          const int j = min(j0 + i, s_last);
+          const int j = min(j0 + i * fold, s_last);
           const int64_t row = (2 * static_cast<int64_t>(j) + (j == s_first ? 1 : 0)) * p.slot_rows + r;
           ml[i] = load2_device(p.ml + row * 2);
           x0[i] = load2_device(p.acc + row * p.D + d);
@@ -629,14 +698,13 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
         }
         float mb = M;
 #pragma unroll
-        for (int i = 0; i < N; ++i) mb = fmaxf(mb, j0 + i <= s_last ? ml[i].x : -INFINITY);
-        const float keep = mb != -INFINITY ? __builtin_amdgcn_exp2f(M - mb) : 1.0f;
+        for (int i = 0; i < N; ++i) mb = fmaxf(mb, j0 + i * fold <= s_last ? ml[i].x : -INFINITY);
+        const float keep = __builtin_amdgcn_exp2f(mb != -INFINITY ? M - mb : 0.0f);
         L *= keep;
         a.x *= keep; a.y *= keep; a.z *= keep; a.w *= keep;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          // a share without a visible key of the row has nothing (its m is -inf, its sum 0)
-          const bool live = j0 + i <= s_last && !(ml[i].x == -INFINITY && ml[i].y == 0.0f);
+          const bool live = j0 + i * fold <= s_last;
           const float f = __builtin_amdgcn_exp2f(live && mb != -INFINITY ? ml[i].x - mb : 0.0f);
           L = live ? fmaf(f, ml[i].y, L) : L;
           a.x = live ? fmaf(f, x0[i].x, a.x) : a.x;
@@ -646,38 +714,63 @@ __global__ __launch_bounds__(64 * kFp4Waves, 2) void fp4_attn_kernel(const Fp4Pa
         }
         M = mb;
       }
-      const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-      T* const o = static_cast<T*>(p.out) + out_at(r0 + r) + d;
-      Elt<T>::store(o + 0, a.x * inv);
-      Elt<T>::store(o + 1, a.y * inv);
-      Elt<T>::store(o + 2, a.z * inv);
-      Elt<T>::store(o + 3, a.w * inv);
+      if (fold > 1) {
+        float* const mine_at = s_part + 6 * tid;
+        mine_at[0] = M; mine_at[1] = L; mine_at[2] = a.x; mine_at[3] = a.y; mine_at[4] = a.z;
+        mine_at[5] = a.w;
+        lds_barrier();
+        if (mine && k == 0) {
+          float mb = M;
+          for (int i = 1; i < fold; ++i) mb = fmaxf(mb, s_part[6 * (tid + i * items)]);
+          const float keep = __builtin_amdgcn_exp2f(mb != -INFINITY ? M - mb : 0.0f);
+          L *= keep;
+          a.x *= keep; a.y *= keep; a.z *= keep; a.w *= keep;
+          for (int i = 1; i < fold; ++i) {
+            const float* const x = s_part + 6 * (tid + i * items);
+            const float f = __builtin_amdgcn_exp2f(mb != -INFINITY ? x[0] - mb : 0.0f);
+            L = fmaf(f, x[1], L);
+            a.x = fmaf(f, x[2], a.x);
+            a.y = fmaf(f, x[3], a.y);
+            a.z = fmaf(f, x[4], a.z);
+            a.w = fmaf(f, x[5], a.w);
+          }
+        }
+        lds_barrier();
+      }
+      if (mine && k == 0) {
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        fp4_store4<T>(static_cast<T*>(p.out) + out_at(r0 + r) + d, a.x * inv, a.y * inv, a.z * inv,
+                      a.w * inv);
+      }
     }
   };
 
   // ---- the share ----
-  using S0 = std::integral_constant<int, 0>;
-  using S1 = std::integral_constant<int, 1>;
-  issue(S0{}, c0);
-  issue(S1{}, c0 + 1);
-  next = places(c0 + 32);
-  begin(c0);
-  auto step = [&](auto slot_c, int q) {
-    consume(slot_c, q);
-    issue(slot_c, q + R);
-    if (q + 1 == c1 || q + 1 == u.u0 + u.n) {
-      finish();
-      if (q + 1 < c1) begin(q + 1);
+  Group even, odd;  // two groups on their way
+  load(even, 0);
+  load(odd, 1);
+  next = places(32);
+  int s = 0;  // the wave's next group
+  for (int q = c0; q < c1;) {
+    begin(q);
+    q = min(c1, u.u0 + u.n);
+    for (int at; (at = c0 + w + kFp4Waves * s) < q; ++s) {
+      if (s - run == 32) {
+        run = s;
+        here = next;
+        next = places(run + 32);
+      }
+      Group x;
+      if (s & 1) {
+        x = odd;
+        load(odd, s + 2);
+      } else {
+        x = even;
+        load(even, s + 2);
+      }
+      consume(x, at);
     }
-  };
-  for (int q = c0; q < c1; q += 2) {
-    if (q - run == 32) {
-      run = q;
-      here = next;
-      next = places(run + 32);
-    }
-    step(S0{}, q);
-    if (q + 1 < c1) step(S1{}, q + 1);
+    finish();
   }
 }
 

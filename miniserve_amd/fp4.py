@@ -220,6 +220,9 @@ def paged_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         out = torch.empty((B, q_len, H, D), dtype=query.dtype, device=dev)
     if B == 0 or q_len == 0:
         return out
+    given = None
+    if out.data_ptr() % 16:  # (the kernel stores 16 bytes at once)
+        given, out = out, torch.empty_like(out)
     q = query.resolve_neg() if query.is_neg() else query
     es = q.element_size()
     if q.stride(3) != 1 or any(s * es % 16 for s in q.stride()[:3]):
@@ -245,4 +248,4 @@ def paged_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         nb, W, max_context, 1 if causal else 0, min(int(window or 0), 2 ** 31 - 1), float(scale),
         code)
     nat.check("msattn_paged_attention_fp4", status)
-    return out
+    return out if given is None else given.copy_(out)
