@@ -71,6 +71,13 @@ struct Fp4Params {
   float* acc;        // [2 shares][slot_rows][D]
 };
 
+// A value the compiler knows nothing of from here on.
+__device__ __forceinline__ void opaque(uint32_t& x) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the constraint names a GPU register class
+  asm volatile("" : "+v"(x));
+#endif
+}
+
 // bf16 parts that a T's value enters a product as.
 template <typename T> constexpr int fp4_parts() {
   return std::is_same<T, bf16_t>::value ? 1 : (std::is_same<T, _Float16>::value ? 2 : 3);
@@ -103,8 +110,8 @@ __device__ __forceinline__ void fp4_store4(T* o, float a, float b, float c, floa
 #ifndef MSATTN_FP4_NT
 #define MSATTN_FP4_NT 0
 #endif
-#ifndef MSATTN_FP4_OCC
-#define MSATTN_FP4_OCC 2
+#ifndef MSATTN_FP4_RING
+#define MSATTN_FP4_RING 3
 #endif
 template <typename V>
 __device__ __forceinline__ V fp4_load(const uint8_t* p) {
@@ -156,6 +163,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   constexpr int LD = DH / 4;             // dims a lane receives of a half
   constexpr int PQ = fp4_parts<T>();
   constexpr int ROWS = 16 * CT;
+  constexpr int kRing = DP == 256 || (CT == 2 && PQ == 3) ? 2 : MSATTN_FP4_RING;
   typedef typename std::conditional<DH == 128, uint4, uint2>::type kraw_t;
 
   __shared__ int s_pre[kFp4MaxEntries + 1];
@@ -225,11 +233,11 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     c1 = share < entries * p.KVH ? 1 : 0;  // its unit's groups, set below
   }
 
-  // The unit holding position q of the list (any lane's own q).
-  auto locate = [&](int q) FP4_INLINE {
+  // The unit holding position q of the list (any lane's own q), in rows a0 .. z0 - 1.
+  auto locate = [&](int q, int a0, int z0) FP4_INLINE {
     Fp4Unit u;
     if (p.split) {
-      int a = 0, z = p.batch;  // the row: KVH s_pre[a rblocks] <= q < KVH s_pre[z rblocks]
+      int a = a0, z = z0;  // the row: KVH s_pre[a rblocks] <= q < KVH s_pre[z rblocks]
       while (z - a > 1) {
         const int m = (a + z) >> 1;
         if (s_pre[m * p.rblocks] * p.KVH <= q) a = m;
@@ -263,7 +271,23 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   };
 
   if (c0 >= c1) return;  // (the workgroup as one)
-  if (!p.split) c1 = __builtin_amdgcn_readfirstlane(locate(0).n);
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  auto unit_at = [&](int q, int a0, int z0) FP4_INLINE {  // locate of one position for the wave
+    Fp4Unit u = locate(q, a0, z0);
+    u.b = uniform(u.b);
+    u.kvh = uniform(u.kvh);
+    u.rb = uniform(u.rb);
+    u.lo = uniform(u.lo);
+    u.hi = uniform(u.hi);
+    u.first = uniform(u.first);
+    u.n = uniform(u.n);
+    u.u0 = uniform(u.u0);
+    return u;
+  };
+  Fp4Unit u = unit_at(c0, 0, p.batch);
+  if (!p.split) c1 = u.n;
+  const int b_end = c1 <= u.u0 + u.n ? u.b + 1 : unit_at(c1 - 1, u.b, p.batch).b + 1;  // the share's rows
+  const int b_first = u.b;
 
   // ---- what a lane holds of a tile: fixed places, one register each ----
   uint32_t k_at[HV], ks_at[HV], v_at[HV], vs_at[HV];
@@ -285,68 +309,94 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     uint4 v[HV];
     uint32_t vs[HV];
   };
-  struct Group {  // two tiles, and where they lie (-1: nowhere)
-    Tile t[2];
-    int64_t at[2];
-  };
+  typedef Tile Group[2];
 
   // Wave w takes positions c0 + w + 8 s of the share. Places of the tiles of its 32 groups from s =
-  // base on: lane i holds tile i's byte offset, -1 where the table has none.
-  auto places = [&](int base) FP4_INLINE {
+  // base on: lane i holds tile i's byte offset, and bit i of `holes` says that the table has none
+  // (the offset is then one that can be read).
+  auto places = [&](int base, uint64_t* holes) FP4_INLINE {
     const int q = c0 + w + kFp4Waves * (base + (lane >> 1));
-    if (q >= c1) return int64_t(-1);
-    const Fp4Unit u = locate(q);
-    const int tile = 2 * (u.first + q - u.u0) + (lane & 1);
-    const int pg = fp4_quot(tile, p.by_tiles);
-    if (tile * kFp4Tile >= u.hi || pg >= p.W) return int64_t(-1);
-    const int phys = p.table[static_cast<int64_t>(u.b) * p.W + pg];
-    if (phys < 0 || phys >= p.num_blocks) return int64_t(-1);
-    const int tpp = p.bs / kFp4Tile;
-    return static_cast<int64_t>(phys) * p.blk_stride + static_cast<int64_t>(u.kvh) * p.head_stride +
-           static_cast<int64_t>(tile - pg * tpp) * fp4_tile_bytes(p.D);
+    int64_t at = -1;
+    if (q < c1) {
+      const Fp4Unit v = locate(q, b_first, b_end);
+      const int tile = 2 * (v.first + q - v.u0) + (lane & 1);
+      const int pg = fp4_quot(tile, p.by_tiles);
+      if (tile * kFp4Tile < v.hi && pg < p.W) {
+        const int phys = p.table[static_cast<int64_t>(v.b) * p.W + pg];
+        if (phys >= 0 && phys < p.num_blocks)
+          at = static_cast<int64_t>(phys) * p.blk_stride + static_cast<int64_t>(v.kvh) * p.head_stride +
+               static_cast<int64_t>(tile - pg * (p.bs / kFp4Tile)) * fp4_tile_bytes(p.D);
+      }
+    }
+    *holes = __ballot(at < 0);
+    return at < 0 ? int64_t(0) : at;
   };
-  int64_t here = places(0), next = -1;  // of this run of 32 groups, and of the next
-  int run = 0;                          // the run's first
-  auto place_of = [&](int s, int t) FP4_INLINE {  // s in this run or the next
-    const int i = 2 * (s - run) + t;
-    auto from = [&](int64_t x) FP4_INLINE {
-      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), i & 63);
-      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), i & 63);
+  uint64_t holes, next_holes = 0;
+  int64_t here = places(0, &holes), next = 0;  // of this run of 32 groups, and of the next
+  int run = 0;                                 // the run's first
+  const int rounds = (c1 - c0 - w + kFp4Waves - 1) / kFp4Waves;  // groups of the wave
+  auto load = [&](Group& x, int s) FP4_INLINE {  // group s, of this run or the next
+    if (s >= rounds) return;
+    const int i = 2 * (s - run);
+    auto from = [&](int64_t places, int t) FP4_INLINE {
+      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(places), (i + t) & 63);
+      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(places >> 32), (i + t) & 63);
       return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
     };
-    if (i < 64) return from(here);  // (a branch: the next run's places may be on their way)
-    return from(next);
-  };
-  auto load = [&](Group& x, int s) FP4_INLINE {
-    if (c0 + w + kFp4Waves * s >= c1) return;
+    int64_t at[2];
+    if (i < 64) {  // (a branch: the next run's places may be on their way)
+      at[0] = from(here, 0);
+      at[1] = from(here, 1);
+    } else {
+      at[0] = from(next, 0);
+      at[1] = from(next, 1);
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      x.at[t] = place_of(s, t);
-      const int64_t at = x.at[t] < 0 ? 0 : x.at[t];
-      const uint8_t* const kt = p.k + at;
-      const uint8_t* const vt = p.v + at;
+      const uint8_t* const kt = p.k + at[t];
+      const uint8_t* const vt = p.v + at[t];
 #pragma unroll
       for (int h = 0; h < HV; ++h) {
-        x.t[t].k[h] = fp4_load<kraw_t>(kt + k_at[h]);
-        x.t[t].ks[h] = fp4_load<uint8_t>(kt + ks_at[h]);
-        x.t[t].v[h] = fp4_load<uint4>(vt + v_at[h]);
-        x.t[t].vs[h] = fp4_load<uint32_t>(vt + vs_at[h]);
+        x[t].k[h] = fp4_load<kraw_t>(kt + k_at[h]);
+        x[t].ks[h] = fp4_load<uint8_t>(kt + ks_at[h]);
+        x[t].v[h] = fp4_load<uint4>(vt + v_at[h]);
+        x[t].vs[h] = fp4_load<uint32_t>(vt + vs_at[h]);
       }
     }
   };
 
   // ---- a unit's state ----
-  Fp4Unit u;
   uint4 qf[CT][HV][NJ][PQ];
   mf_f32x4 acc[CT][HV][VC];
   float m_run[CT], l_run[CT];
   int lo_n[CT], hi_n[CT];  // keys the lane's rows see
   int all_lo, all_hi;      // keys every row of the block sees
-  auto uniform = [](int x) FP4_INLINE { return __builtin_amdgcn_readfirstlane(x); };
-  auto begin = [&](int q) FP4_INLINE {
-    u = locate(q);
-    u.b = uniform(u.b); u.kvh = uniform(u.kvh); u.rb = uniform(u.rb); u.lo = uniform(u.lo);
-    u.hi = uniform(u.hi); u.first = uniform(u.first); u.n = uniform(u.n); u.u0 = uniform(u.u0);
+  constexpr int QW = static_cast<int>(sizeof(T)) / 2;  // 16-byte words of 8 query elements
+  uint4 q_raw[CT][HV][NJ][QW];
+  auto query = [&]() FP4_INLINE {  // u's query rows, requested
+    const int r0 = u.rb * ROWS;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int r = r0 + 16 * ct + n;
+      const bool ok = r < p.rows_per_kvh;
+      const int i = ok ? fp4_quot(r, p.by_g) : 0;
+      const T* const qp = static_cast<const T*>(p.q) + u.b * p.q_st[0] + i * p.q_st[1] +
+                          (u.kvh * p.G + (ok ? r - i * p.G : 0)) * p.q_st[2];
+#pragma unroll
+      for (int h = 0; h < HV; ++h)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int dim = 128 * h + g * LD + 8 * j;
+#pragma unroll
+          for (int x = 0; x < QW; ++x) {
+            q_raw[ct][h][j][x] = make_uint4(0u, 0u, 0u, 0u);
+            if (ok && dim < p.D)
+              q_raw[ct][h][j][x] = *reinterpret_cast<const uint4*>(qp + dim + x * Chunk<T>::kElems);
+          }
+        }
+    }
+  };
+  auto begin = [&]() FP4_INLINE {
     const int ctx = uniform(ctx_of(u.b));
     const int r0 = u.rb * ROWS;
     const int r1 = min(r0 + ROWS, p.rows_per_kvh) - 1;
@@ -356,35 +406,24 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       const int r = r0 + 16 * ct + n;
-      const bool ok = r <= r1;
-      const int i = ok ? fp4_quot(r, p.by_g) : 0;
-      const int qpos = ctx - p.q_len + i;
-      hi_n[ct] = !ok ? 0 : (p.causal ? min(ctx, qpos + 1) : ctx);
+      const int qpos = ctx - p.q_len + fp4_quot(min(r, r1), p.by_g);
+      hi_n[ct] = r > r1 ? 0 : (p.causal ? min(ctx, qpos + 1) : ctx);
       lo_n[ct] = p.window > 0 ? max(0, qpos - p.window + 1) : 0;
       m_run[ct] = -INFINITY;
       l_run[ct] = 0.0f;
-      const T* const qp = static_cast<const T*>(p.q) + u.b * p.q_st[0] + i * p.q_st[1] +
-                          (u.kvh * p.G + (ok ? r - i * p.G : 0)) * p.q_st[2];
 #pragma unroll
       for (int h = 0; h < HV; ++h) {
 #pragma unroll
         for (int c = 0; c < VC; ++c) acc[ct][h][c] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          const int dim = 128 * h + g * LD + 8 * j;
-          uint4 raw[sizeof(T) == 4 ? 2 : 1] = {};
-          if (ok && dim < p.D) {
-#pragma unroll
-            for (int i2 = 0; i2 < static_cast<int>(sizeof(T)) / 2; ++i2)
-              raw[i2] = *reinterpret_cast<const uint4*>(qp + dim + i2 * Chunk<T>::kElems);
-          }
           if constexpr (PQ == 1) {
-            qf[ct][h][j][0] = raw[0];
+            qf[ct][h][j][0] = q_raw[ct][h][j][0];
           } else {
             float x[8];
 #pragma unroll
-            for (int i2 = 0; i2 < static_cast<int>(sizeof(T)) / 2; ++i2)
-              Chunk<T>::unpack(raw[i2], x + i2 * Chunk<T>::kElems);
+            for (int i = 0; i < QW; ++i)
+              Chunk<T>::unpack(q_raw[ct][h][j][i], x + i * Chunk<T>::kElems);
 #pragma unroll
             for (int a = 0; a < PQ; ++a) {
               const uint32_t w0 = fp4_cut2(x[0], x[1]), w1 = fp4_cut2(x[2], x[3]);
@@ -510,12 +549,13 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   };
   auto byte_of = [](uint32_t x, int i) { return (x >> (8 * i)) & 255u; };
 
-  auto consume = [&](Group& x, int q) FP4_INLINE {
-    const int tok = (u.first + q - u.u0) * kFp4Group;
+  auto consume = [&](Group& x, int s) FP4_INLINE {
+    const int tok = (u.first + c0 + w + kFp4Waves * s - u.u0) * kFp4Group;
     mf_f32x4 s0[CT], s1[CT];
-    scores(x.t[0], s0);
-    scores(x.t[1], s1);
-    const bool full = tok >= all_lo && tok + kFp4Group <= all_hi && x.at[0] >= 0 && x.at[1] >= 0;
+    scores(x[0], s0);
+    scores(x[1], s1);
+    const uint32_t hole = static_cast<uint32_t>(holes >> (2 * (s - run))) & 3u;
+    const bool full = tok >= all_lo && tok + kFp4Group <= all_hi && hole == 0;
     float mul = p.scale_log2;
     // Of keys 4 g + i of tile t, bit 4 t + i: where the lane's row sees them, and where a value's
     // block is NaN (in groups that have masked keys).
@@ -527,7 +567,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int key = tok + 16 * (i / 4) + 4 * g + i % 4;
-        const bool live = key >= u.lo && key < u.hi && x.at[i / 4] >= 0;
+        const bool live = key >= u.lo && key < u.hi && !((hole >> (i / 4)) & 1u);
         dead |= live ? 0u : 1u << i;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
@@ -544,17 +584,17 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         bad[h] = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          uint32_t e[4] = {x.t[t].v[h].x, x.t[t].v[h].y, x.t[t].v[h].z, x.t[t].v[h].w};
+          uint32_t e[4] = {x[t].v[h].x, x[t].v[h].y, x[t].v[h].z, x[t].v[h].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const bool gone = (dead >> (4 * t + i)) & 1u;
-            const bool nan = byte_of(x.t[t].vs[h], i) == kFp4NaN;
+            const bool nan = byte_of(x[t].vs[h], i) == kFp4NaN;
             bad[h] |= nan && !gone ? 1u << (4 * t + i) : 0u;
             e[i] = gone || nan ? 0u : e[i];
-            x.t[t].vs[h] = gone || nan ? (x.t[t].vs[h] & ~(255u << (8 * i))) | 127u << (8 * i)
-                                       : x.t[t].vs[h];
+            x[t].vs[h] = gone || nan ? (x[t].vs[h] & ~(255u << (8 * i))) | 127u << (8 * i)
+                                       : x[t].vs[h];
           }
-          x.t[t].v[h] = make_uint4(e[0], e[1], e[2], e[3]);
+          x[t].v[h] = make_uint4(e[0], e[1], e[2], e[3]);
         }
         any_bad |= bad[h];
       }
@@ -565,14 +605,15 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       float sc[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sc[i] = fp4_scale(byte_of(x.t[0].vs[h], i));
-        sc[4 + i] = fp4_scale(byte_of(x.t[1].vs[h], i));
+        sc[i] = fp4_scale(byte_of(x[0].vs[h], i));
+        sc[4 + i] = fp4_scale(byte_of(x[1].vs[h], i));
       }
-      product(hc, x.t[0].v[h], x.t[1].v[h], sc, pw);
+      product(hc, x[0].v[h], x[1].v[h], sc, pw);
     });
     if (!full && __any(any_bad != 0)) {
       // Rows that see a NaN block of dims: ones for the blocks times ones for what the rows see.
       auto ones = [](uint32_t bits) FP4_INLINE {
+        opaque(bits);  // (else the compiler works these out for every group)
         uint32_t y[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -594,13 +635,12 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     }
   };
 
-  auto out_at = [&](int r) FP4_INLINE {  // element offset of row r of the unit's KV head in the output
+  auto out_at = [&](const Fp4Unit& u, int r) FP4_INLINE {  // element offset of row r of the unit's KV head in the output
     const int i = fp4_quot(r, p.by_g);
     return ((static_cast<int64_t>(u.b) * p.q_len + i) * p.H + (u.kvh * p.G + (r - i * p.G))) * p.D;
   };
-  // The waves' parts of the unit joined, 16 rows at a time: normalised rows, or a partial of the
-  // share and perhaps the join of the unit's shares.
-  auto finish = [&]() FP4_INLINE {
+  // The waves' parts of unit u joined, 16 rows at a time: normalised rows, or the share's partial.
+  auto finish = [&](const Fp4Unit& u) FP4_INLINE {
     const int r0 = u.rb * ROWS;
     const int rows = min(ROWS, p.rows_per_kvh - r0);
     const int per = p.D / 4;  // items of a row
@@ -646,7 +686,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         }
         if (whole) {
           const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // (a NaN stays one)
-          fp4_store4<T>(static_cast<T*>(p.out) + out_at(r0 + 16 * ct + r) + d, a.x * inv, a.y * inv,
+          fp4_store4<T>(static_cast<T*>(p.out) + out_at(u, r0 + 16 * ct + r) + d, a.x * inv, a.y * inv,
                         a.z * inv, a.w * inv);
         } else {
           const int64_t row = slot * p.slot_rows + 16 * ct + r;
@@ -657,23 +697,13 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       }
       lds_barrier();
     }
-    if (whole) return;
-    // The shares that hold the unit's groups; the first names its counter. The partials above are
-    // written through (agent scope) before the counter moves, and read the same way after it.
-    const int s_first = u.u0 / chunk, s_last = (u.u0 + u.n - 1) / chunk;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds_barrier();
-    if (tid == 0) {
-      int* const t = p.tickets + s_first;
-      const int old = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const int last = old == s_last - s_first;
-      if (last) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      s_tot[0] = last;
-    }
-    lds_barrier();
-    const int last = uniform(s_tot[0]);
-    asm volatile("" ::: "memory");
-    if (!last) return;
+  };
+  // The join of unit v, whose shares have all left their partials.
+  auto join = [&](const Fp4Unit& v) FP4_INLINE {
+    const int r0 = v.rb * ROWS;
+    const int rows = min(ROWS, p.rows_per_kvh - r0);
+    const int per = p.D / 4;
+    const int s_first = v.u0 / chunk, s_last = (v.u0 + v.n - 1) / chunk;
     // Threads left over take other shares of the same items, and are joined through LDS.
     const int items = rows * per;
     const int fold = items >= kFp4Threads ? 1 : kFp4Threads / items;
@@ -739,38 +769,74 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       }
       if (mine && k == 0) {
         const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        fp4_store4<T>(static_cast<T*>(p.out) + out_at(r0 + r) + d, a.x * inv, a.y * inv, a.z * inv,
+        fp4_store4<T>(static_cast<T*>(p.out) + out_at(v, r0 + r) + d, a.x * inv, a.y * inv, a.z * inv,
                       a.w * inv);
       }
     }
   };
 
   // ---- the share ----
-  Group even, odd;  // two groups on their way
-  load(even, 0);
-  load(odd, 1);
-  next = places(32);
-  int s = 0;  // the wave's next group
-  for (int q = c0; q < c1;) {
-    begin(q);
-    q = min(c1, u.u0 + u.n);
-    for (int at; (at = c0 + w + kFp4Waves * s) < q; ++s) {
+  query();
+  Group ring[kRing];  // the next groups, on their way
+  static_for<kRing>([&](auto i) FP4_INLINE { load(ring[i], i); });
+  if (rounds > 32) next = places(32, &next_holes);
+  const bool head = u.u0 < c0 || u.u0 + u.n > c1;  // the first unit has other shares
+  int s = 0, turn = 0;  // the wave's next group, and where in the ring it is
+  for (;;) {
+    begin();
+    const int end = min(c1, u.u0 + u.n);
+    const int s_end = (end - c0 - w + kFp4Waves - 1) / kFp4Waves;
+    for (; s < s_end; ++s) {
       if (s - run == 32) {
         run = s;
         here = next;
-        next = places(run + 32);
+        holes = next_holes;
+        if (rounds > s + 32) next = places(s + 32, &next_holes);
       }
-      Group x;
-      if (s & 1) {
-        x = odd;
-        load(odd, s + 2);
-      } else {
-        x = even;
-        load(even, s + 2);
-      }
-      consume(x, at);
+      // (a copy of the code for each place of the ring: its registers are not moved)
+      static_for<kRing>([&](auto i) FP4_INLINE {
+        if (turn == i) {
+          consume(ring[i], s);
+          load(ring[i], s + kRing);
+        }
+      });
+      turn = turn == kRing - 1 ? 0 : turn + 1;
     }
-    finish();
+    const Fp4Unit done = u;
+    if (end < c1) {
+      u = unit_at(end, b_first, b_end);
+      query();
+    }
+    finish(done);
+    if (end == c1) break;
+  }
+
+  // ---- the first and the last unit, where they have other shares ----
+  const bool tail = u.u0 + u.n > c1 || u.u0 < c0;  // (u: the last; perhaps the first too)
+  if (!head && !tail) return;
+  // The partials are written through (agent scope) before the counters move, and read the same way
+  // after them. A unit's counter is its first share's, which no other unit split has.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  lds_barrier();
+  const Fp4Unit first = unit_at(c0, b_first, b_end);
+  if (tid < 2) {
+    const Fp4Unit& v = tid == 0 ? first : u;
+    const int mine = tid == 0 ? head && first.u0 != u.u0 : tail;
+    int last = 0;
+    if (mine) {
+      const int s_first = v.u0 / chunk, s_last = (v.u0 + v.n - 1) / chunk;
+      int* const t = p.tickets + s_first;
+      const int old = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      last = old == s_last - s_first;
+      if (last) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    s_tot[tid] = last;
+  }
+  lds_barrier();
+  const int last0 = uniform(s_tot[0]), last1 = uniform(s_tot[1]);
+  asm volatile("" ::: "memory");
+  for (int i = 0; i < 2; ++i) {
+    if (i == 0 ? last0 : last1) join(i == 0 ? first : u);
   }
 }
 
