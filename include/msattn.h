@@ -47,6 +47,7 @@ typedef enum msattn_status {
   MSATTN_ERR_UNSUPPORTED = 2,  /* valid request outside the compiled kernel set */
   MSATTN_ERR_WORKSPACE = 3,    /* workspace smaller than msattn_workspace_bytes() */
   MSATTN_ERR_HIP = 4,          /* a HIP launch reported an error */
+  MSATTN_ERR_OVERLAP = 5,      /* an input shares memory with what the call writes */
 } msattn_status;
 
 /* Kernel routes of msattn_paged_attention (msattn_paged_attention_route). */
@@ -478,13 +479,14 @@ int msattn_gather_kv(const void* cache, int64_t cache_block_stride, int64_t cach
  * msattn_write_kv_fp4: msattn_write_kv_strided into such a cache. A block whose largest magnitude
  * is a takes the power of two 2^e with a / 2^e in (3.5, 7] (e from -126 to 125), its elements
  * x / 2^e to the nearest, ties to the even code, at most 6; one with a NaN or an infinity reads
- * back as NaN. k_strides / v_strides are the batch, token and head strides of k and v in elements.
- * The same row gives the same bytes whatever stands beside it. Two tokens of one call must not
- * land in one slot.
+ * back as NaN. The strides of k and v are in elements. The same row gives the same bytes whatever
+ * stands beside it. Two tokens of one call must not land in one slot. MSATTN_ERR_OVERLAP where k or
+ * v shares memory with a cache.
  */
-int msattn_write_kv_fp4(const void* k, const int64_t* k_strides, const void* v,
-                        const int64_t* v_strides, void* k_cache, void* v_cache,
-                        int64_t cache_block_stride, int64_t cache_head_stride,
+int msattn_write_kv_fp4(const void* k, int64_t k_batch_stride, int64_t k_token_stride,
+                        int64_t k_head_stride, const void* v, int64_t v_batch_stride,
+                        int64_t v_token_stride, int64_t v_head_stride, void* k_cache,
+                        void* v_cache, int64_t cache_block_stride, int64_t cache_head_stride,
                         const int32_t* block_table, const int32_t* starts, int batch, int tokens,
                         int num_kv_heads, int head_dim, int block_size, int num_blocks,
                         int table_width, int src_dtype, void* stream);
@@ -511,15 +513,17 @@ size_t msattn_fp4_workspace_bytes(int batch, int q_len, int num_heads, int num_k
 
 /*
  * msattn_paged_attention over a 4-bit cache: fp32, fp16 or bf16 query, any q_len, causal or not,
- * window as there; one launch. q_strides are the query's batch, token and head strides in elements
- * (16-byte aligned rows); out is contiguous. Rows without a visible key give zeros; an infinity or
+ * window as there; one launch. The query's strides are in elements, its rows and the contiguous out
+ * 16-byte aligned. Rows without a visible key give zeros; an infinity or
  * NaN reaches the queries that see its key alone. Scores and products take the cache's values
  * exactly; the weights of a bf16 query are rounded to bf16, in the numerator and in the sum alike;
  * maxima, sums and accumulators are fp32.
  */
-int msattn_paged_attention_fp4(const void* query, const int64_t* q_strides, const void* k_cache,
-                               const void* v_cache, int64_t cache_block_stride,
-                               int64_t cache_head_stride, const int32_t* block_table,
+int msattn_paged_attention_fp4(const void* query, int64_t q_batch_stride,
+                               int64_t q_token_stride, int64_t q_head_stride,
+                               const void* k_cache, const void* v_cache,
+                               int64_t cache_block_stride, int64_t cache_head_stride,
+                               const int32_t* block_table,
                                const int32_t* context_lens, void* out, void* workspace,
                                size_t workspace_bytes, int batch, int q_len, int num_heads,
                                int num_kv_heads, int head_dim, int block_size, int num_blocks,

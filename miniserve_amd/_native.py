@@ -21,7 +21,7 @@ DTYPE_CODES = {
     torch.float8_e4m3fn: FP8_E4M3,
 }
 
-OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_HIP = 0, 1, 2, 3, 4
+OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_HIP, ERR_OVERLAP = 0, 1, 2, 3, 4, 5
 
 # msattn_route codes: the kernel msattn_paged_attention runs for a call's shape.
 ROUTE_PREFILL, ROUTE_PARTITION_FUSED, ROUTE_PARTITION, ROUTE_STREAMK, ROUTE_GENERIC = 1, 2, 3, 4, 5
@@ -101,14 +101,14 @@ SIGNATURES = {
         c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp,
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
     "msattn_write_kv_fp4": (c_int, [
-        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp,
+        c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp,
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
     "msattn_read_kv_fp4": (c_int, [
         c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp,
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
     "msattn_fp4_workspace_bytes": (c_size, [c_int] * 7),
     "msattn_paged_attention_fp4": (c_int, [
-        c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_size,
+        c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_size,
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
         c_float, c_int, c_vp]),
     "msattn_probe_stream_read": (c_int, [c_vp, c_size, c_vp, c_vp]),

@@ -52,8 +52,8 @@ FILE_FLAGS = {
     "shared_prefix_fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 # The 4-bit cache's attention and the any-layout prefill kernels do the same.
-FILE_FLAGS.update({f"fp4_attn_{q}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-                   for q in ("f32", "f16", "bf16")})
+FILE_FLAGS.update({f"fp4_attn_{q}_{d}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+                   for q in ("f32", "f16", "bf16") for d in (64, 128, 256)})
 FILE_FLAGS.update({f"prefill_any_{q}_{kv}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
                    for q in ("f32", "f16", "bf16") for kv in ("f32", "f16", "bf16", "fp8")})
 

@@ -511,6 +511,7 @@ const char* msattn_status_string(int status) {
     case MSATTN_ERR_UNSUPPORTED: return "unsupported geometry or dtype";
     case MSATTN_ERR_WORKSPACE: return "workspace too small";
     case MSATTN_ERR_HIP: return "HIP error";
+    case MSATTN_ERR_OVERLAP: return "an input shares memory with what the call writes";
     default: return "unknown status";
   }
 }

@@ -73,30 +73,56 @@ bool geometry_ok(int batch, int q_len, int H, int KVH, int D, int max_ctx) {
 
 // How a call is cut: column tiles of 16 query rows a wave, and its shares.
 struct Plan {
-  int ct, rblocks, slot_rows, split, shares;
+  int ct, wk, rblocks, slot_rows, split, shares, xcd_units;
   size_t ml_off, acc_off, total;
 };
 
+int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
-bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int q_dtype, Plan* p) {
-  const int64_t rows = static_cast<int64_t>(q_len) * (H / KVH);
-  const int most = 2;
-  p->ct = rows <= 16 ? 1 : most;
+// Workspace does not depend on causal and window.
+bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causal,
+             int window, int q_dtype, Plan* p) {
+  const int G = H / KVH;
+  const int64_t rows = static_cast<int64_t>(q_len) * G;
+  p->ct = rows <= 16 ? 1 : 2;
   const int per = 16 * p->ct;
   const int64_t rblocks = (rows + per - 1) / per;
   const int64_t units = batch * rblocks * KVH;
   if (rows >= (int64_t(1) << 30) || units >= (int64_t(1) << 30)) return false;
   p->rblocks = static_cast<int>(rblocks);
   p->slot_rows = static_cast<int>(std::min<int64_t>(per, rows));
-  const int64_t groups = max_ctx / kFp4Group + 2;  // of a unit, at most
+  const int64_t want = 256;  // workgroups: one a CU
+  int64_t groups = max_ctx / kFp4Group + 1;  // of a unit, at most
   p->split = batch * rblocks <= kFp4MaxEntries && units * groups < (int64_t(1) << 31);
-    const int64_t want = 256;  // a workgroup a CU
   p->shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, units * groups)));
   const size_t slots = p->split ? 2 * static_cast<size_t>(p->shares) * p->slot_rows : 0;
   p->ml_off = up256((kHdrTickets + kMaxTickets) * sizeof(int));
   p->acc_off = p->ml_off + up256(slots * 2 * sizeof(float));
   p->total = p->acc_off + up256(slots * D * sizeof(float));
+  if (window > 0)
+    groups = std::min<int64_t>(groups, (static_cast<int64_t>(window) + per / G + 1) / kFp4Group + 2);
+  // Without a list, partials and joins: whole units, wk waves each. What each way costs, in a wave's
+  // groups (about 1.3 us at 32 rows, two waves a SIMD): a unit's start and end are about 3 of them,
+  // and about 10 each with a list (its plan, partials and joins, in which all waves of a workgroup
+  // meet). Several rounds of the CUs even out; the last unit to start does not. Measured: 896 units of
+  // 145 groups, wk = 1, 2, 4, 8 and the list, 191, 103, 104, 126, 161 us; 896 of 65, causal, 70, 40, 42,
+  // 62, 231; 4096 of 33, causal, 96, 85, 109, 190, 332. Units of few rows take all waves of a workgroup,
+  // and only where no CU gets two (their contexts may differ; 64 of 64 groups, 14 us against 20).
+  const double load = static_cast<double>(units) / want;
+  const double mean = groups - (causal && window == 0 ? 0.5 * std::min(q_len, max_ctx) / kFp4Group : 0.0);
+  double best = p->split ? units * mean / (want * kFp4Waves) + 10 * (load + 1) : 1e300;
+  p->wk = kFp4Waves;
+  for (int wk = kFp4Waves; wk >= (p->ct == 1 ? kFp4Waves : 1); wk /= 2) {
+    const double longest = ceil(static_cast<double>(groups) / wk) + 3, rounds = load * wk / kFp4Waves;
+    const double cost = rounds <= 1 ? longest : rounds * (mean / wk + 3) + 0.5 * longest;
+    if (cost > best || (rounds > 1 && p->ct == 1 && p->split)) continue;
+    best = cost;
+    p->wk = wk;
+    p->split = 0;
+  }
+  p->xcd_units = static_cast<int>(ceil_div64(ceil_div64(units * p->wk, kFp4Waves), 8));
   return true;
 }
 
@@ -104,18 +130,37 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int q_dty
 
 extern "C" {
 
-int msattn_write_kv_fp4(const void* k, const int64_t* k_strides, const void* v,
-                        const int64_t* v_strides, void* k_cache, void* v_cache,
-                        int64_t cache_block_stride, int64_t cache_head_stride,
+int msattn_write_kv_fp4(const void* k, int64_t k_batch_stride, int64_t k_token_stride,
+                        int64_t k_head_stride, const void* v, int64_t v_batch_stride,
+                        int64_t v_token_stride, int64_t v_head_stride, void* k_cache,
+                        void* v_cache, int64_t cache_block_stride, int64_t cache_head_stride,
                         const int32_t* block_table, const int32_t* starts, int batch, int tokens,
                         int num_kv_heads, int head_dim, int block_size, int num_blocks,
                         int table_width, int src_dtype, void* stream) {
-  if (!k_strides || !v_strides) return MSATTN_ERR_INVALID_ARG;
+  const int64_t ks[3] = {k_batch_stride, k_token_stride, k_head_stride};
+  const int64_t vs[3] = {v_batch_stride, v_token_stride, v_head_stride};
+  for (int i = 0; i < 3; ++i)
+    if (ks[i] < 0 || vs[i] < 0) return MSATTN_ERR_INVALID_ARG;
   Fp4CacheParams p{};
-  const int rc = cache_params(&p, k, v, k_strides, v_strides, k_cache, v_cache, cache_block_stride,
+  const int rc = cache_params(&p, k, v, ks, vs, k_cache, v_cache, cache_block_stride,
                               cache_head_stride, block_table, starts, batch, tokens, num_kv_heads,
                               head_dim, block_size, num_blocks, table_width, src_dtype);
   if (rc != MSATTN_OK || tokens == 0) return rc;
+  // The bytes that k, v and the caches span.
+  const int eb = type_bytes(src_dtype);
+  const int64_t cache_span = (num_blocks - 1) * cache_block_stride +
+                             (num_kv_heads - 1) * cache_head_stride +
+                             static_cast<int64_t>(block_size / kFp4Tile) * fp4_tile_bytes(head_dim);
+  const struct { const void* at; const int64_t* st; } in[2] = {{k, ks}, {v, vs}};
+  for (const auto& x : in) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(x.at);
+    const uintptr_t hi = lo + static_cast<uintptr_t>(((batch - 1) * x.st[0] + (tokens - 1) * x.st[1] +
+                                                      (num_kv_heads - 1) * x.st[2] + head_dim) * eb);
+    for (const void* c : {static_cast<const void*>(k_cache), static_cast<const void*>(v_cache)}) {
+      const uintptr_t clo = reinterpret_cast<uintptr_t>(c);
+      if (lo < clo + static_cast<uintptr_t>(cache_span) && clo < hi) return MSATTN_ERR_OVERLAP;
+    }
+  }
   return status_of(launch_write_fp4(p, src_dtype, static_cast<hipStream_t>(stream)));
 }
 
@@ -140,20 +185,22 @@ size_t msattn_fp4_workspace_bytes(int batch, int q_len, int num_heads, int num_k
   Plan plan;
   if (!geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context) ||
       !float_type(q_dtype) ||
-      !plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, q_dtype, &plan))
+      !plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, 1, 0, q_dtype, &plan))
     return 0;
   return plan.total;
 }
 
-int msattn_paged_attention_fp4(const void* query, const int64_t* q_strides, const void* k_cache,
-                               const void* v_cache, int64_t cache_block_stride,
-                               int64_t cache_head_stride, const int32_t* block_table,
+int msattn_paged_attention_fp4(const void* query, int64_t q_batch_stride,
+                               int64_t q_token_stride, int64_t q_head_stride,
+                               const void* k_cache, const void* v_cache,
+                               int64_t cache_block_stride, int64_t cache_head_stride,
+                               const int32_t* block_table,
                                const int32_t* context_lens, void* out, void* workspace,
                                size_t workspace_bytes, int batch, int q_len, int num_heads,
                                int num_kv_heads, int head_dim, int block_size, int num_blocks,
                                int table_width, int max_context, int causal, int window,
                                float scale, int q_dtype, void* stream) {
-  if (!query || !q_strides || !block_table || !context_lens || !out || !workspace ||
+  if (!query || !block_table || !context_lens || !out || !workspace ||
       !float_type(q_dtype) || window < 0 || std::isnan(scale) ||
       !geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context) ||
       !cache_ok(k_cache, v_cache, cache_block_stride, cache_head_stride, num_kv_heads, head_dim,
@@ -163,10 +210,11 @@ int msattn_paged_attention_fp4(const void* query, const int64_t* q_strides, cons
   if (!on(query, 16) || !on(out, 16) || !on(workspace, 256) || !on(block_table, 4) ||
       !on(context_lens, 4))
     return MSATTN_ERR_INVALID_ARG;
-  for (int i = 0; i < 3; ++i)
-    if (q_strides[i] * eb % 16 != 0) return MSATTN_ERR_INVALID_ARG;
+  const int64_t q_strides[3] = {q_batch_stride, q_token_stride, q_head_stride};
+  for (int64_t x : q_strides)
+    if (x < 0 || x * eb % 16 != 0) return MSATTN_ERR_INVALID_ARG;
   Plan plan;
-  if (!plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, q_dtype, &plan))
+  if (!plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, causal, window, q_dtype, &plan))
     return MSATTN_ERR_UNSUPPORTED;
   if (workspace_bytes < plan.total) return MSATTN_ERR_WORKSPACE;
   char* const ws = static_cast<char*>(workspace);
@@ -200,18 +248,26 @@ int msattn_paged_attention_fp4(const void* query, const int64_t* q_strides, cons
   p.slot_rows = plan.slot_rows;
   p.split = plan.split;
   p.shares = plan.shares;
+  p.xcd_units = plan.xcd_units;
   p.by_tiles = fp4_div(static_cast<uint32_t>(block_size / kFp4Tile));
   p.by_g = fp4_div(static_cast<uint32_t>(p.G));
   p.by_rb = fp4_div(static_cast<uint32_t>(plan.rblocks));
   p.by_kvh = fp4_div(static_cast<uint32_t>(num_kv_heads));
+  p.by_per = fp4_div(static_cast<uint32_t>(head_dim / 4));
   p.tickets = reinterpret_cast<int*>(ws) + kHdrTickets;
   p.ml = reinterpret_cast<float*>(ws + plan.ml_off);
   p.acc = reinterpret_cast<float*>(ws + plan.acc_off);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  auto launch = [&](auto t) {
+    typedef decltype(t) T;
+    if (head_dim <= 64) return launch_fp4_attn<T, 64>(p, plan.ct, plan.wk, st);
+    if (head_dim <= 128) return launch_fp4_attn<T, 128>(p, plan.ct, plan.wk, st);
+    return launch_fp4_attn<T, 256>(p, plan.ct, plan.wk, st);
+  };
   switch (q_dtype) {
-    case MSATTN_F32: return status_of(launch_fp4_attn<float>(p, plan.ct, st));
-    case MSATTN_F16: return status_of(launch_fp4_attn<_Float16>(p, plan.ct, st));
-    default: return status_of(launch_fp4_attn<bf16_t>(p, plan.ct, st));
+    case MSATTN_F32: return status_of(launch(float{}));
+    case MSATTN_F16: return status_of(launch(_Float16{}));
+    default: return status_of(launch(bf16_t{}));
   }
 }
 

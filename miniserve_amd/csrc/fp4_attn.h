@@ -62,10 +62,12 @@ struct Fp4Params {
   int rows_per_kvh;  // q_len * G
   int rblocks;       // ceil(rows_per_kvh / (16 CT))
   int slot_rows;     // rows of a partial: min(16 CT, rows_per_kvh)
-  int split;         // shares planned over all units (else one unit a workgroup)
+  int split;         // shares planned over all units (else units dealt to the workgroups)
+  int xcd_units;     // without split: workgroups an XCD
   int shares;
   Fp4Div by_tiles;   // tiles of a page
   Fp4Div by_g, by_rb, by_kvh;
+  Fp4Div by_per;     // D / 4
   int* tickets;
   float* ml;         // [2 shares][slot_rows][2]
   float* acc;        // [2 shares][slot_rows][D]
@@ -154,7 +156,9 @@ __device__ __forceinline__ int fp4_count(int lo, int hi) {  // at least one, so 
   return hi > lo ? ceil_div(hi, kFp4Group) - lo / kFp4Group : 1;
 }
 
-template <typename T, int DP, int CT>
+// WK waves take a unit's groups in turn. WK = 8: a workgroup takes a share of the list or, without
+// split, one unit; else 8 / WK units, neighbours in the list.
+template <typename T, int DP, int CT, int WK>
 __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Params p) {
   constexpr int HV = DP > 128 ? 2 : 1;   // halves of 128 dims
   constexpr int DH = DP > 128 ? 128 : DP;
@@ -169,20 +173,25 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   __shared__ int s_pre[kFp4MaxEntries + 1];
   __shared__ int s_ctx[kFp4MaxEntries];
   __shared__ int s_tot[kFp4Waves];  // and whether this workgroup joins a unit's shares
-  // The waves' accumulators of 16 rows, rows 4 floats apart beyond DP (so that the 16 rows of a
-  // store fall on different banks), and their maxima and sums.
-  __shared__ float s_acc[kFp4Waves][16][DP + 4];
-  __shared__ float2 s_ml[kFp4Waves][16];
+  // The waves' accumulators of up to 16 rows of a unit, [buffer][wave][rows][RS] (RS: the rows of a
+  // store fall on different banks), and their maxima and sums. Fewer rows leave more buffers.
+  constexpr int RS = DP + 4;
+  __shared__ float s_acc[kFp4Waves * 16 * RS];
+  __shared__ float2 s_ml[kFp4Waves * 16];
+  __shared__ int s_cnt[16], s_done[16];  // of a buffer: waves that have written it, times it was read
 
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n = lane & 15;
   const int share = static_cast<int>(blockIdx.x);
+  constexpr int NU = kFp4Waves / WK;        // units at a time
+  const int wu = w / WK, wk = w % WK;       // the wave's unit, and its place among the unit's waves
+  const bool list = WK == kFp4Waves && p.split;
   const int entries = p.batch * p.rblocks;
 
   auto ctx_of = [&](int b) FP4_INLINE {
-    if (p.split) return s_ctx[b];
+    if (list) return s_ctx[b];
     const int c = p.lens[b];
     return c < 0 ? 0 : (c > p.max_ctx ? p.max_ctx : c);
   };
@@ -193,9 +202,11 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   };
 
+  if (tid < 16) s_cnt[tid] = s_done[tid] = 0;
+  if (!list) lds_barrier();
   // The list: s_pre[e] = groups of one head's units of entries 0 .. e - 1 (entry = row, row block).
   int c0, c1, chunk = 1;
-  if (p.split) {
+  if (list) {
     int base = 0;
     for (int e0 = 0; e0 < entries; e0 += kFp4Threads) {
       const int e = e0 + tid;
@@ -230,13 +241,25 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     c1 = min(c0 + chunk, total);
   } else {
     c0 = 0;
-    c1 = share < entries * p.KVH ? 1 : 0;  // its unit's groups, set below
+    c1 = 1;  // (its unit's groups, set below)
   }
+
+  // Without a list: the wave's unit. Workgroup i runs on XCD i % 8, each of which has an L2 of its
+  // own: an XCD takes a run of units, so that the row blocks of a head, which read the same keys,
+  // share one. Later row blocks first: under a causal mask they have the most keys.
+  auto alone = [&](Fp4Unit* u) FP4_INLINE {
+    const int at = ((share & 7) * p.xcd_units + (share >> 3)) * NU + wu;
+    const int bk = fp4_quot(at, p.by_rb);
+    u->rb = p.rblocks - 1 - (at - bk * p.rblocks);
+    u->b = fp4_quot(bk, p.by_kvh);
+    u->kvh = bk - u->b * p.KVH;
+    return u->b < p.batch;
+  };
 
   // The unit holding position q of the list (any lane's own q), in rows a0 .. z0 - 1.
   auto locate = [&](int q, int a0, int z0) FP4_INLINE {
     Fp4Unit u;
-    if (p.split) {
+    if (list) {
       int a = a0, z = z0;  // the row: KVH s_pre[a rblocks] <= q < KVH s_pre[z rblocks]
       while (z - a > 1) {
         const int m = (a + z) >> 1;
@@ -258,10 +281,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       u.rb = x;
       u.u0 = pre0 * p.KVH + u.kvh * per + (s_pre[e0 + x] - pre0);
     } else {
-      const int bk = fp4_quot(share, p.by_rb);
-      u.rb = share - bk * p.rblocks;
-      u.b = fp4_quot(bk, p.by_kvh);
-      u.kvh = bk - u.b * p.KVH;
+      alone(&u);
       u.u0 = 0;
     }
     fp4_extent<ROWS>(p, ctx_of(u.b), u.rb, &u.lo, &u.hi);
@@ -272,22 +292,46 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
 
   if (c0 >= c1) return;  // (the workgroup as one)
   auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  auto unit_at = [&](int q, int a0, int z0) FP4_INLINE {  // locate of one position for the wave
-    Fp4Unit u = locate(q, a0, z0);
-    u.b = uniform(u.b);
-    u.kvh = uniform(u.kvh);
-    u.rb = uniform(u.rb);
-    u.lo = uniform(u.lo);
-    u.hi = uniform(u.hi);
-    u.first = uniform(u.first);
-    u.n = uniform(u.n);
-    u.u0 = uniform(u.u0);
+  // locate for one position of the wave: 64 entries of the list at a time, one a lane.
+  auto search = [&](int from, int len, int stride, int mul, int key) FP4_INLINE {
+    int lo = 0;  // the last of 0 .. len - 1 with (s_pre[from + lo stride] - s_pre[from]) mul <= key
+    const int base = s_pre[from];
+    while (len > 1) {
+      const int step = (len + 63) >> 6;
+      const int m = (lane + 1) * step;
+      const bool le = m < len && (s_pre[from + (lo + m) * stride] - base) * mul <= key;
+      const int c = __popcll(__ballot(le)) * step;
+      lo += c;
+      len = min(step, len - c);
+    }
+    return lo;
+  };
+  auto unit_at = [&](int q) FP4_INLINE {
+    Fp4Unit u;
+    if (list) {
+      u.b = search(0, p.batch, p.rblocks, p.KVH, q);
+      const int e0 = u.b * p.rblocks;
+      const int pre0 = uniform(s_pre[e0]), per = uniform(s_pre[e0 + p.rblocks]) - pre0;
+      const int rem = q - pre0 * p.KVH;
+      u.kvh = uniform(rem / per);
+      const int in = rem - u.kvh * per;
+      u.rb = p.rblocks == 1 ? 0 : search(e0, p.rblocks, 1, 1, in);
+      u.u0 = pre0 * p.KVH + u.kvh * per + (uniform(s_pre[e0 + u.rb]) - pre0);
+    } else {
+      alone(&u);
+      u.u0 = 0;
+    }
+    fp4_extent<ROWS>(p, uniform(ctx_of(u.b)), u.rb, &u.lo, &u.hi);
+    u.first = fp4_first(u.lo);
+    u.n = fp4_count(u.lo, u.hi);
     return u;
   };
-  Fp4Unit u = unit_at(c0, 0, p.batch);
-  if (!p.split) c1 = u.n;
-  const int b_end = c1 <= u.u0 + u.n ? u.b + 1 : unit_at(c1 - 1, u.b, p.batch).b + 1;  // the share's rows
+  Fp4Unit u{}, any;
+  // (waves past the last unit go on to the barriers, with a unit of no groups)
+  if (list || alone(&any)) u = unit_at(c0);
+  if (!list) c1 = u.n;
   const int b_first = u.b;
+  const int b_end = c1 <= u.u0 + u.n ? u.b + 1 : unit_at(c1 - 1).b + 1;  // the share's rows
 
   // ---- what a lane holds of a tile: fixed places, one register each ----
   uint32_t k_at[HV], ks_at[HV], v_at[HV], vs_at[HV];
@@ -311,11 +355,11 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   };
   typedef Tile Group[2];
 
-  // Wave w takes positions c0 + w + 8 s of the share. Places of the tiles of its 32 groups from s =
+  // The wave takes positions c0 + wk + WK s of the share. Places of the tiles of its 32 groups from s =
   // base on: lane i holds tile i's byte offset, and bit i of `holes` says that the table has none
   // (the offset is then one that can be read).
   auto places = [&](int base, uint64_t* holes) FP4_INLINE {
-    const int q = c0 + w + kFp4Waves * (base + (lane >> 1));
+    const int q = c0 + wk + WK * (base + (lane >> 1));
     int64_t at = -1;
     if (q < c1) {
       const Fp4Unit v = locate(q, b_first, b_end);
@@ -332,9 +376,9 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     return at < 0 ? int64_t(0) : at;
   };
   uint64_t holes, next_holes = 0;
-  int64_t here = places(0, &holes), next = 0;  // of this run of 32 groups, and of the next
+  int64_t here, next = 0;  // of this run of 32 groups, and of the next
   int run = 0;                                 // the run's first
-  const int rounds = (c1 - c0 - w + kFp4Waves - 1) / kFp4Waves;  // groups of the wave
+  const int rounds = (c1 - c0 - wk + WK - 1) / WK;  // groups of the wave
   auto load = [&](Group& x, int s) FP4_INLINE {  // group s, of this run or the next
     if (s >= rounds) return;
     const int i = 2 * (s - run);
@@ -550,7 +594,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   auto byte_of = [](uint32_t x, int i) { return (x >> (8 * i)) & 255u; };
 
   auto consume = [&](Group& x, int s) FP4_INLINE {
-    const int tok = (u.first + c0 + w + kFp4Waves * s - u.u0) * kFp4Group;
+    const int tok = (u.first + c0 + wk + WK * s - u.u0) * kFp4Group;
     mf_f32x4 s0[CT], s1[CT];
     scores(x[0], s0);
     scores(x[1], s1);
@@ -640,62 +684,100 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     return ((static_cast<int64_t>(u.b) * p.q_len + i) * p.H + (u.kvh * p.G + (r - i * p.G))) * p.D;
   };
   // The waves' parts of unit u joined, 16 rows at a time: normalised rows, or the share's partial.
-  auto finish = [&](const Fp4Unit& u) FP4_INLINE {
-    const int r0 = u.rb * ROWS;
-    const int rows = min(ROWS, p.rows_per_kvh - r0);
+  // At the share's end all threads do it, between barriers. Before, a wave leaves its part in a
+  // buffer and goes on to the next unit, and the last to leave one joins them: no wave waits for the
+  // others, unless all buffers hold parts of earlier units.
+  const int brows = WK == kFp4Waves ? min(16, p.slot_rows) : 16, buffers = 16 / brows;
+  int event = 0;
+  auto put = [&](int ct, int buf, int rows) FP4_INLINE {
+    const float l = rows4_sum(l_run[ct]);
+    if (n >= rows) return;
+    const int at = (buf * kFp4Waves + w) * brows + n;
+    if (g == 0) s_ml[at] = make_float2(m_run[ct], l);
+#pragma unroll
+    for (int h = 0; h < HV; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < VC; c += 4)
+          *reinterpret_cast<float4*>(&s_acc[at * RS + 128 * h + LD * g + VC * i + c]) =
+              make_float4(acc[ct][h][c][i], acc[ct][h][c + 1][i], acc[ct][h][c + 2][i],
+                          acc[ct][h][c + 3][i]);
+  };
+  auto fold = [&](const Fp4Unit& u, int r0, int buf, int rows, int t0, int threads) FP4_INLINE {
     const int per = p.D / 4;  // items of a row
     const bool whole = u.u0 >= c0 && u.u0 + u.n <= c1;
     const int64_t slot = 2 * static_cast<int64_t>(share) + (u.u0 >= c0 ? 1 : 0);
+    for (int idx = t0; idx < rows * per; idx += threads) {
+      const int r = fp4_quot(idx, p.by_per), d = 4 * (idx - r * per);
+      float2 ml[WK];
+      float M = -INFINITY, L = 0.0f;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int at = buf * brows + r;  // (buf: the first wave's part)
+#pragma unroll
+      for (int i = 0; i < WK; ++i) {
+        ml[i] = s_ml[at + i * brows];
+        M = fmaxf(M, ml[i].x);
+      }
+#pragma unroll
+      for (int i = 0; i < WK; ++i) {
+        const float f = __builtin_amdgcn_exp2f(M != -INFINITY ? ml[i].x - M : 0.0f);
+        const float4 x = *reinterpret_cast<const float4*>(&s_acc[(at + i * brows) * RS + d]);
+        L = fmaf(f, ml[i].y, L);
+        a.x = fmaf(f, x.x, a.x);
+        a.y = fmaf(f, x.y, a.y);
+        a.z = fmaf(f, x.z, a.z);
+        a.w = fmaf(f, x.w, a.w);
+      }
+      if (whole) {
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // (a NaN stays one)
+        fp4_store4<T>(static_cast<T*>(p.out) + out_at(u, u.rb * ROWS + r0 + r) + d, a.x * inv,
+                      a.y * inv, a.z * inv, a.w * inv);
+      } else {
+        const int64_t row = slot * p.slot_rows + r0 + r;
+        if (d == 0) store2_device(p.ml + row * 2, M, L);
+        store2_device(p.acc + row * p.D + d, a.x, a.y);
+        store2_device(p.acc + row * p.D + d + 2, a.z, a.w);
+      }
+    }
+  };
+  auto finish = [&](const Fp4Unit& u, bool ends) FP4_INLINE {
+    const int rows = u.n == 0 ? 0 : min(ROWS, p.rows_per_kvh - u.rb * ROWS);  // (no unit: none)
+    if (ends) {
+      lds_barrier();  // (the buffers' last parts are read)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const int n_rows = min(16, rows - 16 * ct);  // (units of one workgroup may differ)
+        if (NU == 1 && n_rows <= 0) break;
+        put(ct, 0, n_rows);
+        lds_barrier();
+        fold(u, 16 * ct, wu * WK, n_rows, tid - 64 * WK * wu, 64 * WK);
+        lds_barrier();
+      }
+      return;
+    }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const int here_rows = min(16, rows - 16 * ct);
-      if (here_rows <= 0) break;
-      const float l = rows4_sum(l_run[ct]);
-      if (n < here_rows) {
-        if (g == 0) s_ml[w][n] = make_float2(m_run[ct], l);
-#pragma unroll
-        for (int h = 0; h < HV; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int c = 0; c < VC; c += 4)
-              *reinterpret_cast<float4*>(&s_acc[w][n][128 * h + LD * g + VC * i + c]) =
-                  make_float4(acc[ct][h][c][i], acc[ct][h][c + 1][i], acc[ct][h][c + 2][i],
-                              acc[ct][h][c + 3][i]);
-      }
-      lds_barrier();
-      for (int idx = tid; idx < here_rows * per; idx += kFp4Threads) {
-        const int r = idx / per, d = 4 * (idx - r * per);
-        float2 ml[kFp4Waves];
-        float M = -INFINITY, L = 0.0f;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < kFp4Waves; ++i) {
-          ml[i] = s_ml[i][r];
-          M = fmaxf(M, ml[i].x);
-        }
-#pragma unroll
-        for (int i = 0; i < kFp4Waves; ++i) {
-          const float f = __builtin_amdgcn_exp2f(M != -INFINITY ? ml[i].x - M : 0.0f);
-          const float4 x = *reinterpret_cast<const float4*>(&s_acc[i][r][d]);
-          L = fmaf(f, ml[i].y, L);
-          a.x = fmaf(f, x.x, a.x);
-          a.y = fmaf(f, x.y, a.y);
-          a.z = fmaf(f, x.z, a.z);
-          a.w = fmaf(f, x.w, a.w);
-        }
-        if (whole) {
-          const float inv = L != 0.0f ? 1.0f / L : 0.0f;  // (a NaN stays one)
-          fp4_store4<T>(static_cast<T*>(p.out) + out_at(u, r0 + 16 * ct + r) + d, a.x * inv, a.y * inv,
-                        a.z * inv, a.w * inv);
-        } else {
-          const int64_t row = slot * p.slot_rows + 16 * ct + r;
-          if (d == 0) store2_device(p.ml + row * 2, M, L);
-          store2_device(p.acc + row * p.D + d, a.x, a.y);
-          store2_device(p.acc + row * p.D + d + 2, a.z, a.w);
-        }
-      }
-      lds_barrier();
+      const int n_rows = min(16, rows - 16 * ct);
+      if (n_rows <= 0) break;
+      const int gen = event / buffers, buf = event - gen * buffers;
+      ++event;
+      // (every wave leaves its part of each event in turn, so that the one waited for comes)
+      while (__hip_atomic_load(&s_done[buf], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) < gen)
+        __builtin_amdgcn_s_sleep(1);
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+      put(ct, buf, n_rows);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+      int old = 0;
+      if (lane == 0)
+        old = __hip_atomic_fetch_add(&s_cnt[buf], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      old = uniform(old);
+      if (old != kFp4Waves * gen + kFp4Waves - 1) continue;
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+      fold(u, 16 * ct, buf * kFp4Waves, n_rows, lane, 64);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+      if (lane == 0)
+        __hip_atomic_store(&s_done[buf], gen + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
   };
   // The join of unit v, whose shares have all left their partials.
@@ -706,21 +788,21 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     const int s_first = v.u0 / chunk, s_last = (v.u0 + v.n - 1) / chunk;
     // Threads left over take other shares of the same items, and are joined through LDS.
     const int items = rows * per;
-    const int fold = items >= kFp4Threads ? 1 : kFp4Threads / items;
-    float* const s_part = &s_acc[0][0][0];  // [thread][6]
+    const int parts = items >= kFp4Threads ? 1 : kFp4Threads / items;
+    float* const s_part = s_acc;  // [thread][6]
     for (int i0 = 0; i0 < items; i0 += kFp4Threads) {
-      const int k = fold == 1 ? 0 : tid / items;
-      const int idx = fold == 1 ? i0 + tid : tid - k * items;
-      const bool mine = idx < items && k < fold;
-      const int r = mine ? idx / per : 0, d = mine ? 4 * (idx - r * per) : 0;
+      const int k = parts == 1 ? 0 : tid / items;
+      const int idx = parts == 1 ? i0 + tid : tid - k * items;
+      const bool mine = idx < items && k < parts;
+      const int r = mine ? fp4_quot(idx, p.by_per) : 0, d = mine ? 4 * (idx - r * per) : 0;
       float M = -INFINITY, L = 0.0f;
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
       constexpr int N = 4;
-      for (int j0 = s_first + k; mine && j0 <= s_last; j0 += N * fold) {
+      for (int j0 = s_first + k; mine && j0 <= s_last; j0 += N * parts) {
         float2 x0[N], x1[N], ml[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {  // shares past the last repeat it, unused
-          const int j = min(j0 + i * fold, s_last);
+          const int j = min(j0 + i * parts, s_last);
           const int64_t row = (2 * static_cast<int64_t>(j) + (j == s_first ? 1 : 0)) * p.slot_rows + r;
           ml[i] = load2_device(p.ml + row * 2);
           x0[i] = load2_device(p.acc + row * p.D + d);
@@ -728,13 +810,13 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         }
         float mb = M;
 #pragma unroll
-        for (int i = 0; i < N; ++i) mb = fmaxf(mb, j0 + i * fold <= s_last ? ml[i].x : -INFINITY);
+        for (int i = 0; i < N; ++i) mb = fmaxf(mb, j0 + i * parts <= s_last ? ml[i].x : -INFINITY);
         const float keep = __builtin_amdgcn_exp2f(mb != -INFINITY ? M - mb : 0.0f);
         L *= keep;
         a.x *= keep; a.y *= keep; a.z *= keep; a.w *= keep;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const bool live = j0 + i * fold <= s_last;
+          const bool live = j0 + i * parts <= s_last;
           const float f = __builtin_amdgcn_exp2f(live && mb != -INFINITY ? ml[i].x - mb : 0.0f);
           L = live ? fmaf(f, ml[i].y, L) : L;
           a.x = live ? fmaf(f, x0[i].x, a.x) : a.x;
@@ -744,18 +826,18 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         }
         M = mb;
       }
-      if (fold > 1) {
+      if (parts > 1) {
         float* const mine_at = s_part + 6 * tid;
         mine_at[0] = M; mine_at[1] = L; mine_at[2] = a.x; mine_at[3] = a.y; mine_at[4] = a.z;
         mine_at[5] = a.w;
         lds_barrier();
         if (mine && k == 0) {
           float mb = M;
-          for (int i = 1; i < fold; ++i) mb = fmaxf(mb, s_part[6 * (tid + i * items)]);
+          for (int i = 1; i < parts; ++i) mb = fmaxf(mb, s_part[6 * (tid + i * items)]);
           const float keep = __builtin_amdgcn_exp2f(mb != -INFINITY ? M - mb : 0.0f);
           L *= keep;
           a.x *= keep; a.y *= keep; a.z *= keep; a.w *= keep;
-          for (int i = 1; i < fold; ++i) {
+          for (int i = 1; i < parts; ++i) {
             const float* const x = s_part + 6 * (tid + i * items);
             const float f = __builtin_amdgcn_exp2f(mb != -INFINITY ? x[0] - mb : 0.0f);
             L = fmaf(f, x[1], L);
@@ -777,6 +859,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
 
   // ---- the share ----
   query();
+  here = places(0, &holes);
   Group ring[kRing];  // the next groups, on their way
   static_for<kRing>([&](auto i) FP4_INLINE { load(ring[i], i); });
   if (rounds > 32) next = places(32, &next_holes);
@@ -785,7 +868,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   for (;;) {
     begin();
     const int end = min(c1, u.u0 + u.n);
-    const int s_end = (end - c0 - w + kFp4Waves - 1) / kFp4Waves;
+    const int s_end = (end - c0 - wk + WK - 1) / WK;
     for (; s < s_end; ++s) {
       if (s - run == 32) {
         run = s;
@@ -802,12 +885,16 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       });
       turn = turn == kRing - 1 ? 0 : turn + 1;
     }
+    if constexpr (WK != kFp4Waves) {
+      finish(u, true);
+      return;
+    }
     const Fp4Unit done = u;
     if (end < c1) {
-      u = unit_at(end, b_first, b_end);
+      u = unit_at(end);
       query();
     }
-    finish(done);
+    finish(done, end == c1);
     if (end == c1) break;
   }
 
@@ -818,7 +905,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   // after them. A unit's counter is its first share's, which no other unit split has.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   lds_barrier();
-  const Fp4Unit first = unit_at(c0, b_first, b_end);
+  const Fp4Unit first = unit_at(c0);
   if (tid < 2) {
     const Fp4Unit& v = tid == 0 ? first : u;
     const int mine = tid == 0 ? head && first.u0 != u.u0 : tail;
@@ -840,11 +927,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   }
 }
 
-// Rows a wave takes, in column tiles of 16: as many as the KV head has, up to what the registers
-// hold beside two groups in flight.
-template <typename T> constexpr int fp4_max_ct() { return fp4_parts<T>() == 1 ? 4 : 2; }
-
-template <typename T>
-hipError_t launch_fp4_attn(const Fp4Params& p, int ct, hipStream_t stream);
+template <typename T, int DP>
+hipError_t launch_fp4_attn(const Fp4Params& p, int ct, int wk, hipStream_t stream);
 
 }  // namespace msattn

@@ -1,0 +1,6 @@
+// The 4-bit cache's attention kernel for f16 queries and head sizes above 64.
+#include "fp4_attn_launch.h"
+
+namespace msattn {
+template hipError_t launch_fp4_attn<_Float16, 128>(const Fp4Params&, int, int, hipStream_t);
+}

@@ -13,7 +13,6 @@ its own methods. The layout is msattn.h's: uint8 [num_blocks, kv_heads, block_si
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -21,11 +20,10 @@ import torch
 from . import _native as nat
 from .attention import (_require_gpu, _workspace, block_table_i32, context_lens_i32, narrow_i32,
                         starts_i32)
-from .rotary import _source, _spans, current, extent, on_16_bytes, on_device
+from .rotary import current, extent, on_device
 
 TILE = 16     # tokens of a tile
 BLOCK = 32    # elements that share a scale
-_I64x3 = ctypes.c_int64 * 3
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -56,28 +54,38 @@ def is_fp4_cache(cache: torch.Tensor) -> bool:
     return cache.dtype == torch.uint8
 
 
-def _cache_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int]:
-    """(num_blocks, kv_heads, block_size, head_dim) of a pair of 4-bit caches, which it checks."""
-    if not (k_cache.is_cuda and v_cache.is_cuda):
+def _cache_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor
+                    ) -> tuple[int, int, int, int, int, tuple]:
+    """(device index, num_blocks, kv_heads, block_size, head_dim, strides) of a pair of 4-bit
+    caches, which it checks (all but what the library's entry points check)."""
+    at, shape, stride = k_cache.get_device(), k_cache.shape, k_cache.stride()
+    if at < 0 or v_cache.get_device() != at:
         _require_gpu(k_cache, "k_cache")
         _require_gpu(v_cache, "v_cache")
-    stride = k_cache.stride()
-    if k_cache.ndim != 4 or k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8 or \
-            k_cache.shape != v_cache.shape or stride != v_cache.stride():
+        raise ValueError("the caches must be on one device")
+    if len(shape) != 4 or shape != v_cache.shape or stride != v_cache.stride() or \
+            k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
         raise ValueError("k_cache and v_cache must share a uint8 [num_blocks, kv_heads, "
                          "block_size / 16, 17 * head_dim / 2] shape and strides")
-    nb, KVH, tiles, nbytes = k_cache.shape
+    nb, KVH, tiles, nbytes = shape
     D = nbytes * 2 // 17
     if nbytes != _tile_bytes(D) or D <= 0 or D % BLOCK or D > nat.MAX_HEAD_DIM:
         raise ValueError(f"a tile of {nbytes} bytes: a 4-bit cache has 17 * head_dim / 2, head_dim "
                          f"a multiple of {BLOCK} up to {nat.MAX_HEAD_DIM}")
-    if nb == 0 or KVH == 0 or tiles == 0:
+    if not (nb and KVH and tiles):
         raise ValueError("an empty cache")
-    if stride[3] != 1 or tiles > 1 and stride[2] != nbytes or stride[0] % 16 or stride[1] % 16 or \
-            k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
-        raise ValueError("the tiles of a page and head must be contiguous, pages and heads on 16 "
-                         "bytes")
-    return nb, KVH, tiles * TILE, D
+    if stride[3] != 1 or stride[2] != nbytes and tiles > 1:
+        raise ValueError("the tiles of a page and head must be contiguous")
+    return at, nb, KVH, tiles * TILE, D, stride
+
+
+def _check(fn: str, status: int, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
+    """nat.check, naming what a refusal of the caches is about."""
+    if status == nat.ERR_INVALID_ARG and (
+            any(x % 16 for x in k_cache.stride()[:2]) or k_cache.data_ptr() % 16 or
+            v_cache.data_ptr() % 16):
+        raise ValueError(f"{fn}: a 4-bit cache's pages and heads lie on 16 bytes")
+    nat.check(fn, status)
 
 
 def write_kv_fp4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -93,41 +101,52 @@ def write_kv_fp4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     among them read back as NaN. A row's bytes do not depend on what is written beside it. Two
     tokens of one call must not land in one slot: parts of either's rows may remain there.
     """
-    nb, KVH, bs, D = _cache_geometry(k_cache, v_cache)
-    dev, dtype = k_cache.device, k.dtype
-    if not (k.is_cuda and v.is_cuda):
+    at, nb, KVH, bs, D, stride = _cache_geometry(k_cache, v_cache)
+    if k.get_device() != at or v.get_device() != at:
         _require_gpu(k, "k")
         _require_gpu(v, "v")
-    if k.ndim != 4 or k.shape != v.shape:
+        raise ValueError("k, v and the caches must be on one device")
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 4 or shape != v.shape:
         raise ValueError("k and v must both be [batch, tokens, kv_heads, head_dim]")
-    B, T = k.shape[:2]
-    if k.shape[2] != KVH or k.shape[3] != D:
+    B, T = shape[:2]
+    if shape[2] != KVH or shape[3] != D:
         raise ValueError("k/v heads or head_dim do not match the cache")
     if v.dtype != dtype:
         raise ValueError("k and v must share a dtype")
     if dtype not in _TYPES:
         raise ValueError(f"unsupported dtype for a 4-bit cache: {dtype}")
-    if v_cache.device != dev or k.device != dev or v.device != dev:
-        raise ValueError("k, v and the caches must be on one device")
     if B == 0 or T == 0:
         return
+    dev = k_cache.device
     table = block_table_i32(block_table, dev)
-    if table.shape[0] < B:
+    rows, W = table.shape
+    if rows < B:
         raise ValueError("block_table has fewer rows than k")
-    if table.shape[1] == 0:
+    if W == 0:
         raise ValueError("block_table has no columns")
     if isinstance(start, torch.Tensor):
         start = narrow_i32(start)
     starts = starts_i32(start, B, dev)
-    written = _spans((k_cache, v_cache))
-    ks, vs = _source(k, written), _source(v, written)
-    stride = k_cache.stride()
-    status = on_device(
-        dev, nat.lib().msattn_write_kv_fp4, ks.data_ptr(), _I64x3(*ks.stride()[:3]), vs.data_ptr(),
-        _I64x3(*vs.stride()[:3]), k_cache.data_ptr(), v_cache.data_ptr(), stride[0], stride[1],
-        table.data_ptr(), starts.data_ptr(), B, T, KVH, D, bs, nb, table.shape[1],
-        nat.dtype_code(dtype))
-    nat.check("msattn_write_kv_fp4", status)
+    ks, vs = k.stride(), v.stride()
+    fn, code = nat.lib().msattn_write_kv_fp4, nat.DTYPE_CODES[dtype]
+    if ks[3] != 1 or vs[3] != 1 or k.is_neg() or v.is_neg():
+        status = nat.ERR_OVERLAP
+    else:
+        status = on_device(
+            dev, fn, k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+            k_cache.data_ptr(), v_cache.data_ptr(), stride[0], stride[1], table.data_ptr(),
+            starts.data_ptr(), B, T, KVH, D, bs, nb, W, code)
+    if status == nat.ERR_OVERLAP:  # rows that cannot be read where they lie: a copy
+        with current(dev):
+            k, v = (x.resolve_neg().clone(memory_format=torch.contiguous_format) for x in (k, v))
+        ks = k.stride()
+        status = on_device(
+            dev, fn, k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), ks[0], ks[1], ks[2],
+            k_cache.data_ptr(), v_cache.data_ptr(), stride[0], stride[1], table.data_ptr(),
+            starts.data_ptr(), B, T, KVH, D, bs, nb, W, code)
+    if status:
+        _check("msattn_write_kv_fp4", status, k_cache, v_cache)
 
 
 def read_kv_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table, start, tokens: int, *,
@@ -137,32 +156,29 @@ def read_kv_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table, start
     entry per row, or an int tensor). fp32 and bf16 hold them exactly. Positions on holes, outside
     the table or below 0 give zeros; those past a row's context give whatever its pages hold.
     """
-    nb, KVH, bs, D = _cache_geometry(k_cache, v_cache)
-    dev = k_cache.device
-    if v_cache.device != dev:
-        raise ValueError("the caches must be on one device")
+    _, nb, KVH, bs, D, stride = _cache_geometry(k_cache, v_cache)
     if dtype not in _TYPES:
         raise ValueError(f"unsupported dtype for a 4-bit cache's values: {dtype}")
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
+    dev = k_cache.device
     table = block_table_i32(block_table, dev)
     B, W = table.shape
     if W == 0:
         raise ValueError("block_table has no columns")
-    k = torch.empty((B, tokens, KVH, D), dtype=dtype, device=dev)
-    v = torch.empty_like(k)
-    if k.numel() == 0:
+    k, v = torch.empty((2, B, tokens, KVH, D), dtype=dtype, device=dev).unbind(0)
+    if B == 0 or tokens == 0:
         return k, v
     if isinstance(start, torch.Tensor):
         start = narrow_i32(start)
     starts = starts_i32(start, B, dev)
-    stride = k_cache.stride()
     status = on_device(
         dev, nat.lib().msattn_read_kv_fp4, k_cache.data_ptr(), v_cache.data_ptr(), stride[0],
         stride[1], table.data_ptr(), starts.data_ptr(), k.data_ptr(), v.data_ptr(), B, tokens, KVH,
-        D, bs, nb, W, nat.dtype_code(dtype))
-    nat.check("msattn_read_kv_fp4", status)
+        D, bs, nb, W, nat.DTYPE_CODES[dtype])
+    if status:
+        _check("msattn_read_kv_fp4", status, k_cache, v_cache)
     return k, v
 
 
@@ -177,75 +193,70 @@ def paged_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     alone. A view of the query in 16-byte rows is read where it lies. Nothing is read by the host
     where ``context_lens`` is a device tensor, so the call is safe to capture.
     """
-    nb, KVH, bs, Dk = _cache_geometry(k_cache, v_cache)
-    if not query.is_cuda:
+    at, nb, KVH, bs, Dk, stride = _cache_geometry(k_cache, v_cache)
+    if query.get_device() != at:
         _require_gpu(query, "query")
-    if query.ndim != 4:
+        raise ValueError("query and the caches must be on one device")
+    shape, dtype = query.shape, query.dtype
+    if len(shape) != 4:
         raise ValueError("query must be [batch, q_len, heads, head_dim]")
-    B, q_len, H, D = query.shape
+    B, q_len, H, D = shape
     if Dk != D:
         raise ValueError(f"head_dim mismatch: query {D}, cache {Dk}")
     if H == 0 or H % KVH:
         raise ValueError("num_heads must be a multiple of num_kv_heads")
-    if query.dtype not in _TYPES:
-        raise ValueError(f"unsupported dtype for a query over a 4-bit cache: {query.dtype}")
+    if dtype not in _TYPES:
+        raise ValueError(f"unsupported dtype for a query over a 4-bit cache: {dtype}")
     if window is not None and window <= 0:
         raise ValueError("window must be positive")
     dev = query.device
-    if k_cache.device != dev or v_cache.device != dev:
-        raise ValueError("query and the caches must be on one device")
     table = block_table_i32(block_table, dev)
-    if table.shape[0] != B:
-        raise ValueError(f"block_table has {table.shape[0]} rows for a batch of {B}")
-    W = table.shape[1]
+    rows, W = table.shape
+    if rows != B:
+        raise ValueError(f"block_table has {rows} rows for a batch of {B}")
     if W == 0:
         raise ValueError("block_table has no columns")
-    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or
-                            out.device != dev or not out.is_contiguous()):
-        raise ValueError("out must be contiguous, of the query's shape, dtype and device")
     if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
         raise ValueError("workspace must be contiguous and on the query's device")
-    with current(dev):
-        lens, host_max = context_lens_i32(context_lens, dev, B)
+    lens, host_max = context_lens_i32(context_lens, dev, B)
     cap = W * bs
     if max_context is None:
         max_context = cap if host_max is None else host_max
     if host_max is not None and host_max > cap:
         raise ValueError(f"context length {host_max} exceeds the block table capacity {cap}")
     max_context = max(0, min(int(max_context), cap, 2 ** 31 - 1))
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
-    fresh = out is None
-    if fresh:
-        out = torch.empty((B, q_len, H, D), dtype=query.dtype, device=dev)
+    given = None  # an output that the kernel, which stores 16 bytes at once, does not write itself
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    elif out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of the query's shape, dtype and device")
+    else:
+        (lo, hi), (olo, ohi) = extent(query), extent(out)
+        if lo < ohi and olo < hi:  # a wave reads its rows while another's are written
+            query = query.clone()
+        if olo % 16:
+            given, out = out, torch.empty_like(out)
     if B == 0 or q_len == 0:
-        return out
-    given = None
-    if out.data_ptr() % 16:  # (the kernel stores 16 bytes at once)
-        given, out = out, torch.empty_like(out)
-    q = query.resolve_neg() if query.is_neg() else query
-    es = q.element_size()
-    if q.stride(3) != 1 or any(s * es % 16 for s in q.stride()[:3]):
-        q = q.contiguous()
-    q = on_16_bytes(q)
-    if q is query and not fresh:  # a wave reads its rows while another's are written
-        (lo, hi), (olo, ohi) = extent(q), extent(out)
-        if lo < ohi and olo < hi:
-            q = q.clone(memory_format=torch.contiguous_format)
-    lib = nat.lib()
-    code = nat.dtype_code(q.dtype)
+        return out if given is None else given
+    qs = query.stride()
+    es = 16 // query.element_size()
+    if qs[3] != 1 or qs[0] % es or qs[1] % es or qs[2] % es or query.data_ptr() % 16 or \
+            query.is_neg():
+        query = query.resolve_neg().clone(memory_format=torch.contiguous_format)
+        qs = query.stride()
+    lib, code = nat.lib(), nat.DTYPE_CODES[dtype]
     ws_bytes = lib.msattn_fp4_workspace_bytes(B, q_len, H, KVH, D, max_context, code)
     if ws_bytes == 0:
         raise ValueError("unsupported attention geometry")
     if workspace is None or workspace.numel() * workspace.element_size() < ws_bytes:
         with current(dev):
             workspace = _workspace(dev, ws_bytes)
-    stride = k_cache.stride()
     status = on_device(
-        dev, lib.msattn_paged_attention_fp4, q.data_ptr(), _I64x3(*q.stride()[:3]),
+        dev, lib.msattn_paged_attention_fp4, query.data_ptr(), qs[0], qs[1], qs[2],
         k_cache.data_ptr(), v_cache.data_ptr(), stride[0], stride[1], table.data_ptr(),
         lens.data_ptr(), out.data_ptr(), workspace.data_ptr(), ws_bytes, B, q_len, H, KVH, D, bs,
-        nb, W, max_context, 1 if causal else 0, min(int(window or 0), 2 ** 31 - 1), float(scale),
-        code)
-    nat.check("msattn_paged_attention_fp4", status)
+        nb, W, max_context, 1 if causal else 0, min(window or 0, 2 ** 31 - 1),
+        1.0 / math.sqrt(D) if scale is None else float(scale), code)
+    if status:
+        _check("msattn_paged_attention_fp4", status, k_cache, v_cache)
     return out if given is None else given.copy_(out)

@@ -1,18 +1,13 @@
 """CPU checks of the 4-bit cache's entry points: refusals, workspace sizes, CPU tensors."""
-import ctypes
-
 import pytest
 import torch
 
 from miniserve_amd import (PagedAttention, _native as nat, allocate_fp4_cache, paged_attention_fp4,
                            read_kv_fp4, write_kv_fp4)
 
-I64x3 = ctypes.c_int64 * 3
-ST = I64x3(4 * 128, 128, 128)
-
 
 def write_args(**over):
-    a = dict(k=1024, ks=ST, v=2048, vs=ST, kc=4096, vc=8192, blk=1088 * 2, head=1088, table=256,
+    a = dict(k=1 << 20, k0=768, k1=256, k2=128, v=1 << 21, v0=768, v1=256, v2=128, kc=4096, vc=1 << 17, blk=1088 * 2, head=1088, table=256,
              starts=512, B=2, T=3, KVH=2, D=128, bs=16, nb=10, W=4, t=nat.BF16, stream=None)
     a.update(over)
     return list(a.values())
@@ -30,7 +25,8 @@ def named(d):
 
 
 @pytest.mark.parametrize("bad,status", BAD_CACHE + [
-    (dict(k=None), 1), (dict(v=None), 1), (dict(ks=None), 1), (dict(vs=None), 1),
+    (dict(k=None), 1), (dict(v=None), 1), (dict(k1=-1), 1), (dict(v0=-256), 1),
+    (dict(k=4096 + 9 * 2176 + 2000), 5), (dict(v=(1 << 17) - 2 * 1536 + 16), 5), (dict(k=4096 - 100, k2=1 << 20), 5),
     (dict(starts=None), 1), (dict(starts=514), 1), (dict(k=1025), 1), (dict(T=-1), 1),
     (dict(B=1 << 20, T=1 << 11), 2)], ids=named)
 def test_write_refuses(bad, status):
@@ -52,7 +48,7 @@ def test_read_refuses(bad, status):
 
 
 def attend_args(**over):
-    a = dict(q=1024, qs=I64x3(8 * 128, 8 * 128, 128), kc=4096, vc=8192, blk=1088 * 2, head=1088,
+    a = dict(q=1024, q0=1024, q1=1024, q2=128, kc=4096, vc=8192, blk=1088 * 2, head=1088,
              table=256, lens=512, out=2048, ws=1 << 20, ws_bytes=1 << 40, B=2, q_len=1, H=8, KVH=2,
              D=128, bs=16, nb=10, W=4, max_context=64, causal=1, window=0, scale=0.1, t=nat.BF16,
              stream=None)
@@ -61,11 +57,11 @@ def attend_args(**over):
 
 
 @pytest.mark.parametrize("bad,status", BAD_CACHE + [
-    (dict(q=None), 1), (dict(qs=None), 1), (dict(lens=None), 1), (dict(lens=513), 1),
-    (dict(out=None), 1), (dict(ws=None), 1), (dict(q=1032), 1), (dict(out=2049), 1),
+    (dict(q=None), 1), (dict(q1=-1024), 1), (dict(lens=None), 1), (dict(lens=513), 1),
+    (dict(out=None), 1), (dict(ws=None), 1), (dict(q=1032), 1), (dict(out=2056), 1),
     (dict(ws=(1 << 20) + 64), 1), (dict(q_len=0), 1), (dict(H=0), 1), (dict(H=3), 1),
     (dict(max_context=-1), 1), (dict(window=-1), 1), (dict(scale=float("nan")), 1),
-    (dict(qs=I64x3(1028, 1024, 128)), 1), (dict(qs=I64x3(1024, 1024, 132)), 1),
+    (dict(q0=1028), 1), (dict(q2=132), 1),
     (dict(ws_bytes=1024), 3), (dict(q_len=1 << 29), 2)], ids=named)
 def test_attention_refuses(bad, status):
     assert nat.lib().msattn_paged_attention_fp4(*attend_args(**bad)) == status
