@@ -37,8 +37,10 @@ int cache_params(Fp4CacheParams* p, const void* k, const void* v, const int64_t*
     return MSATTN_ERR_INVALID_ARG;
   const int eb = type_bytes(dtype);
   if (!on(k, eb) || !on(v, eb) || !on(table, 4) || !on(starts, 4)) return MSATTN_ERR_INVALID_ARG;
-  if (static_cast<int64_t>(batch) * tokens >= (int64_t(1) << 31) ||
-      static_cast<int64_t>(KVH) * (D / 8) >= (int64_t(1) << 22))
+  // tokens positions from anywhere in a tile; the wave's index fits 31 bits
+  p->tiles = static_cast<int>((static_cast<int64_t>(tokens) + 2 * (kFp4Tile - 1)) / kFp4Tile);
+  p->items = static_cast<int64_t>(batch) * p->tiles;
+  if (p->items >= (int64_t(1) << 31) || (p->items *= KVH) >= (int64_t(1) << 31))
     return MSATTN_ERR_UNSUPPORTED;
   p->k_cache = static_cast<uint8_t*>(k_cache);
   p->v_cache = static_cast<uint8_t*>(v_cache);
@@ -61,8 +63,8 @@ int cache_params(Fp4CacheParams* p, const void* k, const void* v, const int64_t*
   p->bs = bs;
   p->num_blocks = num_blocks;
   p->W = W;
-  p->by_tokens = fp4_div(static_cast<uint32_t>(tokens > 0 ? tokens : 1));
-  p->by_octets = fp4_div(static_cast<uint32_t>(D / 8));
+  p->by_tiles = fp4_div(static_cast<uint32_t>(p->tiles > 0 ? p->tiles : 1));
+  p->by_heads = fp4_div(static_cast<uint32_t>(KVH));
   p->by_bs = fp4_div(static_cast<uint32_t>(bs));
   return MSATTN_OK;
 }

@@ -63,7 +63,9 @@ struct Fp4CacheParams {
   int64_t k_st[3], v_st[3];         // batch, token and head strides of k and v (elements)
   int batch, tokens, KVH, D, bs, num_blocks, W;
   int vec;                          // rows of k and v on 16 bytes
-  Fp4Div by_tokens, by_octets, by_bs;
+  int tiles;                        // that a row's tokens may touch
+  int64_t items;                    // rows x tiles x heads: a wave each
+  Fp4Div by_tiles, by_heads, by_bs;
 };
 
 hipError_t launch_write_fp4(const Fp4CacheParams& p, int src_dtype, hipStream_t stream);

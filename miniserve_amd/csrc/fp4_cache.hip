@@ -3,9 +3,12 @@
 //   write   cache[table[b, pos / bs], pos % bs] = quantise(src[b, t]),  pos = starts[b] + t
 //   read    dst[b, t] = values of cache[table[b, pos / bs], pos % bs]
 //
-// One thread takes 8 elements of a row of K and of V: 16 bytes of a 16-bit row, 4 bytes of the
-// cache. The four threads of a 32-element block are neighbours, so that the block's largest
-// magnitude is two lane exchanges away.
+// A wave takes one tile (16 tokens of one head) of K and of V, four lanes a token: in step j lane
+// (t, q) = (l / 4, l % 4) has dims 32 j + 8 q .. + 7 of token t, 16 bytes of a 16-bit row and 4 of the
+// cache, so that a block's largest magnitude is two lane exchanges away. Rows move in pieces of 64
+// bytes; values' tiles in whole lines, since octet 4 j + q lies at 64 (4 j + q) + 4 t; keys' too, once
+// the four lanes of a token have exchanged their words of four steps. (A thread for each 8 elements,
+// row by row, wrote the values' words 64 bytes apart: 4 x 8191 tokens of 8 x 128 bf16 in 51 us.)
 #include "fp4_cache.h"
 
 namespace msattn {
@@ -88,110 +91,172 @@ __device__ __forceinline__ void widen8(uint32_t w, uint32_t byte, float (&x)[8])
   for (int i = 0; i < 8; ++i) x[i] = byte == kFp4NaN ? __uint_as_float(0x7fc00000u) : y[i];
 }
 
-// What a thread works on: 8 dims from 8 o of head h of token t of row b, and the tile and place
-// of the token (tile < 0: a hole, or outside the table).
+// What a wave works on: head h and the tokens of one tile of row b, and where the tile lies (at < 0:
+// a hole, or outside the table).
 struct Fp4Item {
-  int b, t, h, o;
-  int64_t tile;  // byte offset of the tile in either cache
-  int place;     // token within the tile
+  int b, h;
+  int t;       // the lane's token (in the call's rows)
+  bool live;   // which is one of the call's
+  int64_t at;  // byte offset of the tile in either cache
 };
 
-// Threads a token, a power of two up to the workgroup's; the grid's y covers what is left.
-__host__ __device__ inline int fp4_lanes(int items) {
-  int n = 4;
-  while (n < items && n < kFp4Threads) n <<= 1;
-  return n;
-}
-
-__device__ __forceinline__ bool fp4_item(const Fp4CacheParams& p, int lanes, int shift, Fp4Item* it) {
-  const int tid = static_cast<int>(threadIdx.x);
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) << (8 - shift)) + (tid >> shift);
-  const int item = static_cast<int>(blockIdx.y) * lanes + (tid & (lanes - 1));
-  const int octets = p.D / 8;
-  if (row >= static_cast<int64_t>(p.batch) * p.tokens || item >= p.KVH * octets) return false;
-  it->b = fp4_quot(static_cast<int>(row), p.by_tokens);
-  it->t = static_cast<int>(row) - it->b * p.tokens;
-  it->h = fp4_quot(item, p.by_octets);
-  it->o = item - it->h * octets;
-  it->tile = -1;
-  it->place = 0;
-  const int64_t pos = static_cast<int64_t>(p.starts[it->b]) + it->t;
-  if (pos < 0 || pos >= static_cast<int64_t>(p.W) * p.bs || pos >= (int64_t(1) << 31)) return true;
-  const int pg = fp4_quot(static_cast<int>(pos), p.by_bs);
-  const int phys = p.table[static_cast<int64_t>(it->b) * p.W + pg];
+__device__ __forceinline__ bool fp4_item(const Fp4CacheParams& p, Fp4Item* it) {
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int64_t i64 = static_cast<int64_t>(blockIdx.x) * (kFp4Threads / 64) + wave;
+  if (i64 >= p.items) return false;
+  const int i = static_cast<int>(i64);
+  const int bk = fp4_quot(i, p.by_heads);  // (head fastest: its neighbours' rows are the memory's)
+  it->h = i - bk * p.KVH;
+  it->b = fp4_quot(bk, p.by_tiles);
+  const int k = bk - it->b * p.tiles;      // the row's tile, from the one its first token lies in
+  const int64_t start = p.starts[it->b];
+  const int64_t first = ((start >> 4) + k) << 4;  // the tile's first position
+  it->t = static_cast<int>(first - start) + (static_cast<int>(threadIdx.x) & 63) / 4;
+  it->live = it->t >= 0 && it->t < p.tokens;
+  it->at = -1;
+  if (first < 0 || first >= static_cast<int64_t>(p.W) * p.bs || first >= (int64_t(1) << 31)) return true;
+  const int pg = fp4_quot(static_cast<int>(first), p.by_bs);
+  const int phys = __builtin_amdgcn_readfirstlane(p.table[static_cast<int64_t>(it->b) * p.W + pg]);
   if (phys < 0 || phys >= p.num_blocks) return true;
-  const int in = static_cast<int>(pos) - pg * p.bs;
-  it->tile = static_cast<int64_t>(phys) * p.blk_stride + static_cast<int64_t>(it->h) * p.head_stride +
-             static_cast<int64_t>(in / kFp4Tile) * fp4_tile_bytes(p.D);
-  it->place = in % kFp4Tile;
+  it->at = static_cast<int64_t>(phys) * p.blk_stride + static_cast<int64_t>(it->h) * p.head_stride +
+           static_cast<int64_t>((static_cast<int>(first) - pg * p.bs) / kFp4Tile) * fp4_tile_bytes(p.D);
   return true;
 }
 
-__device__ __forceinline__ int64_t source_at(const int64_t (&st)[3], const Fp4Item& it) {
-  return it.b * st[0] + it.t * st[1] + it.h * st[2] + 8 * it.o;
-}
-
-template <typename T, bool VEC>
-__global__ __launch_bounds__(kFp4Threads) void write_fp4_kernel(const Fp4CacheParams p, int lanes,
-                                                                int shift) {
-  Fp4Item it;
-  if (!fp4_item(p, lanes, shift, &it) || it.tile < 0) return;
-  float k[8], v[8];
-  load8<T, VEC>(static_cast<const T*>(p.k) + source_at(p.k_st, it), k);
-  load8<T, VEC>(static_cast<const T*>(p.v) + source_at(p.v_st, it), v);
-  uint32_t kb, vb;
-  const uint32_t kw = quantise8(k, &kb), vw = quantise8(v, &vb);
-  uint8_t* const kt = p.k_cache + it.tile;
-  uint8_t* const vt = p.v_cache + it.tile;
-  *reinterpret_cast<uint32_t*>(kt + it.place * (p.D / 2) + 4 * it.o) = kw;
-  *reinterpret_cast<uint32_t*>(vt + 64 * it.o + 4 * it.place) = vw;
-  if (it.o % 4 == 0) {
-    const int at = 8 * p.D + 4 * it.o + it.place;
-    kt[at] = static_cast<uint8_t>(kb);
-    vt[at] = static_cast<uint8_t>(vb);
-  }
-}
-
-template <typename T, bool VEC>
-__global__ __launch_bounds__(kFp4Threads) void read_fp4_kernel(const Fp4CacheParams p, int lanes,
-                                                               int shift) {
-  Fp4Item it;
-  if (!fp4_item(p, lanes, shift, &it)) return;
-  float k[8], v[8];
+// Words x[j] of lanes q = 0 .. 3 of a quad, transposed: x[j] of lane q becomes x[q] of lane j.
+__device__ __forceinline__ void quad_transpose(uint32_t (&x)[4], int q) {
+  auto swapped = [](uint32_t v, auto ctrl) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v),
+                                                             decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  using X1 = std::integral_constant<int, 0xB1>;  // lane q ^ 1
+  using X2 = std::integral_constant<int, 0x4E>;  // lane q ^ 2
 #pragma unroll
-  for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.0f;
-  if (it.tile >= 0) {
-    const uint8_t* const kt = p.k_cache + it.tile;
-    const uint8_t* const vt = p.v_cache + it.tile;
-    const int at = 8 * p.D + 16 * (it.o / 4) + it.place;
-    widen8(*reinterpret_cast<const uint32_t*>(kt + it.place * (p.D / 2) + 4 * it.o), kt[at], k);
-    widen8(*reinterpret_cast<const uint32_t*>(vt + 64 * it.o + 4 * it.place), vt[at], v);
+  for (int j = 0; j < 4; j += 2) {  // the off-diagonal words of each 2 x 2, then the 2 x 2s
+    const uint32_t send = q & 1 ? x[j] : x[j + 1];
+    const uint32_t got = swapped(send, X1{});
+    if (q & 1) x[j] = got;
+    else x[j + 1] = got;
   }
-  store8<T, VEC>(static_cast<T*>(p.k) + source_at(p.k_st, it), k);
-  store8<T, VEC>(static_cast<T*>(p.v) + source_at(p.v_st, it), v);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t send = q & 2 ? x[j] : x[j + 2];
+    const uint32_t got = swapped(send, X2{});
+    if (q & 2) x[j] = got;
+    else x[j + 2] = got;
+  }
+}
+
+template <typename T, bool VEC, int NB>
+__global__ __launch_bounds__(kFp4Threads) void write_fp4_kernel(const Fp4CacheParams p) {
+  Fp4Item it;
+  if (!fp4_item(p, &it) || it.at < 0 || !it.live) return;  // (a token's four lanes as one)
+  const int lane = static_cast<int>(threadIdx.x) & 63, t = lane >> 2, q = lane & 3;
+  const T* const kp = static_cast<const T*>(p.k) + it.b * p.k_st[0] + it.t * p.k_st[1] + it.h * p.k_st[2] + 8 * q;
+  const T* const vp = static_cast<const T*>(p.v) + it.b * p.v_st[0] + it.t * p.v_st[1] + it.h * p.v_st[2] + 8 * q;
+  uint8_t* const kt = p.k_cache + it.at;
+  uint8_t* const vt = p.v_cache + it.at;
+  uint32_t kw[NB], kb[NB], vw[NB], vb[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    float x[8];
+    load8<T, VEC>(kp + 32 * j, x);
+    kw[j] = quantise8(x, &kb[j]);
+    load8<T, VEC>(vp + 32 * j, x);
+    vw[j] = quantise8(x, &vb[j]);
+  }
+#pragma unroll
+  for (int j = 0; j + 4 <= NB; j += 4) {
+    uint32_t x[4] = {kw[j], kw[j + 1], kw[j + 2], kw[j + 3]};
+    quad_transpose(x, q);  // lane q: all of block j + q
+    *reinterpret_cast<uint4*>(kt + t * (16 * NB) + 16 * (j + q)) = make_uint4(x[0], x[1], x[2], x[3]);
+  }
+#pragma unroll
+  for (int j = NB / 4 * 4; j < NB; ++j)
+    *reinterpret_cast<uint32_t*>(kt + t * (16 * NB) + 16 * j + 4 * q) = kw[j];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+    *reinterpret_cast<uint32_t*>(vt + 64 * (4 * j + q) + 4 * t) = vw[j];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {  // (lane j % 4 stores block j's bytes)
+    if (q != j % 4) continue;
+    kt[256 * NB + 16 * j + t] = static_cast<uint8_t>(kb[j]);
+    vt[256 * NB + 16 * j + t] = static_cast<uint8_t>(vb[j]);
+  }
+}
+
+template <typename T, bool VEC, int NB>
+__global__ __launch_bounds__(kFp4Threads) void read_fp4_kernel(const Fp4CacheParams p) {
+  Fp4Item it;
+  if (!fp4_item(p, &it) || !it.live) return;
+  const int lane = static_cast<int>(threadIdx.x) & 63, t = lane >> 2, q = lane & 3;
+  const int64_t at = it.b * p.k_st[0] + it.t * p.k_st[1] + it.h * p.k_st[2] + 8 * q;
+  uint32_t kw[NB], kb[NB], vw[NB], vb[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) kw[j] = vw[j] = kb[j] = vb[j] = 0;
+  if (it.at >= 0) {
+    const uint8_t* const kt = p.k_cache + it.at;
+    const uint8_t* const vt = p.v_cache + it.at;
+#pragma unroll
+    for (int j = 0; j + 4 <= NB; j += 4) {
+      const uint4 w = *reinterpret_cast<const uint4*>(kt + t * (16 * NB) + 16 * (j + q));
+      uint32_t x[4] = {w.x, w.y, w.z, w.w};
+      quad_transpose(x, q);  // lane q: octet q of blocks j .. j + 3
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kw[j + i] = x[i];
+    }
+#pragma unroll
+    for (int j = NB / 4 * 4; j < NB; ++j)
+      kw[j] = *reinterpret_cast<const uint32_t*>(kt + t * (16 * NB) + 16 * j + 4 * q);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      vw[j] = *reinterpret_cast<const uint32_t*>(vt + 64 * (4 * j + q) + 4 * t);
+      kb[j] = kt[256 * NB + 16 * j + t];
+      vb[j] = vt[256 * NB + 16 * j + t];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    float x[8];
+    widen8(kw[j], kb[j], x);
+    store8<T, VEC>(static_cast<T*>(p.k) + at + 32 * j, x);
+    widen8(vw[j], vb[j], x);
+    store8<T, VEC>(static_cast<T*>(p.v) + at + 32 * j, x);
+  }
+}
+
+template <typename T, bool VEC, int NB>
+static hipError_t launch_ops(const Fp4CacheParams& p, bool write, hipStream_t stream) {
+  constexpr int per = kFp4Threads / 64;
+  const dim3 grid(static_cast<unsigned>((p.items + per - 1) / per));
+  if (write)
+    hipLaunchKernelGGL((write_fp4_kernel<T, VEC, NB>), grid, dim3(kFp4Threads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((read_fp4_kernel<T, VEC, NB>), grid, dim3(kFp4Threads), 0, stream, p);
+  return hipGetLastError();
 }
 
 template <typename T, bool VEC>
-static hipError_t launch_ops(const Fp4CacheParams& p, bool write, hipStream_t stream) {
-  const int items = p.KVH * (p.D / 8);
-  const int lanes = fp4_lanes(items);
-  const int shift = __builtin_ctz(static_cast<unsigned>(lanes));
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens, per = kFp4Threads / lanes;
-  const dim3 grid(static_cast<unsigned>((rows + per - 1) / per),
-                  static_cast<unsigned>((items + lanes - 1) / lanes));
-  if (write)
-    hipLaunchKernelGGL((write_fp4_kernel<T, VEC>), grid, dim3(kFp4Threads), 0, stream, p, lanes, shift);
-  else
-    hipLaunchKernelGGL((read_fp4_kernel<T, VEC>), grid, dim3(kFp4Threads), 0, stream, p, lanes, shift);
-  return hipGetLastError();
+static hipError_t launch_blocks(const Fp4CacheParams& p, bool write, hipStream_t stream) {
+  switch (p.D / kFp4Block) {
+    case 1: return launch_ops<T, VEC, 1>(p, write, stream);
+    case 2: return launch_ops<T, VEC, 2>(p, write, stream);
+    case 3: return launch_ops<T, VEC, 3>(p, write, stream);
+    case 4: return launch_ops<T, VEC, 4>(p, write, stream);
+    case 5: return launch_ops<T, VEC, 5>(p, write, stream);
+    case 6: return launch_ops<T, VEC, 6>(p, write, stream);
+    case 7: return launch_ops<T, VEC, 7>(p, write, stream);
+    case 8: return launch_ops<T, VEC, 8>(p, write, stream);
+    default: return hipErrorNotSupported;
+  }
 }
 
 template <bool VEC>
 static hipError_t launch_types(const Fp4CacheParams& p, int dtype, bool write, hipStream_t stream) {
   switch (dtype) {
-    case 0: return launch_ops<float, VEC>(p, write, stream);
-    case 1: return launch_ops<_Float16, VEC>(p, write, stream);
-    case 2: return launch_ops<bf16_t, VEC>(p, write, stream);
+    case 0: return launch_blocks<float, VEC>(p, write, stream);
+    case 1: return launch_blocks<_Float16, VEC>(p, write, stream);
+    case 2: return launch_blocks<bf16_t, VEC>(p, write, stream);
     default: return hipErrorNotSupported;
   }
 }

@@ -28,7 +28,7 @@ def named(d):
     (dict(k=None), 1), (dict(v=None), 1), (dict(k1=-1), 1), (dict(v0=-256), 1),
     (dict(k=4096 + 9 * 2176 + 2000), 5), (dict(v=(1 << 17) - 2 * 1536 + 16), 5), (dict(k=4096 - 100, k2=1 << 20), 5),
     (dict(starts=None), 1), (dict(starts=514), 1), (dict(k=1025), 1), (dict(T=-1), 1),
-    (dict(B=1 << 20, T=1 << 11), 2)], ids=named)
+    (dict(B=1 << 20, T=1 << 15), 2)], ids=named)
 def test_write_refuses(bad, status):
     assert nat.lib().msattn_write_kv_fp4(*write_args(**bad)) == status
 
@@ -42,7 +42,7 @@ def read_args(**over):
 
 @pytest.mark.parametrize("bad,status", BAD_CACHE + [
     (dict(k=None), 1), (dict(v=None), 1), (dict(starts=None), 1), (dict(v=2049), 1),
-    (dict(T=-1), 1), (dict(B=1 << 20, T=1 << 11), 2)], ids=named)
+    (dict(T=-1), 1), (dict(B=1 << 20, T=1 << 15), 2)], ids=named)
 def test_read_refuses(bad, status):
     assert nat.lib().msattn_read_kv_fp4(*read_args(**bad)) == status
 
