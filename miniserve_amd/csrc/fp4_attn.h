@@ -112,6 +112,9 @@ __device__ __forceinline__ void fp4_store4(T* o, float a, float b, float c, floa
 #ifndef MSATTN_FP4_NT
 #define MSATTN_FP4_NT 0
 #endif
+#ifndef MSATTN_FP4_BALANCE
+#define MSATTN_FP4_BALANCE 1
+#endif
 #ifndef MSATTN_FP4_RING
 #define MSATTN_FP4_RING 3
 #endif
@@ -137,6 +140,7 @@ __device__ __forceinline__ V fp4_load(const uint8_t* p) {
 // Keys a query row, and a block of rows, may see, and a unit's place in the work list.
 struct Fp4Unit {
   int b, kvh, rb;
+  int ctx;           // the row's context
   int lo, hi;        // keys that some row of the block sees
   int first, n;      // its groups of keys
   int u0;            // position of its first group in the list
@@ -178,6 +182,8 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   constexpr int RS = DP + 4;
   __shared__ float s_acc[kFp4Waves * 16 * RS];
   __shared__ float2 s_ml[kFp4Waves * 16];
+  __shared__ int s_prog[kFp4Waves];  // groups that a wave has taken
+  __shared__ int s_first[5];         // the share's first unit
   __shared__ int s_cnt[16], s_done[16];  // of a buffer: waves that have written it, times it was read
 
   const int tid = static_cast<int>(threadIdx.x);
@@ -190,11 +196,6 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   const bool list = WK == kFp4Waves && p.split;
   const int entries = p.batch * p.rblocks;
 
-  auto ctx_of = [&](int b) FP4_INLINE {
-    if (list) return s_ctx[b];
-    const int c = p.lens[b];
-    return c < 0 ? 0 : (c > p.max_ctx ? p.max_ctx : c);
-  };
   // Barrier for what lies in LDS: loads into registers stay on their way.
   auto lds_barrier = [&]() FP4_INLINE {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -203,98 +204,77 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   };
 
   if (tid < 16) s_cnt[tid] = s_done[tid] = 0;
-  if (!list) lds_barrier();
-  // The list: s_pre[e] = groups of one head's units of entries 0 .. e - 1 (entry = row, row block).
-  int c0, c1, chunk = 1;
+  if (tid < kFp4Waves) s_prog[tid] = 0;
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  auto clamped = [&](int c) FP4_INLINE { return c < 0 ? 0 : (c > p.max_ctx ? p.max_ctx : c); };
+  // The list: groups of one head's units of entries 0 .. e - 1 (entry = row, row block). A batch of
+  // up to 64 rows of one block each has it in registers, entry e's sum with its own groups and its
+  // context in lane e of every wave; others in LDS.
+  const bool regs = p.rblocks == 1 && p.batch <= 64;
+  int c0 = 0, c1 = 0, chunk = 1, lane_sum = 0, lane_ctx = 0;
   if (list) {
-    int base = 0;
-    for (int e0 = 0; e0 < entries; e0 += kFp4Threads) {
-      const int e = e0 + tid;
+    int sum = 0;
+    if (regs) {
       int cnt = 0;
-      if (e < entries) {
-        const int b = fp4_quot(e, p.by_rb), rb = e - b * p.rblocks;
-        const int c = p.lens[b], ctx = c < 0 ? 0 : (c > p.max_ctx ? p.max_ctx : c);
-        if (rb == 0) s_ctx[b] = ctx;
+      if (lane < p.batch) {
+        lane_ctx = clamped(p.lens[lane]);
         int lo, hi;
-        fp4_extent<ROWS>(p, ctx, rb, &lo, &hi);
+        fp4_extent<ROWS>(p, lane_ctx, 0, &lo, &hi);
         cnt = fp4_count(lo, hi);
       }
-      const int incl = wave_inclusive_sum(cnt);
-      if (lane == 63) s_tot[w] = incl;
-      __syncthreads();
-      int before = base;
+      lane_sum = wave_inclusive_sum(cnt);
+      sum = __builtin_amdgcn_readlane(lane_sum, 63);
+    } else {
+      for (int e0 = 0; e0 < entries; e0 += kFp4Threads) {
+        const int e = e0 + tid;
+        int cnt = 0;
+        if (e < entries) {
+          const int b = fp4_quot(e, p.by_rb), rb = e - b * p.rblocks, ctx = clamped(p.lens[b]);
+          if (rb == 0) s_ctx[b] = ctx;
+          int lo, hi;
+          fp4_extent<ROWS>(p, ctx, rb, &lo, &hi);
+          cnt = fp4_count(lo, hi);
+        }
+        const int incl = wave_inclusive_sum(cnt);
+        if (lane == 63) s_tot[w] = incl;
+        __syncthreads();
+        int before = sum;
 #pragma unroll
-      for (int i = 0; i < kFp4Waves; ++i) {
-        const int t = s_tot[i];
-        if (i < w) before += t;
-        base += t;
+        for (int i = 0; i < kFp4Waves; ++i) {
+          const int t = s_tot[i];
+          if (i < w) before += t;
+          sum += t;
+        }
+        if (e < entries) s_pre[e + 1] = before + incl;
+        if (e == 0) s_pre[0] = 0;
+        __syncthreads();
       }
-      if (e < entries) s_pre[e + 1] = before + incl;
-      __syncthreads();
+      sum = uniform(sum);
     }
-    if (tid == 0) s_pre[0] = 0;
-    __syncthreads();
-    const int total = __builtin_amdgcn_readfirstlane(base) * p.KVH;
+    const int total = sum * p.KVH;
     // whole rounds of the waves: a part of one takes as long, and leaves more to join
     chunk = ceil_div(ceil_div(total, p.shares), kFp4Waves) * kFp4Waves;
     c0 = static_cast<int>(min(static_cast<int64_t>(share) * chunk, static_cast<int64_t>(total)));
     c1 = min(c0 + chunk, total);
-  } else {
-    c0 = 0;
-    c1 = 1;  // (its unit's groups, set below)
+    if (c0 >= c1) return;  // (the workgroup as one)
   }
-
-  // Without a list: the wave's unit. Workgroup i runs on XCD i % 8, each of which has an L2 of its
-  // own: an XCD takes a run of units, so that the row blocks of a head, which read the same keys,
-  // share one. Later row blocks first: under a causal mask they have the most keys.
-  auto alone = [&](Fp4Unit* u) FP4_INLINE {
-    const int at = ((share & 7) * p.xcd_units + (share >> 3)) * NU + wu;
-    const int bk = fp4_quot(at, p.by_rb);
-    u->rb = p.rblocks - 1 - (at - bk * p.rblocks);
-    u->b = fp4_quot(bk, p.by_kvh);
-    u->kvh = bk - u->b * p.KVH;
-    return u->b < p.batch;
+  auto sum_before = [&](int e) FP4_INLINE {
+    if (!regs) return uniform(s_pre[e]);
+    return e == 0 ? 0 : __builtin_amdgcn_readlane(lane_sum, e - 1);
   };
-
-  // The unit holding position q of the list (any lane's own q), in rows a0 .. z0 - 1.
-  auto locate = [&](int q, int a0, int z0) FP4_INLINE {
-    Fp4Unit u;
-    if (list) {
-      int a = a0, z = z0;  // the row: KVH s_pre[a rblocks] <= q < KVH s_pre[z rblocks]
-      while (z - a > 1) {
-        const int m = (a + z) >> 1;
-        if (s_pre[m * p.rblocks] * p.KVH <= q) a = m;
-        else z = m;
-      }
-      u.b = a;
-      const int e0 = a * p.rblocks;
-      const int pre0 = s_pre[e0], per = s_pre[e0 + p.rblocks] - pre0;
-      const int rem = q - pre0 * p.KVH;
-      u.kvh = rem / per;
-      const int in = rem - u.kvh * per;
-      int x = 0, y = p.rblocks;
-      while (y - x > 1) {
-        const int m = (x + y) >> 1;
-        if (s_pre[e0 + m] - pre0 <= in) x = m;
-        else y = m;
-      }
-      u.rb = x;
-      u.u0 = pre0 * p.KVH + u.kvh * per + (s_pre[e0 + x] - pre0);
-    } else {
-      alone(&u);
-      u.u0 = 0;
-    }
-    fp4_extent<ROWS>(p, ctx_of(u.b), u.rb, &u.lo, &u.hi);
+  auto context = [&](int b) FP4_INLINE {
+    if (!list) return uniform(clamped(p.lens[b]));
+    return regs ? __builtin_amdgcn_readlane(lane_ctx, b) : uniform(s_ctx[b]);
+  };
+  auto extents = [&](Fp4Unit& u) FP4_INLINE {
+    fp4_extent<ROWS>(p, u.ctx, u.rb, &u.lo, &u.hi);
     u.first = fp4_first(u.lo);
     u.n = fp4_count(u.lo, u.hi);
-    return u;
   };
-
-  if (c0 >= c1) return;  // (the workgroup as one)
-  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  // locate for one position of the wave: 64 entries of the list at a time, one a lane.
+  // The last of 0 .. len - 1 with (s_pre[from + i stride] - s_pre[from]) mul <= key: 64 entries at a
+  // time, one a lane.
   auto search = [&](int from, int len, int stride, int mul, int key) FP4_INLINE {
-    int lo = 0;  // the last of 0 .. len - 1 with (s_pre[from + lo stride] - s_pre[from]) mul <= key
+    int lo = 0;
     const int base = s_pre[from];
     while (len > 1) {
       const int step = (len + 63) >> 6;
@@ -306,32 +286,52 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     }
     return lo;
   };
-  auto unit_at = [&](int q) FP4_INLINE {
-    Fp4Unit u;
-    if (list) {
-      u.b = search(0, p.batch, p.rblocks, p.KVH, q);
-      const int e0 = u.b * p.rblocks;
-      const int pre0 = uniform(s_pre[e0]), per = uniform(s_pre[e0 + p.rblocks]) - pre0;
-      const int rem = q - pre0 * p.KVH;
-      u.kvh = uniform(rem / per);
-      const int in = rem - u.kvh * per;
-      u.rb = p.rblocks == 1 ? 0 : search(e0, p.rblocks, 1, 1, in);
-      u.u0 = pre0 * p.KVH + u.kvh * per + (uniform(s_pre[e0 + u.rb]) - pre0);
-    } else {
-      alone(&u);
-      u.u0 = 0;
+  // The unit of the wave that holds position c0 of the list.
+  Fp4Unit u{};
+  if (list) {
+    u.b = regs ? __popcll(__ballot(lane < p.batch - 1 && lane_sum * p.KVH <= c0))
+               : search(0, p.batch, p.rblocks, p.KVH, c0);
+    const int e0 = u.b * p.rblocks;
+    const int pre0 = sum_before(e0), per = sum_before(e0 + p.rblocks) - pre0;
+    const int rem = c0 - pre0 * p.KVH;
+    u.kvh = rem / per;
+    const int in = rem - u.kvh * per;
+    u.rb = p.rblocks == 1 ? 0 : search(e0, p.rblocks, 1, 1, in);
+    u.u0 = pre0 * p.KVH + u.kvh * per + (sum_before(e0 + u.rb) - pre0);
+    u.ctx = context(u.b);
+    extents(u);
+  } else {
+    // Without a list. Workgroup i runs on XCD i % 8, each of which has an L2 of its own: an XCD takes
+    // a run of units, so that the row blocks of a head, which read the same keys, share one. Later
+    // row blocks first: under a causal mask they have the most keys.
+    const int at = ((share & 7) * p.xcd_units + (share >> 3)) * NU + wu;
+    const int bk = fp4_quot(at, p.by_rb);
+    const int b = fp4_quot(bk, p.by_kvh);
+    if (b < p.batch) {  // (waves past the last unit go on to the barriers, with one of no groups)
+      u.rb = p.rblocks - 1 - (at - bk * p.rblocks);
+      u.b = b;
+      u.kvh = bk - b * p.KVH;
+      u.ctx = context(b);
+      extents(u);
     }
-    fp4_extent<ROWS>(p, uniform(ctx_of(u.b)), u.rb, &u.lo, &u.hi);
-    u.first = fp4_first(u.lo);
-    u.n = fp4_count(u.lo, u.hi);
-    return u;
+    c1 = u.n;
+  }
+  const bool head = u.u0 < c0 || u.u0 + u.n > c1;  // the first unit has other shares
+  if (list && tid == 0) {
+    s_first[0] = u.b; s_first[1] = u.kvh; s_first[2] = u.rb; s_first[3] = u.u0; s_first[4] = u.n;
+  }
+  // The next unit of the list (the caller knows that there is one).
+  auto advance = [&](Fp4Unit& u) FP4_INLINE {
+    u.u0 += u.n;
+    if (++u.rb == p.rblocks) {
+      u.rb = 0;
+      if (++u.kvh == p.KVH) {
+        u.kvh = 0;
+        u.ctx = context(++u.b);
+      }
+    }
+    extents(u);
   };
-  Fp4Unit u{}, any;
-  // (waves past the last unit go on to the barriers, with a unit of no groups)
-  if (list || alone(&any)) u = unit_at(c0);
-  if (!list) c1 = u.n;
-  const int b_first = u.b;
-  const int b_end = c1 <= u.u0 + u.n ? u.b + 1 : unit_at(c1 - 1).b + 1;  // the share's rows
 
   // ---- what a lane holds of a tile: fixed places, one register each ----
   uint32_t k_at[HV], ks_at[HV], v_at[HV], vs_at[HV];
@@ -358,19 +358,29 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   // The wave takes positions c0 + wk + WK s of the share. Places of the tiles of its 32 groups from s =
   // base on: lane i holds tile i's byte offset, and bit i of `holes` says that the table has none
   // (the offset is then one that can be read).
+  Fp4Unit ahead = u;  // the unit that the last places reached
   auto places = [&](int base, uint64_t* holes) FP4_INLINE {
-    const int q = c0 + wk + WK * (base + (lane >> 1));
-    int64_t at = -1;
-    if (q < c1) {
-      const Fp4Unit v = locate(q, b_first, b_end);
-      const int tile = 2 * (v.first + q - v.u0) + (lane & 1);
-      const int pg = fp4_quot(tile, p.by_tiles);
-      if (tile * kFp4Tile < v.hi && pg < p.W) {
-        const int phys = p.table[static_cast<int64_t>(v.b) * p.W + pg];
-        if (phys >= 0 && phys < p.num_blocks)
-          at = static_cast<int64_t>(phys) * p.blk_stride + static_cast<int64_t>(v.kvh) * p.head_stride +
-               static_cast<int64_t>(tile - pg * (p.bs / kFp4Tile)) * fp4_tile_bytes(p.D);
+    const int q0 = c0 + wk + WK * base, q = q0 + WK * (lane >> 1), q_end = min(c1, q0 + WK * 32);
+    int tile = 0, hi = 0;
+    int64_t row = 0, head = 0;
+    for (;;) {
+      const int at = q - ahead.u0;
+      if (at >= 0 && at < ahead.n) {
+        tile = 2 * (ahead.first + at) + (lane & 1);
+        hi = ahead.hi;
+        row = static_cast<int64_t>(ahead.b) * p.W;
+        head = ahead.kvh * p.head_stride;
       }
+      if (ahead.u0 + ahead.n >= q_end) break;
+      advance(ahead);
+    }
+    int64_t at = -1;
+    const int pg = fp4_quot(tile, p.by_tiles);
+    if (q < c1 && tile * kFp4Tile < hi && pg < p.W) {
+      const int phys = p.table[row + pg];
+      if (phys >= 0 && phys < p.num_blocks)
+        at = static_cast<int64_t>(phys) * p.blk_stride + head +
+             static_cast<int64_t>(tile - pg * (p.bs / kFp4Tile)) * fp4_tile_bytes(p.D);
     }
     *holes = __ballot(at < 0);
     return at < 0 ? int64_t(0) : at;
@@ -441,7 +451,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     }
   };
   auto begin = [&]() FP4_INLINE {
-    const int ctx = uniform(ctx_of(u.b));
+    const int ctx = u.ctx;
     const int r0 = u.rb * ROWS;
     const int r1 = min(r0 + ROWS, p.rows_per_kvh) - 1;
     const int q0 = ctx - p.q_len + fp4_quot(r0, p.by_g), q1 = ctx - p.q_len + fp4_quot(r1, p.by_g);
@@ -863,7 +873,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   Group ring[kRing];  // the next groups, on their way
   static_for<kRing>([&](auto i) FP4_INLINE { load(ring[i], i); });
   if (rounds > 32) next = places(32, &next_holes);
-  const bool head = u.u0 < c0 || u.u0 + u.n > c1;  // the first unit has other shares
+  lds_barrier();  // (the counters are set)
   int s = 0, turn = 0;  // the wave's next group, and where in the ring it is
   for (;;) {
     begin();
@@ -884,6 +894,15 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         }
       });
       turn = turn == kRing - 1 ? 0 : turn + 1;
+      if constexpr (MSATTN_FP4_BALANCE && WK == kFp4Waves && CT == 1) {
+        // Of a SIMD's two waves the older one's loads are served first: the one that is not ahead
+        // issues at a raised priority.
+        __hip_atomic_store(&s_prog[w], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        const int other = uniform(__hip_atomic_load(&s_prog[w ^ 4], __ATOMIC_RELAXED,
+                                                    __HIP_MEMORY_SCOPE_WORKGROUP));
+        if (s <= other) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+      }
     }
     if constexpr (WK != kFp4Waves) {
       finish(u, true);
@@ -891,7 +910,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     }
     const Fp4Unit done = u;
     if (end < c1) {
-      u = unit_at(end);
+      advance(u);
       query();
     }
     finish(done, end == c1);
@@ -905,7 +924,12 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   // after them. A unit's counter is its first share's, which no other unit split has.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   lds_barrier();
-  const Fp4Unit first = unit_at(c0);
+  Fp4Unit first{};
+  first.b = uniform(s_first[0]);
+  first.kvh = uniform(s_first[1]);
+  first.rb = uniform(s_first[2]);
+  first.u0 = uniform(s_first[3]);
+  first.n = uniform(s_first[4]);
   if (tid < 2) {
     const Fp4Unit& v = tid == 0 ? first : u;
     const int mine = tid == 0 ? head && first.u0 != u.u0 : tail;
