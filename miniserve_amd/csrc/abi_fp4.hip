@@ -97,8 +97,8 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   p->slot_rows = static_cast<int>(std::min<int64_t>(per, rows));
   const int64_t want = 256;  // workgroups: one a CU
   int64_t groups = max_ctx / kFp4Group + 1;  // of a unit, at most
-  p->split = batch * rblocks <= kFp4MaxEntries && units * groups < (int64_t(1) << 31);
-  p->shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, units * groups)));
+  p->split = batch * rblocks <= kFp4MaxEntries && units * (groups + kFp4Head) < (int64_t(1) << 30);
+  p->shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, units * (groups + kFp4Head))));
   const size_t slots = p->split ? 2 * static_cast<size_t>(p->shares) * p->slot_rows : 0;
   p->ml_off = up256((kHdrTickets + kMaxTickets) * sizeof(int));
   p->acc_off = p->ml_off + up256(slots * 2 * sizeof(float));
@@ -112,19 +112,34 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   // 145 groups, wk = 1, 2, 4, 8 and the list, 191, 103, 104, 126, 161 us; 896 of 65, causal, 70, 40, 42,
   // 62, 231; 4096 of 33, causal, 96, 85, 109, 190, 332. Units of few rows take all waves of a workgroup,
   // and only where no CU gets two (their contexts may differ; 64 of 64 groups, 14 us against 20).
-  const double load = static_cast<double>(units) / want;
   const double mean = groups - (causal && window == 0 ? 0.5 * std::min(q_len, max_ctx) / kFp4Group : 0.0);
-  double best = p->split ? units * mean / (want * kFp4Waves) + 10 * (load + 1) : 1e300;
+  double best = p->split ? units * mean / (want * kFp4Waves) + 10 * (static_cast<double>(units) / want + 1)
+                         : 1e300;
   p->wk = kFp4Waves;
-  for (int wk = kFp4Waves; wk >= (p->ct == 1 ? kFp4Waves : 1); wk /= 2) {
+  auto consider = [&](int ct, int wk, double round) {  // round: of a group of 16 ct rows
+    const int64_t blocks = (rows + 16 * ct - 1) / (16 * ct);
+    const double load = static_cast<double>(batch * blocks * KVH) / want;
     const double longest = ceil(static_cast<double>(groups) / wk) + 3, rounds = load * wk / kFp4Waves;
-    const double cost = rounds <= 1 ? longest : rounds * (mean / wk + 3) + 0.5 * longest;
-    if (cost > best || (rounds > 1 && p->ct == 1 && p->split)) continue;
+    const double cost = round * (rounds <= 1 ? longest : rounds * (mean / wk + 3) + 0.5 * longest);
+    if (cost > best || (rounds > 1 && ct == 1 && p->split)) return;
     best = cost;
+    p->ct = ct;
     p->wk = wk;
     p->split = 0;
+    p->rblocks = static_cast<int>(blocks);
+  };
+  if (p->ct == 1) {
+    consider(1, kFp4Waves, 1.0);
+  } else {
+#ifndef ROUND4
+#define ROUND4 1.8
+#endif
+    for (int wk = kFp4Waves; wk >= 1; wk /= 2) consider(2, wk, 1.0);
+    if (q_dtype == MSATTN_BF16 && D <= 128 && rows > 32)
+      for (int wk = 4; wk >= 1; wk /= 2) consider(4, wk, ROUND4);
   }
-  p->xcd_units = static_cast<int>(ceil_div64(ceil_div64(units * p->wk, kFp4Waves), 8));
+  const int64_t dealt = static_cast<int64_t>(batch) * p->rblocks * KVH;  // units
+  p->xcd_units = static_cast<int>(ceil_div64(ceil_div64(dealt * p->wk, kFp4Waves), 8));
   return true;
 }
 

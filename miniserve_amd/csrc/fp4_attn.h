@@ -44,7 +44,12 @@ constexpr int kFp4Group = 32;            // tokens of a group
 constexpr int kFp4MaxEntries = 2048;     // (row, row block) pairs whose shares are planned in LDS
 constexpr int kFp4MaxShares = 4096;      // one arrival counter each, at most kMaxTickets
 static_assert(kFp4MaxShares <= kMaxTickets, "a counter a share");
-constexpr float kFp4Slack = 8.0f;        // base-2 headroom before a running maximum moves
+// Positions of the list ahead of a unit's groups that hold no work: what its start and end cost a
+// workgroup, in groups.
+#ifndef MSATTN_FP4_HEAD
+#define MSATTN_FP4_HEAD 24
+#endif
+constexpr int kFp4Head = MSATTN_FP4_HEAD;
 
 struct Fp4Params {
   const void* q;
@@ -109,32 +114,41 @@ __device__ __forceinline__ void fp4_store4(T* o, float a, float b, float c, floa
   else *reinterpret_cast<uint2*>(o) = make_uint2(Pack2<T>::pack(a, b), Pack2<T>::pack(c, d));
 }
 
-#ifndef MSATTN_FP4_NT
-#define MSATTN_FP4_NT 0
+#ifndef MSATTN_FP4_BALANCE_EVERY
+#define MSATTN_FP4_BALANCE_EVERY 1
 #endif
 #ifndef MSATTN_FP4_BALANCE
 #define MSATTN_FP4_BALANCE 1
 #endif
+#ifndef MSATTN_FP4_RING4
+#define MSATTN_FP4_RING4 1
+#endif
 #ifndef MSATTN_FP4_RING
 #define MSATTN_FP4_RING 3
 #endif
+// A lane's bytes of a tile, through the tile's descriptor. (Nontemporal loads took 61 -> 73 us on 64
+// rows of H32/KVH8/D128: a tile's first and last lines are its neighbours' too.)
 template <typename V>
-__device__ __forceinline__ V fp4_load(const uint8_t* p) {
-#if MSATTN_FP4_NT
+__device__ __forceinline__ V fp4_load(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+  const int off = static_cast<int>(at);
   if constexpr (sizeof(V) == 16) {
-    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-    const u4 x = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p));
+    const mf_u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
     return V{x.x, x.y, x.z, x.w};
   } else if constexpr (sizeof(V) == 8) {
     typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-    const u2 x = __builtin_nontemporal_load(reinterpret_cast<const u2*>(p));
+    const u2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
     return V{x.x, x.y};
+  } else if constexpr (sizeof(V) == 4) {
+    return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
   } else {
-    return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    return __builtin_amdgcn_raw_buffer_load_b8(r, off, 0, 0);
   }
-#else
-  return *reinterpret_cast<const V*>(p);
-#endif
+}
+
+// The power of two of byte i of w, as the widening instruction takes it: it reads the exponent's bits
+// alone (checked on all bytes, whatever the others).
+__device__ __forceinline__ float fp4_scale_of(uint32_t w, int i) {
+  return __uint_as_float(i == 0 ? w << 23 : i == 1 ? w << 15 : i == 2 ? w << 7 : w >> 1);
 }
 
 // Keys a query row, and a block of rows, may see, and a unit's place in the work list.
@@ -144,6 +158,8 @@ struct Fp4Unit {
   int lo, hi;        // keys that some row of the block sees
   int first, n;      // its groups of keys
   int u0;            // position of its first group in the list
+  // Of the share: the unit's groups skip .. skip + cnt - 1, which are the share's r0 .. r0 + cnt - 1
+  int skip, cnt, r0;
 };
 
 template <int ROWS>
@@ -171,7 +187,9 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   constexpr int LD = DH / 4;             // dims a lane receives of a half
   constexpr int PQ = fp4_parts<T>();
   constexpr int ROWS = 16 * CT;
-  constexpr int kRing = DP == 256 || (CT == 2 && PQ == 3) ? 2 : MSATTN_FP4_RING;
+  constexpr bool QLDS = CT == 4;         // the query's operands in LDS, where a unit's waves share them
+  constexpr int kRing = QLDS ? MSATTN_FP4_RING4 : DP == 256 || (CT == 2 && PQ == 3) ? 2 : MSATTN_FP4_RING;
+  constexpr bool kEarly = QLDS;          // keys of the group after requested before its values
   typedef typename std::conditional<DH == 128, uint4, uint2>::type kraw_t;
 
   __shared__ int s_pre[kFp4MaxEntries + 1];
@@ -180,7 +198,9 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   // The waves' accumulators of up to 16 rows of a unit, [buffer][wave][rows][RS] (RS: the rows of a
   // store fall on different banks), and their maxima and sums. Fewer rows leave more buffers.
   constexpr int RS = DP + 4;
-  __shared__ float s_acc[kFp4Waves * 16 * RS];
+  constexpr int kAccWords = kFp4Waves * 16 * RS, kQueryWords = QLDS ? kFp4Waves / WK * CT * HV * NJ * 64 * 4 : 0;
+  __shared__ __attribute__((aligned(16))) float
+      s_acc[kAccWords > kQueryWords ? kAccWords : kQueryWords];  // (and the query's operands before)
   __shared__ float2 s_ml[kFp4Waves * 16];
   __shared__ int s_prog[kFp4Waves];  // groups that a wave has taken
   __shared__ int s_first[5];         // the share's first unit
@@ -220,7 +240,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         lane_ctx = clamped(p.lens[lane]);
         int lo, hi;
         fp4_extent<ROWS>(p, lane_ctx, 0, &lo, &hi);
-        cnt = fp4_count(lo, hi);
+        cnt = fp4_count(lo, hi) + kFp4Head;
       }
       lane_sum = wave_inclusive_sum(cnt);
       sum = __builtin_amdgcn_readlane(lane_sum, 63);
@@ -233,7 +253,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
           if (rb == 0) s_ctx[b] = ctx;
           int lo, hi;
           fp4_extent<ROWS>(p, ctx, rb, &lo, &hi);
-          cnt = fp4_count(lo, hi);
+          cnt = fp4_count(lo, hi) + kFp4Head;
         }
         const int incl = wave_inclusive_sum(cnt);
         if (lane == 63) s_tot[w] = incl;
@@ -252,7 +272,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       sum = uniform(sum);
     }
     const int total = sum * p.KVH;
-    // whole rounds of the waves: a part of one takes as long, and leaves more to join
+    // (whole rounds of the waves)
     chunk = ceil_div(ceil_div(total, p.shares), kFp4Waves) * kFp4Waves;
     c0 = static_cast<int>(min(static_cast<int64_t>(share) * chunk, static_cast<int64_t>(total)));
     c1 = min(c0 + chunk, total);
@@ -297,9 +317,11 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     u.kvh = rem / per;
     const int in = rem - u.kvh * per;
     u.rb = p.rblocks == 1 ? 0 : search(e0, p.rblocks, 1, 1, in);
-    u.u0 = pre0 * p.KVH + u.kvh * per + (sum_before(e0 + u.rb) - pre0);
+    u.u0 = pre0 * p.KVH + u.kvh * per + (sum_before(e0 + u.rb) - pre0) + kFp4Head;
     u.ctx = context(u.b);
     extents(u);
+    u.skip = max(0, c0 - u.u0);
+    u.cnt = min(u.n, c1 - u.u0) - u.skip;
   } else {
     // Without a list. Workgroup i runs on XCD i % 8, each of which has an L2 of its own: an XCD takes
     // a run of units, so that the row blocks of a head, which read the same keys, share one. Later
@@ -314,15 +336,18 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       u.ctx = context(b);
       extents(u);
     }
-    c1 = u.n;
+    c1 = u.cnt = u.n;
   }
-  const bool head = u.u0 < c0 || u.u0 + u.n > c1;  // the first unit has other shares
+  if (list && u.cnt <= 0) return;  // (a share of the head of a unit alone; the workgroup as one)
+  const bool head = u.cnt < u.n;   // the first unit has other shares
   if (list && tid == 0) {
     s_first[0] = u.b; s_first[1] = u.kvh; s_first[2] = u.rb; s_first[3] = u.u0; s_first[4] = u.n;
   }
-  // The next unit of the list (the caller knows that there is one).
+  // Whether the share goes on behind u, and the unit it goes on with.
+  auto more = [&](const Fp4Unit& u) FP4_INLINE { return u.u0 + u.n + kFp4Head < c1; };
   auto advance = [&](Fp4Unit& u) FP4_INLINE {
-    u.u0 += u.n;
+    u.u0 += u.n + kFp4Head;
+    u.r0 += u.cnt;
     if (++u.rb == p.rblocks) {
       u.rb = 0;
       if (++u.kvh == p.KVH) {
@@ -331,7 +356,18 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       }
     }
     extents(u);
+    u.skip = 0;
+    u.cnt = min(u.n, c1 - u.u0);
   };
+  int groups = u.cnt;  // of the share
+  if constexpr (WK == kFp4Waves) {
+    if (more(u)) {
+      Fp4Unit v = u;
+      do advance(v);
+      while (more(v));
+      groups = v.r0 + v.cnt;
+    }
+  }
 
   // ---- what a lane holds of a tile: fixed places, one register each ----
   uint32_t k_at[HV], ks_at[HV], v_at[HV], vs_at[HV];
@@ -355,72 +391,93 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   };
   typedef Tile Group[2];
 
-  // The wave takes positions c0 + wk + WK s of the share. Places of the tiles of its 32 groups from s =
-  // base on: lane i holds tile i's byte offset, and bit i of `holes` says that the table has none
-  // (the offset is then one that can be read).
+  // The wave takes the share's groups wk + WK s. Places of the tiles of its 32 groups from s = base on:
+  // lane i holds tile i's byte offset, and bit i of `holes` says that the table has none (the offset
+  // is then one that can be read). The table is asked first, and its answer taken up later.
   Fp4Unit ahead = u;  // the unit that the last places reached
-  auto places = [&](int base, uint64_t* holes) FP4_INLINE {
-    const int q0 = c0 + wk + WK * base, q = q0 + WK * (lane >> 1), q_end = min(c1, q0 + WK * 32);
+  struct Asked {
+    int page;      // as the table has it
+    int64_t rest;  // the tile's bytes from its page's start on
+  };
+  auto ask = [&](int base) FP4_INLINE {
+    const int r_first = wk + WK * base, r = r_first + WK * (lane >> 1);
+    const int r_end = min(groups, r_first + WK * 32);
     int tile = 0, hi = 0;
     int64_t row = 0, head = 0;
     for (;;) {
-      const int at = q - ahead.u0;
-      if (at >= 0 && at < ahead.n) {
-        tile = 2 * (ahead.first + at) + (lane & 1);
+      const int at = r - ahead.r0;
+      if (at >= 0 && at < ahead.cnt) {
+        tile = 2 * (ahead.first + ahead.skip + at) + (lane & 1);
         hi = ahead.hi;
         row = static_cast<int64_t>(ahead.b) * p.W;
         head = ahead.kvh * p.head_stride;
       }
-      if (ahead.u0 + ahead.n >= q_end) break;
+      if (ahead.r0 + ahead.cnt >= r_end) break;
       advance(ahead);
     }
-    int64_t at = -1;
+    Asked x;
+    x.page = -1;
     const int pg = fp4_quot(tile, p.by_tiles);
-    if (q < c1 && tile * kFp4Tile < hi && pg < p.W) {
-      const int phys = p.table[row + pg];
-      if (phys >= 0 && phys < p.num_blocks)
-        at = static_cast<int64_t>(phys) * p.blk_stride + head +
-             static_cast<int64_t>(tile - pg * (p.bs / kFp4Tile)) * fp4_tile_bytes(p.D);
-    }
-    *holes = __ballot(at < 0);
-    return at < 0 ? int64_t(0) : at;
+    x.rest = head + static_cast<int64_t>(tile - pg * (p.bs / kFp4Tile)) * fp4_tile_bytes(p.D);
+    if (tile * kFp4Tile < hi && pg < p.W) x.page = p.table[row + pg];
+    return x;
+  };
+  auto answer = [&](const Asked& x, uint64_t* holes) FP4_INLINE {
+    const bool has = x.page >= 0 && x.page < p.num_blocks;
+    *holes = __ballot(!has);
+    return has ? static_cast<int64_t>(x.page) * p.blk_stride + x.rest : int64_t(0);
   };
   uint64_t holes, next_holes = 0;
   int64_t here, next = 0;  // of this run of 32 groups, and of the next
-  int run = 0;                                 // the run's first
-  const int rounds = (c1 - c0 - wk + WK - 1) / WK;  // groups of the wave
-  auto load = [&](Group& x, int s) FP4_INLINE {  // group s, of this run or the next
+  Asked asked{};           // of the next, until the run's last groups
+  int run = 0;             // the run's first
+  const int rounds = (groups - wk + WK - 1) / WK;  // groups of the wave
+  // Keys (1), values (2) or both (3) of group s, of this run or the next, requested. Values alone come
+  // after the same group's keys.
+  int64_t at[2] = {0, 0};
+  auto load = [&](Group& x, int s, auto parts_c) FP4_INLINE {
+    constexpr int parts = decltype(parts_c)::value;
     if (s >= rounds) return;
-    const int i = 2 * (s - run);
-    auto from = [&](int64_t places, int t) FP4_INLINE {
-      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(places), (i + t) & 63);
-      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(places >> 32), (i + t) & 63);
-      return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-    };
-    int64_t at[2];
-    if (i < 64) {  // (a branch: the next run's places may be on their way)
-      at[0] = from(here, 0);
-      at[1] = from(here, 1);
-    } else {
-      at[0] = from(next, 0);
-      at[1] = from(next, 1);
+    if constexpr ((parts & 1) != 0) {
+      const int i = 2 * (s - run);
+      auto from = [&](int64_t places, int t) FP4_INLINE {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(places), (i + t) & 63);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(places >> 32), (i + t) & 63);
+        return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+      };
+      if (i < 64) {  // (a branch: the next run's places may be on their way)
+        at[0] = from(here, 0);
+        at[1] = from(here, 1);
+      } else {
+        at[0] = from(next, 0);
+        at[1] = from(next, 1);
+      }
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint8_t* const kt = p.k + at[t];
-      const uint8_t* const vt = p.v + at[t];
+      const __amdgpu_buffer_rsrc_t kt = tile_rsrc(p.k + at[t], fp4_tile_bytes(p.D));
+      const __amdgpu_buffer_rsrc_t vt = tile_rsrc(p.v + at[t], fp4_tile_bytes(p.D));
 #pragma unroll
       for (int h = 0; h < HV; ++h) {
-        x[t].k[h] = fp4_load<kraw_t>(kt + k_at[h]);
-        x[t].ks[h] = fp4_load<uint8_t>(kt + ks_at[h]);
-        x[t].v[h] = fp4_load<uint4>(vt + v_at[h]);
-        x[t].vs[h] = fp4_load<uint32_t>(vt + vs_at[h]);
+        if constexpr ((parts & 1) != 0) {
+          x[t].k[h] = fp4_load<kraw_t>(kt, k_at[h]);
+          x[t].ks[h] = fp4_load<uint8_t>(kt, ks_at[h]);
+        }
+        if constexpr ((parts & 2) != 0) {
+          x[t].v[h] = fp4_load<uint4>(vt, v_at[h]);
+          x[t].vs[h] = fp4_load<uint32_t>(vt, vs_at[h]);
+        }
       }
     }
   };
+  using Keys = std::integral_constant<int, 1>;
+  using Values = std::integral_constant<int, 2>;
+  using Both = std::integral_constant<int, 3>;
 
   // ---- a unit's state ----
-  uint4 qf[CT][HV][NJ][PQ];
+  uint4 qf[QLDS ? 1 : CT][HV][NJ][PQ];
+  static_assert(!QLDS || PQ == 1, "one part a query element");
+  uint4* const s_q = reinterpret_cast<uint4*>(s_acc) + wu * (CT * HV * NJ * 64) + lane;
   mf_f32x4 acc[CT][HV][VC];
   float m_run[CT], l_run[CT];
   int lo_n[CT], hi_n[CT];  // keys the lane's rows see
@@ -471,7 +528,10 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         for (int c = 0; c < VC; ++c) acc[ct][h][c] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          if constexpr (PQ == 1) {
+          if constexpr (QLDS) {  // (the unit's waves hold the same rows: one of them stores each)
+            if ((ct * HV + h) * NJ + j == wk + ((ct * HV + h) * NJ + j) / WK * WK)
+              s_q[((ct * HV + h) * NJ + j) * 64] = q_raw[ct][h][j][0];
+          } else if constexpr (PQ == 1) {
             qf[ct][h][j][0] = q_raw[ct][h][j][0];
           } else {
             float x[8];
@@ -490,24 +550,69 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     }
   };
 
-  // Scores of one tile.
-  auto scores = [&](const Tile& k, mf_f32x4 (&s)[CT]) FP4_INLINE {
+  // Scores of the group's two tiles.
+  auto scores = [&](const Group& x, mf_f32x4 (&s0)[CT], mf_f32x4 (&s1)[CT]) FP4_INLINE {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) s[ct] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int ct = 0; ct < CT; ++ct) s0[ct] = s1[ct] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+    float sc[HV][2];
 #pragma unroll
-    for (int h = 0; h < HV; ++h) {
-      const float sc = fp4_scale(k_in[h] ? k.ks[h] : 127u);
-      static_for<NJ>([&](auto jc) FP4_INLINE {
-        constexpr int j = decltype(jc)::value;
-        uint32_t x;
-        if constexpr (DH == 128) x = j == 0 ? k.k[h].x : j == 1 ? k.k[h].y : j == 2 ? k.k[h].z : k.k[h].w;
-        else x = j == 0 ? k.k[h].x : k.k[h].y;
-        const uint4 ka = make_uint4(fp4_widen2<0>(x, sc), fp4_widen2<1>(x, sc),
-                                    fp4_widen2<2>(x, sc), fp4_widen2<3>(x, sc));
+    for (int h = 0; h < HV; ++h)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
+      for (int t = 0; t < 2; ++t) sc[h][t] = fp4_scale(k_in[h] ? x[t].ks[h] : 127u);
+    // Word i of the 4 of step st (half st / NJ, product st % NJ) of tile t's operand.
+    auto widen = [&](auto step_c, int t, int i) FP4_INLINE {
+      constexpr int st = decltype(step_c)::value, h = st / NJ, j = st % NJ;
+      const kraw_t& r = x[t].k[h];
+      uint32_t w;
+      if constexpr (DH == 128) w = j == 0 ? r.x : j == 1 ? r.y : j == 2 ? r.z : r.w;
+      else w = j == 0 ? r.x : r.y;
+      return i == 0 ? fp4_widen2<0>(w, sc[h][t]) : i == 1 ? fp4_widen2<1>(w, sc[h][t])
+             : i == 2 ? fp4_widen2<2>(w, sc[h][t]) : fp4_widen2<3>(w, sc[h][t]);
+    };
+    if constexpr (!QLDS) {
 #pragma unroll
-          for (int a = 0; a < PQ; ++a) s[ct] = Mfma16<bf16_t>::mac(ka, qf[ct][h][j][a], s[ct]);
+      for (int t = 0; t < 2; ++t)
+        static_for<HV * NJ>([&](auto st_c) FP4_INLINE {
+          constexpr int st = decltype(st_c)::value;
+          const uint4 k = make_uint4(widen(st_c, t, 0), widen(st_c, t, 1), widen(st_c, t, 2), widen(st_c, t, 3));
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int a = 0; a < PQ; ++a) {
+              mf_f32x4& s = t == 0 ? s0[ct] : s1[ct];
+              s = Mfma16<bf16_t>::mac(k, qf[ct][st / NJ][st % NJ][a], s);
+            }
+        });
+    } else {
+      // One read of the query for both tiles, three of them on their way, and the keys of the next
+      // step widened between the products of one (a wave issues in order).
+      constexpr int kAhead = 3, kSteps = HV * NJ;
+      uint32_t k[2][2][4];  // of the step's parity, by tile
+      uint4 qv[kAhead];
+      auto q_at = [&](int i) FP4_INLINE { return s_q[((i % CT * HV + i / CT / NJ) * NJ + i / CT % NJ) * 64]; };
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k[0][i / 4][i % 4] = widen(std::integral_constant<int, 0>{}, i / 4, i % 4);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) qv[i] = q_at(i);
+      static_for<kSteps>([&](auto st_c) FP4_INLINE {
+        constexpr int st = decltype(st_c)::value;
+        const uint4 k0 = make_uint4(k[st & 1][0][0], k[st & 1][0][1], k[st & 1][0][2], k[st & 1][0][3]);
+        const uint4 k1 = make_uint4(k[st & 1][1][0], k[st & 1][1][1], k[st & 1][1][2], k[st & 1][1][3]);
+        int i = 0;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const int n = st * CT + ct;
+          const uint4 q = qv[n % kAhead];
+          s0[ct] = Mfma16<bf16_t>::mac(k0, q, s0[ct]);
+          s1[ct] = Mfma16<bf16_t>::mac(k1, q, s1[ct]);
+          if (n + kAhead < kSteps * CT) qv[n % kAhead] = q_at(n + kAhead);
+          if constexpr (st + 1 < kSteps) {
+#pragma unroll
+            for (; i < 8 * (ct + 1) / CT; ++i)
+              k[(st + 1) & 1][i / 4][i % 4] = widen(std::integral_constant<int, st + 1>{}, i / 4, i % 4);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       });
     }
   };
@@ -580,34 +685,45 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
 #pragma unroll
       for (int t = 0; t < 8; ++t) x[t] >>= sh;
     }
+    // The operands of dims 2 c and 2 c + 1, widened step by step between the products of the two dims
+    // before (a wave issues in order: the matrix core runs while it widens).
+    uint32_t e[2][4], o[2][4], y[2];
+    auto step = [&](auto c_c, int t) FP4_INLINE {
+      constexpr int c = decltype(c_c)::value;
+      y[t & 1] = fp4_widen2<c>(x[t], sc[t]);
+      if (t & 1) {
+        e[c & 1][t / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x05040100u);
+        o[c & 1][t / 2] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302u);
+      }
+    };
+#pragma unroll
+    for (int t = 0; t < 8; ++t) step(std::integral_constant<int, 0>{}, t);
     static_for<VC / 2>([&](auto cc) FP4_INLINE {
       constexpr int c = decltype(cc)::value;
-      uint32_t y[8];
+      const uint4 ea = make_uint4(e[c & 1][0], e[c & 1][1], e[c & 1][2], e[c & 1][3]);
+      const uint4 oa = make_uint4(o[c & 1][0], o[c & 1][1], o[c & 1][2], o[c & 1][3]);
+      constexpr int N = CT * PQ;  // pairs of products
+      int t = 0;
 #pragma unroll
-      for (int t = 0; t < 8; ++t) y[t] = fp4_widen2<c>(x[t], sc[t]);
-      uint32_t e[4], o[4];
+      for (int i = 0; i < N; ++i) {
+        const int ct = i / PQ, a = i % PQ;
+        acc[ct][h][2 * c] = Mfma16<bf16_t>::mac(ea, b[ct][a], acc[ct][h][2 * c]);
+        acc[ct][h][2 * c + 1] = Mfma16<bf16_t>::mac(oa, b[ct][a], acc[ct][h][2 * c + 1]);
+        if constexpr (c + 1 < VC / 2) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        e[t] = __builtin_amdgcn_perm(y[2 * t + 1], y[2 * t], 0x05040100u);
-        o[t] = __builtin_amdgcn_perm(y[2 * t + 1], y[2 * t], 0x07060302u);
-      }
-      const uint4 ea = make_uint4(e[0], e[1], e[2], e[3]), oa = make_uint4(o[0], o[1], o[2], o[3]);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int a = 0; a < PQ; ++a) {
-          acc[ct][h][2 * c] = Mfma16<bf16_t>::mac(ea, b[ct][a], acc[ct][h][2 * c]);
-          acc[ct][h][2 * c + 1] = Mfma16<bf16_t>::mac(oa, b[ct][a], acc[ct][h][2 * c + 1]);
+          for (; t < 8 * (i + 1) / N; ++t) step(std::integral_constant<int, c + 1>{}, t);
         }
+        if constexpr (CT > 1) __builtin_amdgcn_sched_barrier(0);
+      }
     });
   };
   auto byte_of = [](uint32_t x, int i) { return (x >> (8 * i)) & 255u; };
 
   auto consume = [&](Group& x, int s) FP4_INLINE {
-    const int tok = (u.first + c0 + wk + WK * s - u.u0) * kFp4Group;
+    const int tok = (u.first + u.skip + wk + WK * s - u.r0) * kFp4Group;
     mf_f32x4 s0[CT], s1[CT];
-    scores(x[0], s0);
-    scores(x[1], s1);
+    scores(x, s0, s1);
+    if constexpr (kEarly) load(x, s + kRing, Keys{});  // (the keys' registers are free)
     const uint32_t hole = static_cast<uint32_t>(holes >> (2 * (s - run))) & 3u;
     const bool full = tok >= all_lo && tok + kFp4Group <= all_hi && hole == 0;
     float mul = p.scale_log2;
@@ -659,8 +775,8 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       float sc[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sc[i] = fp4_scale(byte_of(x[0].vs[h], i));
-        sc[4 + i] = fp4_scale(byte_of(x[1].vs[h], i));
+        sc[i] = fp4_scale_of(x[0].vs[h], i);
+        sc[4 + i] = fp4_scale_of(x[1].vs[h], i);
       }
       product(hc, x[0].v[h], x[1].v[h], sc, pw);
     });
@@ -716,8 +832,8 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   };
   auto fold = [&](const Fp4Unit& u, int r0, int buf, int rows, int t0, int threads) FP4_INLINE {
     const int per = p.D / 4;  // items of a row
-    const bool whole = u.u0 >= c0 && u.u0 + u.n <= c1;
-    const int64_t slot = 2 * static_cast<int64_t>(share) + (u.u0 >= c0 ? 1 : 0);
+    const bool whole = u.cnt == u.n;
+    const int64_t slot = 2 * static_cast<int64_t>(share) + (u.skip == 0 ? 1 : 0);
     for (int idx = t0; idx < rows * per; idx += threads) {
       const int r = fp4_quot(idx, p.by_per), d = 4 * (idx - r * per);
       float2 ml[WK];
@@ -868,33 +984,35 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   };
 
   // ---- the share ----
+  asked = ask(0);
   query();
-  here = places(0, &holes);
+  here = answer(asked, &holes);
   Group ring[kRing];  // the next groups, on their way
-  static_for<kRing>([&](auto i) FP4_INLINE { load(ring[i], i); });
-  if (rounds > 32) next = places(32, &next_holes);
+  static_for<kRing>([&](auto i) FP4_INLINE { load(ring[i], i, Both{}); });
+  if (rounds > 32) asked = ask(32);
   lds_barrier();  // (the counters are set)
   int s = 0, turn = 0;  // the wave's next group, and where in the ring it is
   for (;;) {
     begin();
-    const int end = min(c1, u.u0 + u.n);
-    const int s_end = (end - c0 - wk + WK - 1) / WK;
+    if constexpr (QLDS) lds_barrier();  // (units of their own: each wave comes here once)
+    const int s_end = (u.r0 + u.cnt - wk + WK - 1) / WK;
     for (; s < s_end; ++s) {
+      if (s - run == 32 - kRing) next = answer(asked, &next_holes);
       if (s - run == 32) {
         run = s;
         here = next;
         holes = next_holes;
-        if (rounds > s + 32) next = places(s + 32, &next_holes);
+        if (rounds > s + 32) asked = ask(s + 32);
       }
       // (a copy of the code for each place of the ring: its registers are not moved)
       static_for<kRing>([&](auto i) FP4_INLINE {
         if (turn == i) {
           consume(ring[i], s);
-          load(ring[i], s + kRing);
+          load(ring[i], s + kRing, typename std::conditional<kEarly, Values, Both>::type{});
         }
       });
       turn = turn == kRing - 1 ? 0 : turn + 1;
-      if constexpr (MSATTN_FP4_BALANCE && WK == kFp4Waves && CT == 1) {
+      if (MSATTN_FP4_BALANCE && WK == kFp4Waves && CT == 1 && (s & MSATTN_FP4_BALANCE_EVERY) == 0) {
         // Of a SIMD's two waves the older one's loads are served first: the one that is not ahead
         // issues at a raised priority.
         __hip_atomic_store(&s_prog[w], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -909,16 +1027,17 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       return;
     }
     const Fp4Unit done = u;
-    if (end < c1) {
+    const bool go_on = more(u);
+    if (go_on) {
       advance(u);
       query();
     }
-    finish(done, end == c1);
-    if (end == c1) break;
+    finish(done, !go_on);
+    if (!go_on) break;
   }
 
   // ---- the first and the last unit, where they have other shares ----
-  const bool tail = u.u0 + u.n > c1 || u.u0 < c0;  // (u: the last; perhaps the first too)
+  const bool tail = u.cnt < u.n;  // (u: the last; perhaps the first too)
   if (!head && !tail) return;
   // The partials are written through (agent scope) before the counters move, and read the same way
   // after them. A unit's counter is its first share's, which no other unit split has.
@@ -949,6 +1068,11 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   for (int i = 0; i < 2; ++i) {
     if (i == 0 ? last0 : last1) join(i == 0 ? first : u);
   }
+}
+
+// Column tiles of 16 query rows a wave takes at most.
+template <typename T, int DP> constexpr int fp4_max_ct() {
+  return std::is_same<T, bf16_t>::value && DP <= 128 ? 4 : 2;
 }
 
 template <typename T, int DP>

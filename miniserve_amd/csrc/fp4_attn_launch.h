@@ -16,6 +16,11 @@ static hipError_t fp4_launch(const Fp4Params& p, hipStream_t stream) {
 template <typename T, int DP>
 hipError_t launch_fp4_attn(const Fp4Params& p, int ct, int wk, hipStream_t stream) {
   if (ct == 1) return fp4_launch<T, DP, 1, 8>(p, stream);
+  if constexpr (fp4_max_ct<T, DP>() == 4) {
+    if (ct == 4 && wk == 1) return fp4_launch<T, DP, 4, 1>(p, stream);
+    if (ct == 4 && wk == 2) return fp4_launch<T, DP, 4, 2>(p, stream);
+    if (ct == 4) return fp4_launch<T, DP, 4, 4>(p, stream);
+  }
   switch (wk) {
     case 1: return fp4_launch<T, DP, 2, 1>(p, stream);
     case 2: return fp4_launch<T, DP, 2, 2>(p, stream);
