@@ -18,8 +18,8 @@ import math
 import torch
 
 from . import _native as nat
-from .attention import (_require_gpu, _workspace, block_table_i32, context_lens_i32, narrow_i32,
-                        starts_i32)
+from .attention import (_require_gpu, _workspace, _workspaces, block_table_i32,
+                        context_lens_i32, narrow_i32, starts_i32)
 from .rotary import current, extent, on_device
 
 TILE = 16     # tokens of a tile
@@ -54,7 +54,7 @@ def is_fp4_cache(cache: torch.Tensor) -> bool:
     return cache.dtype == torch.uint8
 
 
-def _cache_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor
+def cache_geometry(k_cache: torch.Tensor, v_cache: torch.Tensor
                     ) -> tuple[int, int, int, int, int, tuple]:
     """(device index, num_blocks, kv_heads, block_size, head_dim, strides) of a pair of 4-bit
     caches, which it checks (all but what the library's entry points check)."""
@@ -101,7 +101,7 @@ def write_kv_fp4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     among them read back as NaN. A row's bytes do not depend on what is written beside it. Two
     tokens of one call must not land in one slot: parts of either's rows may remain there.
     """
-    at, nb, KVH, bs, D, stride = _cache_geometry(k_cache, v_cache)
+    at, nb, KVH, bs, D, stride = cache_geometry(k_cache, v_cache)
     if k.get_device() != at or v.get_device() != at:
         _require_gpu(k, "k")
         _require_gpu(v, "v")
@@ -156,7 +156,7 @@ def read_kv_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table, start
     entry per row, or an int tensor). fp32 and bf16 hold them exactly. Positions on holes, outside
     the table or below 0 give zeros; those past a row's context give whatever its pages hold.
     """
-    _, nb, KVH, bs, D, stride = _cache_geometry(k_cache, v_cache)
+    _, nb, KVH, bs, D, stride = cache_geometry(k_cache, v_cache)
     if dtype not in _TYPES:
         raise ValueError(f"unsupported dtype for a 4-bit cache's values: {dtype}")
     tokens = int(tokens)
@@ -182,6 +182,14 @@ def read_kv_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table, start
     return k, v
 
 
+def _kept_workspace(dev: torch.device, index: int) -> torch.Tensor | None:
+    """The workspace that calls on `dev`'s current stream share (None where there is none yet, and
+    under capture, where a graph gets one of its own)."""
+    if torch._C._cuda_getDevice() != index or torch.cuda.is_current_stream_capturing():
+        return None
+    return _workspaces.get((index, nat.stream_handle(dev)))
+
+
 def paged_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                         block_table, context_lens, *, causal: bool = True,
                         window: int | None = None, scale: float | None = None,
@@ -193,7 +201,7 @@ def paged_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     alone. A view of the query in 16-byte rows is read where it lies. Nothing is read by the host
     where ``context_lens`` is a device tensor, so the call is safe to capture.
     """
-    at, nb, KVH, bs, Dk, stride = _cache_geometry(k_cache, v_cache)
+    at, nb, KVH, bs, Dk, stride = cache_geometry(k_cache, v_cache)
     if query.get_device() != at:
         _require_gpu(query, "query")
         raise ValueError("query and the caches must be on one device")
@@ -245,18 +253,22 @@ def paged_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         query = query.resolve_neg().clone(memory_format=torch.contiguous_format)
         qs = query.stride()
     lib, code = nat.lib(), nat.DTYPE_CODES[dtype]
-    ws_bytes = lib.msattn_fp4_workspace_bytes(B, q_len, H, KVH, D, max_context, code)
-    if ws_bytes == 0:
-        raise ValueError("unsupported attention geometry")
-    if workspace is None or workspace.numel() * workspace.element_size() < ws_bytes:
+    args = (query.data_ptr(), qs[0], qs[1], qs[2], k_cache.data_ptr(), v_cache.data_ptr(),
+            stride[0], stride[1], table.data_ptr(), lens.data_ptr(), out.data_ptr())
+    sizes = (B, q_len, H, KVH, D, bs, nb, W, max_context, 1 if causal else 0,
+             min(window or 0, 2 ** 31 - 1), 1.0 / math.sqrt(D) if scale is None else float(scale),
+             code)
+    status, call = nat.ERR_WORKSPACE, lib.msattn_paged_attention_fp4
+    if workspace is None:  # the stream's, as large as earlier calls needed it
+        workspace = _kept_workspace(dev, at)
+    if workspace is not None:
+        status = on_device(dev, call, *args, workspace.data_ptr(),
+                           workspace.numel() * workspace.element_size(), *sizes)
+    if status == nat.ERR_WORKSPACE:
+        nbytes = lib.msattn_fp4_workspace_bytes(B, q_len, H, KVH, D, max_context, code)
         with current(dev):
-            workspace = _workspace(dev, ws_bytes)
-    status = on_device(
-        dev, lib.msattn_paged_attention_fp4, query.data_ptr(), qs[0], qs[1], qs[2],
-        k_cache.data_ptr(), v_cache.data_ptr(), stride[0], stride[1], table.data_ptr(),
-        lens.data_ptr(), out.data_ptr(), workspace.data_ptr(), ws_bytes, B, q_len, H, KVH, D, bs,
-        nb, W, max_context, 1 if causal else 0, min(window or 0, 2 ** 31 - 1),
-        1.0 / math.sqrt(D) if scale is None else float(scale), code)
+            workspace = _workspace(dev, nbytes)
+        status = on_device(dev, call, *args, workspace.data_ptr(), nbytes, *sizes)
     if status:
         _check("msattn_paged_attention_fp4", status, k_cache, v_cache)
     return out if given is None else given.copy_(out)

@@ -35,6 +35,7 @@ import torch
 
 from . import _native as nat
 from .attention import PagedAttention, paged_attention, paged_attention_append
+from .fp4 import cache_geometry, is_fp4_cache, paged_attention_fp4, write_kv_fp4
 from .rotary import on_16_bytes, rope_table, write_kv_rope
 
 
@@ -89,7 +90,9 @@ class GraphedDecodeRunner:
         which are rotated at each row's new position on the way, in the same launches. The two
         calls round the rotated query to its type, where the one may keep more of its digits
         (paged_attention_append): the same caches, outputs that may differ in the last place. A
-        step that has a position past the tables is refused."""
+        step that has a position past the tables is refused.
+        Layers with 4-bit caches (allocate_fp4_cache) are written and attended over in two calls,
+        whatever fused_append, and take no rope: their keys come rotated."""
         buckets = list(buckets)
         if not buckets or sorted(buckets) != buckets or buckets[0] < 1:
             raise ValueError("buckets must be sorted, start at 1")
@@ -109,10 +112,17 @@ class GraphedDecodeRunner:
         if kc0.device.type != "cuda":
             raise RuntimeError("GraphedDecodeRunner needs caches on a ROCm GPU device")
         self._device = kc0.device
-        self.block_size = kc0.shape[1]
         self.num_heads = pa0.num_heads
-        self.num_kv_heads = kc0.shape[2]
-        self.head_dim = kc0.shape[3]
+        self.fp4 = is_fp4_cache(kc0)
+        if any(is_fp4_cache(layer.k_cache) != self.fp4 for layer in self.layers):
+            raise ValueError("either all layers have 4-bit caches, or none")
+        if self.fp4:
+            if rope is not None:
+                raise ValueError("a 4-bit cache takes rotated keys: no rope")
+            _, _, self.num_kv_heads, self.block_size, self.head_dim, _ = \
+                cache_geometry(kc0, self.layers[0].v_cache)
+        else:
+            self.block_size, self.num_kv_heads, self.head_dim = kc0.shape[1:]
         self.dtype = dtype or pa0.dtype
         L, Bm, H, KVH, D = (len(self.layers), self.max_batch, self.num_heads,
                             self.num_kv_heads, self.head_dim)
@@ -147,8 +157,12 @@ class GraphedDecodeRunner:
         self._stage_ev: list = [None, None]
         self._out = torch.zeros((L, Bm, 1, H, D), dtype=self.dtype, device=dev)
         self.max_context = self.table_width * self.block_size
-        ws_bytes = max(nat.lib().msattn_workspace_bytes(b, 1, H, KVH, D, self.max_context)
-                       for b in self.buckets)
+        if self.fp4:
+            ws_bytes = max(nat.lib().msattn_fp4_workspace_bytes(
+                b, 1, H, KVH, D, self.max_context, nat.dtype_code(self.dtype)) for b in self.buckets)
+        else:
+            ws_bytes = max(nat.lib().msattn_workspace_bytes(b, 1, H, KVH, D, self.max_context)
+                           for b in self.buckets)
         self._ws = torch.zeros(ws_bytes, dtype=torch.uint8, device=dev)
 
     # ---------------------------------------------------------------- step
@@ -158,6 +172,13 @@ class GraphedDecodeRunner:
         start = buf["start"][:bucket]
         lens = buf["lens"][:bucket]
         for li, layer in enumerate(self.layers):
+            if self.fp4:
+                write_kv_fp4(buf["k"][li, :bucket], buf["v"][li, :bucket], layer.k_cache,
+                             layer.v_cache, table, start)
+                paged_attention_fp4(buf["q"][li, :bucket], layer.k_cache, layer.v_cache, table, lens,
+                                    window=layer.pa.window, max_context=self.max_context,
+                                    workspace=self._ws, out=self._out[li, :bucket])
+                continue
             if self.fused_append and buf["k"].dtype == buf["q"].dtype:
                 # write_kv at lens - 1 (= start for real rows; pad rows have lens 0 and
                 # write nothing) and the decode, in one launch where the partition

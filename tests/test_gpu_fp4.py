@@ -17,6 +17,7 @@ import torch
 
 from miniserve_amd import (PagedAttention, _native as nat, allocate_fp4_cache, paged_attention_fp4,
                            read_kv_fp4, write_kv_fp4)
+from miniserve_amd.graphs import DecodeLayer, GraphedDecodeRunner
 from oracle import dense, fp4
 
 pytestmark = pytest.mark.gpu
@@ -232,6 +233,18 @@ CASES = {
     "pages of 256": (8, 2, 64, F16, [513, 600, 1000], 1, 256, True, None),
     "long": (4, 1, 128, BF16, [20000, 11000, 3], 1, 16, True, None),
     "long, fp32": (2, 1, 64, F32, [17700, 30001], 1, 64, True, None),
+    "wide chunk, one a wave": (16, 2, 128, BF16, [700, 640], 600, 16, True, None),
+    "wide chunk, 64 dims": (16, 8, 64, BF16, [300] * 4, 270, 16, True, None),
+    "wide chunk, window": (16, 2, 128, BF16, [700, 90], 300, 32, True, 100),
+    "wide chunk, not causal": (8, 2, 96, BF16, [333, 1000], 200, 16, False, None),
+    "wide chunk, fp32": (16, 2, 128, F32, [500, 430], 400, 16, True, None),
+    "wide chunk, 256 dims": (8, 1, 256, F16, [300, 170], 150, 16, True, None),
+    "drafts in a list": (28, 4, 128, BF16, [2500 - 37 * i for i in range(20)], 3, 16, True, None),
+    "ragged in a list": (32, 8, 64, BF16, [1 + (i * 977) % 3100 for i in range(70)], 1, 16, True, None),
+    "ragged in a list, fp32": (8, 4, 128, F32, [1 + (i * 977) % 3100 for i in range(30)], 1, 16, True, None),
+    "ragged in a list, 256 dims": (4, 4, 256, F16, [1 + (i * 977) % 3100 for i in range(25)], 1, 16, True, None),
+    "ragged in a list, window": (32, 8, 128, F16, [(i * 977) % 5100 for i in range(40)], 2, 16, True, 1500),
+    "16 rows in a list": (16, 1, 64, BF16, [9000, 4000, 12000, 70, 0], 1, 16, True, None),
     "many rows": (8, 8, 64, BF16, [1 + (i * 37) % 150 for i in range(300)], 1, 16, True, None),
 }
 
@@ -395,6 +408,42 @@ def test_captured_and_replayed(device):
             torch.cuda.synchronize()
             got = out.clone()
             assert torch.equal(got, step())
+
+
+def test_graphed_runner(device):
+    """Bucketed graphs over 4-bit caches: three layers, padded buckets, against eager steps."""
+    H, KVH, D, bs, L = 8, 2, 64, 16, 3
+    g = torch.Generator(device).manual_seed(3)
+
+    def layers():
+        out = []
+        for _ in range(L):
+            pa = PagedAttention(H, KVH, D, num_blocks=24, block_size=bs, dtype=BF16, device=device,
+                                kv_dtype=torch.float4_e2m1fn_x2)
+            out.append(DecodeLayer(pa, *pa.allocate_kv_cache()))
+        return out
+
+    pair = [GraphedDecodeRunner(layers(), 6, buckets=(1, 2, 4), dtype=BF16) for _ in range(2)]
+    assert (pair[0].block_size, pair[0].num_kv_heads, pair[0].head_dim) == (bs, KVH, D)
+    tables_ = [[0, 5, 9], [1, 2], [3, 4, 6, 7], [8]]
+    for step, (rows, ctx) in enumerate([((0, 1, 2), [0, 0, 0]), ((0, 1, 2, 3), [1, 1, 1, 0]),
+                                        ((2,), [2]), ((0, 1, 2), [2, 2, 3]), ((3, 0), [1, 3])]):
+        B = len(rows)
+        q = torch.randn(L, B, 1, H, D, device=device, generator=g).to(BF16)
+        k, v = (torch.randn(L, B, 1, KVH, D, device=device, generator=g).to(BF16) for _ in range(2))
+        note(f"runner step {step}")
+        a, b = (r.decode(q, k, v, [tables_[i] for i in rows], ctx, use_graph=use)
+                for r, use in zip(pair, (True, False)))
+        torch.cuda.synchronize()
+        assert torch.equal(a, b)
+        for x, y in zip(pair[0].layers, pair[1].layers):
+            assert torch.equal(x.k_cache, y.k_cache) and torch.equal(x.v_cache, y.v_cache)
+        if ctx[0] == 0:  # one key: its value, as stored
+            want = fp4.values(*fp4.quantise(v[:, 0].cpu()))
+            got = a[:, 0].cpu().double().reshape(L, 1, KVH, H // KVH, D)
+            assert np.array_equal(got.numpy(), np.broadcast_to(want[:, :, :, None], got.shape))
+    with pytest.raises(ValueError, match="no rope"):
+        GraphedDecodeRunner(layers(), 6, dtype=BF16, rope=(torch.ones(9, D), torch.zeros(9, D)))
 
 
 def test_on_another_stream(device):
