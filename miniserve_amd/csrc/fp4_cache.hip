@@ -185,10 +185,30 @@ __global__ __launch_bounds__(kFp4Threads) void write_fp4_kernel(const Fp4CachePa
   }
 }
 
+// Lanes l and l + 4 (bit 2 of l clear) hold dims 32 j .. (a) and 32 (j + 1) .. (b) of two tokens in
+// turn; afterwards l's a and l + 4's a are the first token's 64 dims, and their b the second's.
+__device__ __forceinline__ void swap_halves(uint4& a, uint4& b) {
+  const bool second = (static_cast<int>(threadIdx.x) & 4) != 0;
+  const auto one = [second](uint32_t& x, uint32_t& y) {
+    const int send = static_cast<int>(second ? x : y);
+    const uint32_t from_next =
+        static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, send, 0x104, 0xF, 0xF, true));
+    const uint32_t from_last =
+        static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, send, 0x114, 0xF, 0xF, true));
+    const uint32_t kept = second ? y : x;
+    x = second ? from_last : kept;
+    y = second ? kept : from_next;
+  };
+  one(a.x, b.x);
+  one(a.y, b.y);
+  one(a.z, b.z);
+  one(a.w, b.w);
+}
+
 template <typename T, bool VEC, int NB>
 __global__ __launch_bounds__(kFp4Threads) void read_fp4_kernel(const Fp4CacheParams p) {
   Fp4Item it;
-  if (!fp4_item(p, &it) || !it.live) return;
+  if (!fp4_item(p, &it)) return;  // (a wave at a time; lanes without a token only pass words on)
   const int lane = static_cast<int>(threadIdx.x) & 63, t = lane >> 2, q = lane & 3;
   const int64_t at = it.b * p.k_st[0] + it.t * p.k_st[1] + it.h * p.k_st[2] + 8 * q;
   uint32_t kw[NB], kb[NB], vw[NB], vb[NB];
@@ -215,13 +235,41 @@ __global__ __launch_bounds__(kFp4Threads) void read_fp4_kernel(const Fp4CachePar
       vb[j] = vt[256 * NB + 16 * j + t];
     }
   }
+  // Rows of 16-bit elements leave two blocks a step, so that eight lanes write a line of 128 bytes at
+  // once: with four lanes' 64 bytes a store (what other types and a last odd block do), answers
+  // larger than a cache were read and written back a half line at a time (134 MB in 52.5 us, now
+  // 37.2; 67 MB in 29.5, now 20.3; the same below 34 MB). Stores past the caches were as fast here, and
+  // cost the answer's reader more than that (134 MB read and reduced in 136 us, against 109).
+  constexpr bool kPairs = VEC && sizeof(T) == 2;
+  constexpr int kPaired = kPairs ? NB / 2 * 2 : 0;
+  T* const out[2] = {static_cast<T*>(p.k) + at, static_cast<T*>(p.v) + at};
+  if constexpr (kPairs) {
+    const int second = t & 1;
+    const int64_t from = 32 * second - (second ? p.k_st[1] : 0);
+    const int t0 = it.t - second;
+    const bool live0 = t0 >= 0 && t0 < p.tokens, live1 = t0 + 1 >= 0 && t0 + 1 < p.tokens;
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
+    for (int of = 0; of < 2; ++of)
+#pragma unroll
+      for (int j = 0; j < kPaired; j += 2) {
+        float x[8], y[8];
+        widen8(of ? vw[j] : kw[j], of ? vb[j] : kb[j], x);
+        widen8(of ? vw[j + 1] : kw[j + 1], of ? vb[j + 1] : kb[j + 1], y);
+        uint4 a = Chunk<T>::pack(x), b = Chunk<T>::pack(y);
+        swap_halves(a, b);
+        T* const o = out[of] + from + 32 * j;
+        if (live0) *reinterpret_cast<uint4*>(o) = a;
+        if (live1) *reinterpret_cast<uint4*>(o + p.k_st[1]) = b;
+      }
+  }
+  if (!it.live) return;
+#pragma unroll
+  for (int j = kPaired; j < NB; ++j) {
     float x[8];
     widen8(kw[j], kb[j], x);
-    store8<T, VEC>(static_cast<T*>(p.k) + at + 32 * j, x);
+    store8<T, VEC>(out[0] + 32 * j, x);
     widen8(vw[j], vb[j], x);
-    store8<T, VEC>(static_cast<T*>(p.v) + at + 32 * j, x);
+    store8<T, VEC>(out[1] + 32 * j, x);
   }
 }
 
