@@ -495,7 +495,7 @@ int msattn_write_kv_fp4(const void* k, int64_t k_batch_stride, int64_t k_token_s
  * The values that positions starts[b] .. starts[b] + tokens - 1 of each row stand for, to k and v
  * [batch, tokens, num_kv_heads, head_dim], contiguous, of type dst_dtype (fp32 and bf16 hold them
  * exactly, fp16 rounds them to nearest); positions on holes, outside the table or below 0 give
- * zeros.
+ * zeros. k and v must share no memory with each other or the caches.
  */
 int msattn_read_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_block_stride,
                        int64_t cache_head_stride, const int32_t* block_table,
@@ -514,8 +514,9 @@ size_t msattn_fp4_workspace_bytes(int batch, int q_len, int num_heads, int num_k
 /*
  * msattn_paged_attention over a 4-bit cache: fp32, fp16 or bf16 query, any q_len, causal or not,
  * window as there; one launch. The query's strides are in elements, its rows and the contiguous out
- * 16-byte aligned. Rows without a visible key give zeros; an infinity or
- * NaN reaches the queries that see its key alone. Scores and products take the cache's values
+ * 16-byte aligned; out shares no memory with the query or the caches. max_context is at most 2^30
+ * (MSATTN_ERR_UNSUPPORTED past it). Rows without a visible key give zeros; an infinity or NaN reaches
+ * the queries that see its key alone. Scores and products take the cache's values
  * exactly; the weights of a bf16 query are rounded to bf16, in the numerator and in the sum alike;
  * maxima, sums and accumulators are fp32.
  */

@@ -83,6 +83,15 @@ int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
+// A wave's time for a group with 64 query rows over that with 32: less than twice, since the keys and
+// values are widened once. 512 queries of H28/KVH4/D128 behind 4096 keys, 2 rows: 92 us against 103;
+// 1024 queries of H32/KVH8/D128 by themselves, 4 rows, where half as many units fill the CUs less
+// evenly: 96 against 88, and this factor chooses the latter.
+constexpr double kRound64 = 1.8;
+
+// Contexts go up to this: a position plus a query's offset or a window fits 31 bits.
+constexpr int kMaxContext = 1 << 30;
+
 // Workspace does not depend on causal and window.
 bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causal,
              int window, int q_dtype, Plan* p) {
@@ -92,10 +101,10 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   const int per = 16 * p->ct;
   const int64_t rblocks = (rows + per - 1) / per;
   const int64_t units = batch * rblocks * KVH;
-  if (rows >= (int64_t(1) << 30) || units >= (int64_t(1) << 30)) return false;
+  if (rows >= (int64_t(1) << 30) || units >= (int64_t(1) << 30) || max_ctx > kMaxContext) return false;
   p->rblocks = static_cast<int>(rblocks);
   p->slot_rows = static_cast<int>(std::min<int64_t>(per, rows));
-  const int64_t want = 256;  // workgroups: one a CU
+  const int64_t want = kFp4Shares;  // workgroups: one a CU
   int64_t groups = max_ctx / kFp4Group + 1;  // of a unit, at most
   p->split = batch * rblocks <= kFp4MaxEntries && units * (groups + kFp4Head) < (int64_t(1) << 30);
   p->shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, units * (groups + kFp4Head))));
@@ -131,12 +140,9 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   if (p->ct == 1) {
     consider(1, kFp4Waves, 1.0);
   } else {
-#ifndef ROUND4
-#define ROUND4 1.8
-#endif
     for (int wk = kFp4Waves; wk >= 1; wk /= 2) consider(2, wk, 1.0);
     if (q_dtype == MSATTN_BF16 && D <= 128 && rows > 32)
-      for (int wk = 4; wk >= 1; wk /= 2) consider(4, wk, ROUND4);
+      for (int wk = 4; wk >= 1; wk /= 2) consider(4, wk, kRound64);
   }
   const int64_t dealt = static_cast<int64_t>(batch) * p->rblocks * KVH;  // units
   p->xcd_units = static_cast<int>(ceil_div64(ceil_div64(dealt * p->wk, kFp4Waves), 8));

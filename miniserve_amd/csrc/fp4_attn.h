@@ -2,15 +2,24 @@
 //
 // A unit is a (batch row, KV head, block of up to 16 CT query rows); rows are the pairs (query
 // token i, head g of the KV head's group) r = i G + g. Its keys are cut into groups of 32 tokens
-// (two tiles), and all groups of all units, in order, are dealt in equal contiguous shares, one a
-// workgroup, whatever the lengths (read on the device, so a call is capture-safe). A share's part of a
-// unit leaves, for each query row,
+// (two tiles). A workgroup has 8 waves, two a SIMD, and units come to it in one of two ways
+// (plan_of in abi_fp4.hip chooses, by what each costs):
+//   list   all groups of all units, in order, a unit's behind kFp4Head empty positions, are cut
+//          into one contiguous share a CU, whatever the lengths (read on the device, so a call is
+//          capture-safe). A workgroup's waves take its share's groups in turn, and go on from unit
+//          to unit without waiting for each other. For few long rows, and ragged ones: 64 rows of 1024 to
+//          8192 keys of H32/KVH8/D128 take 49.6 us, 4.4 TB/s of the cache, 5.4 to 6.8 inside a share.
+//   dealt  a unit is whole: WK waves take its groups in turn, and 8 / WK units share a workgroup.
+//          For chunks of prompts, with thousands of units: no partials and no joins.
+// What a wave or a share leaves of a unit is, for each query row,
 //   m,  l = sum_j 2^(s_j - m),  acc = sum_j 2^(s_j - m) V_j,   s_j = scale log2(e) q.K_j
-// over its visible keys; a unit that lies within one share is normalised and written, the shares of
-// another leave partials, and the last of them to arrive joins them.
+// over its visible keys. The waves' parts are joined in LDS; a unit that lies within one share is then
+// normalised and written, the shares of another leave partials in the workspace, and the last of them
+// to arrive joins them.
 //
 // A wave loads a tile's keys and values straight into the registers of the matrix operands, 16
-// bytes a lane, contiguous (fp4_cache.h), two groups ahead. Lane (g, n) = (l / 16, l % 16):
+// bytes a lane, contiguous (fp4_cache.h); the next kRing groups are on their way while it works on
+// one. Lane (g, n) = (l / 16, l % 16):
 //   * S^T = K Q^T on v_mfma_f32_16x16x32_bf16: the lane holds 32 dims of key n of the tile (at
 //     D = 128), widened by v_cvt_scalef32_pk_bf16_fp4, which is exact, and the same dims of query
 //     row n; it receives row n's scores of keys 4 g .. 4 g + 3 of the tile.
@@ -21,9 +30,17 @@
 // The scaled 4-bit matrix instructions are not used: with an e4m3 operand beside the 4-bit one,
 // sums of 128 products came out up to 9e-5 of the sum of magnitudes off, bf16 ones exactly rounded.
 //
+// What bounds it. A decode: the cache's bytes in the middle of a share, and about 7 us of start (the
+// plan, the table, the first tiles) and end (parts and joins) around it, all there is to a small call.
+// A chunk: the widening. A tile is widened once for each unit that reads it, so units of few rows spend
+// their time on it: with 64 rows a wave (CT = 4, their query in LDS) 512 queries of H28/KVH4/D128 behind
+// 4096 keys, two rows of them, take 90 us, with 32 in registers 103; matrix instructions issue for 26 %
+// of that time, vector ones for 45 %.
+//
 // fp16 and fp32 queries, and their weights, enter the products as 2 and 3 bf16 parts, which hold
 // all their digits (for a weight, 16 and 24 of them); a bf16 query's weights are rounded to bf16
-// once, in the numerator and in the sum alike. Maxima, sums and accumulators are fp32.
+// once, in the numerator and in the sum alike. Maxima, sums and accumulators are fp32. (The chunk
+// above: fp16 147 us, fp32 219.)
 //
 // A masked key's score is -inf, and where a group has masked keys, values that some row must not see
 // are taken as zeros, and their NaN, if any, is given to the rows that do see them.
@@ -42,14 +59,13 @@ constexpr int kFp4Waves = 8;             // waves of a workgroup, two a SIMD
 constexpr int kFp4Threads = 64 * kFp4Waves;
 constexpr int kFp4Group = 32;            // tokens of a group
 constexpr int kFp4MaxEntries = 2048;     // (row, row block) pairs whose shares are planned in LDS
-constexpr int kFp4MaxShares = 4096;      // one arrival counter each, at most kMaxTickets
-static_assert(kFp4MaxShares <= kMaxTickets, "a counter a share");
+constexpr int kFp4Shares = 256;          // of a list, at most: one a CU, an arrival counter each
+static_assert(kFp4Shares <= kMaxTickets, "a counter a share");
 // Positions of the list ahead of a unit's groups that hold no work: what its start and end cost a
-// workgroup, in groups.
-#ifndef MSATTN_FP4_HEAD
-#define MSATTN_FP4_HEAD 24
-#endif
-constexpr int kFp4Head = MSATTN_FP4_HEAD;
+// workgroup, in groups. Without them a share of many short units ends last: 64 rows of H32/KVH8/D128
+// with 1024 to 8192 keys, 0, 8, 24 and 48 of them, 58.0, 53.0, 49.6 and 51.6 us; 16 rows of 16384 keys
+// each, where every share has the same, 56.3, 60.3, 59.3 and 59.5.
+constexpr int kFp4Head = 24;
 
 struct Fp4Params {
   const void* q;
@@ -123,18 +139,6 @@ __device__ __forceinline__ void fp4_store4(T* o, float a, float b, float c, floa
   else *reinterpret_cast<uint2*>(o) = make_uint2(Pack2<T>::pack(a, b), Pack2<T>::pack(c, d));
 }
 
-#ifndef MSATTN_FP4_BALANCE_EVERY
-#define MSATTN_FP4_BALANCE_EVERY 1
-#endif
-#ifndef MSATTN_FP4_BALANCE
-#define MSATTN_FP4_BALANCE 1
-#endif
-#ifndef MSATTN_FP4_RING4
-#define MSATTN_FP4_RING4 1
-#endif
-#ifndef MSATTN_FP4_RING
-#define MSATTN_FP4_RING 3
-#endif
 // A lane's bytes of a tile, through the tile's descriptor. (Nontemporal loads took 61 -> 73 us on 64
 // rows of H32/KVH8/D128: a tile's first and last lines are its neighbours' too.)
 template <typename V>
@@ -197,8 +201,10 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   constexpr int PQ = fp4_parts<T>();
   constexpr int ROWS = 16 * CT;
   constexpr bool QLDS = CT == 4;         // the query's operands in LDS, where a unit's waves share them
-  constexpr int kRing = QLDS ? MSATTN_FP4_RING4 : DP == 256 || (CT == 2 && PQ == 3) ? 2 : MSATTN_FP4_RING;
-  constexpr bool kEarly = QLDS;          // keys of the group after requested before its values
+  // Groups on their way while one is worked on: as many as the registers hold. With CT = 4 one, its
+  // keys requested as soon as the group before has used its own, before that one's softmax.
+  constexpr int kRing = QLDS ? 1 : DP == 256 || (CT == 2 && PQ == 3) ? 2 : 3;
+  constexpr bool kEarly = QLDS;
   typedef typename std::conditional<DH == 128, uint4, uint2>::type kraw_t;
 
   __shared__ int s_pre[kFp4MaxEntries + 1];
@@ -1021,7 +1027,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         }
       });
       turn = turn == kRing - 1 ? 0 : turn + 1;
-      if (MSATTN_FP4_BALANCE && WK == kFp4Waves && CT == 1 && (s & MSATTN_FP4_BALANCE_EVERY) == 0) {
+      if (WK == kFp4Waves && CT == 1 && (s & 1) == 0) {
         // Of a SIMD's two waves the older one's loads are served first: the one that is not ahead
         // issues at a raised priority.
         __hip_atomic_store(&s_prog[w], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);

@@ -62,7 +62,8 @@ def attend_args(**over):
     (dict(ws=(1 << 20) + 64), 1), (dict(q_len=0), 1), (dict(H=0), 1), (dict(H=3), 1),
     (dict(max_context=-1), 1), (dict(window=-1), 1), (dict(scale=float("nan")), 1),
     (dict(q0=1028), 1), (dict(q2=132), 1),
-    (dict(ws_bytes=1024), 3), (dict(q_len=1 << 29), 2)], ids=named)
+    (dict(ws_bytes=1024), 3), (dict(q_len=1 << 29), 2),
+    (dict(max_context=(1 << 30) + 1), 2)], ids=named)
 def test_attention_refuses(bad, status):
     assert nat.lib().msattn_paged_attention_fp4(*attend_args(**bad)) == status
 

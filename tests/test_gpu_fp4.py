@@ -3,7 +3,7 @@
 Tolerance of the attention. The cache's values are exact. Scores are fp32 sums of exact products:
 off by at most |ds| = (P D + 8) 2^-24 scale |q||k| (P products of bf16 parts a dim, their additions,
 the scale), so a weight is off by a factor e^(2 |ds|). The weights of a bf16 query are rounded once,
-in numerator and sum alike (u = 2^-9); of an fp16 one they lose at most 2^-15 to its two parts, of an
+in numerator and sum alike (u = 2^-8); of an fp16 one they lose at most 2^-15 to its two parts, of an
 fp32 one nothing. Sums over n keys go in steps of 32: (n / 32 + 40) 2^-23; the hardware's 2^x, its
 argument and the joins 2^-18, as for the 16-bit caches. The output is rounded once. Outputs are
 weighted means of V: the whole is at most
@@ -245,6 +245,12 @@ CASES = {
     "ragged in a list, 256 dims": (4, 4, 256, F16, [1 + (i * 977) % 3100 for i in range(25)], 1, 16, True, None),
     "ragged in a list, window": (32, 8, 128, F16, [(i * 977) % 5100 for i in range(40)], 2, 16, True, 1500),
     "16 rows in a list": (16, 1, 64, BF16, [9000, 4000, 12000, 70, 0], 1, 16, True, None),
+    "two row blocks in a list": (8, 2, 64, BF16, [9000, 3000, 5, 0], 10, 16, True, None),
+    "row blocks in a list, fp32": (12, 2, 96, F32, [5000, 7100], 17, 32, True, None),
+    "row blocks in a list, window": (8, 2, 128, BF16, [9000, 4100], 11, 16, True, 3500),
+    "row blocks in a list, 192 dims": (8, 1, 192, F16, [6000, 4100], 9, 16, False, None),
+    "more rows than a list takes": (1, 1, 64, BF16, [(i * 37) % 70 for i in range(2100)], 1, 16, True, None),
+    "more rows than a list takes, drafts": (7, 1, 32, F16, [(i * 37) % 50 for i in range(2100)], 3, 16, True, None),
     "many rows": (8, 8, 64, BF16, [1 + (i * 37) % 150 for i in range(300)], 1, 16, True, None),
 }
 
@@ -455,6 +461,122 @@ def test_on_another_stream(device):
         got = x.call()
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_two_streams_and_graphs_at_once(device):
+    """Shares and joins of four calls that run together, eager ones and replayed ones, each with its
+    stream's or graph's workspace; 16-bit calls on the same workspace in between."""
+    x = Batch(8, 2, 64, BF16, [9000, 3000, 700, 12000], 1)
+    table, q = x.table.to(device), x.q.to(device)
+    lens = torch.tensor(x.lens, dtype=torch.int32, device=device)
+    want = x.call()
+    x.check(want)
+    pa = PagedAttention(8, 2, 64, num_blocks=64, block_size=16, dtype=BF16, device=device)
+    kc, vc = (torch.randn(t.shape, device=device, generator=torch.Generator(device).manual_seed(3))
+              .to(BF16) for t in pa.allocate_kv_cache())
+    table16 = torch.arange(64, dtype=torch.int32, device=device).view(1, 64)
+    want16 = pa(q[:1], kc, vc, table16, [1000])
+    streams = [torch.cuda.Stream(device) for _ in range(2)]
+    graphs = []
+    note("capture")
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream(device))
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = paged_attention_fp4(q, *x.caches, table, lens)
+        graphs.append((gr, out))
+    torch.cuda.synchronize()
+    for i in range(3):
+        note(f"together {i}")
+        outs = []
+        for s, (gr, out) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    outs.append(paged_attention_fp4(q, *x.caches, table, lens))
+                    gr.replay()
+                    got16 = pa(q[:1], kc, vc, table16, [1000])
+                outs += [out, outs[-1]]
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+        assert torch.equal(got16, want16)
+        for _, out in graphs:
+            out.zero_()
+        torch.cuda.synchronize()
+
+
+def test_caches_past_4_gib(device):
+    """Pages 2^29 bytes apart: written, read and attended over as the same pages side by side."""
+    x = Batch(8, 2, 64, BF16, [70, 33], 1)
+    nb = x.caches[0].shape[0]
+    kc, vc = (c.new_empty((nb - 1) * 2 ** 29 + 8 * 4096).as_strided(c.shape, (2 ** 29, 4096, 544, 1))
+              for c in x.caches)
+    kc.copy_(x.caches[0])
+    vc.copy_(x.caches[1])
+    g = torch.Generator().manual_seed(9)
+    new = [torch.randn(2, 12, 2, 64, generator=g).to(BF16).to(device) for _ in range(2)]
+    table, start = x.table.to(device), [n - 12 for n in x.lens]
+    note("far pages")
+    for caches in ((kc, vc), x.caches):
+        write_kv_fp4(*new, *caches, table, start)
+    assert torch.equal(kc, x.caches[0]) and torch.equal(vc, x.caches[1])
+    for a, b in zip(read_kv_fp4(kc, vc, table, 0, 70), read_kv_fp4(*x.caches, table, 0, 70)):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    lens = torch.tensor(x.lens, dtype=torch.int32, device=device)
+    want = x.call()
+    assert torch.equal(paged_attention_fp4(x.q.to(device), kc, vc, table, lens), want)
+
+
+def test_shared_and_expanded_inputs(device):
+    """One tensor as keys and values, heads and tokens of one row by stride 0, one query for all
+    rows, and k inside the cache's own memory."""
+    x = Batch(8, 2, 64, BF16, [64, 64, 64], 1)
+    table = x.table.to(device)
+    row = torch.randn(3, 1, 1, 64, device=device, generator=torch.Generator(device).manual_seed(1)).to(BF16)
+    fresh = [torch.zeros_like(c) for c in x.caches]
+    note("expanded")
+    wide = row.expand(3, 20, 2, 64)
+    write_kv_fp4(wide, wide, *x.caches, table, 7)
+    write_kv_fp4(wide.contiguous(), wide.clone(), *fresh, table, 7)
+    k, v = read_kv_fp4(*x.caches, table, 7, 20)
+    assert torch.equal(k, v) and all(torch.equal(a, b) for a, b in
+                                     zip((k, v), read_kv_fp4(*fresh, table, 7, 20)))
+    lens = torch.tensor(x.lens, dtype=torch.int32, device=device)
+    q = x.q[:1].to(device)
+    assert torch.equal(paged_attention_fp4(q.expand(3, 1, 8, 64), *x.caches, table, lens),
+                       paged_attention_fp4(q.repeat(3, 1, 1, 1), *x.caches, table, lens))
+    # the last pages of the caches, which no table names, as the keys' and values' memory
+    pool = torch.zeros(2, 8, 2, 1, 544, dtype=torch.uint8, device=device)
+    kc, vc = pool.unbind(0)
+    own = [c[6].view(-1)[:512].view(BF16).view(1, 2, 2, 64) for c in (kc, vc)]
+    for t in own:
+        t.normal_()
+    kept = [t.clone() for t in own]
+    one = torch.zeros(1, 2, dtype=torch.int32, device=device)
+    write_kv_fp4(*own, kc, vc, one, 3)
+    want = allocate_fp4_cache(8, 16, 2, 64, device=device)
+    write_kv_fp4(*kept, *want, one, 3)
+    assert torch.equal(kc[0], want[0][0]) and torch.equal(vc[0], want[1][0])
+    assert all(torch.equal(a, b) for a, b in zip(own, kept))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_parts_of_tiles_read_back(device, dtype):
+    """Every start in a tile and every number of tokens up to two tiles: what lies beside the answer
+    in its buffer is the next row's."""
+    KVH, D = 2, 96
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(1, 64, KVH, D, generator=g).to(BF16).to(device)
+    kc, vc = allocate_fp4_cache(5, 16, KVH, D, device=device)
+    table = torch.tensor([[3, 1, 4, 0]], dtype=torch.int32, device=device)
+    write_kv_fp4(x, -x, kc, vc, table)
+    k, v = read_kv_fp4(kc, vc, table, 0, 64, dtype=dtype)
+    two = table.expand(16, 4)
+    starts = torch.arange(16, dtype=torch.int32, device=device)
+    note(f"parts {dtype}")
+    for n in (1, 2, 3, 15, 16, 17, 31, 32, 33):
+        a, b = read_kv_fp4(kc, vc, two, starts, n, dtype=dtype)
+        for i in range(16):
+            assert torch.equal(a[i], k[0, i:i + n]) and torch.equal(b[i], v[0, i:i + n])
 
 
 def test_views_outputs_and_pages_apart(device):
