@@ -226,6 +226,8 @@ def paged_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise ValueError("block_table has no columns")
     if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
         raise ValueError("workspace must be contiguous and on the query's device")
+    if isinstance(context_lens, torch.Tensor):
+        context_lens = narrow_i32(context_lens)
     lens, host_max = context_lens_i32(context_lens, dev, B)
     cap = W * bs
     if max_context is None:

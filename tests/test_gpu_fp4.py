@@ -293,6 +293,10 @@ def test_a_larger_table_and_a_bound_on_the_context(device):
     note("max_context")
     want = x.call()
     x.check(want)
+    wide = torch.tensor(x.lens, dtype=torch.int64, device=device)
+    assert torch.equal(want, x.call(lens=wide))
+    wide[2] += 2 ** 32  # past any table: as many keys as max_context
+    x.check(x.call(lens=wide, max_context=200), rows=[0, 1, 2])
     x.check(x.call(lens=x.lens))  # (host lengths: the bound is their largest)
     full = torch.tensor(x.lens, dtype=torch.int32, device=device)
     x.lens = [min(n, 150) for n in x.lens]
