@@ -89,6 +89,10 @@ size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 // evenly: 96 against 88, and this factor chooses the latter.
 constexpr double kRound64 = 1.8;
 
+// And with 16. 32 rows of 4 drafts of H28/KVH4/D128 under a window of 2048, 128 units of 28 rows: 24.8
+// us, as 256 of 16 19.8; the chunk above 143.
+constexpr double kRound16 = 0.65;
+
 // Contexts go up to this: a position plus a query's offset or a window fits 31 bits.
 constexpr int kMaxContext = 1 << 30;
 
@@ -97,7 +101,10 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
              int window, int q_dtype, Plan* p) {
   const int G = H / KVH;
   const int64_t rows = static_cast<int64_t>(q_len) * G;
-  p->ct = rows <= 16 ? 1 : 2;
+  const int DP = D <= 64 ? 64 : (D <= 128 ? 128 : 256);
+  const int parts = q_dtype == MSATTN_BF16 ? 1 : (q_dtype == MSATTN_F16 ? 2 : 3);
+  const int list_ct = fp4_list_ct(parts, DP), max_ct = fp4_max_ct(parts, DP);
+  p->ct = rows <= 16 ? 1 : list_ct;
   const int per = 16 * p->ct;
   const int64_t rblocks = (rows + per - 1) / per;
   const int64_t units = batch * rblocks * KVH;
@@ -122,7 +129,7 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   // 62, 231; 4096 of 33, causal, 96, 85, 109, 190, 332. Units of few rows take all waves of a workgroup,
   // and only where no CU gets two (their contexts may differ; 64 of 64 groups, 14 us against 20).
   const double mean = groups - (causal && window == 0 ? 0.5 * std::min(q_len, max_ctx) / kFp4Group : 0.0);
-  double best = p->split ? units * mean / (want * kFp4Waves) + 10 * (static_cast<double>(units) / want + 1)
+  double best = p->split ? (rows > 16 && list_ct == 1 ? kRound16 : 1.0) * units * mean / (want * kFp4Waves) + 10 * (static_cast<double>(units) / want + 1)
                          : 1e300;
   p->wk = kFp4Waves;
   auto consider = [&](int ct, int wk, double round) {  // round: of a group of 16 ct rows
@@ -130,18 +137,19 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
     const double load = static_cast<double>(batch * blocks * KVH) / want;
     const double longest = ceil(static_cast<double>(groups) / wk) + 3, rounds = load * wk / kFp4Waves;
     const double cost = round * (rounds <= 1 ? longest : rounds * (mean / wk + 3) + 0.5 * longest);
-    if (cost > best || (rounds > 1 && ct == 1 && p->split)) return;
+    if (cost > best || (rounds > 1 && rows <= 16 && p->split)) return;
     best = cost;
     p->ct = ct;
     p->wk = wk;
     p->split = 0;
     p->rblocks = static_cast<int>(blocks);
   };
-  if (p->ct == 1) {
+  if (rows <= 16) {
     consider(1, kFp4Waves, 1.0);
   } else {
-    for (int wk = kFp4Waves; wk >= 1; wk /= 2) consider(2, wk, 1.0);
-    if (q_dtype == MSATTN_BF16 && D <= 128 && rows > 32)
+    for (int wk = kFp4Waves; wk >= 1; wk /= 2) consider(1, wk, kRound16);
+    for (int wk = kFp4Waves; max_ct >= 2 && wk >= 1; wk /= 2) consider(2, wk, 1.0);
+    if (max_ct == 4 && rows > 32)
       for (int wk = 4; wk >= 1; wk /= 2) consider(4, wk, kRound64);
   }
   const int64_t dealt = static_cast<int64_t>(batch) * p->rblocks * KVH;  // units

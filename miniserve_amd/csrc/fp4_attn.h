@@ -189,9 +189,9 @@ __device__ __forceinline__ int fp4_count(int lo, int hi) {  // at least one, so 
   return hi > lo ? ceil_div(hi, kFp4Group) - lo / kFp4Group : 1;
 }
 
-// WK waves take a unit's groups in turn. WK = 8: a workgroup takes a share of the list or, without
-// split, one unit; else 8 / WK units, neighbours in the list.
-template <typename T, int DP, int CT, int WK>
+// WK waves take a unit's groups in turn. LIST (WK = 8): a workgroup takes a share of the list; else 8 / WK
+// units, neighbours in it.
+template <typename T, int DP, int CT, int WK, bool LIST>
 __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Params p) {
   constexpr int HV = DP > 128 ? 2 : 1;   // halves of 128 dims
   constexpr int DH = DP > 128 ? 128 : DP;
@@ -203,8 +203,8 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   constexpr bool QLDS = CT == 4;         // the query's operands in LDS, where a unit's waves share them
   // Groups on their way while one is worked on: as many as the registers hold. With CT = 4 one, its
   // keys requested as soon as the group before has used its own, before that one's softmax.
-  constexpr int kRing = QLDS ? 1 : DP == 256 || (CT == 2 && PQ == 3) ? 2 : 3;
-  constexpr bool kEarly = QLDS;
+  constexpr int kRing = QLDS || (DP == 256 && PQ > 1) ? 1 : DP == 256 || (CT == 2 && PQ == 3) ? 2 : 3;
+  constexpr bool kEarly = kRing == 1;
   typedef typename std::conditional<DH == 128, uint4, uint2>::type kraw_t;
 
   __shared__ int s_pre[kFp4MaxEntries + 1];
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   const int share = static_cast<int>(blockIdx.x);
   constexpr int NU = kFp4Waves / WK;        // units at a time
   const int wu = w / WK, wk = w % WK;       // the wave's unit, and its place among the unit's waves
-  const bool list = WK == kFp4Waves && p.split;
+  static_assert(!LIST || WK == kFp4Waves, "a share's groups are all waves'");
   const int entries = p.batch * p.rblocks;
 
   // Barrier for what lies in LDS: loads into registers stay on their way.
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   // context in lane e of every wave; others in LDS.
   const bool regs = p.rblocks == 1 && p.batch <= 64;
   int c0 = 0, c1 = 0, chunk = 1, lane_sum = 0, lane_ctx = 0;
-  if (list) {
+  if constexpr (LIST) {
     int sum = 0;
     if (regs) {
       int cnt = 0;
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     return e == 0 ? 0 : __builtin_amdgcn_readlane(lane_sum, e - 1);
   };
   auto context = [&](int b) FP4_INLINE {
-    if (!list) return uniform(clamped(p.lens[b]));
+    if constexpr (!LIST) return uniform(clamped(p.lens[b]));
     return regs ? __builtin_amdgcn_readlane(lane_ctx, b) : uniform(s_ctx[b]);
   };
   auto extents = [&](Fp4Unit& u) FP4_INLINE {
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   };
   // The unit of the wave that holds position c0 of the list.
   Fp4Unit u{};
-  if (list) {
+  if constexpr (LIST) {
     u.b = regs ? __popcll(__ballot(lane < p.batch - 1 && lane_sum * p.KVH <= c0))
                : search(0, p.batch, p.rblocks, p.KVH, c0);
     const int e0 = u.b * p.rblocks;
@@ -353,9 +353,9 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     }
     c1 = u.cnt = u.n;
   }
-  if (list && u.cnt <= 0) return;  // (a share of the head of a unit alone; the workgroup as one)
+  if (LIST && u.cnt <= 0) return;  // (a share of the head of a unit alone; the workgroup as one)
   const bool head = u.cnt < u.n;   // the first unit has other shares
-  if (list && tid == 0) {
+  if (LIST && tid == 0) {
     s_first[0] = u.b; s_first[1] = u.kvh; s_first[2] = u.rb; s_first[3] = u.u0; s_first[4] = u.n;
   }
   // Whether the share goes on behind u, and the unit it goes on with.
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     u.cnt = min(u.n, c1 - u.u0);
   };
   int groups = u.cnt;  // of the share
-  if constexpr (WK == kFp4Waves) {
+  if constexpr (LIST) {
     if (more(u)) {
       Fp4Unit v = u;
       do advance(v);
@@ -828,7 +828,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   // At the share's end all threads do it, between barriers. Before, a wave leaves its part in a
   // buffer and goes on to the next unit, and the last to leave one joins them: no wave waits for the
   // others, unless all buffers hold parts of earlier units.
-  const int brows = WK == kFp4Waves ? min(16, p.slot_rows) : 16, buffers = 16 / brows;
+  const int brows = LIST ? min(16, p.slot_rows) : 16, buffers = 16 / brows;
   int event = 0;
   auto put = [&](int ct, int buf, int rows) FP4_INLINE {
     const float l = rows4_sum(l_run[ct]);
@@ -1037,7 +1037,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         else __builtin_amdgcn_s_setprio(0);
       }
     }
-    if constexpr (WK != kFp4Waves) {
+    if constexpr (!LIST) {
       finish(u, true);
       return;
     }
@@ -1085,10 +1085,16 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   }
 }
 
-// Column tiles of 16 query rows a wave takes at most.
-template <typename T, int DP> constexpr int fp4_max_ct() {
-  return std::is_same<T, bf16_t>::value && DP <= 128 ? 4 : 2;
+// Blocks of 16 query rows that a wave takes at most, by the bf16 parts of a query element: what its
+// registers hold of accumulators, query and the groups on their way. Past it they spill: at 256 dims two
+// blocks 500 bytes a lane and more (40 rows of 4 drafts of H8/KVH1, 300 to 2000 keys: 105 us against
+// 24), fp32 of 128 dims 150 (2 x 512 queries of H28/KVH4 behind 4096 keys: 219 against 201).
+constexpr int fp4_max_ct(int parts, int DP) {
+  return DP > 128 || (DP > 64 && parts == 3) ? 1 : (parts == 1 ? 4 : 2);
 }
+// Of a list, whose kernel holds more besides (two blocks of fp16 of 128 dims 270 bytes: 32 rows of 4 drafts
+// of H28/KVH4, 600 to 4096 keys, 60 us against 30).
+constexpr int fp4_list_ct(int parts, int DP) { return DP > 128 || (DP > 64 && parts > 1) ? 1 : 2; }
 
 template <typename T, int DP>
 hipError_t launch_fp4_attn(const Fp4Params& p, int ct, int wk, hipStream_t stream);

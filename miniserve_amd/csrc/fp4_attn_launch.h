@@ -6,27 +6,36 @@
 
 namespace msattn {
 
-template <typename T, int DP, int CT, int WK>
+template <typename T, int DP, int CT, int WK, bool LIST>
 static hipError_t fp4_launch(const Fp4Params& p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.split ? p.shares : 8 * p.xcd_units));
-  hipLaunchKernelGGL((fp4_attn_kernel<T, DP, CT, WK>), grid, dim3(kFp4Threads), 0, stream, p);
+  const dim3 grid(static_cast<unsigned>(LIST ? p.shares : 8 * p.xcd_units));
+  hipLaunchKernelGGL((fp4_attn_kernel<T, DP, CT, WK, LIST>), grid, dim3(kFp4Threads), 0, stream, p);
   return hipGetLastError();
+}
+
+template <typename T, int DP, int CT>
+static hipError_t fp4_launch_waves(const Fp4Params& p, int wk, hipStream_t stream) {
+  if constexpr (CT <= fp4_list_ct(fp4_parts<T>(), DP))
+    if (p.split) return fp4_launch<T, DP, CT, kFp4Waves, true>(p, stream);
+  if constexpr (CT < 4)
+    if (wk == 8) return fp4_launch<T, DP, CT, 8, false>(p, stream);
+  switch (wk) {
+    case 1: return fp4_launch<T, DP, CT, 1, false>(p, stream);
+    case 2: return fp4_launch<T, DP, CT, 2, false>(p, stream);
+    case 4: return fp4_launch<T, DP, CT, 4, false>(p, stream);
+    default: return hipErrorNotSupported;
+  }
 }
 
 template <typename T, int DP>
 hipError_t launch_fp4_attn(const Fp4Params& p, int ct, int wk, hipStream_t stream) {
-  if (ct == 1) return fp4_launch<T, DP, 1, 8>(p, stream);
-  if constexpr (fp4_max_ct<T, DP>() == 4) {
-    if (ct == 4 && wk == 1) return fp4_launch<T, DP, 4, 1>(p, stream);
-    if (ct == 4 && wk == 2) return fp4_launch<T, DP, 4, 2>(p, stream);
-    if (ct == 4) return fp4_launch<T, DP, 4, 4>(p, stream);
-  }
-  switch (wk) {
-    case 1: return fp4_launch<T, DP, 2, 1>(p, stream);
-    case 2: return fp4_launch<T, DP, 2, 2>(p, stream);
-    case 4: return fp4_launch<T, DP, 2, 4>(p, stream);
-    default: return fp4_launch<T, DP, 2, 8>(p, stream);
-  }
+  constexpr int most = fp4_max_ct(fp4_parts<T>(), DP);
+  if (ct == 1) return fp4_launch_waves<T, DP, 1>(p, wk, stream);
+  if constexpr (most >= 2)
+    if (ct == 2) return fp4_launch_waves<T, DP, 2>(p, wk, stream);
+  if constexpr (most >= 4)
+    if (ct == 4) return fp4_launch_waves<T, DP, 4>(p, wk, stream);
+  return hipErrorNotSupported;
 }
 
 }  // namespace msattn

@@ -239,6 +239,12 @@ CASES = {
     "wide chunk, not causal": (8, 2, 96, BF16, [333, 1000], 200, 16, False, None),
     "wide chunk, fp32": (16, 2, 128, F32, [500, 430], 400, 16, True, None),
     "wide chunk, 256 dims": (8, 1, 256, F16, [300, 170], 150, 16, True, None),
+    "wide chunk, 256 dims, fp32": (8, 1, 256, F32, [300, 170], 150, 16, True, None),
+    "wide chunk, 256 dims, one a wave": (8, 1, 256, BF16, [700, 640, 333, 610], 600, 16, True, None),
+    "wide chunk, 256 dims, fp32, two a wave": (8, 1, 256, F32, [400, 340, 333, 377], 320, 16, False, 90),
+    "wide chunk, fp16, one a wave": (16, 2, 128, F16, [700, 640], 600, 16, True, None),
+    "two blocks of 16 rows": (28, 4, 128, BF16, [(i * 97) % 900 for i in range(30)], 4, 16, True, 300),
+    "two blocks of 16 rows, fp32": (6, 2, 224, F32, [(i * 97) % 900 for i in range(30)], 7, 16, True, None),
     "drafts in a list": (28, 4, 128, BF16, [2500 - 37 * i for i in range(20)], 3, 16, True, None),
     "ragged in a list": (32, 8, 64, BF16, [1 + (i * 977) % 3100 for i in range(70)], 1, 16, True, None),
     "ragged in a list, fp32": (8, 4, 128, F32, [1 + (i * 977) % 3100 for i in range(30)], 1, 16, True, None),
