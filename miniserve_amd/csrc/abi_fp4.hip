@@ -126,8 +126,7 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   // and about 10 each with a list (its plan, partials and joins, in which all waves of a workgroup
   // meet). Several rounds of the CUs even out; the last unit to start does not. Measured: 896 units of
   // 145 groups, wk = 1, 2, 4, 8 and the list, 191, 103, 104, 126, 161 us; 896 of 65, causal, 70, 40, 42,
-  // 62, 231; 4096 of 33, causal, 96, 85, 109, 190, 332. Units of few rows take all waves of a workgroup,
-  // and only where no CU gets two (their contexts may differ; 64 of 64 groups, 14 us against 20).
+  // 62, 231; 4096 of 33, causal, 96, 85, 109, 190, 332. Units of few rows take all waves of a workgroup.
   const double mean = groups - (causal && window == 0 ? 0.5 * std::min(q_len, max_ctx) / kFp4Group : 0.0);
   double best = p->split ? (rows > 16 && list_ct == 1 ? kRound16 : 1.0) * units * mean / (want * kFp4Waves) + 10 * (static_cast<double>(units) / want + 1)
                          : 1e300;
@@ -137,7 +136,7 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
     const double load = static_cast<double>(batch * blocks * KVH) / want;
     const double longest = ceil(static_cast<double>(groups) / wk) + 3, rounds = load * wk / kFp4Waves;
     const double cost = round * (rounds <= 1 ? longest : rounds * (mean / wk + 3) + 0.5 * longest);
-    if (cost > best || (rounds > 1 && rows <= 16 && p->split)) return;
+    if (cost > best) return;
     best = cost;
     p->ct = ct;
     p->wk = wk;
@@ -145,7 +144,16 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
     p->rblocks = static_cast<int>(blocks);
   };
   if (rows <= 16) {
-    consider(1, kFp4Waves, 1.0);
+    // Where a CU gets several units of few rows, in us: dealt, each round of them starts anew (about 3.7
+    // on top of 5), and a list shares their groups evenly (10, 5 a unit and CU). Dealt units take longer
+    // for their groups where these stream at the memory's rate, bf16 above 64 dims, than where the
+    // waves' own work bounds them. List / dealt: H32/KVH8/D128, 64 rows up to 640 keys 26.0 / 16.4, 1300
+    // 32.6 / 25.8, 1024 to 8192 49.1 / 58.6; 100 rows of 1000 39.3 / 38.9, of 2500 62.7 / 67.7; in fp32
+    // 64 of 2500 54.0 / 46.5; H12/KVH12/D64, 64 of 2500 51.6 / 39.1, 100 in fp32 84.5 / 74.9.
+    const double load = static_cast<double>(units) / want, shared = load * groups / kFp4Waves;
+    const double slower = parts > 1 || D <= 64 ? 0.2 : 0.45;  // us a wave's group
+    if (load <= 1 || !p->split) consider(1, kFp4Waves, 1.0);
+    else if (slower * shared < 5 + 1.3 * load) best = 1e300, consider(1, kFp4Waves, 1.0);
   } else {
     for (int wk = kFp4Waves; wk >= 1; wk /= 2) consider(1, wk, kRound16);
     for (int wk = kFp4Waves; max_ct >= 2 && wk >= 1; wk /= 2) consider(2, wk, 1.0);
