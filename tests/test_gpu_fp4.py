@@ -269,6 +269,19 @@ def test_against_64_bits(device, name):
     x.check(x.call(causal=causal, window=window), causal, window)
 
 
+@pytest.mark.parametrize("name", ["around a tile", "ragged", "ragged in a list", "ragged in a list, fp32",
+                                  "ragged in a list, 256 dims", "many rows", "33 rows a head", "32 dims",
+                                  "drafts in a list", "a chunk", "a chunk, fp16", "96 dims, fp32",
+                                  "256 dims, 20 rows", "no context", "pages of 48"])
+def test_short_contexts_under_wide_tables(device, name):
+    """A table that could hold 40000 tokens: many short units in each share of a list, its plan in
+    registers or LDS, and joins of units that several shares have."""
+    H, KVH, D, dtype, lens, q_len, bs, causal, window = CASES[name]
+    x = Batch(H, KVH, D, dtype, lens, q_len, bs, extra=40000 // bs)
+    note(f"wide table {name}")
+    x.check(x.call(causal=causal, window=window), causal, window)
+
+
 @pytest.mark.parametrize("q_len", [1, 40])
 def test_every_byte_it_reads_is_written(device, q_len):
     """A workspace of NaN past the header, which stays zero; twice: bit for bit the same."""
