@@ -73,9 +73,9 @@ bool geometry_ok(int batch, int q_len, int H, int KVH, int D, int max_ctx) {
   return batch > 0 && q_len > 0 && H > 0 && KVH > 0 && H % KVH == 0 && dim_ok(D) && max_ctx >= 0;
 }
 
-// How a call is cut: column tiles of 16 query rows a wave, and its shares.
+// How a call is cut: the way, blocks of 16 query rows a wave, waves of a unit, shares or parts.
 struct Plan {
-  int ct, wk, rblocks, slot_rows, split, shares, xcd_units;
+  int way, ct, wk, rblocks, slot_rows, shares, parts, xcd_units;
   size_t ml_off, acc_off, total;
 };
 
@@ -113,9 +113,11 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   p->slot_rows = static_cast<int>(std::min<int64_t>(per, rows));
   const int64_t want = kFp4Shares;  // workgroups: one a CU
   int64_t groups = max_ctx / kFp4Group + 1;  // of a unit, at most
-  p->split = batch * rblocks <= kFp4MaxEntries && units * (groups + kFp4Head) < (int64_t(1) << 30);
+  const bool split = batch * rblocks <= kFp4MaxEntries && units * (groups + kFp4Head) < (int64_t(1) << 30);
+  p->way = split ? kFp4List : kFp4Dealt;
+  p->parts = 1;
   p->shares = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, units * (groups + kFp4Head))));
-  const size_t slots = p->split ? 2 * static_cast<size_t>(p->shares) * p->slot_rows : 0;
+  const size_t slots = split ? 2 * static_cast<size_t>(p->shares) * p->slot_rows : 0;
   p->ml_off = up256((kHdrTickets + kMaxTickets) * sizeof(int));
   p->acc_off = p->ml_off + up256(slots * 2 * sizeof(float));
   p->total = p->acc_off + up256(slots * D * sizeof(float));
@@ -128,8 +130,10 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   // 145 groups, wk = 1, 2, 4, 8 and the list, 191, 103, 104, 126, 161 us; 896 of 65, causal, 70, 40, 42,
   // 62, 231; 4096 of 33, causal, 96, 85, 109, 190, 332. Units of few rows take all waves of a workgroup.
   const double mean = groups - (causal && window == 0 ? 0.5 * std::min(q_len, max_ctx) / kFp4Group : 0.0);
-  double best = p->split ? (rows > 16 && list_ct == 1 ? kRound16 : 1.0) * units * mean / (want * kFp4Waves) + 10 * (static_cast<double>(units) / want + 1)
-                         : 1e300;
+  const double listed = static_cast<double>(units) / want;  // units a CU
+  double best = 1e300;
+  if (split)
+    best = (rows > 16 && list_ct == 1 ? kRound16 : 1.0) * listed * mean / kFp4Waves + 10 * (listed + 1);
   p->wk = kFp4Waves;
   auto consider = [&](int ct, int wk, double round) {  // round: of a group of 16 ct rows
     const int64_t blocks = (rows + 16 * ct - 1) / (16 * ct);
@@ -140,7 +144,7 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
     best = cost;
     p->ct = ct;
     p->wk = wk;
-    p->split = 0;
+    p->way = kFp4Dealt;
     p->rblocks = static_cast<int>(blocks);
   };
   if (rows <= 16) {
@@ -150,17 +154,36 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
     // waves' own work bounds them. List / dealt: H32/KVH8/D128, 64 rows up to 640 keys 26.0 / 16.4, 1300
     // 32.6 / 25.8, 1024 to 8192 49.1 / 58.6; 100 rows of 1000 39.3 / 38.9, of 2500 62.7 / 67.7; in fp32
     // 64 of 2500 54.0 / 46.5; H12/KVH12/D64, 64 of 2500 51.6 / 39.1, 100 in fp32 84.5 / 74.9.
-    const double load = static_cast<double>(units) / want, shared = load * groups / kFp4Waves;
     const double slower = parts > 1 || D <= 64 ? 0.2 : 0.45;  // us a wave's group
-    if (load <= 1 || !p->split) consider(1, kFp4Waves, 1.0);
-    else if (slower * shared < 5 + 1.3 * load) best = 1e300, consider(1, kFp4Waves, 1.0);
+    const bool few = slower * listed * groups / kFp4Waves < 5 + 1.3 * listed;
+    if (split && listed > 1) best = few ? 1e300 : 0;
+    consider(1, kFp4Waves, 1.0);
   } else {
     for (int wk = kFp4Waves; wk >= 1; wk /= 2) consider(1, wk, kRound16);
     for (int wk = kFp4Waves; max_ct >= 2 && wk >= 1; wk /= 2) consider(2, wk, 1.0);
     if (max_ct == 4 && rows > 32)
       for (int wk = 4; wk >= 1; wk /= 2) consider(4, wk, kRound64);
   }
-  const int64_t dealt = static_cast<int64_t>(batch) * p->rblocks * KVH;  // units
+  // Few units: each cut into as many parts as there are CUs for it, a workgroup a part, joined like
+  // shares but without a list's plan. Start, partials and join cost 7 groups, 5 of the longer ones above
+  // 128 dims. List / parts: 16 rows of 1024 to 4096 keys of H28/KVH4/D128 in fp16 20.5 / 16.1 us, 16 of
+  // 16384 of H32/KVH8/D128 58.6 / 52.7, 32 of 1024 to 8192 of H8/KVH1/D256 in fp32 44.8 / 30.1. Dealt /
+  // parts: 4 rows of H32/KVH8/D128 up to 600 keys 9.0 / 11.2, 1000 10.8 / 11.4, 1400 12.3 / 11.7, 2000
+  // 14.4 / 12.2; 16 of H8/KVH1/D256 up to 600 13.5 / 12.9, 2000 22.2 / 14.4.
+  const int64_t most = std::min<int64_t>(want / units, (groups + kFp4Waves - 1) / kFp4Waves);
+  if (split && most > 1) {
+    const double cost = (rows > 16 && list_ct == 1 ? kRound16 : 1.0) *
+                            ceil(static_cast<double>(groups) / (most * kFp4Waves)) +
+                        (D > 128 ? 5 : 7);
+    if (cost < best) {
+      p->way = kFp4Parts;
+      p->ct = rows <= 16 ? 1 : list_ct;
+      p->wk = kFp4Waves;
+      p->rblocks = static_cast<int>(rblocks);
+      p->parts = static_cast<int>(most);
+    }
+  }
+  const int64_t dealt = static_cast<int64_t>(batch) * p->rblocks * KVH * p->parts;  // units, or parts of them
   p->xcd_units = static_cast<int>(ceil_div64(ceil_div64(dealt * p->wk, kFp4Waves), 8));
   return true;
 }
@@ -285,12 +308,13 @@ int msattn_paged_attention_fp4(const void* query, int64_t q_batch_stride,
   p.rows_per_kvh = q_len * p.G;
   p.rblocks = plan.rblocks;
   p.slot_rows = plan.slot_rows;
-  p.split = plan.split;
+  p.parts = plan.parts;
   p.shares = plan.shares;
   p.xcd_units = plan.xcd_units;
   p.by_tiles = fp4_div(static_cast<uint32_t>(block_size / kFp4Tile));
   p.by_g = fp4_div(static_cast<uint32_t>(p.G));
   p.by_rb = fp4_div(static_cast<uint32_t>(plan.rblocks));
+  p.by_parts = fp4_div(static_cast<uint32_t>(plan.parts));
   p.by_kvh = fp4_div(static_cast<uint32_t>(num_kv_heads));
   p.by_per = fp4_div(static_cast<uint32_t>(head_dim / 4));
   p.tickets = reinterpret_cast<int*>(ws) + kHdrTickets;
@@ -299,9 +323,9 @@ int msattn_paged_attention_fp4(const void* query, int64_t q_batch_stride,
   const hipStream_t st = static_cast<hipStream_t>(stream);
   auto launch = [&](auto t) {
     typedef decltype(t) T;
-    if (head_dim <= 64) return launch_fp4_attn<T, 64>(p, plan.ct, plan.wk, st);
-    if (head_dim <= 128) return launch_fp4_attn<T, 128>(p, plan.ct, plan.wk, st);
-    return launch_fp4_attn<T, 256>(p, plan.ct, plan.wk, st);
+    if (head_dim <= 64) return launch_fp4_attn<T, 64>(p, plan.way, plan.ct, plan.wk, st);
+    if (head_dim <= 128) return launch_fp4_attn<T, 128>(p, plan.way, plan.ct, plan.wk, st);
+    return launch_fp4_attn<T, 256>(p, plan.way, plan.ct, plan.wk, st);
   };
   switch (q_dtype) {
     case MSATTN_F32: return status_of(launch(float{}));

@@ -2,20 +2,25 @@
 //
 // A unit is a (batch row, KV head, block of up to 16 CT query rows); rows are the pairs (query
 // token i, head g of the KV head's group) r = i G + g. Its keys are cut into groups of 32 tokens
-// (two tiles). A workgroup has 8 waves, two a SIMD, and units come to it in one of two ways
+// (two tiles). A workgroup has 8 waves, two a SIMD, and units come to it in one of three ways
 // (plan_of in abi_fp4.hip chooses, by what each costs):
 //   list   all groups of all units, in order, a unit's behind kFp4Head empty positions, are cut
 //          into one contiguous share a CU, whatever the lengths (read on the device, so a call is
 //          capture-safe). A workgroup's waves take its share's groups in turn, and go on from unit
-//          to unit without waiting for each other. For few long rows, and ragged ones: 64 rows of 1024 to
-//          8192 keys of H32/KVH8/D128 take 49.6 us, 4.4 TB/s of the cache, 5.4 to 6.8 inside a share.
+//          to unit without waiting for each other. For more units than CUs, long and ragged: 64 rows
+//          of 1024 to 8192 keys of H32/KVH8/D128 take 49 us, 4.4 TB/s of the cache, 5.4 to 6.8 inside
+//          a share.
+//   parts  a unit is cut into equal parts, a workgroup each, joined as shares are but without a
+//          plan. For few long units: 16 rows of 1024 to 4096 keys of H28/KVH4/D128 in fp16 take 16
+//          us, as a list 20.5.
 //   dealt  a unit is whole: WK waves take its groups in turn, and 8 / WK units share a workgroup.
-//          For chunks of prompts, with thousands of units: no partials and no joins.
+//          For chunks of prompts, with thousands of units, and for short contexts: no plan, no
+//          partials and no joins.
 // What a wave or a share leaves of a unit is, for each query row,
 //   m,  l = sum_j 2^(s_j - m),  acc = sum_j 2^(s_j - m) V_j,   s_j = scale log2(e) q.K_j
 // over its visible keys. The waves' parts are joined in LDS; a unit that lies within one share is then
 // normalised and written, the shares of another leave partials in the workspace, and the last of them
-// to arrive joins them.
+// to arrive joins them; so too with parts.
 //
 // A wave loads a tile's keys and values straight into the registers of the matrix operands, 16
 // bytes a lane, contiguous (fp4_cache.h); the next kRing groups are on their way while it works on
@@ -40,7 +45,7 @@
 // fp16 and fp32 queries, and their weights, enter the products as 2 and 3 bf16 parts, which hold
 // all their digits (for a weight, 16 and 24 of them); a bf16 query's weights are rounded to bf16
 // once, in the numerator and in the sum alike. Maxima, sums and accumulators are fp32. (The chunk
-// above: fp16 147 us, fp32 219.)
+// above: fp16 146 us, fp32 202.)
 //
 // A masked key's score is -inf, and where a group has masked keys, values that some row must not see
 // are taken as zeros, and their NaN, if any, is given to the rows that do see them.
@@ -83,11 +88,11 @@ struct Fp4Params {
   int rows_per_kvh;  // q_len * G
   int rblocks;       // ceil(rows_per_kvh / (16 CT))
   int slot_rows;     // rows of a partial: min(16 CT, rows_per_kvh)
-  int split;         // shares planned over all units (else units dealt to the workgroups)
-  int xcd_units;     // without split: workgroups an XCD
-  int shares;
+  int xcd_units;     // without a list: workgroups an XCD
+  int shares;        // of a list
+  int parts;         // of a unit
   Fp4Div by_tiles;   // tiles of a page
-  Fp4Div by_g, by_rb, by_kvh;
+  Fp4Div by_g, by_rb, by_kvh, by_parts;
   Fp4Div by_per;     // D / 4
   int* tickets;
   float* ml;         // [2 shares][slot_rows][2]
@@ -189,10 +194,15 @@ __device__ __forceinline__ int fp4_count(int lo, int hi) {  // at least one, so 
   return hi > lo ? ceil_div(hi, kFp4Group) - lo / kFp4Group : 1;
 }
 
-// WK waves take a unit's groups in turn. LIST (WK = 8): a workgroup takes a share of the list; else 8 / WK
-// units, neighbours in it.
-template <typename T, int DP, int CT, int WK, bool LIST>
+// How units come to the workgroups.
+enum : int { kFp4Dealt, kFp4Parts, kFp4List };
+
+// WK waves take a unit's groups in turn. WAY = kFp4List (WK = 8): a workgroup takes a share of the list;
+// kFp4Parts (WK = 8): one of p.parts parts of a unit; else 8 / WK units, neighbours in the list.
+template <typename T, int DP, int CT, int WK, int WAY>
 __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Params p) {
+  constexpr bool LIST = WAY == kFp4List, PARTS = WAY == kFp4Parts;
+  static_assert(WAY == kFp4Dealt || WK == kFp4Waves, "a share's groups are all waves'");
   constexpr int HV = DP > 128 ? 2 : 1;   // halves of 128 dims
   constexpr int DH = DP > 128 ? 128 : DP;
   constexpr int NJ = DH / 32;            // score products of a half; dwords of keys a lane holds
@@ -207,8 +217,8 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   constexpr bool kEarly = kRing == 1;
   typedef typename std::conditional<DH == 128, uint4, uint2>::type kraw_t;
 
-  __shared__ int s_pre[kFp4MaxEntries + 1];
-  __shared__ int s_ctx[kFp4MaxEntries];
+  __shared__ int s_pre[LIST ? kFp4MaxEntries + 1 : 1];
+  __shared__ int s_ctx[LIST ? kFp4MaxEntries : 1];
   __shared__ int s_tot[kFp4Waves];  // and whether this workgroup joins a unit's shares
   // The waves' accumulators of up to 16 rows of a unit, [buffer][wave][rows][RS] (RS: the rows of a
   // store fall on different banks), and their maxima and sums. Fewer rows leave more buffers.
@@ -228,7 +238,6 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   const int share = static_cast<int>(blockIdx.x);
   constexpr int NU = kFp4Waves / WK;        // units at a time
   const int wu = w / WK, wk = w % WK;       // the wave's unit, and its place among the unit's waves
-  static_assert(!LIST || WK == kFp4Waves, "a share's groups are all waves'");
   const int entries = p.batch * p.rblocks;
 
   // Barrier for what lies in LDS: loads into registers stay on their way.
@@ -323,6 +332,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   };
   // The unit of the wave that holds position c0 of the list.
   Fp4Unit u{};
+  int unit = 0;  // without a list: its number
   if constexpr (LIST) {
     u.b = regs ? __popcll(__ballot(lane < p.batch - 1 && lane_sum * p.KVH <= c0))
                : search(0, p.batch, p.rblocks, p.KVH, c0);
@@ -342,16 +352,29 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     // a run of units, so that the row blocks of a head, which read the same keys, share one. Later
     // row blocks first: under a causal mask they have the most keys.
     const int at = ((share & 7) * p.xcd_units + (share >> 3)) * NU + wu;
-    const int bk = fp4_quot(at, p.by_rb);
+    if constexpr (PARTS) unit = fp4_quot(at, p.by_parts);
+    else unit = at;
+    const int bk = fp4_quot(unit, p.by_rb);
     const int b = fp4_quot(bk, p.by_kvh);
     if (b < p.batch) {  // (waves past the last unit go on to the barriers, with one of no groups)
-      u.rb = p.rblocks - 1 - (at - bk * p.rblocks);
+      u.rb = p.rblocks - 1 - (unit - bk * p.rblocks);
       u.b = b;
       u.kvh = bk - b * p.KVH;
       u.ctx = context(b);
       extents(u);
     }
-    c1 = u.cnt = u.n;
+    u.cnt = u.n;
+    if constexpr (PARTS) {
+      // Parts of equal length; a unit of a round of the waves or less is the first part's.
+      const int part = at - unit * p.parts, q = fp4_quot(u.n, p.by_parts), more = u.n - q * p.parts;
+      if (u.n > kFp4Waves) {
+        u.skip = part * q + min(part, more);
+        u.cnt = q + (part < more ? 1 : 0);
+      } else if (part > 0 || u.n == 0) {
+        return;  // (the workgroup as one)
+      }
+    }
+    c1 = u.cnt;
   }
   if (LIST && u.cnt <= 0) return;  // (a share of the head of a unit alone; the workgroup as one)
   const bool head = u.cnt < u.n;   // the first unit has other shares
@@ -848,7 +871,8 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   auto fold = [&](const Fp4Unit& u, int r0, int buf, int rows, int t0, int threads) FP4_INLINE {
     const int per = p.D / 4;  // items of a row
     const bool whole = u.cnt == u.n;
-    const int64_t slot = 2 * static_cast<int64_t>(share) + (u.skip == 0 ? 1 : 0);
+    const int64_t slot = PARTS ? static_cast<int64_t>((share & 7) * p.xcd_units + (share >> 3))
+                               : 2 * static_cast<int64_t>(share) + (u.skip == 0 ? 1 : 0);
     for (int idx = t0; idx < rows * per; idx += threads) {
       const int r = fp4_quot(idx, p.by_per), d = 4 * (idx - r * per);
       float2 ml[WK];
@@ -926,7 +950,8 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     const int r0 = v.rb * ROWS;
     const int rows = min(ROWS, p.rows_per_kvh - r0);
     const int per = p.D / 4;
-    const int s_first = v.u0 / chunk, s_last = (v.u0 + v.n - 1) / chunk;
+    const int s_first = PARTS ? unit * p.parts : v.u0 / chunk;
+    const int s_last = PARTS ? s_first + p.parts - 1 : (v.u0 + v.n - 1) / chunk;
     // Threads left over take other shares of the same items, and are joined through LDS.
     const int items = rows * per;
     const int parts = items >= kFp4Threads ? 1 : kFp4Threads / items;
@@ -944,7 +969,8 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
 #pragma unroll
         for (int i = 0; i < N; ++i) {  // shares past the last repeat it, unused
           const int j = min(j0 + i * parts, s_last);
-          const int64_t row = (2 * static_cast<int64_t>(j) + (j == s_first ? 1 : 0)) * p.slot_rows + r;
+          const int64_t slot = PARTS ? j : 2 * static_cast<int64_t>(j) + (j == s_first ? 1 : 0);
+          const int64_t row = slot * p.slot_rows + r;
           ml[i] = load2_device(p.ml + row * 2);
           x0[i] = load2_device(p.acc + row * p.D + d);
           x1[i] = load2_device(p.acc + row * p.D + d + 2);
@@ -1039,7 +1065,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     }
     if constexpr (!LIST) {
       finish(u, true);
-      return;
+      break;
     }
     const Fp4Unit done = u;
     const bool go_on = more(u);
@@ -1051,6 +1077,25 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     if (!go_on) break;
   }
 
+  if constexpr (WAY == kFp4Dealt) return;
+  if constexpr (PARTS) {
+    if (u.cnt == u.n) return;
+    // (as below, with a counter a unit)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    if (tid == 0) {
+      int* const t = p.tickets + unit;
+      const int old = __hip_atomic_fetch_add(t, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const bool last = old == p.parts - 1;
+      if (last) __hip_atomic_store(t, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_tot[0] = last;
+    }
+    lds_barrier();
+    const int last = uniform(s_tot[0]);
+    asm volatile("" ::: "memory");
+    if (last) join(u);
+    return;
+  }
   // ---- the first and the last unit, where they have other shares ----
   const bool tail = u.cnt < u.n;  // (u: the last; perhaps the first too)
   if (!head && !tail) return;
@@ -1097,6 +1142,6 @@ constexpr int fp4_max_ct(int parts, int DP) {
 constexpr int fp4_list_ct(int parts, int DP) { return DP > 128 || (DP > 64 && parts > 1) ? 1 : 2; }
 
 template <typename T, int DP>
-hipError_t launch_fp4_attn(const Fp4Params& p, int ct, int wk, hipStream_t stream);
+hipError_t launch_fp4_attn(const Fp4Params& p, int way, int ct, int wk, hipStream_t stream);
 
 }  // namespace msattn

@@ -2,5 +2,5 @@
 #include "fp4_attn_launch.h"
 
 namespace msattn {
-template hipError_t launch_fp4_attn<bf16_t, 128>(const Fp4Params&, int, int, hipStream_t);
+template hipError_t launch_fp4_attn<bf16_t, 128>(const Fp4Params&, int, int, int, hipStream_t);
 }

@@ -298,6 +298,24 @@ def test_every_byte_it_reads_is_written(device, q_len):
     assert torch.equal(a, x.call(workspace=ws, max_context=600))
 
 
+@pytest.mark.parametrize("KVH,q_len", [(1, 1), (2, 4), (8, 1), (20, 1), (40, 3)])
+def test_partials_are_written_before_they_are_read(device, KVH, q_len):
+    """The same where units are cut: parts of few units, among them ones of no key, of one and of
+    fewer groups than parts, and a list's shares."""
+    lens = [0, 1, 40, 257, 300, 900, 9000, 2300]
+    x = Batch(KVH, KVH, 64, F16, lens, q_len, extra=1500)
+    nbytes = nat.lib().msattn_fp4_workspace_bytes(8, q_len, KVH, KVH, 64, 30000, nat.F16)
+    ws = torch.full((nbytes,), 255, dtype=torch.uint8, device=device)
+    header = (64 + 4096) * 4
+    ws[:header] = 0
+    note(f"poisoned partials {KVH} {q_len}")
+    a = x.call(workspace=ws, max_context=30000)
+    x.check(a)
+    assert not ws[:header].any()
+    ws[header:] = 255
+    assert torch.equal(a, x.call(workspace=ws, max_context=30000))
+
+
 @pytest.mark.parametrize("q_len", [1, 3, 50])
 def test_holes_are_not_read(device, q_len):
     x = Batch(8, 2, 128, BF16, [300, 250, 193, 200, 90], q_len)
