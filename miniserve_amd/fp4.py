@@ -237,7 +237,7 @@ def paged_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     max_context = max(0, min(int(max_context), cap, 2 ** 31 - 1))
     given = None  # an output that the kernel, which stores 16 bytes at once, does not write itself
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be contiguous, of the query's shape, dtype and device")
     else:
