@@ -45,7 +45,7 @@
 // fp16 and fp32 queries, and their weights, enter the products as 2 and 3 bf16 parts, which hold
 // all their digits (for a weight, 16 and 24 of them); a bf16 query's weights are rounded to bf16
 // once, in the numerator and in the sum alike. Maxima, sums and accumulators are fp32. (The chunk
-// above: fp16 146 us, fp32 202.)
+// above: fp16 139 us, fp32 203.)
 //
 // A masked key's score is -inf, and where a group has masked keys, values that some row must not see
 // are taken as zeros, and their NaN, if any, is given to the rows that do see them.
@@ -213,7 +213,10 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   constexpr bool QLDS = CT == 4;         // the query's operands in LDS, where a unit's waves share them
   // Groups on their way while one is worked on: as many as the registers hold. With CT = 4 one, its
   // keys requested as soon as the group before has used its own, before that one's softmax.
-  constexpr int kRing = QLDS || (DP == 256 && PQ > 1) ? 1 : DP == 256 || (CT == 2 && PQ == 3) ? 2 : 3;
+  // Three where a list streams; two are enough for a unit or a part of one, which begins with all of them
+  // (64 rows of H32/KVH8/D128 up to 1300 keys, two, three and four: 24.1, 25.8, 27.9 us).
+  constexpr int kRing = QLDS || (DP == 256 && PQ > 1) ? 1
+                        : !LIST || DP == 256 || (CT == 2 && PQ == 3) ? 2 : 3;
   constexpr bool kEarly = kRing == 1;
   typedef typename std::conditional<DH == 128, uint4, uint2>::type kraw_t;
 
