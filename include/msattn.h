@@ -516,9 +516,9 @@ size_t msattn_fp4_workspace_bytes(int batch, int q_len, int num_heads, int num_k
  * window as there; one launch. The query's strides are in elements, its rows and the contiguous out
  * 16-byte aligned; out shares no memory with the query or the caches. max_context is at most 2^30
  * (MSATTN_ERR_UNSUPPORTED past it). Rows without a visible key give zeros; an infinity or NaN reaches
- * the queries that see its key alone. Scores and products take the cache's values
- * exactly; the weights of a bf16 query are rounded to bf16, in the numerator and in the sum alike;
- * maxima, sums and accumulators are fp32.
+ * the queries that see its key alone. Scores and products take the cache's values exactly, and the
+ * query's; a weight enters the products with 16 digits (fp32 queries: 24), and the sum in fp32, as are
+ * maxima and accumulators.
  */
 int msattn_paged_attention_fp4(const void* query, int64_t q_batch_stride,
                                int64_t q_token_stride, int64_t q_head_stride,

@@ -38,14 +38,15 @@
 // What bounds it. A decode: the cache's bytes in the middle of a share, and about 7 us of start (the
 // plan, the table, the first tiles) and end (parts and joins) around it, all there is to a small call.
 // A chunk: the widening. A tile is widened once for each unit that reads it, so units of few rows spend
-// their time on it: with 64 rows a wave (CT = 4, their query in LDS) 512 queries of H28/KVH4/D128 behind
-// 4096 keys, two rows of them, take 90 us, with 32 in registers 103; matrix instructions issue for 26 %
-// of that time, vector ones for 45 %.
+// their time on it, 64 a wave (CT = 4, their query in LDS) less than 32 in registers (abi_fp4.hip has
+// both sides).
 //
-// fp16 and fp32 queries, and their weights, enter the products as 2 and 3 bf16 parts, which hold
-// all their digits (for a weight, 16 and 24 of them); a bf16 query's weights are rounded to bf16
-// once, in the numerator and in the sum alike. Maxima, sums and accumulators are fp32. (The chunk
-// above: fp16 139 us, fp32 203.)
+// fp16 and fp32 queries enter the products as 2 and 3 bf16 parts, which hold all their digits; weights,
+// which are fp32, as 2 parts for 16-bit queries and 3 for fp32 ones (16 and 24 digits). Maxima, sums and
+// accumulators are fp32. (One part was rounded to 8 digits, whose error in a bf16 answer, a mean of
+// values weighed so, was as large as the answer's own rounding: mean relative error against 64 bits
+// 0.0023, with two parts 0.0017. 512 queries of H28/KVH4/D128 behind 4096 keys, two rows of them, take
+// 103 us with two parts, 92 with one; decodes are level. The chunk in fp16 126 us, in fp32 194.)
 //
 // A masked key's score is -inf, and where a group has masked keys, values that some row must not see
 // are taken as zeros, and their NaN, if any, is given to the rows that do see them.
@@ -121,11 +122,17 @@ __device__ __forceinline__ uint32_t fp4_cut2(float& a, float& b) {
 }
 
 // The same of finite weights (or NaN), each part rounded to nearest: what is left has as many digits
-// less, and a sign. (Half the instructions: 2 x 512 fp16 queries behind 4096 keys 162 -> 147 us.)
+// less, and a sign, and is exact (a dot product with (-1, 0) or (0, -1) takes a part away; the other
+// weight of the pair is the same row's, so that its NaN changes no answer. 2 x 512 fp16 queries behind
+// 4096 keys: cut off 162 us, rounded 147, with the dot products 126 against 139).
 __device__ __forceinline__ uint32_t fp4_part2(float& a, float& b) {
   const uint32_t w = Pack2<bf16_t>::pack(a, b);
-  a -= __uint_as_float(w << 16);
-  b -= __uint_as_float(w & 0xffff0000u);
+  uint32_t first = 0x0000bf80u;  // (-1, 0)
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("" : "+s"(first));  // (as a constant it is encoded as -1.0f, which is (0, -1))
+#endif
+  a = Dot2<bf16_t>::dot(w, first, a);
+  b = Dot2<bf16_t>::dot(w, 0xbf800000u, b);
   return w;
 }
 
@@ -209,6 +216,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   constexpr int VC = DH / 16;            // value products of a half: dims a lane holds of a token
   constexpr int LD = DH / 4;             // dims a lane receives of a half
   constexpr int PQ = fp4_parts<T>();
+  constexpr int PW = PQ == 1 ? 2 : PQ;   // bf16 parts of a weight
   constexpr int ROWS = 16 * CT;
   constexpr bool QLDS = CT == 4;         // the query's operands in LDS, where a unit's waves share them
   // Groups on their way while one is worked on: as many as the registers hold. With CT = 4 one, its
@@ -521,7 +529,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
   uint4* const s_q = reinterpret_cast<uint4*>(s_acc) + wu * (CT * HV * NJ * 64) + lane;
   mf_f32x4 acc[CT][HV][VC];
   float m_run[CT], l_run[CT];
-  int lo_n[CT], hi_n[CT];  // keys the lane's rows see
+  int lo_n[QLDS ? 1 : CT], hi_n[QLDS ? 1 : CT];  // keys the lane's rows see
   int all_lo, all_hi;      // keys every row of the block sees
   constexpr int QW = static_cast<int>(sizeof(T)) / 2;  // 16-byte words of 8 query elements
   uint4 q_raw[CT][HV][NJ][QW];
@@ -548,6 +556,12 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         }
     }
   };
+  auto seen_keys = [&](const Fp4Unit& u, int r, int* lo, int* hi) FP4_INLINE {  // of row r of the KV head
+    const int r1 = min(u.rb * ROWS + ROWS, p.rows_per_kvh) - 1;
+    const int qpos = u.ctx - p.q_len + fp4_quot(min(r, r1), p.by_g);
+    *hi = r > r1 ? 0 : (p.causal ? min(u.ctx, qpos + 1) : u.ctx);
+    *lo = p.window > 0 ? max(0, qpos - p.window + 1) : 0;
+  };
   auto begin = [&]() FP4_INLINE {
     const int ctx = u.ctx;
     const int r0 = u.rb * ROWS;
@@ -557,10 +571,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     all_lo = p.window > 0 ? max(0, q1 - p.window + 1) : 0;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const int r = r0 + 16 * ct + n;
-      const int qpos = ctx - p.q_len + fp4_quot(min(r, r1), p.by_g);
-      hi_n[ct] = r > r1 ? 0 : (p.causal ? min(ctx, qpos + 1) : ctx);
-      lo_n[ct] = p.window > 0 ? max(0, qpos - p.window + 1) : 0;
+      if constexpr (!QLDS) seen_keys(u, r0 + 16 * ct + n, &lo_n[ct], &hi_n[ct]);
       m_run[ct] = -INFINITY;
       l_run[ct] = 0.0f;
 #pragma unroll
@@ -658,7 +669,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     }
   };
 
-  uint4 pw[CT][PQ];  // the weights, as the B operand of the value products
+  uint4 pw[CT][PW];  // the weights, as the B operand of the value products
   float psum[CT];
   auto weights = [&](int ct, const mf_f32x4& s0, const mf_f32x4& s1, float mul) FP4_INLINE {
     const float m = m_run[ct] != -INFINITY ? m_run[ct] : 0.0f;
@@ -668,21 +679,12 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       x[i] = __builtin_amdgcn_exp2f(fmaf(s0[i], mul, -m));
       x[4 + i] = __builtin_amdgcn_exp2f(fmaf(s1[i], mul, -m));
     }
-    if constexpr (PQ == 1) {
-      const uint4 y = make_uint4(Pack2<bf16_t>::pack(x[0], x[1]), Pack2<bf16_t>::pack(x[2], x[3]),
-                                 Pack2<bf16_t>::pack(x[4], x[5]), Pack2<bf16_t>::pack(x[6], x[7]));
-      const uint32_t one = 0x3f803f80u;
-      psum[ct] = Dot2<bf16_t>::dot(y.x, one, Dot2<bf16_t>::dot(y.y, one, 0.0f)) +
-                 Dot2<bf16_t>::dot(y.z, one, Dot2<bf16_t>::dot(y.w, one, 0.0f));
-      pw[ct][0] = y;
-    } else {
-      psum[ct] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    psum[ct] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
-      for (int a = 0; a < PQ; ++a) {
-        const uint32_t w0 = fp4_part2(x[0], x[1]), w1 = fp4_part2(x[2], x[3]);
-        const uint32_t w2 = fp4_part2(x[4], x[5]), w3 = fp4_part2(x[6], x[7]);
-        pw[ct][a] = make_uint4(w0, w1, w2, w3);
-      }
+    for (int a = 0; a < PW; ++a) {
+      const uint32_t w0 = fp4_part2(x[0], x[1]), w1 = fp4_part2(x[2], x[3]);
+      const uint32_t w2 = fp4_part2(x[4], x[5]), w3 = fp4_part2(x[6], x[7]);
+      pw[ct][a] = make_uint4(w0, w1, w2, w3);
     }
   };
   // The weights with the running maximum as it stands, and only where one of them exceeds 2^8 (or
@@ -718,7 +720,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
 
   // O^T += V^T P^T for half h: d0, d1 the tiles' elements, sc the 8 tokens' scales.
   auto product = [&](auto h_c, const uint4& d0, const uint4& d1, const float (&sc)[8],
-                     const uint4 (&b)[CT][PQ]) FP4_INLINE {
+                     const uint4 (&b)[CT][PW]) FP4_INLINE {
     constexpr int h = decltype(h_c)::value;
     uint32_t x[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
     if constexpr (DH == 64) {  // two lanes share 8 dims
@@ -743,11 +745,11 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
       constexpr int c = decltype(cc)::value;
       const uint4 ea = make_uint4(e[c & 1][0], e[c & 1][1], e[c & 1][2], e[c & 1][3]);
       const uint4 oa = make_uint4(o[c & 1][0], o[c & 1][1], o[c & 1][2], o[c & 1][3]);
-      constexpr int N = CT * PQ;  // pairs of products
+      constexpr int N = CT * PW;  // pairs of products
       int t = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int ct = i / PQ, a = i % PQ;
+        const int ct = i / PW, a = i % PW;
         acc[ct][h][2 * c] = Mfma16<bf16_t>::mac(ea, b[ct][a], acc[ct][h][2 * c]);
         acc[ct][h][2 * c + 1] = Mfma16<bf16_t>::mac(oa, b[ct][a], acc[ct][h][2 * c + 1]);
         if constexpr (c + 1 < VC / 2) {
@@ -773,8 +775,19 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
     uint32_t seen[CT], bad[HV], any_bad = 0;
     if (!full) {
       uint32_t dead = 0;  // no row sees it, or the table has no page
+      int lo_r[CT], hi_r[CT];
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) seen[ct] = 0;
+      for (int ct = 0; ct < CT; ++ct) {
+        seen[ct] = 0;
+        if constexpr (QLDS) {  // (worked out here: the registers are the accumulators')
+          uint32_t row = u.rb * ROWS + 16 * ct + n;
+          opaque(row);
+          seen_keys(u, static_cast<int>(row), &lo_r[ct], &hi_r[ct]);
+        } else {
+          lo_r[ct] = lo_n[ct];
+          hi_r[ct] = hi_n[ct];
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int key = tok + 16 * (i / 4) + 4 * g + i % 4;
@@ -782,7 +795,7 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
         dead |= live ? 0u : 1u << i;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          const bool see = live && key >= lo_n[ct] && key < hi_n[ct];
+          const bool see = live && key >= lo_r[ct] && key < hi_r[ct];
           seen[ct] |= see ? 1u << i : 0u;
           // (scaled first: a scale of 0 or below must not touch the mask)
           if (i < 4) s0[ct][i % 4] = see ? s0[ct][i % 4] * p.scale_log2 : -INFINITY;
