@@ -113,9 +113,11 @@ template <typename T> constexpr int fp4_parts() {
 }
 
 // One packed pair of bf16 parts of a and b, cut off (not rounded, so that no part overflows), and
-// what is left of them. A part that is not finite leaves nothing.
+// what is left of them. A part that is not finite leaves nothing. (A NaN is made quiet: one whose
+// payload lies in the lower half alone would be cut to an infinity.)
 __device__ __forceinline__ uint32_t fp4_cut2(float& a, float& b) {
-  const uint32_t x = __float_as_uint(a) & 0xffff0000u, y = __float_as_uint(b) & 0xffff0000u;
+  const uint32_t x = (__float_as_uint(a) | (a != a ? 0x400000u : 0u)) & 0xffff0000u;
+  const uint32_t y = (__float_as_uint(b) | (b != b ? 0x400000u : 0u)) & 0xffff0000u;
   a = (x & 0x7f800000u) == 0x7f800000u ? 0.0f : a - __uint_as_float(x);
   b = (y & 0x7f800000u) == 0x7f800000u ? 0.0f : b - __uint_as_float(y);
   return (x >> 16) | y;
