@@ -481,7 +481,8 @@ int msattn_gather_kv(const void* cache, int64_t cache_block_stride, int64_t cach
  * x / 2^e to the nearest, ties to the even code, at most 6; one with a NaN or an infinity reads
  * back as NaN. The strides of k and v are in elements. The same row gives the same bytes whatever
  * stands beside it. Two tokens of one call must not land in one slot. MSATTN_ERR_OVERLAP where k or
- * v shares memory with a cache.
+ * v shares memory with a cache. MSATTN_ERR_UNSUPPORTED for batch * num_kv_heads * (tokens + 30) / 16
+ * (rounded down) from about 2^26 on, more than a launch holds; so too of the read.
  */
 int msattn_write_kv_fp4(const void* k, int64_t k_batch_stride, int64_t k_token_stride,
                         int64_t k_head_stride, const void* v, int64_t v_batch_stride,
@@ -515,7 +516,8 @@ size_t msattn_fp4_workspace_bytes(int batch, int q_len, int num_heads, int num_k
  * msattn_paged_attention over a 4-bit cache: fp32, fp16 or bf16 query, any q_len, causal or not,
  * window as there; one launch. The query's strides are in elements, its rows and the contiguous out
  * 16-byte aligned; out shares no memory with the query or the caches. max_context is at most 2^30
- * (MSATTN_ERR_UNSUPPORTED past it). Rows without a visible key give zeros; an infinity or NaN reaches
+ * (MSATTN_ERR_UNSUPPORTED past it, and where a launch would have 2^32 threads: from about 2^23 units
+ * of a row, a KV head and 16 of its query rows on, where eight waves take a unit). Rows without a visible key give zeros; an infinity or NaN reaches
  * the queries that see its key alone. Scores and products take the cache's values exactly, and the
  * query's; a weight enters the products with 16 digits (fp32 queries: 24), and the sum in fp32, as are
  * maxima and accumulators.

@@ -25,6 +25,9 @@ bool cache_ok(const void* k, const void* v, int64_t blk, int64_t head, int KVH, 
          W > 0;
 }
 
+// A launch has fewer than 2^32 threads.
+bool grid_ok(int64_t workgroups, int threads) { return workgroups * threads < (int64_t(1) << 32); }
+
 int status_of(hipError_t e) { return e == hipSuccess ? MSATTN_OK : MSATTN_ERR_HIP; }
 
 // Write or read: the parameters that both have.
@@ -37,10 +40,11 @@ int cache_params(Fp4CacheParams* p, const void* k, const void* v, const int64_t*
     return MSATTN_ERR_INVALID_ARG;
   const int eb = type_bytes(dtype);
   if (!on(k, eb) || !on(v, eb) || !on(table, 4) || !on(starts, 4)) return MSATTN_ERR_INVALID_ARG;
-  // tokens positions from anywhere in a tile; the wave's index fits 31 bits
+  // tokens positions from anywhere in a tile, a wave for each tile they may touch
   p->tiles = static_cast<int>((static_cast<int64_t>(tokens) + 2 * (kFp4Tile - 1)) / kFp4Tile);
   p->items = static_cast<int64_t>(batch) * p->tiles;
-  if (p->items >= (int64_t(1) << 31) || (p->items *= KVH) >= (int64_t(1) << 31))
+  if (p->items >= (int64_t(1) << 31) || !grid_ok(p->items *= KVH, 64) ||
+      !grid_ok(fp4_cache_workgroups(p->items), kFp4CacheThreads))
     return MSATTN_ERR_UNSUPPORTED;
   p->k_cache = static_cast<uint8_t*>(k_cache);
   p->v_cache = static_cast<uint8_t*>(v_cache);
@@ -277,6 +281,8 @@ int msattn_paged_attention_fp4(const void* query, int64_t q_batch_stride,
     if (x < 0 || x * eb % 16 != 0) return MSATTN_ERR_INVALID_ARG;
   Plan plan;
   if (!plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, causal, window, q_dtype, &plan))
+    return MSATTN_ERR_UNSUPPORTED;
+  if (plan.way != kFp4List && !grid_ok(8 * static_cast<int64_t>(plan.xcd_units), kFp4Threads))
     return MSATTN_ERR_UNSUPPORTED;
   if (workspace_bytes < plan.total) return MSATTN_ERR_WORKSPACE;
   char* const ws = static_cast<char*>(workspace);

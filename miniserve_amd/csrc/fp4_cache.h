@@ -68,6 +68,11 @@ struct Fp4CacheParams {
   Fp4Div by_tiles, by_heads, by_bs;
 };
 
+constexpr int kFp4CacheThreads = 256;  // of a workgroup of theirs
+constexpr int64_t fp4_cache_workgroups(int64_t items) {
+  return (items + kFp4CacheThreads / 64 - 1) / (kFp4CacheThreads / 64);
+}
+
 hipError_t launch_write_fp4(const Fp4CacheParams& p, int src_dtype, hipStream_t stream);
 hipError_t launch_read_fp4(const Fp4CacheParams& p, int dst_dtype, hipStream_t stream);
 

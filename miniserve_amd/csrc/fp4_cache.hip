@@ -13,8 +13,6 @@
 
 namespace msattn {
 
-constexpr int kFp4Threads = 256;
-
 // Eight elements of a row in fp32. VEC: 16-byte accesses.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
@@ -102,7 +100,7 @@ struct Fp4Item {
 
 __device__ __forceinline__ bool fp4_item(const Fp4CacheParams& p, Fp4Item* it) {
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-  const int64_t i64 = static_cast<int64_t>(blockIdx.x) * (kFp4Threads / 64) + wave;
+  const int64_t i64 = static_cast<int64_t>(blockIdx.x) * (kFp4CacheThreads / 64) + wave;
   if (i64 >= p.items) return false;
   const int i = static_cast<int>(i64);
   const int bk = fp4_quot(i, p.by_heads);  // (head fastest: its neighbours' rows are the memory's)
@@ -148,7 +146,7 @@ __device__ __forceinline__ void quad_transpose(uint32_t (&x)[4], int q) {
 }
 
 template <typename T, bool VEC, int NB>
-__global__ __launch_bounds__(kFp4Threads) void write_fp4_kernel(const Fp4CacheParams p) {
+__global__ __launch_bounds__(kFp4CacheThreads) void write_fp4_kernel(const Fp4CacheParams p) {
   Fp4Item it;
   if (!fp4_item(p, &it) || it.at < 0 || !it.live) return;  // (a token's four lanes as one)
   const int lane = static_cast<int>(threadIdx.x) & 63, t = lane >> 2, q = lane & 3;
@@ -206,7 +204,7 @@ __device__ __forceinline__ void swap_halves(uint4& a, uint4& b) {
 }
 
 template <typename T, bool VEC, int NB>
-__global__ __launch_bounds__(kFp4Threads) void read_fp4_kernel(const Fp4CacheParams p) {
+__global__ __launch_bounds__(kFp4CacheThreads) void read_fp4_kernel(const Fp4CacheParams p) {
   Fp4Item it;
   if (!fp4_item(p, &it)) return;  // (a wave at a time; lanes without a token only pass words on)
   const int lane = static_cast<int>(threadIdx.x) & 63, t = lane >> 2, q = lane & 3;
@@ -275,12 +273,11 @@ __global__ __launch_bounds__(kFp4Threads) void read_fp4_kernel(const Fp4CachePar
 
 template <typename T, bool VEC, int NB>
 static hipError_t launch_ops(const Fp4CacheParams& p, bool write, hipStream_t stream) {
-  constexpr int per = kFp4Threads / 64;
-  const dim3 grid(static_cast<unsigned>((p.items + per - 1) / per));
+  const dim3 grid(static_cast<unsigned>(fp4_cache_workgroups(p.items)));
   if (write)
-    hipLaunchKernelGGL((write_fp4_kernel<T, VEC, NB>), grid, dim3(kFp4Threads), 0, stream, p);
+    hipLaunchKernelGGL((write_fp4_kernel<T, VEC, NB>), grid, dim3(kFp4CacheThreads), 0, stream, p);
   else
-    hipLaunchKernelGGL((read_fp4_kernel<T, VEC, NB>), grid, dim3(kFp4Threads), 0, stream, p);
+    hipLaunchKernelGGL((read_fp4_kernel<T, VEC, NB>), grid, dim3(kFp4CacheThreads), 0, stream, p);
   return hipGetLastError();
 }
 

@@ -109,3 +109,28 @@ def test_cpu_tensors_raise():
         read_kv_fp4(k, v, table, 0, 1)
     with pytest.raises(RuntimeError, match="no CPU path"):
         paged_attention_fp4(x, k, v, table, [1])
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """A wave a tile: 2^26 - 4 of them are 2^32 - 256 threads, one more a workgroup too many. Inputs
+    that overlap the cache, and a workspace too small, end the calls below the limit."""
+    L, most = nat.lib(), 4 * (2 ** 24 - 1)
+    for KVH, B, T in ((1, most, 1), (4, most // 4, 1), (1, 1, 16 * most - 30), (4, 1, 4 * most - 15)):
+        below = write_args(k=4096, B=B, KVH=KVH, T=T)
+        assert L.msattn_write_kv_fp4(*below) == nat.ERR_OVERLAP, (KVH, B, T)
+        above = dict(T=T + 16) if B == 1 else dict(B=B + 1)
+        assert L.msattn_write_kv_fp4(*write_args(k=4096, KVH=KVH, **{**dict(B=B, T=T), **above})) == \
+            nat.ERR_UNSUPPORTED, (KVH, B, T)
+        assert L.msattn_read_kv_fp4(*read_args(KVH=KVH, **{**dict(B=B, T=T), **above})) == \
+            nat.ERR_UNSUPPORTED, (KVH, B, T)
+
+
+@pytest.mark.parametrize("KVH,H", [(8, 8), (1, 1)])
+def test_attention_of_too_many_threads_is_refused(KVH, H):
+    """Short contexts: whole units of eight waves, a workgroup of 512 threads each."""
+    L, most = nat.lib(), (2 ** 23 - 8) // KVH
+    args = dict(H=H, KVH=KVH, q_len=1, max_context=16, ws_bytes=1024)
+    assert L.msattn_paged_attention_fp4(*attend_args(B=most, **args)) == nat.ERR_WORKSPACE
+    for B in (most + 8, 1 << 27):
+        assert L.msattn_paged_attention_fp4(*attend_args(B=B, **{**args, "ws_bytes": 1 << 40})) == \
+            nat.ERR_UNSUPPORTED
