@@ -396,7 +396,8 @@ class PagedAttention:
         ``prefix_groups`` = (group_rows, prefix_pages): groups of rows, each behind shared pages
         of its own (paged_attention_shared), read once a group where the call is causal and
         without a window or RoPE. Over 4-bit caches (``paged_attention_fp4``) neither changes how
-        pages are read, and "triton_flash" is refused as over FP8 ones.
+        pages are read (malformed ones are refused all the same), and "triton_flash" is refused as
+        over FP8 ones.
         """
         if backend not in _BACKENDS:
             raise ValueError(f"unknown attention backend: {backend!r}")
@@ -404,9 +405,20 @@ class PagedAttention:
             if backend == "triton_flash":
                 raise ValueError("triton_flash does not support a 4-bit KV cache")
             from .fp4 import paged_attention_fp4
+            window = self.window if window is None else window
+            if causal and window is None and query.ndim == 4 and \
+                    (prefix_groups is not None or shared_prefix_pages):
+                # (refused where the other caches' calls are)
+                B, q_len = query.shape[:2]
+                block_table = block_table_i32(block_table, query.device)
+                W = block_table.shape[1]
+                if prefix_groups is not None:
+                    from .shared import check_groups
+                    check_groups(*prefix_groups, B, W, query.device)
+                elif q_len == 1 and not 0 <= int(shared_prefix_pages) <= W:
+                    raise ValueError(f"prefix_pages {shared_prefix_pages} outside [0, {W}]")
             return paged_attention_fp4(query, k_cache, v_cache, block_table, context_lens,
-                                       causal=causal, scale=scale,
-                                       window=self.window if window is None else window)
+                                       causal=causal, scale=scale, window=window)
         if backend == "triton_flash":
             if not causal:
                 raise ValueError("triton_flash supports causal decode only")

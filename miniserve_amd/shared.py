@@ -17,17 +17,16 @@ from .attention import (_host_ints_to_device, _require_gpu, _workspace, block_ta
 from .rotary import current, extent, on_device
 
 
-def _groups_i32(group_rows, prefix_pages, batch: int, width: int, dev: torch.device
-                ) -> tuple[torch.Tensor, torch.Tensor]:
-    """(int32 [groups + 1], int32 [groups]) on `dev`; host values are checked."""
+def check_groups(group_rows, prefix_pages, batch: int, width: int, dev: torch.device) -> list:
+    """[group_rows, prefix_pages], host values checked and as lists, tensors on `dev` as they are (the
+    host does not read them); as many of the one as the other needs."""
     out = []
     for name, x, most in (("group_rows", group_rows, batch), ("prefix_pages", prefix_pages, width)):
         if isinstance(x, torch.Tensor) and (x.dtype.is_floating_point or x.dtype.is_complex or
                                             x.dtype == torch.bool):
             raise ValueError(f"{name} must hold whole numbers")
         if isinstance(x, torch.Tensor) and x.device == dev:
-            x = x if x.ndim == 1 else x.reshape(-1)
-            out.append(narrow_i32(x, 0, most).contiguous())
+            out.append(x if x.ndim == 1 else x.reshape(-1))
             continue
         given = x.reshape(-1).tolist() if isinstance(x, torch.Tensor) else list(x)
         values = [int(v) for v in given]
@@ -39,11 +38,20 @@ def _groups_i32(group_rows, prefix_pages, batch: int, width: int, dev: torch.dev
                 raise ValueError(f"group_rows must ascend within [0, {batch}]")
         elif any(not 0 <= v <= width for v in values):
             raise ValueError(f"prefix_pages must lie within [0, {width}]")
-        out.append(_host_ints_to_device(values, dev))
-    rows, pages = out
-    if rows.numel() != pages.numel() + 1 and not (rows.numel() == 0 and pages.numel() == 0):
-        raise ValueError(f"{pages.numel()} groups need {pages.numel() + 1} group_rows, not "
-                         f"{rows.numel()}")
+        out.append(values)
+    rows, pages = map(len, out)
+    if rows != pages + 1 and not (rows == 0 and pages == 0):
+        raise ValueError(f"{pages} groups need {pages + 1} group_rows, not {rows}")
+    return out
+
+
+def _groups_i32(group_rows, prefix_pages, batch: int, width: int, dev: torch.device
+                ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(int32 [groups + 1], int32 [groups]) on `dev`; host values are checked."""
+    rows, pages = (
+        narrow_i32(x, 0, most).contiguous() if isinstance(x, torch.Tensor) else
+        _host_ints_to_device(x, dev)
+        for x, most in zip(check_groups(group_rows, prefix_pages, batch, width, dev), (batch, width)))
     return rows, pages
 
 

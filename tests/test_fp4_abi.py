@@ -134,3 +134,30 @@ def test_attention_of_too_many_threads_is_refused(KVH, H):
     for B in (most + 8, 1 << 27):
         assert L.msattn_paged_attention_fp4(*attend_args(B=B, **{**args, "ws_bytes": 1 << 40})) == \
             nat.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("given,match", [
+    (dict(shared_prefix_pages=4), "outside"), (dict(shared_prefix_pages=-1), "outside"),
+    (dict(prefix_groups=([0, 3], [1])), "ascend"), (dict(prefix_groups=([1, 0], [1])), "ascend"),
+    (dict(prefix_groups=([0, 2], [4])), "within"), (dict(prefix_groups=([0, 2], [1, 1])), "need"),
+    (dict(prefix_groups=([0, 1.5], [1])), "whole"),
+    (dict(prefix_groups=(torch.tensor([0.0, 2.0]), [1])), "whole")], ids=str)
+def test_malformed_prefixes_are_refused_though_unused(given, match):
+    pa = PagedAttention(4, 2, 64, num_blocks=8, block_size=16, kv_dtype=torch.float4_e2m1fn_x2)
+    kc, vc = pa.allocate_kv_cache()
+    q, table = torch.zeros(2, 1, 4, 64), torch.zeros(2, 3, dtype=torch.int32)
+    with pytest.raises(ValueError, match=match):
+        pa(q, kc, vc, table, [1, 1], **given)
+    # as over other caches, where they are not looked at: under a window, not causal, as far as the GPU
+    for kw in (dict(window=5), dict(causal=False)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            pa(q, kc, vc, table, [1, 1], **given, **kw)
+
+
+@pytest.mark.parametrize("given", [{}, dict(shared_prefix_pages=3), dict(shared_prefix_pages=0),
+                                   dict(prefix_groups=([0, 2], [3])), dict(prefix_groups=([], []))], ids=str)
+def test_prefixes_are_accepted(given):
+    pa = PagedAttention(4, 2, 64, num_blocks=8, block_size=16, kv_dtype=torch.float4_e2m1fn_x2)
+    kc, vc = pa.allocate_kv_cache()
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        pa(torch.zeros(2, 1, 4, 64), kc, vc, torch.zeros(2, 3, dtype=torch.int32), [1, 1], **given)
