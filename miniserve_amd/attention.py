@@ -38,7 +38,7 @@ _BACKENDS = ("sdpa", "triton_flash")
 # tensor is unchanged, list lengths go through pinned memory, and a call without a
 # workspace reuses one zeroed workspace per (device, stream).
 _cache_lock = threading.Lock()
-_table_cache: dict[tuple, tuple] = {}   # (id, device) -> (weakref, version, meta, int32 table)
+_table_cache: dict[tuple, tuple] = {}   # (id, device, stream) -> (weakref, version, meta, int32 table)
 _TABLE_CACHE_MAX = 16
 _workspaces: dict[tuple, torch.Tensor] = {}  # (device index, stream handle) -> uint8 tensor
 
@@ -116,7 +116,8 @@ def block_table_i32(block_table, device: torch.device) -> torch.Tensor:
     A device tensor that needs converting (the reference keeps int64 tables,
     attention.py:237) is converted once and reused while it is unchanged: same object,
     same torch version counter (every in-place write through torch bumps it), same shape
-    and strides. Not during graph capture, whose conversions must be captured."""
+    and strides, by calls on one stream (another's would neither wait for the conversion nor keep
+    its memory). Not during graph capture, whose conversions must be captured."""
     if isinstance(block_table, torch.Tensor) and block_table.dtype == torch.int32 and \
             block_table.ndim == 2 and block_table.device == device and block_table.is_contiguous():
         return block_table
@@ -127,7 +128,7 @@ def block_table_i32(block_table, device: torch.device) -> torch.Tensor:
         version = block_table._version
     except RuntimeError:  # inference-mode tensors keep no version counter: no reuse
         return _convert_table(block_table)
-    key = (id(block_table), str(device))
+    key = (id(block_table), str(device), nat.stream_handle(device) if device.type == "cuda" else 0)
     meta = (block_table.data_ptr(), tuple(block_table.shape), block_table.stride(),
             block_table.dtype)
     with _cache_lock:
