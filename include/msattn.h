@@ -513,6 +513,15 @@ size_t msattn_fp4_workspace_bytes(int batch, int q_len, int num_heads, int num_k
                                   int head_dim, int max_context, int q_dtype);
 
 /*
+ * How msattn_paged_attention_fp4 takes a call of these sizes (what it returns is the same either
+ * way, but for the order of sums): plan[0] 0 units of a row, a KV head and some of its query rows dealt
+ * whole to waves, 1 units cut into parts, 2 equal shares of a list of all units' keys; plan[1] blocks of
+ * 16 query rows a unit has, plan[2] waves a unit, plan[3] parts a unit. Nothing is launched.
+ */
+int msattn_fp4_plan(int batch, int q_len, int num_heads, int num_kv_heads, int head_dim,
+                    int max_context, int causal, int window, int q_dtype, int* plan);
+
+/*
  * msattn_paged_attention over a 4-bit cache: fp32, fp16 or bf16 query, any q_len, causal or not,
  * window as there; one launch. The query's strides are in elements, its rows and the contiguous out
  * 16-byte aligned; out shares no memory with the query or the caches. max_context is at most 2^30

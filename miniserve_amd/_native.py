@@ -107,6 +107,7 @@ SIGNATURES = {
         c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp,
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp]),
     "msattn_fp4_workspace_bytes": (c_size, [c_int] * 7),
+    "msattn_fp4_plan": (c_int, [c_int] * 9 + [ctypes.POINTER(c_int)]),
     "msattn_paged_attention_fp4": (c_int, [
         c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_size,
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,

@@ -192,6 +192,10 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   return true;
 }
 
+bool launch_ok(const Plan& p) {
+  return p.way == kFp4List || grid_ok(8 * static_cast<int64_t>(p.xcd_units), kFp4Threads);
+}
+
 }  // namespace
 
 extern "C" {
@@ -256,6 +260,22 @@ size_t msattn_fp4_workspace_bytes(int batch, int q_len, int num_heads, int num_k
   return plan.total;
 }
 
+int msattn_fp4_plan(int batch, int q_len, int num_heads, int num_kv_heads, int head_dim,
+                    int max_context, int causal, int window, int q_dtype, int* plan) {
+  Plan p;
+  if (!plan || window < 0 || !float_type(q_dtype) ||
+      !geometry_ok(batch, q_len, num_heads, num_kv_heads, head_dim, max_context))
+    return MSATTN_ERR_INVALID_ARG;
+  if (!plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, causal, window, q_dtype, &p) ||
+      !launch_ok(p))
+    return MSATTN_ERR_UNSUPPORTED;
+  plan[0] = p.way;
+  plan[1] = p.ct;
+  plan[2] = p.wk;
+  plan[3] = p.parts;
+  return MSATTN_OK;
+}
+
 int msattn_paged_attention_fp4(const void* query, int64_t q_batch_stride,
                                int64_t q_token_stride, int64_t q_head_stride,
                                const void* k_cache, const void* v_cache,
@@ -280,9 +300,8 @@ int msattn_paged_attention_fp4(const void* query, int64_t q_batch_stride,
   for (int64_t x : q_strides)
     if (x < 0 || x * eb % 16 != 0) return MSATTN_ERR_INVALID_ARG;
   Plan plan;
-  if (!plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, causal, window, q_dtype, &plan))
-    return MSATTN_ERR_UNSUPPORTED;
-  if (plan.way != kFp4List && !grid_ok(8 * static_cast<int64_t>(plan.xcd_units), kFp4Threads))
+  if (!plan_of(batch, q_len, num_heads, num_kv_heads, head_dim, max_context, causal, window, q_dtype, &plan) ||
+      !launch_ok(plan))
     return MSATTN_ERR_UNSUPPORTED;
   if (workspace_bytes < plan.total) return MSATTN_ERR_WORKSPACE;
   char* const ws = static_cast<char*>(workspace);

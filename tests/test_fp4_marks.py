@@ -50,7 +50,7 @@ class Marked:
         self.caches = []
         kept = []
         for x, is_values in ((k, False), (v, True)):
-            codes, scale = fp4.quantise(x)
+            codes, scale = quantise(x)
             kept.append(fp4.values(codes, scale))
             codes[~seen], scale[~seen] = 15, 255
             self.caches.append(pack(codes, scale, is_values))
@@ -111,6 +111,19 @@ class Marked:
                         (b, i, h, int(over.argmax()), over.max(), limit[over.argmax()])
 
 
+def quantise(x):
+    """fp4.quantise by the exponents of the largest magnitudes: the tests' contexts are long."""
+    blocks = x.double().unflatten(-1, (-1, 32))
+    top = blocks.abs().amax(-1, keepdim=True)
+    mant, exp = torch.frexp(top)  # top = mant 2^exp, mant in [0.5, 1)
+    exp = torch.where(top > 0, exp - 3 + (mant > 0.875), -126).clamp(-126, 125)
+    y = torch.ldexp(blocks.abs(), -exp)
+    code = sum((y > m if i % 2 == 0 else y >= m).to(torch.uint8) for i, m in
+               enumerate((0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)))
+    code |= torch.signbit(blocks).to(torch.uint8) << 3
+    return code.flatten(-2).numpy(), (exp[..., 0] + 127).to(torch.uint8).numpy()
+
+
 def pack(codes, scale, is_values):
     """fp4.pack without a loop over elements: the tests' contexts are long."""
     nb, bs, H, D = codes.shape
@@ -123,7 +136,11 @@ def pack(codes, scale, is_values):
 
 
 def test_packing():
-    codes, scale = fp4.quantise(torch.randn(2, 32, 3, 96, generator=torch.Generator().manual_seed(0)))
+    x = torch.randn(2, 32, 3, 96, generator=torch.Generator().manual_seed(0))
+    x[0, 0, 0, :12] = torch.tensor([6, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, -0.0, -5, 5.01, -0.25])
+    x[0, 1, 0, :32], x[0, 2, 0, 0], x[0, 3, 0, 0] = 0.0, 7.0, 1e-40
+    codes, scale = fp4.quantise(x)
+    assert (quantise(x)[0] == codes).all() and (quantise(x)[1] == scale).all()
     for is_values in (False, True):
         assert torch.equal(pack(codes, scale, is_values), fp4.pack(codes, scale, is_values))
 
