@@ -88,13 +88,13 @@ int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 // A wave's time for a group with 64 query rows over that with 32: less than twice, since the keys and
-// values are widened once. 512 queries of H28/KVH4/D128 behind 4096 keys, 2 rows: 92 us against 103;
+// values are widened once. 512 queries of H28/KVH4/D128 behind 4096 keys, 2 rows: 103 us against 111;
 // 1024 queries of H32/KVH8/D128 by themselves, 4 rows, where half as many units fill the CUs less
-// evenly: 96 against 88, and this factor chooses the latter.
+// evenly: 99 against 90, and this factor chooses the latter.
 constexpr double kRound64 = 1.8;
 
-// And with 16. 32 rows of 4 drafts of H28/KVH4/D128 under a window of 2048, 128 units of 28 rows: 24.8
-// us, as 256 of 16 19.8; the chunk above 143.
+// And with 16. 32 rows of 4 drafts of H28/KVH4/D128 under a window of 2048, 128 units of 28 rows: 24.1
+// us, as 256 of 16 18.6; the chunk above 147.
 constexpr double kRound16 = 0.65;
 
 // Contexts go up to this: a position plus a query's offset or a window fits 31 bits.
@@ -131,8 +131,9 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   // groups (about 1.3 us at 32 rows, two waves a SIMD): a unit's start and end are about 3 of them,
   // and about 10 each with a list (its plan, partials and joins, in which all waves of a workgroup
   // meet). Several rounds of the CUs even out; the last unit to start does not. Measured: 896 units of
-  // 145 groups, wk = 1, 2, 4, 8 and the list, 191, 103, 104, 126, 161 us; 896 of 65, causal, 70, 40, 42,
-  // 62, 231; 4096 of 33, causal, 96, 85, 109, 190, 332. Units of few rows take all waves of a workgroup.
+  // 32 rows and 144 groups, wk = 1, 2, 4, 8 and the list, 210, 111, 113, 124, 161 us; of 65 groups 101,
+  // 58, 59, 70, 105; 4096 of 32, causal, 105, 90, 114, 160, 301. Units of few rows take all waves of a
+  // workgroup.
   const double mean = groups - (causal && window == 0 ? 0.5 * std::min(q_len, max_ctx) / kFp4Group : 0.0);
   const double listed = static_cast<double>(units) / want;  // units a CU
   double best = 1e300;
@@ -155,9 +156,10 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
     // Where a CU gets several units of few rows, in us: dealt, each round of them starts anew (about 3.7
     // on top of 5), and a list shares their groups evenly (10, 5 a unit and CU). Dealt units take longer
     // for their groups where these stream at the memory's rate, bf16 above 64 dims, than where the
-    // waves' own work bounds them. List / dealt: H32/KVH8/D128, 64 rows up to 640 keys 26.0 / 16.4, 1300
-    // 32.6 / 25.8, 1024 to 8192 49.1 / 58.6; 100 rows of 1000 39.3 / 38.9, of 2500 62.7 / 67.7; in fp32
-    // 64 of 2500 54.0 / 46.5; H12/KVH12/D64, 64 of 2500 51.6 / 39.1, 100 in fp32 84.5 / 74.9.
+    // waves' own work bounds them. List / dealt: H32/KVH8/D128, 64 rows of 640 keys 19.5 / 17.5, of 1300
+    // 33.5 / 25.8, of 1024 to 8192 49.5 / 59.6; 100 rows of 1000 39.6 / 36.4, of 2500 62.7 / 65.4; in
+    // fp32 64 of 2500 55.0 / 44.0; H12/KVH12/D64, 64 of 2500 51.8 / 30.1, 100 in fp32 82.1 / 71.8. (64 of
+    // 5000 there, which these figures leave to a list: 77.7 / 50.1.)
     const double slower = parts > 1 || D <= 64 ? 0.2 : 0.45;  // us a wave's group
     const bool few = slower * listed * groups / kFp4Waves < 5 + 1.3 * listed;
     if (split && listed > 1) best = few ? 1e300 : 0;
@@ -170,10 +172,10 @@ bool plan_of(int batch, int q_len, int H, int KVH, int D, int max_ctx, int causa
   }
   // Few units: each cut into as many parts as there are CUs for it, a workgroup a part, joined like
   // shares but without a list's plan. Start, partials and join cost 7 groups, 5 of the longer ones above
-  // 128 dims. List / parts: 16 rows of 1024 to 4096 keys of H28/KVH4/D128 in fp16 20.5 / 16.1 us, 16 of
-  // 16384 of H32/KVH8/D128 58.6 / 52.7, 32 of 1024 to 8192 of H8/KVH1/D256 in fp32 44.8 / 30.1. Dealt /
-  // parts: 4 rows of H32/KVH8/D128 up to 600 keys 9.0 / 11.2, 1000 10.8 / 11.4, 1400 12.3 / 11.7, 2000
-  // 14.4 / 12.2; 16 of H8/KVH1/D256 up to 600 13.5 / 12.9, 2000 22.2 / 14.4.
+  // 128 dims. List / parts: 16 rows of 1024 to 4096 keys of H28/KVH4/D128 in fp16 20.7 / 16.1 us, 16 of
+  // 16384 of H32/KVH8/D128 58.6 / 51.8, 32 of 1024 to 8192 of H8/KVH1/D256 in fp32 42.1 / 31.5. Dealt /
+  // parts: 4 rows of H32/KVH8/D128 up to 600 keys 9.0 / 11.1, 1000 10.8 / 11.3, 1400 12.3 / 11.4, 2000
+  // 14.5 / 12.0; 16 of H8/KVH1/D256 up to 600 13.9 / 13.3, 2000 22.8 / 14.6.
   const int64_t most = std::min<int64_t>(want / units, (groups + kFp4Waves - 1) / kFp4Waves);
   if (split && most > 1) {
     const double cost = (rows > 16 && list_ct == 1 ? kRound16 : 1.0) *

@@ -8,11 +8,11 @@
 //          into one contiguous share a CU, whatever the lengths (read on the device, so a call is
 //          capture-safe). A workgroup's waves take its share's groups in turn, and go on from unit
 //          to unit without waiting for each other. For more units than CUs, long and ragged: 64 rows
-//          of 1024 to 8192 keys of H32/KVH8/D128 take 49 us, 4.4 TB/s of the cache, 5.4 to 6.8 inside
+//          of 1024 to 8192 keys of H32/KVH8/D128 take 50 us, 4.3 TB/s of the cache, 5.4 to 6.8 inside
 //          a share.
 //   parts  a unit is cut into equal parts, a workgroup each, joined as shares are but without a
 //          plan. For few long units: 16 rows of 1024 to 4096 keys of H28/KVH4/D128 in fp16 take 16
-//          us, as a list 20.5.
+//          us, as a list 20.7.
 //   dealt  a unit is whole: WK waves take its groups in turn, and 8 / WK units share a workgroup.
 //          For chunks of prompts, with thousands of units, and for short contexts: no plan, no
 //          partials and no joins.
@@ -69,8 +69,8 @@ constexpr int kFp4Shares = 256;          // of a list, at most: one a CU, an arr
 static_assert(kFp4Shares <= kMaxTickets, "a counter a share");
 // Positions of the list ahead of a unit's groups that hold no work: what its start and end cost a
 // workgroup, in groups. Without them a share of many short units ends last: 64 rows of H32/KVH8/D128
-// with 1024 to 8192 keys, 0, 8, 24 and 48 of them, 58.0, 53.0, 49.6 and 51.6 us; 16 rows of 16384 keys
-// each, where every share has the same, 56.3, 60.3, 59.3 and 59.5.
+// with 1024 to 8192 keys, 0, 8, 24 and 48 of them, 58.2, 52.8, 50.0 and 52.0 us; with 4096 each, where
+// every share has the same, 56.6, 56.7, 57.7 and 57.2.
 constexpr int kFp4Head = 24;
 
 struct Fp4Params {
@@ -1150,8 +1150,9 @@ __global__ __launch_bounds__(kFp4Threads, 2) void fp4_attn_kernel(const Fp4Param
 
 // Blocks of 16 query rows that a wave takes at most, by the bf16 parts of a query element: what its
 // registers hold of accumulators, query and the groups on their way. Past it they spill: at 256 dims two
-// blocks 500 bytes a lane and more (40 rows of 4 drafts of H8/KVH1, 300 to 2000 keys: 105 us against
-// 24), fp32 of 128 dims 150 (2 x 512 queries of H28/KVH4 behind 4096 keys: 219 against 201).
+// blocks 500 bytes a lane and more (40 rows of 4 drafts of H8/KVH1, 300 to 2000 keys, as units of eight
+// waves: 99 us against 25), fp32 of 128 dims 150 (2 x 512 queries of H28/KVH4 behind 4096 keys, units of
+// two waves: 205 against 191).
 constexpr int fp4_max_ct(int parts, int DP) {
   return DP > 128 || (DP > 64 && parts == 3) ? 1 : (parts == 1 ? 4 : 2);
 }

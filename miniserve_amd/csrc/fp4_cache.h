@@ -3,11 +3,12 @@
 // Elements are e2m1 (a sign and 0, 0.5, 1, 1.5, 2, 3, 4, 6); each 32 of a row share a power of
 // two, held as its exponent + 127 in a byte (the OCP microscaling format MXFP4, which gfx950
 // widens and rounds in one instruction each). For a block whose largest magnitude is a the
-// power is the one that puts a / 2^e in (3.5, 7]: a rounds to 4 or 6, off by at most 1/7 of it.
+// power is the one that puts a / 2^e in (3.5, 7]: a rounds to 4 or 6, off by at most a fifth of it
+// (5 to 4), and no element by more than 2^e.
 // (The rms error of normal values is 0.1119 of theirs, against 0.1149 for the exponent of a alone
 // and 0.1155 for the smallest power that saturates nothing.) Elements round to the nearest, ties to
 // the even code. The bytes 1 .. 252 are used, so that both the power and 6 times it are normal in
-// fp32 and bf16. A block with a NaN or an infinity has the byte 255: all of it reads as NaN.
+// fp32 and bf16; past 7 2^125 a saturates at 6 2^125, below 3.5 2^-126 it takes 2^-126. A block with a NaN or an infinity has the byte 255: all of it reads as NaN.
 //
 // A cache is uint8 [num_blocks, kv_heads, block_size / 16, 17 D / 2]: one tile, contiguous, for 16
 // tokens of one head, its 8 D bytes of elements and then its scales as [D / 32][16 tokens]. Two

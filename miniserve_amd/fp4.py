@@ -95,9 +95,10 @@ def write_kv_fp4(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
 
     Row b's token t goes to position start[b] + t (``start``: an int, one entry per row, or an int
     tensor); tokens on holes of the block table or outside it are not written. Each 32 elements of
-    a row take the power of two 2^e for which the largest magnitude lies in (3.5, 7] 2^e, and go to
-    the nearest of 0, 0.5, 1, 1.5, 2, 3, 4 and 6 times it (ties to the even code, at most 6), so
-    that none is off by more than 2^e, a 3.5th of the largest; 32 elements with a NaN or an infinity
+    a row take the power of two 2^e for which the largest magnitude lies in (3.5, 7] 2^e (-126 <= e
+    <= 125), and go to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4 and 6 times it (ties to the even code,
+    at most 6), so that none is off by more than 2^e, a 3.5th of the largest, where that is from
+    4.1e-38 to 2.9e38 (larger ones saturate at 6 2^125); 32 elements with a NaN or an infinity
     among them read back as NaN. A row's bytes do not depend on what is written beside it. Two
     tokens of one call must not land in one slot: parts of either's rows may remain there.
     """
