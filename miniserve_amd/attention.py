@@ -34,7 +34,7 @@ _BACKENDS = ("sdpa", "triton_flash")
 
 # Per-call host work of the eager path (the reference runner calls forward once per layer
 # with an int64 device table and a Python-list context_lens, model_runner.py:72-83) is kept
-# off the common case: the int32 table of a source tensor is converted once while the
+# off the common case: the int32 table of a source tensor is converted once a stream while the
 # tensor is unchanged, list lengths go through pinned memory, and a call without a
 # workspace reuses one zeroed workspace per (device, stream).
 _cache_lock = threading.Lock()
